@@ -869,6 +869,27 @@ int pxl_dma_launch_captured(void* slot0, void* slot1);
 void pxl_elt_pair_begin(void);
 int pxl_elt_pair_end(void);
 
+/* ------------------------------------------------------------------------------------------ */
+/* Layer normalisation (csrc/layernorm.hip): what a torch TaskModel of a plugin takes next to BatchNorm / IBNorm              */
+/* ------------------------------------------------------------------------------------------ */
+/* u = (x - mean) / sqrt(var + eps), y = u * w + b; mean / var over the C features of a row, in fp32.
+ * dtype: type of x, y, dy, dx; pdtype: type of w, b, dw, db -- PXL_F32 or dtype; w / b NULL: 1 / 0.
+ * rows form: x [R] rows of C contiguous features, x_stride elements apart (>= C); y, dy, dx are [R][C] without gaps.
+ * nchw form: x [N][C][S] without gaps, normalised over C at each of the N * S positions.
+ * mean, rstd: fp32, one per row / position, written by _fwd (both NULL: not kept) and read by _bwd.
+ * _bwd: dx, dw, db may each be NULL (not wanted); ws: *_bwd_workspace bytes when dw or db is wanted.  R == 0 / N * S == 0: dw and
+ * db are zero, nothing else is touched.  Sums have one order: equal inputs give equal bits.  No atomics, capturable. */
+int pxl_layer_norm_fwd(int dtype, int pdtype, long R, int C, long x_stride, const void* x, const void* w, const void* b, float eps,
+                       void* y, float* mean, float* rstd, void* stream);
+size_t pxl_layer_norm_bwd_workspace(long R, int C);
+int pxl_layer_norm_bwd(int dtype, int pdtype, long R, int C, long x_stride, const void* x, const void* dy, const void* w, const float* mean,
+                       const float* rstd, void* dx, void* dw, void* db, void* ws, size_t ws_bytes, void* stream);
+int pxl_layer_norm_nchw_fwd(int dtype, int pdtype, long N, int C, long S, const void* x, const void* w, const void* b, float eps, void* y,
+                            float* mean, float* rstd, void* stream);
+size_t pxl_layer_norm_nchw_bwd_workspace(long N, int C, long S);
+int pxl_layer_norm_nchw_bwd(int dtype, int pdtype, long N, int C, long S, const void* x, const void* dy, const void* w, const float* mean,
+                            const float* rstd, void* dx, void* dw, void* db, void* ws, size_t ws_bytes, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -274,6 +274,12 @@ SIGNATURES = {
     "pxl_net_cons_head_supported": (_I, [_P]),
     "pxl_net_cons_head_fwd": (_I, [_P, _P, _P, _P, _Z, _P, _P]),
     "pxl_net_cons_head_bwd": (_I, [_P, _P, _Z, _P, _P]),
+    "pxl_layer_norm_fwd": (_I, [_I, _I, _L, _I, _L, _P, _P, _P, _F, _P, _P, _P, _P]),
+    "pxl_layer_norm_bwd_workspace": (_Z, [_L, _I]),
+    "pxl_layer_norm_bwd": (_I, [_I, _I, _L, _I, _L, _P, _P, _P, _P, _P, _P, _P, _P, _P, _Z, _P]),
+    "pxl_layer_norm_nchw_fwd": (_I, [_I, _I, _L, _I, _L, _P, _P, _P, _F, _P, _P, _P, _P]),
+    "pxl_layer_norm_nchw_bwd_workspace": (_Z, [_L, _I, _L]),
+    "pxl_layer_norm_nchw_bwd": (_I, [_I, _I, _L, _I, _L, _P, _P, _P, _P, _P, _P, _P, _P, _P, _Z, _P]),
     "pxl_net_backward": (_I, [_P, _P, _P, _P, _P, _P, _P, _P, _Z, _P, _Z, _I, _P]),
 }
 

@@ -1,8 +1,8 @@
-"""Fused per-pixel losses (autograd Functions over libpixelhip kernels, NCHW fp32 tensors)."""
+"""Fused per-pixel losses (NCHW fp32 tensors) and layer normalisation (fp32 / bf16), autograd Functions over libpixelhip kernels."""
 import torch
 
 from . import _lib
-from ._lib import check, lib, ptr, stream_ptr
+from ._lib import check, dtype_code, lib, ptr, stream_ptr
 
 
 def _gpu(*ts):
@@ -270,3 +270,132 @@ class _SoftmaxChannels(torch.autograd.Function):
 def softmax_channels(x):
     """F.softmax(x, dim=1) of an NCHW fp32 prediction (the sseg activation), differentiable."""
     return _SoftmaxChannels.apply(x)
+
+
+# ---- layer normalisation (csrc/layernorm.hip) ---------------------------------------------------------------------------------
+def _launch(dev, fn, *args):
+    """fn(*args, stream) on the current stream of `dev`, which need not be the current device"""
+    if dev.index == torch.cuda.current_device():
+        check(fn(*args, stream_ptr()))
+    else:
+        with torch.cuda.device(dev):
+            check(fn(*args, stream_ptr()))
+
+
+def _row_stride(x):
+    """elements between the rows of a tensor whose last axis is contiguous and whose leading axes form one evenly spaced run
+    without overlap; None where they do not"""
+    C = x.shape[-1]
+    if x.stride(-1) != 1 and C > 1:
+        return None
+    step, span = None, 1
+    for k in range(x.dim() - 2, -1, -1):
+        n = x.shape[k]
+        if n == 1:
+            continue
+        if step is None:
+            step = x.stride(k)
+        elif x.stride(k) != step * span:
+            return None
+        span *= n
+    if step is None:
+        return C
+    return step if step >= C else None
+
+
+def _ln_forward(x, weight, bias, eps, channels, keep):
+    """-> (x as the kernel read it, geometry, y, mean, rstd); mean / rstd None unless `keep`"""
+    code = dtype_code(x.dtype)
+    pcode = code if weight is None and bias is None else dtype_code((bias if weight is None else weight).dtype)
+    if channels:
+        x = x.contiguous()
+        N, C = x.shape[0], x.shape[1]
+        S = x.numel() // (N * C) if x.numel() else 0
+        geo = (code, pcode, N, C, S)
+        rows, fn = N * S, lib().pxl_layer_norm_nchw_fwd
+        y = torch.empty_like(x)
+    else:
+        C = x.shape[-1]
+        stride = C if x.is_contiguous() else _row_stride(x)
+        if stride is None:
+            x, stride = x.contiguous(), C
+        rows = x.numel() // C
+        geo = (code, pcode, rows, C, stride)
+        fn = lib().pxl_layer_norm_fwd
+        y = torch.empty(x.shape, device=x.device, dtype=x.dtype)
+    stats = torch.empty(2, rows, device=x.device, dtype=torch.float32) if keep else None
+    mean = stats.data_ptr() if keep else None
+    _launch(x.device, fn, *geo, ptr(x), ptr(weight), ptr(bias), eps, ptr(y), mean, mean + 4 * rows if keep else None)
+    return x, geo, y, stats
+
+
+class _LayerNorm(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, weight, bias, eps, channels):
+        x, ctx.geo, y, stats = _ln_forward(x, weight, bias, eps, channels, True)
+        ctx.save_for_backward(x, weight, stats)
+        ctx.channels, ctx.pdtype = channels, None if weight is None and bias is None else (bias if weight is None else weight).dtype
+        return y
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, dy):
+        x, weight, stats = ctx.saved_tensors
+        dy = dy.contiguous()
+        geo, C = ctx.geo, ctx.geo[3]
+        rows = stats.shape[1]
+        need_x, need_w, need_b = ctx.needs_input_grad[:3]
+        dev = x.device
+        dx = torch.empty(x.shape, device=dev, dtype=x.dtype) if need_x else None
+        dw = torch.empty(C, device=dev, dtype=ctx.pdtype) if need_w else None
+        db = torch.empty(C, device=dev, dtype=ctx.pdtype) if need_b else None
+        h = lib()
+        ws, nbytes = None, 0
+        if need_w or need_b:
+            nbytes = h.pxl_layer_norm_nchw_bwd_workspace(geo[2], C, geo[4]) if ctx.channels else h.pxl_layer_norm_bwd_workspace(rows, C)
+            ws = torch.empty(nbytes, device=dev, dtype=torch.uint8)
+        mean = stats.data_ptr()
+        _launch(dev, h.pxl_layer_norm_nchw_bwd if ctx.channels else h.pxl_layer_norm_bwd, *geo, ptr(x), ptr(dy), ptr(weight), mean,
+                mean + 4 * rows, ptr(dx), ptr(dw), ptr(db), ptr(ws), nbytes)
+        return dx, dw, db, None, None
+
+
+def _layer_norm(name, x, weight, bias, eps, channels):
+    axis = 1 if channels else -1
+    if x.dim() < (2 if channels else 1) or x.shape[axis] == 0:
+        raise ValueError("%s: no features to normalise over in %s" % (name, tuple(x.shape)))
+    C = x.shape[axis]
+    for what, t in (("weight", weight), ("bias", bias)):
+        if t is None:
+            continue
+        if t.dim() != 1 or t.shape[0] != C:
+            raise ValueError("%s: %s %s for %d features" % (name, what, tuple(t.shape), C))
+        if t.dtype not in (torch.float32, x.dtype) or (weight is not None and t.dtype != weight.dtype):
+            raise ValueError("%s: weight and bias are both float32 or both of the type of x (%s), got %s" % (name, x.dtype, t.dtype))
+        if t.device != x.device:
+            raise ValueError("%s: %s on %s, x on %s" % (name, what, t.device, x.device))
+    if x.dtype not in (torch.float32, torch.bfloat16):
+        raise ValueError("%s: float32 or bfloat16, got %s" % (name, x.dtype))
+    if not eps >= 0:
+        raise ValueError("%s: eps %r" % (name, eps))
+    _gpu(x)
+    weight = weight.contiguous() if weight is not None else None
+    bias = bias.contiguous() if bias is not None else None
+    if torch.is_grad_enabled() and (x.requires_grad or (weight is not None and weight.requires_grad) or (bias is not None and bias.requires_grad)):
+        return _LayerNorm.apply(x, weight, bias, float(eps), channels)
+    return _ln_forward(x, weight, bias, float(eps), channels, False)[2]
+
+
+def layer_norm(x, weight=None, bias=None, eps=1e-5):
+    """(x - mean) / sqrt(var + eps) * weight + bias over the LAST axis of x (fp32 or bf16; any leading axes, rows may lie apart in
+    memory), statistics in fp32; weight / bias [C]: fp32 or the type of x.  Differentiable once in x, weight and bias; gradients
+    are the same bits from call to call."""
+    return _layer_norm("layer_norm", x, weight, bias, eps, False)
+
+
+def layer_norm_channels(x, weight=None, bias=None, eps=1e-5):
+    """`layer_norm` over axis 1 of an [N, C, ...] map at each position (a map stored channels last is read as it lies)."""
+    if x.dim() == 4 and x.dtype in (torch.float32, torch.bfloat16) and not x.is_contiguous() and \
+            x.is_contiguous(memory_format=torch.channels_last):
+        return _layer_norm("layer_norm_channels", x.permute(0, 2, 3, 1), weight, bias, eps, False).permute(0, 3, 1, 2)
+    return _layer_norm("layer_norm_channels", x, weight, bias, eps, True)

@@ -55,3 +55,28 @@ class GaussianNoiseLayer(nn.Module):
         mm = torch.empty(B, 2, device=inp.device, dtype=torch.float32)
         check(lib().pxl_gaussian_noise_apply(B, inp.numel() // B, ptr(inp), ptr(self.noise), ptr(mm), stream_ptr()))
         return inp
+
+
+class LayerNorm(nn.Module):
+    """Layer normalisation over the last axis, or over axis 1 of an [N, C, ...] map (channels_first=True), on the fused kernels
+    (functional.layer_norm / layer_norm_channels): for the torch task models a plugin brings, next to SynchronizedBatchNorm2d.
+    Parameter names and shapes are torch.nn.LayerNorm's for one normalised axis."""
+
+    def __init__(self, num_features, eps=1e-5, affine=True, channels_first=False):
+        super().__init__()
+        self.num_features, self.eps, self.channels_first = int(num_features), float(eps), bool(channels_first)
+        if self.num_features < 1 or not self.eps >= 0:
+            raise ValueError("LayerNorm: num_features %r, eps %r" % (num_features, eps))
+        self.weight = nn.Parameter(torch.ones(self.num_features)) if affine else None
+        self.bias = nn.Parameter(torch.zeros(self.num_features)) if affine else None
+
+    def forward(self, x):
+        from .. import functional as PF
+        axis = 1 if self.channels_first else -1
+        if x.dim() < (2 if self.channels_first else 1) or x.shape[axis] != self.num_features:
+            raise ValueError("LayerNorm: %s has no axis of %d features at %d" % (tuple(x.shape), self.num_features, axis))
+        f = PF.layer_norm_channels if self.channels_first else PF.layer_norm
+        return f(x, self.weight, self.bias, self.eps)
+
+    def extra_repr(self):
+        return "%d, eps=%g, affine=%s, channels_first=%s" % (self.num_features, self.eps, self.weight is not None, self.channels_first)
