@@ -890,6 +890,34 @@ size_t pxl_layer_norm_nchw_bwd_workspace(long N, int C, long S);
 int pxl_layer_norm_nchw_bwd(int dtype, int pdtype, long N, int C, long S, const void* x, const void* dy, const void* w, const float* mean,
                             const float* rstd, void* dx, void* dw, void* db, void* ws, size_t ws_bytes, void* stream);
 
+/* ------------------------------------------------------------------------------------------ */
+/* Orthogonalised updates (csrc/muon.hip): the Muon optimizer next to SGD / Adam                */
+/* ------------------------------------------------------------------------------------------ */
+/* One matrix [rows][cols] without gaps.  pxl_orthogonalize: p <- the result, g: the matrix, mom / scale unused.
+ * pxl_muon_step: p the parameter, g its gradient (type `dtype`), mom the momentum (fp32), scale: the factor on lr of this matrix. */
+typedef struct pxl_ns_item {
+  void* p;
+  const void* g;
+  float* mom;
+  int32_t rows, cols;
+  float scale;
+  int32_t reserved;
+} pxl_ns_item;
+/* items: HOST array; n matrices of any mix of shapes, none of which overlap (p of one against anything of another); p == g is allowed
+ * in pxl_orthogonalize.  coef: HOST array [steps][3], 1 .. 16 steps;
+ *   X = G / max(|G|_F, eps);  per step  X <- a X + (b L + c L^2) X,  L = X X'  (of the transposed matrix when rows > cols)
+ * fp32 results: every product to 22 bits and more, sums in fp32;  bf16: the result rounded once.  Coefficients that let singular values in
+ * [0, 1] grow past 16 are refused.
+ * pxl_muon_step:  mom <- momentum * mom + (1 - momentum) * g;  u = nesterov ? (1 - momentum) * g + momentum * mom : mom;
+ *                 p <- p * (1 - lr * weight_decay) - lr * scale * orthogonalised(u)
+ * ws: pxl_ns_workspace(dtype, items, n) bytes (0: a bad argument), 256-byte aligned, not shared with another call in flight.
+ * The item list is copied at the call (kernel arguments): nothing of it is read later.  Equal inputs give equal bits; capturable. */
+size_t pxl_ns_workspace(int dtype, const pxl_ns_item* items, int n);
+int pxl_orthogonalize(int dtype, const pxl_ns_item* items, int n, int steps, const float* coef, float eps, void* ws, size_t ws_bytes,
+                      void* stream);
+int pxl_muon_step(int dtype, const pxl_ns_item* items, int n, int steps, const float* coef, float eps, double lr, double momentum, int nesterov,
+                  double weight_decay, void* ws, size_t ws_bytes, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

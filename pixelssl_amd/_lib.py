@@ -49,6 +49,11 @@ class UpdSeg(C.Structure):
     _fields_ = [("off", C.c_int64), ("n", C.c_int64), ("s_pk", C.c_int64), ("t_pk", C.c_int64)]
 
 
+class NsItem(C.Structure):
+    _fields_ = [("p", C.c_void_p), ("g", C.c_void_p), ("mom", C.c_void_p), ("rows", C.c_int32), ("cols", C.c_int32),
+                ("scale", C.c_float), ("reserved", C.c_int32)]
+
+
 class BnDesc(C.Structure):
     _fields_ = [("C", C.c_int32), ("gamma_off", C.c_int32), ("beta_off", C.c_int32),
                 ("rmean_off", C.c_int32), ("rvar_off", C.c_int32), ("eps", C.c_float),
@@ -280,6 +285,9 @@ SIGNATURES = {
     "pxl_layer_norm_nchw_fwd": (_I, [_I, _I, _L, _I, _L, _P, _P, _P, _F, _P, _P, _P, _P]),
     "pxl_layer_norm_nchw_bwd_workspace": (_Z, [_L, _I, _L]),
     "pxl_layer_norm_nchw_bwd": (_I, [_I, _I, _L, _I, _L, _P, _P, _P, _P, _P, _P, _P, _P, _P, _Z, _P]),
+    "pxl_ns_workspace": (_Z, [_I, _P, _I]),
+    "pxl_orthogonalize": (_I, [_I, _P, _I, _I, _P, _F, _P, _Z, _P]),
+    "pxl_muon_step": (_I, [_I, _P, _I, _I, _P, _F, C.c_double, C.c_double, _I, C.c_double, _P, _Z, _P]),
     "pxl_net_backward": (_I, [_P, _P, _P, _P, _P, _P, _P, _P, _Z, _P, _Z, _I, _P]),
 }
 

@@ -1,4 +1,8 @@
-"""Fused per-pixel losses (NCHW fp32 tensors) and layer normalisation (fp32 / bf16), autograd Functions over libpixelhip kernels."""
+"""Fused per-pixel losses (NCHW fp32 tensors) and layer normalisation (fp32 / bf16), autograd Functions over libpixelhip kernels;
+orthogonalised updates of weight matrices."""
+import ctypes
+import functools
+
 import torch
 
 from . import _lib
@@ -399,3 +403,124 @@ def layer_norm_channels(x, weight=None, bias=None, eps=1e-5):
             x.is_contiguous(memory_format=torch.channels_last):
         return _layer_norm("layer_norm_channels", x.permute(0, 2, 3, 1), weight, bias, eps, False).permute(0, 3, 1, 2)
     return _layer_norm("layer_norm_channels", x, weight, bias, eps, True)
+
+
+# ---- orthogonalised updates (csrc/muon.hip) -----------------------------------------------------------------------------------
+NEWTON_SCHULZ = (3.4445, -4.7750, 2.0315)      # (a, b, c) of x (a + b x^2 + c x^4): singular values to 0.7 .. 1.2 in five steps
+
+
+@functools.lru_cache(maxsize=64)
+def _ns_coefficients(steps, coefficients):
+    """(a, b, c) for every step, or one triple per step -> float[steps * 3]"""
+    if coefficients and not isinstance(coefficients[0], tuple):
+        coefficients = (coefficients,) * steps
+    if steps < 1 or len(coefficients) != steps or any(len(t) != 3 for t in coefficients):
+        raise ValueError("Newton-Schulz: %d steps need one (a, b, c) or as many, got %r" % (steps, coefficients))
+    flat = [float(v) for t in coefficients for v in t]
+    return (ctypes.c_float * len(flat))(*flat)
+
+
+def _coefficients(steps, coefficients):
+    c = tuple(tuple(t) if isinstance(t, (tuple, list)) else float(t) for t in coefficients)
+    return _ns_coefficients(int(steps), c)
+
+
+def orthogonalize(x, steps=5, coefficients=NEWTON_SCHULZ, eps=1e-7):
+    """Every matrix of x [..., rows, cols] (fp32 or bf16) with its singular values driven to about 1 by `steps` of the Newton-Schulz
+    iteration X <- (a + b L + c L^2) X, L = X X', from X = x / max(|x|, eps) (Frobenius norm); for rows > cols on the transposed
+    matrix.  coefficients: one (a, b, c) or one per step.  A NaN or an infinity makes its own matrix NaN.  Not differentiable."""
+    if x.dim() < 2:
+        raise ValueError("orthogonalize: %s is no matrix" % (tuple(x.shape),))
+    if x.dtype not in (torch.float32, torch.bfloat16):
+        raise ValueError("orthogonalize: float32 or bfloat16, got %s" % x.dtype)
+    if not eps > 0:
+        raise ValueError("orthogonalize: eps %r" % (eps,))
+    coef = _coefficients(steps, coefficients)
+    if torch.is_grad_enabled() and x.requires_grad:
+        raise _lib.PixelHipError("orthogonalize has no gradient: call it under torch.no_grad() or on a detached tensor")
+    _gpu(x)
+    x = x.detach().contiguous()
+    out = torch.empty_like(x)
+    rows, cols = x.shape[-2], x.shape[-1]
+    if x.numel():
+        size = rows * cols * x.element_size()
+        src, dst = x.data_ptr(), out.data_ptr()
+        n = x.numel() // (rows * cols)
+        items = (_lib.NsItem * n)(*[(dst + k * size, src + k * size, None, rows, cols, 1.0, 0) for k in range(n)])
+        _run_ns(lib().pxl_orthogonalize, x.device, dtype_code(x.dtype), items, n, steps, coef, eps)
+    return out
+
+
+def _run_ns(fn, dev, code, items, n, steps, coef, eps, *scalars):
+    nbytes = lib().pxl_ns_workspace(code, items, n)
+    if nbytes == 0:
+        raise _lib.PixelHipError("libpixelhip: %s" % lib().pxl_last_error().decode())
+    ws = torch.empty(nbytes, device=dev, dtype=torch.uint8)
+    _launch(dev, fn, code, items, n, int(steps), coef, float(eps), *scalars, ptr(ws), nbytes)
+
+
+def _dense_strides(t):
+    """strides of the axes that have any length, when t fills one run of memory with its first axis outermost (contiguous or
+    channels last); None otherwise"""
+    if not (t.is_contiguous() or (t.dim() == 4 and t.is_contiguous(memory_format=torch.channels_last))):
+        return None
+    return tuple(s for s, n in zip(t.stride(), t.shape) if n > 1)
+
+
+def muon_scale(shape, adjust="original"):
+    """factor on the learning rate of a [rows, ...] parameter: 'original': sqrt(max(1, rows / cols)); 'match_rms_adamw': 0.2 sqrt(max(rows,
+    cols)) (an update of the size AdamW's has); 'none': 1.  cols: the product of the other axes."""
+    rows, cols = shape[0], 1
+    for n in shape[1:]:
+        cols *= n
+    if adjust == "original":
+        return max(1.0, rows / cols) ** 0.5
+    if adjust == "match_rms_adamw":
+        return 0.2 * max(rows, cols) ** 0.5
+    if adjust == "none":
+        return 1.0
+    raise ValueError("muon: adjust is 'original', 'match_rms_adamw' or 'none', got %r" % (adjust,))
+
+
+def muon_update(params, grads, momenta, lr, momentum=0.95, nesterov=True, weight_decay=0.0, steps=5, coefficients=NEWTON_SCHULZ, eps=1e-7,
+                adjust="original"):
+    """One Muon step on lists of parameters [rows, ...] (two axes or more; a convolution's [out, in, kh, kw] is the matrix of its
+    rows), in place, all matrices of all shapes together:
+        momentum_k <- momentum * momentum_k + (1 - momentum) * grad_k
+        u = (1 - momentum) * grad_k + momentum * momentum_k  (nesterov)  or  momentum_k
+        param_k <- param_k * (1 - lr * weight_decay) - lr * muon_scale(...) * orthogonalize(u)
+    params / grads fp32 or bf16 (one type per parameter), momenta fp32 with the parameter's memory layout (contiguous or channels
+    last).  Parameters and momenta may overlap nothing."""
+    params, grads, momenta = list(params), list(grads), list(momenta)
+    if not len(params) == len(grads) == len(momenta):
+        raise ValueError("muon_update: %d parameters, %d gradients, %d momenta" % (len(params), len(grads), len(momenta)))
+    lr, momentum, weight_decay = float(lr), float(momentum), float(weight_decay)
+    if not 0 <= momentum < 1 or not eps > 0 or not abs(lr) < float("inf") or not abs(weight_decay) < float("inf"):
+        raise ValueError("muon_update: lr %r, momentum %r (0 <= momentum < 1), weight decay %r, eps %r" % (lr, momentum, weight_decay, eps))
+    coef = _coefficients(steps, coefficients)
+    work, keep, scales = {}, [], {}
+    for k, (p, g, m) in enumerate(zip(params, grads, momenta)):
+        shape = p.shape
+        if p.dim() < 2 or g.shape != shape or m.shape != shape:
+            raise ValueError("muon_update: entry %d: parameter %s, gradient %s, momentum %s" % (k, tuple(shape), tuple(g.shape), tuple(m.shape)))
+        if p.dtype not in (torch.float32, torch.bfloat16) or g.dtype != p.dtype or m.dtype != torch.float32:
+            raise ValueError("muon_update: entry %d: parameter and gradient both float32 or both bfloat16, momentum float32; got %s, %s, %s" %
+                             (k, p.dtype, g.dtype, m.dtype))
+        strides = _dense_strides(p)
+        if strides is None or _dense_strides(m) != strides:
+            raise ValueError("muon_update: entry %d: a parameter and its momentum are dense and lie alike in memory" % k)
+        if g.device != p.device or m.device != p.device:
+            raise ValueError("muon_update: entry %d lies on %s, %s and %s" % (k, p.device, g.device, m.device))
+        _gpu(p)
+        if p.numel() == 0:
+            continue
+        if _dense_strides(g) != strides:
+            g = torch.empty_like(p, requires_grad=False).copy_(g.detach())
+            keep.append(g)
+        if shape not in scales:
+            scales[shape] = (shape[0], p.numel() // shape[0], muon_scale(shape, adjust), 0)
+        work.setdefault((p.device, p.dtype), []).append((p.data_ptr(), g.data_ptr(), m.data_ptr()) + scales[shape])
+    for (dev, dtype), entries in work.items():
+        _run_ns(lib().pxl_muon_step, dev, dtype_code(dtype), (_lib.NsItem * len(entries))(*entries), len(entries), steps, coef, eps, lr, momentum,
+                int(bool(nesterov)), weight_decay)
+    torch.autograd.graph.increment_version([t for t in params + momenta if t.numel()])
