@@ -918,6 +918,17 @@ int pxl_orthogonalize(int dtype, const pxl_ns_item* items, int n, int steps, con
 int pxl_muon_step(int dtype, const pxl_ns_item* items, int n, int steps, const float* coef, float eps, double lr, double momentum, int nesterov,
                   double weight_decay, void* ws, size_t ws_bytes, void* stream);
 
+/* pxl_adam_step without weight decay on n tensors, 40 to a launch: the vectors that the Muon optimizer leaves to Adam.  items: HOST array,
+ * copied at the call; p / g of type dtype, moments fp32; the tensors may not overlap. */
+typedef struct pxl_adam_item {
+  void* p;
+  const void* g;
+  float* exp_avg;
+  float* exp_avg_sq;
+  int64_t n;
+} pxl_adam_item;
+int pxl_adam_list(int dtype, const pxl_adam_item* items, int n, double lr, double beta1, double beta2, double eps, int step, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

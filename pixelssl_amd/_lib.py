@@ -54,6 +54,10 @@ class NsItem(C.Structure):
                 ("scale", C.c_float), ("reserved", C.c_int32)]
 
 
+class AdamItem(C.Structure):
+    _fields_ = [("p", C.c_void_p), ("g", C.c_void_p), ("exp_avg", C.c_void_p), ("exp_avg_sq", C.c_void_p), ("n", C.c_int64)]
+
+
 class BnDesc(C.Structure):
     _fields_ = [("C", C.c_int32), ("gamma_off", C.c_int32), ("beta_off", C.c_int32),
                 ("rmean_off", C.c_int32), ("rvar_off", C.c_int32), ("eps", C.c_float),
@@ -288,6 +292,7 @@ SIGNATURES = {
     "pxl_ns_workspace": (_Z, [_I, _P, _I]),
     "pxl_orthogonalize": (_I, [_I, _P, _I, _I, _P, _F, _P, _Z, _P]),
     "pxl_muon_step": (_I, [_I, _P, _I, _I, _P, _F, C.c_double, C.c_double, _I, C.c_double, _P, _Z, _P]),
+    "pxl_adam_list": (_I, [_I, _P, _I, C.c_double, C.c_double, C.c_double, C.c_double, _I, _P]),
     "pxl_net_backward": (_I, [_P, _P, _P, _P, _P, _P, _P, _P, _Z, _P, _Z, _I, _P]),
 }
 

@@ -142,6 +142,25 @@ __global__ __launch_bounds__(256) void adam_kernel(long n, float* __restrict__ p
   }
 }
 
+// the same update on a list of tensors: one grid row per tensor, the list in the kernel arguments.  A few hundred short vectors (the
+// BatchNorm / LayerNorm parameters and biases that Muon leaves to Adam) are bound by launches, not by bytes
+struct AdamList { pxl_adam_item it[40]; };
+template <typename T>
+__global__ __launch_bounds__(256) void adam_list_kernel(AdamList list, float step_size, float beta1, float beta2, float nu1, float nu2, float eps,
+                                                        float inv_sqrt_bc2) {
+  const pxl_adam_item& e = list.it[blockIdx.y];
+  T* p = reinterpret_cast<T*>(e.p);
+  const T* g = reinterpret_cast<const T*>(e.g);
+  for (long i = blockIdx.x * 256L + threadIdx.x; i < e.n; i += gridDim.x * 256L) {
+    const float gi = to_f(g[i]);
+    const float mi = beta1 * e.exp_avg[i] + nu1 * gi;
+    const float vi = beta2 * e.exp_avg_sq[i] + nu2 * gi * gi;
+    e.exp_avg[i] = mi;
+    e.exp_avg_sq[i] = vi;
+    p[i] = from_f<T>(to_f(p[i]) - step_size * mi / (sqrtf(vi) * inv_sqrt_bc2 + eps));
+  }
+}
+
 __global__ __launch_bounds__(256) void scale_kernel(long n, float* __restrict__ x, float a) {
   for (long i = blockIdx.x * (long)blockDim.x + threadIdx.x; i < n; i += (long)gridDim.x * blockDim.x) x[i] *= a;
 }
@@ -264,6 +283,33 @@ extern "C" int pxl_adam_step_wd(long n, float* p, const float* g, float* exp_avg
   hipLaunchKernelGGL(adam_kernel, dim3(grid_for(n)), dim3(256), 0, reinterpret_cast<hipStream_t>(stream), n, p, g,
                      exp_avg, exp_avg_sq, (float)(lr / bc1), beta1, beta2, eps, (float)(1.0 / sqrt(bc2)), weight_decay);
   PXL_LAUNCH_CHECK();
+  return PXL_OK;
+}
+
+extern "C" int pxl_adam_list(int dtype, const pxl_adam_item* items, int n, double lr, double beta1, double beta2, double eps, int step, void* stream) {
+  PXL_REQUIRE(dtype == PXL_F32 || dtype == PXL_BF16, "adam_list: dtype %d is neither PXL_F32 nor PXL_BF16", dtype);
+  PXL_REQUIRE(n >= 0 && (n == 0 || items != nullptr) && step >= 1 && beta1 >= 0 && beta1 < 1 && beta2 >= 0 && beta2 < 1 && eps > 0,
+              "adam_list: bad argument (step counts from 1)");
+  for (int k = 0; k < n; ++k)
+    PXL_REQUIRE(items[k].p && items[k].g && items[k].exp_avg && items[k].exp_avg_sq && items[k].n >= 1, "adam_list: item %d: null pointer or no elements", k);
+  const double bc1 = 1.0 - pow(beta1, step), bc2 = 1.0 - pow(beta2, step);
+  for (int at = 0; at < n; at += 40) {
+    AdamList list;
+    const int cnt = n - at < 40 ? n - at : 40;
+    long most = 0;
+    for (int k = 0; k < cnt; ++k) { list.it[k] = items[at + k]; most = most > items[at + k].n ? most : items[at + k].n; }
+    for (int k = cnt; k < 40; ++k) list.it[k] = list.it[0];
+    const long blocks = (most + 1023) / 1024;
+    const dim3 grid((unsigned)(blocks < 1024 ? blocks : 1024), (unsigned)cnt);
+    hipStream_t st = reinterpret_cast<hipStream_t>(stream);
+    if (dtype == PXL_F32)
+      hipLaunchKernelGGL(adam_list_kernel<float>, grid, dim3(256), 0, st, list, (float)(lr / bc1), (float)beta1, (float)beta2, (float)(1.0 - beta1),
+                         (float)(1.0 - beta2), (float)eps, (float)(1.0 / sqrt(bc2)));
+    else
+      hipLaunchKernelGGL(adam_list_kernel<bf16_t>, grid, dim3(256), 0, st, list, (float)(lr / bc1), (float)beta1, (float)beta2, (float)(1.0 - beta1),
+                         (float)(1.0 - beta2), (float)eps, (float)(1.0 / sqrt(bc2)));
+    PXL_LAUNCH_CHECK();
+  }
   return PXL_OK;
 }
 

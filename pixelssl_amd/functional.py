@@ -489,7 +489,7 @@ def muon_update(params, grads, momenta, lr, momentum=0.95, nesterov=True, weight
         momentum_k <- momentum * momentum_k + (1 - momentum) * grad_k
         u = (1 - momentum) * grad_k + momentum * momentum_k  (nesterov)  or  momentum_k
         param_k <- param_k * (1 - lr * weight_decay) - lr * muon_scale(...) * orthogonalize(u)
-    params / grads fp32 or bf16 (one type per parameter), momenta fp32 with the parameter's memory layout (contiguous or channels
+    adjust: the rule of muon_scale, or one factor per parameter in its place.  params / grads fp32 or bf16 (one type per parameter), momenta fp32 with the parameter's memory layout (contiguous or channels
     last).  Parameters and momenta may overlap nothing."""
     params, grads, momenta = list(params), list(grads), list(momenta)
     if not len(params) == len(grads) == len(momenta):
@@ -498,6 +498,9 @@ def muon_update(params, grads, momenta, lr, momentum=0.95, nesterov=True, weight
     if not 0 <= momentum < 1 or not eps > 0 or not abs(lr) < float("inf") or not abs(weight_decay) < float("inf"):
         raise ValueError("muon_update: lr %r, momentum %r (0 <= momentum < 1), weight decay %r, eps %r" % (lr, momentum, weight_decay, eps))
     coef = _coefficients(steps, coefficients)
+    named = isinstance(adjust, str)
+    if not named and (len(adjust) != len(params) or not all(abs(float(a)) < float("inf") for a in adjust)):
+        raise ValueError("muon_update: adjust is a name or one finite factor per parameter, got %r" % (adjust,))
     work, keep, scales = {}, [], {}
     for k, (p, g, m) in enumerate(zip(params, grads, momenta)):
         shape = p.shape
@@ -518,9 +521,42 @@ def muon_update(params, grads, momenta, lr, momentum=0.95, nesterov=True, weight
             g = torch.empty_like(p, requires_grad=False).copy_(g.detach())
             keep.append(g)
         if shape not in scales:
-            scales[shape] = (shape[0], p.numel() // shape[0], muon_scale(shape, adjust), 0)
-        work.setdefault((p.device, p.dtype), []).append((p.data_ptr(), g.data_ptr(), m.data_ptr()) + scales[shape])
+            scales[shape] = (shape[0], p.numel() // shape[0], muon_scale(shape, adjust) if named else 0.0, 0)
+        geo = scales[shape] if named else scales[shape][:2] + (float(adjust[k]), 0)
+        work.setdefault((p.device, p.dtype), []).append((p.data_ptr(), g.data_ptr(), m.data_ptr()) + geo)
     for (dev, dtype), entries in work.items():
         _run_ns(lib().pxl_muon_step, dev, dtype_code(dtype), (_lib.NsItem * len(entries))(*entries), len(entries), steps, coef, eps, lr, momentum,
                 int(bool(nesterov)), weight_decay)
     torch.autograd.graph.increment_version([t for t in params + momenta if t.numel()])
+
+
+def adam_update(params, grads, exp_avgs, exp_avg_sqs, lr, betas=(0.9, 0.999), eps=1e-8, step=1):
+    """torch.optim.Adam's update without weight decay (FusedAdam's arithmetic) on lists of tensors, in place, many in one launch: the
+    vectors beside muon_update's matrices.  params / grads fp32 or bf16, exp_avgs / exp_avg_sqs fp32, all four of an entry dense and
+    alike in memory (a gradient may lie otherwise).  step counts from 1."""
+    b1, b2 = float(betas[0]), float(betas[1])
+    if not (0 <= b1 < 1 and 0 <= b2 < 1 and eps > 0 and int(step) >= 1):
+        raise ValueError("adam_update: betas %r, eps %r, step %r" % (betas, eps, step))
+    work, keep, touched = {}, [], []
+    for k, (p, g, m, v) in enumerate(zip(params, grads, exp_avgs, exp_avg_sqs)):
+        if not g.shape == m.shape == v.shape == p.shape:
+            raise ValueError("adam_update: entry %d: shapes %s, %s, %s, %s" % (k, tuple(p.shape), tuple(g.shape), tuple(m.shape), tuple(v.shape)))
+        if p.dtype not in (torch.float32, torch.bfloat16) or g.dtype != p.dtype or m.dtype != torch.float32 or v.dtype != torch.float32:
+            raise ValueError("adam_update: entry %d: parameter and gradient both float32 or both bfloat16, the moments float32" % k)
+        strides = _dense_strides(p)
+        if strides is None or _dense_strides(m) != strides or _dense_strides(v) != strides:
+            raise ValueError("adam_update: entry %d: a parameter and its moments are dense and lie alike in memory" % k)
+        if not g.device == m.device == v.device == p.device:
+            raise ValueError("adam_update: entry %d lies on several devices" % k)
+        _gpu(p)
+        if p.numel() == 0:
+            continue
+        if _dense_strides(g) != strides:
+            g = torch.empty_like(p, requires_grad=False).copy_(g.detach())
+            keep.append(g)
+        work.setdefault((p.device, p.dtype), []).append((p.data_ptr(), g.data_ptr(), m.data_ptr(), v.data_ptr(), p.numel()))
+        touched += [p, m, v]
+    for (dev, dtype), entries in work.items():
+        _launch(dev, lib().pxl_adam_list, dtype_code(dtype), (_lib.AdamItem * len(entries))(*entries), len(entries), float(lr), b1, b2, float(eps),
+                int(step))
+    torch.autograd.graph.increment_version(touched)

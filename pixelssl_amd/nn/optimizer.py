@@ -8,7 +8,7 @@ from ..utils import cmd
 from .. import _lib
 from .. import ops
 
-VALID_OPTIMIZER = ['sgd', 'adam']
+VALID_OPTIMIZER = ['sgd', 'adam']          # the reference's names; `muon` below is this framework's own
 
 
 def add_parser_arguments(parser):
@@ -96,6 +96,9 @@ class _FlatStateMixin:
 
     _STATE_KEYS = ()          # (state_dict key, store attribute)
 
+    def _keys_of(self, p):
+        return self._STATE_KEYS
+
     def _param_list(self):
         return [p for g in self.param_groups for p in g['params']]
 
@@ -110,7 +113,7 @@ class _FlatStateMixin:
                     continue
                 store = p._pxl_flat[0]
                 entry = {k: _flat_view(store, getattr(store, attr), p).detach().clone().contiguous()
-                         for k, attr in self._STATE_KEYS}
+                         for k, attr in self._keys_of(p)}
                 entry.update(self._extra_state())
                 state[idx] = entry
         sd['state'] = state
@@ -141,7 +144,7 @@ class _FlatStateMixin:
                     steps = max(steps, self._steps_of(entry))
                     continue
                 store = p._pxl_flat[0]
-                for k, attr in self._STATE_KEYS:
+                for k, attr in self._keys_of(p):
                     if entry.get(k) is not None:
                         _flat_view(store, getattr(store, attr), p).copy_(entry[k].to(store.params.device))
                 steps = max(steps, self._steps_of(entry))
@@ -509,6 +512,133 @@ class FusedAdam(_FlatStateMixin, Optimizer):
                     p.grad = None if set_to_none else p.grad.detach().zero_()
 
 
+class FusedMuon(_FlatStateMixin, Optimizer):
+    """Muon: every matrix parameter (two axes or more; a convolution's weight is the matrix of its output channels) steps along its
+    orthogonalised momentum, all matrices of all groups with equal settings in one call (functional.muon_update has the formulas);
+    every vector, and every parameter of a group with muon=False, takes an Adam step of learning rate lr * vector_scale without
+    weight decay, all of a group in one launch per 40.  The arithmetic is the same for engine parameters (flat fp32 store) and for any
+    other GPU tensor (fp32 or bf16, dense).  One process per GPU: gradients are the mean over ranks before the step and the step has
+    one summation order, so replicas stay equal.
+
+    momentum / nesterov / weight_decay / ns_steps / ns_coefficients / ns_eps / adjust_lr: of the matrices; betas / eps: of the vectors."""
+
+    _ALL_KEYS = (('momentum_buffer', 'momentum'), ('exp_avg', 'exp_avg'), ('exp_avg_sq', 'exp_avg_sq'))
+    _STATE_KEYS = _ALL_KEYS
+
+    def __init__(self, params, lr=0.02, momentum=0.95, nesterov=True, weight_decay=0.0, ns_steps=5, ns_coefficients=None, ns_eps=1e-7,
+                 adjust_lr='original', betas=(0.9, 0.999), eps=1e-8, vector_scale=0.015, muon=True):
+        from .. import functional as PF
+        coefs = PF.NEWTON_SCHULZ if ns_coefficients is None else ns_coefficients
+        super().__init__(params, dict(lr=lr, momentum=momentum, nesterov=nesterov, weight_decay=weight_decay, ns_steps=ns_steps,
+                                      ns_coefficients=coefs, ns_eps=ns_eps, adjust_lr=adjust_lr, betas=tuple(betas), eps=eps,
+                                      vector_scale=vector_scale, muon=muon))
+        self._foreign = []
+        self._stores = {}
+        for group in self.param_groups:
+            if not 0 <= group['momentum'] < 1:
+                raise ValueError('FusedMuon: momentum %r' % (group['momentum'],))
+            b1, b2 = group['betas']
+            if not (0 <= b1 < 1 and 0 <= b2 < 1) or not group['eps'] > 0 or not group['ns_eps'] > 0:
+                raise ValueError('FusedMuon: betas %r, eps %r, ns_eps %r' % (group['betas'], group['eps'], group['ns_eps']))
+            PF.muon_scale((1, 1), group['adjust_lr'])
+            PF._coefficients(group['ns_steps'], group['ns_coefficients'])
+            self._foreign.append(_foreign(group['params']))
+            for p in self._foreign[-1]:
+                if p.dtype not in (torch.float32, torch.bfloat16) or PF._dense_strides(p) is None:
+                    raise ValueError('FusedMuon: parameters are dense float32 or bfloat16 tensors, got %s of strides %s' % (p.dtype, p.stride()))
+            for p in group['params']:
+                if getattr(p, '_pxl_flat', None) is not None:
+                    self._stores[id(p._pxl_flat[0])] = p._pxl_flat[0]
+        for store in self._stores.values():
+            for _, attr in self._ALL_KEYS:
+                if not hasattr(store, attr):
+                    setattr(store, attr, torch.zeros_like(store.params))
+        self._matrix = {id(p): bool(group['muon']) and p.dim() >= 2 for group in self.param_groups for p in group['params']}
+        self._step = 0
+        self._steps_taken = 0
+
+    def _keys_of(self, p):
+        return self._ALL_KEYS[:1] if self._matrix[id(p)] else self._ALL_KEYS[1:]
+
+    def _extra_state(self):
+        return {'step': torch.tensor(float(self._step))}
+
+    def _steps_of(self, entry):
+        st = entry.get('step', 0)
+        return int(st.item() if torch.is_tensor(st) else st)
+
+    def _after_load(self, steps):
+        self._step = steps
+        for foreign in self._foreign:
+            for p in foreign:                   # moments in fp32 that lie like their parameter, whatever the checkpoint's do
+                st = self.state.get(p)
+                for k, _ in self._keys_of(p) if st else ():
+                    if st.get(k) is not None:
+                        st[k] = torch.empty_like(p, dtype=torch.float32, requires_grad=False).copy_(st[k])
+
+    @staticmethod
+    def _slot(flat, p):
+        """the slot of `p` in a flat buffer of its store as [rows, columns] / [n], padding included (zero, and staying zero)"""
+        _, off, n = p._pxl_flat
+        rows = (getattr(p, '_pxl_alloc', None) or tuple(p.shape))[0]
+        return flat[off:off + n].view(rows, n // rows) if p.dim() >= 2 else flat[off:off + n]
+
+    @torch.no_grad()
+    def step(self, closure=None):
+        from .. import functional as PF
+        from .. import graph as pgraph
+        if pgraph.current_hyper() is not None or (torch.cuda.is_available() and torch.cuda.is_current_stream_capturing()):
+            raise _lib.PixelHipError('FusedMuon: a captured training step is not supported (learning rates are kernel arguments)')
+        loss = None
+        if closure is not None:
+            with torch.enable_grad():
+                loss = closure()
+        _sync_foreign_grads(self._foreign)
+        self._step += 1
+        self._steps_taken = self._step
+        calls = {}                      # settings -> the matrices that share them
+        for group in self.param_groups:
+            b1, b2 = group['betas']
+            vectors = []
+            for p in group['params']:
+                ref = getattr(p, '_pxl_flat', None)
+                matrix = self._matrix[id(p)]
+                if ref is None:
+                    if p.grad is None:
+                        continue
+                    st = self.state[p]
+                    for k, _ in self._keys_of(p):
+                        if st.get(k) is None:
+                            st[k] = torch.zeros_like(p, dtype=torch.float32)
+                    st['step'] = torch.tensor(float(self._step))
+                    entry = (p, p.grad) + tuple(st[k] for k, _ in self._keys_of(p))
+                else:
+                    entry = tuple(self._slot(getattr(ref[0], k), p) for k in ('params', 'grads') + tuple(a for _, a in self._keys_of(p)))
+                if matrix:
+                    scale = PF.muon_scale(p.shape, group['adjust_lr'])
+                    key = tuple(group[k] for k in ('lr', 'momentum', 'nesterov', 'weight_decay', 'ns_steps', 'ns_coefficients', 'ns_eps'))
+                    calls.setdefault(key, []).append(entry + (scale,))
+                else:
+                    vectors.append(entry)
+            if vectors:
+                PF.adam_update(*zip(*vectors), lr=float(group['lr']) * float(group['vector_scale']), betas=(b1, b2), eps=group['eps'], step=self._step)
+        for (lr, momentum, nesterov, wd, steps, coefs, eps), entries in calls.items():
+            p, g, m, scales = zip(*entries)
+            PF.muon_update(p, g, m, lr=lr, momentum=momentum, nesterov=nesterov, weight_decay=wd, steps=steps, coefficients=coefs, eps=eps,
+                           adjust=scales)
+        for store in self._stores.values():
+            store.touch()
+        return loss
+
+    def zero_grad(self, set_to_none=False):
+        for store in self._stores.values():
+            store.grads.zero_()
+        for foreign in self._foreign:
+            for p in foreign:
+                if p.grad is not None:
+                    p.grad = None if set_to_none else p.grad.detach().zero_()
+
+
 def sgd(args):
     args.lr = 0.01 if args.lr == -1 else args.lr
     args.weight_decay = 0 if args.weight_decay == -1 else args.weight_decay
@@ -535,3 +665,21 @@ def adam(args):
                          weight_decay=args.weight_decay)
 
     return adam_wrapper
+
+
+def muon(args):
+    """`muon(args)`: an optimizer of this framework (not one of VALID_OPTIMIZER, which are the reference's), chosen like them
+    -- `nn.optimizer.muon(args)(param_groups)`.  The shared flags: --lr (default 0.02), --momentum (0.95), --nesterov, --weight-decay (0),
+    and --beta1 / --beta2 / --eps (0.9, 0.999, 1e-8) of the vectors' Adam step."""
+    args.lr = 0.02 if args.lr == -1 else args.lr
+    args.momentum = 0.95 if args.momentum == -1 else args.momentum
+    args.weight_decay = 0.0 if args.weight_decay == -1 else args.weight_decay
+    args.beta1 = 0.9 if args.beta1 == -1 else args.beta1
+    args.beta2 = 0.999 if args.beta2 == -1 else args.beta2
+    args.eps = 1e-08 if args.eps == -1 else args.eps
+
+    def muon_wrapper(param_groups):
+        return FusedMuon(param_groups, lr=args.lr, momentum=args.momentum, nesterov=args.nesterov, weight_decay=args.weight_decay,
+                         betas=(args.beta1, args.beta2), eps=args.eps)
+
+    return muon_wrapper
