@@ -149,15 +149,382 @@ __global__ __launch_bounds__(256) void ln_chan_dwb_loop(long P, int C, long S, c
   }
 }
 
-// part[G][2][C] -> dw[C], db[C] (either may be absent), groups in ascending order
+// ---- 16-byte pieces at any element alignment --------------------------------------------------------------------------------
+template <typename T> struct Piece {
+  static constexpr int N = 16 / (int)sizeof(T);
+  // `valid` elements from p on (all N: one unaligned 16-byte access), the others 0
+  static __device__ __forceinline__ uint4 load(const T* p, int valid) {
+    uint4 v = make_uint4(0u, 0u, 0u, 0u);
+    if (valid >= N) {
+      __builtin_memcpy(&v, p, 16);
+    } else if (valid > 0) {
+      T t[N];
+#pragma unroll
+      for (int e = 0; e < N; ++e) t[e] = e < valid ? p[e] : T(0);
+      __builtin_memcpy(&v, t, 16);
+    }
+    return v;
+  }
+  static __device__ __forceinline__ void store(T* p, const float* f, int valid) {
+    const uint4 v = Chunk<T>::pack(f);
+    if (valid >= N) {
+      __builtin_memcpy(p, &v, 16);
+    } else if (valid > 0) {
+#pragma unroll
+      for (int e = 0; e < N; ++e)
+        if (e < valid) p[e] = from_f<T>(f[e]);
+    }
+  }
+};
+
+template <int LPR> __device__ __forceinline__ float row_sum(float v, float* sh) {
+  if constexpr (LPR == 256) return block_sum<256>(v, sh);
+#pragma unroll
+  for (int o = LPR / 2; o > 0; o >>= 1) v += __shfl_xor(v, o, 64);
+  return v;
+}
+
+// ---- rows that fit into registers: LPR lanes hold a row in NV pieces each, one sweep over memory; weight and bias stay in registers
+// over the rows of a workgroup --------------------------------------------------------------------------------------------------
+template <typename T, int LPR, int NV>
+__global__ __launch_bounds__(256) void ln_rows_fwd(long R, int C, long xs, const T* __restrict__ x, LnParam w, LnParam b, float eps,
+                                                   T* __restrict__ y, float* __restrict__ mean, float* __restrict__ rstd) {
+  constexpr int V = Piece<T>::N, RPB = 256 / LPR;
+  __shared__ float sh[4];
+  const int lane = threadIdx.x % LPR;
+  float wv[NV][V], bv[NV][V];
+#pragma unroll
+  for (int j = 0; j < NV; ++j)
+#pragma unroll
+    for (int e = 0; e < V; ++e) {
+      const int c = (j * LPR + lane) * V + e;
+      wv[j][e] = c < C ? w.get<T>(c, 1.f) : 0.f;
+      bv[j][e] = c < C ? b.get<T>(c, 0.f) : 0.f;
+    }
+  const float inv = 1.f / C;
+  for (long r0 = (long)blockIdx.x * RPB; r0 < R; r0 += (long)gridDim.x * RPB) {
+    const long r = r0 + threadIdx.x / LPR;
+    const bool live = RPB == 1 || r < R;
+    float f[NV][V];
+    float s = 0.f;
+#pragma unroll
+    for (int j = 0; j < NV; ++j) {
+      const int c = (j * LPR + lane) * V;
+      Chunk<T>::unpack(Piece<T>::load(x + r * xs + c, live ? C - c : 0), f[j]);
+#pragma unroll
+      for (int e = 0; e < V; ++e) s += f[j][e];
+    }
+    const float m = row_sum<LPR>(s, sh) / C;           // (divided: a row of equal values has its mean exactly)
+    float q = 0.f;
+#pragma unroll
+    for (int j = 0; j < NV; ++j) {
+      const int left = C - (j * LPR + lane) * V;
+#pragma unroll
+      for (int e = 0; e < V; ++e) {
+        f[j][e] -= m;
+        if (e < left) q += f[j][e] * f[j][e];
+      }
+    }
+    const float rs = 1.f / sqrtf(row_sum<LPR>(q, sh) * inv + eps);
+#pragma unroll
+    for (int j = 0; j < NV; ++j) {
+      const int c = (j * LPR + lane) * V;
+#pragma unroll
+      for (int e = 0; e < V; ++e) f[j][e] = f[j][e] * rs * wv[j][e] + bv[j][e];
+      Piece<T>::store(y + r * C + c, f[j], live ? C - c : 0);
+    }
+    if (mean != nullptr && lane == 0 && live) { mean[r] = m; rstd[r] = rs; }
+  }
+}
+
+// dx and, kept in registers over the rows of a workgroup, its share of dw / db -> part[workgroup][2][C]
+template <typename T, int LPR, int NV>
+__global__ __launch_bounds__(256) void ln_rows_bwd(long R, int C, long xs, const T* __restrict__ x, const T* __restrict__ dy, LnParam w,
+                                                   const float* __restrict__ mean, const float* __restrict__ rstd, T* __restrict__ dx,
+                                                   float* __restrict__ part) {
+  constexpr int V = Piece<T>::N, RPB = 256 / LPR;
+  __shared__ float sh[4];
+  const int lane = threadIdx.x % LPR, sub = threadIdx.x / LPR;
+  float wv[NV][V], aw[NV][V], ab[NV][V];
+#pragma unroll
+  for (int j = 0; j < NV; ++j)
+#pragma unroll
+    for (int e = 0; e < V; ++e) {
+      const int c = (j * LPR + lane) * V + e;
+      wv[j][e] = c < C ? w.get<T>(c, 1.f) : 0.f;
+      aw[j][e] = ab[j][e] = 0.f;
+    }
+  const float inv = 1.f / C;
+  for (long r0 = (long)blockIdx.x * RPB; r0 < R; r0 += (long)gridDim.x * RPB) {
+    const long r = r0 + sub;
+    const bool live = RPB == 1 || r < R;
+    const float m = live ? mean[r] : 0.f, rs = live ? rstd[r] : 0.f;
+    float u[NV][V], g[NV][V];
+    float s1 = 0.f, s2 = 0.f;
+#pragma unroll
+    for (int j = 0; j < NV; ++j) {
+      const int c = (j * LPR + lane) * V;
+      Chunk<T>::unpack(Piece<T>::load(x + r * xs + c, live ? C - c : 0), u[j]);
+      Chunk<T>::unpack(Piece<T>::load(dy + r * C + c, live ? C - c : 0), g[j]);
+    }
+#pragma unroll
+    for (int j = 0; j < NV; ++j)
+#pragma unroll
+      for (int e = 0; e < V; ++e) {
+        u[j][e] = (u[j][e] - m) * rs;
+        const float d = g[j][e];            // 0 behind the row's end
+        if (part != nullptr) {
+          aw[j][e] += d * u[j][e];
+          ab[j][e] += d;
+        }
+        g[j][e] = d * wv[j][e];
+        s1 += g[j][e];
+        s2 += g[j][e] * u[j][e];
+      }
+    if (dx == nullptr) continue;
+    const float a1 = row_sum<LPR>(s1, sh) * inv, a2 = row_sum<LPR>(s2, sh) * inv;
+#pragma unroll
+    for (int j = 0; j < NV; ++j) {
+      const int c = (j * LPR + lane) * V;
+#pragma unroll
+      for (int e = 0; e < V; ++e) g[j][e] = rs * (g[j][e] - a1 - u[j][e] * a2);
+      Piece<T>::store(dx + r * C + c, g[j], live ? C - c : 0);
+    }
+  }
+  if (part == nullptr) return;
+  float* p = part + (long)blockIdx.x * 2 * C;
+  if constexpr (RPB == 1) {
+#pragma unroll
+    for (int j = 0; j < NV; ++j) {
+      const int c = (j * LPR + lane) * V;
+      Piece<float>::store(p + c, aw[j], C - c);
+      Piece<float>::store(p + C + c, ab[j], C - c);
+      if constexpr (V == 8) {
+        Piece<float>::store(p + c + 4, aw[j] + 4, C - c - 4);
+        Piece<float>::store(p + C + c + 4, ab[j] + 4, C - c - 4);
+      }
+    }
+  } else {
+    // the row lanes of the workgroup one after the other into one copy
+    __shared__ float acc[2][LPR * NV * V];
+    for (int k = 0; k < RPB; ++k) {
+      if (sub == k) {
+#pragma unroll
+        for (int j = 0; j < NV; ++j)
+#pragma unroll
+          for (int e = 0; e < V; ++e) {
+            const int at = (j * V + e) * LPR + lane;
+            acc[0][at] = k == 0 ? aw[j][e] : acc[0][at] + aw[j][e];
+            acc[1][at] = k == 0 ? ab[j][e] : acc[1][at] + ab[j][e];
+          }
+      }
+      __syncthreads();
+    }
+    for (int c = threadIdx.x; c < C; c += 256) {
+      const int piece = c / V, e = c - piece * V, j = piece / LPR, l = piece - j * LPR;
+      p[c] = acc[0][(j * V + e) * LPR + l];
+      p[C + c] = acc[1][(j * V + e) * LPR + l];
+    }
+  }
+}
+
+// ---- channels that fit into registers: a workgroup takes all C channels of TSV pieces of consecutive positions; a thread holds NV
+// channels (CY apart) of one piece ------------------------------------------------------------------------------------------------
+// sums over the channels, per position of the piece: over the lanes of the wave, then over the waves through LDS
+template <int THREADS, int TSV, int V, int NS>
+__device__ __forceinline__ void chan_sum(float (&s)[NS][V], float* sh) {
+  constexpr int NW = THREADS / 64;
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, sv = threadIdx.x % TSV;
+#pragma unroll
+  for (int o = TSV; o < 64; o <<= 1)
+#pragma unroll
+    for (int k = 0; k < NS; ++k)
+#pragma unroll
+      for (int e = 0; e < V; ++e) s[k][e] += __shfl_xor(s[k][e], o, 64);
+  constexpr int W = NS * TSV * V;                     // values per wave
+  if (lane < TSV) {
+#pragma unroll
+    for (int k = 0; k < NS; ++k)
+#pragma unroll
+      for (int e = 0; e < V; ++e) sh[wave * W + (k * TSV + sv) * V + e] = s[k][e];
+  }
+  __syncthreads();
+  if (threadIdx.x < W) {
+    float t = sh[threadIdx.x];
+#pragma unroll
+    for (int q = 1; q < NW; ++q) t += sh[q * W + threadIdx.x];
+    sh[NW * W + threadIdx.x] = t;
+  }
+  __syncthreads();
+#pragma unroll
+  for (int k = 0; k < NS; ++k)
+#pragma unroll
+    for (int e = 0; e < V; ++e) s[k][e] = sh[NW * W + (k * TSV + sv) * V + e];
+}
+
+template <typename T, int THREADS, int TSV, int NV>
+__global__ __launch_bounds__(THREADS) void ln_chan_fwd(int tiles, int per, int C, long S, const T* __restrict__ x, LnParam w, LnParam b, float eps,
+                                                       T* __restrict__ y, float* __restrict__ mean, float* __restrict__ rstd) {
+  constexpr int V = Piece<T>::N, CY = THREADS / TSV, TS = TSV * V;
+  __shared__ float sh[(THREADS / 64 + 1) * TS];
+  const int sv = threadIdx.x % TSV, cy = threadIdx.x / TSV;
+  const float inv = 1.f / C;
+  const int t = xcd_remap(blockIdx.x, tiles);
+  const long n = t / per;
+  const long s0 = (long)(t - n * per) * TS + sv * V;
+  const int left = S - s0 >= V ? V : (S - s0 > 0 ? (int)(S - s0) : 0);
+  const long base = n * C * S + s0;
+  uint4 raw[NV];
+#pragma unroll
+  for (int j = 0; j < NV; ++j) {
+    const int c = j * CY + cy;
+    raw[j] = Piece<T>::load(x + base + c * S, c < C ? left : 0);
+  }
+  float s[1][V];
+#pragma unroll
+  for (int e = 0; e < V; ++e) s[0][e] = 0.f;
+#pragma unroll
+  for (int j = 0; j < NV; ++j) {
+    float f[V];
+    Chunk<T>::unpack(raw[j], f);
+#pragma unroll
+    for (int e = 0; e < V; ++e) s[0][e] += f[e];
+  }
+  chan_sum<THREADS, TSV, V, 1>(s, sh);
+  float m[V];
+#pragma unroll
+  for (int e = 0; e < V; ++e) { m[e] = s[0][e] / C; s[0][e] = 0.f; }           // (divided: equal values have their mean exactly)
+#pragma unroll
+  for (int j = 0; j < NV; ++j) {
+    float f[V];
+    Chunk<T>::unpack(raw[j], f);
+    if (j * CY + cy < C) {
+#pragma unroll
+      for (int e = 0; e < V; ++e) s[0][e] += (f[e] - m[e]) * (f[e] - m[e]);
+    }
+  }
+  __syncthreads();                    // the last readers of sh are done
+  chan_sum<THREADS, TSV, V, 1>(s, sh);
+  float rs[V];
+#pragma unroll
+  for (int e = 0; e < V; ++e) rs[e] = 1.f / sqrtf(s[0][e] * inv + eps);
+#pragma unroll
+  for (int j = 0; j < NV; ++j) {
+    const int c = j * CY + cy;
+    if (c >= C) continue;
+    const float wc = w.get<T>(c, 1.f), bc = b.get<T>(c, 0.f);
+    float f[V];
+    Chunk<T>::unpack(raw[j], f);
+#pragma unroll
+    for (int e = 0; e < V; ++e) f[e] = (f[e] - m[e]) * rs[e] * wc + bc;
+    Piece<T>::store(y + base + c * S, f, left);
+  }
+  if (mean != nullptr && cy == 0) {
+#pragma unroll
+    for (int e = 0; e < V; ++e)
+      if (e < left) { mean[n * S + s0 + e] = m[e]; rstd[n * S + s0 + e] = rs[e]; }
+  }
+}
+
+template <typename T, int THREADS, int TSV, int NV>
+__global__ __launch_bounds__(THREADS) void ln_chan_bwd(int tiles, int per, int C, long S, const T* __restrict__ x, const T* __restrict__ dy, LnParam w,
+                                                       const float* __restrict__ mean, const float* __restrict__ rstd, T* __restrict__ dx,
+                                                       float* __restrict__ part) {
+  constexpr int V = Piece<T>::N, CY = THREADS / TSV, TS = TSV * V;
+  __shared__ float sh[(THREADS / 64 + 1) * 2 * TS];
+  const int sv = threadIdx.x % TSV, cy = threadIdx.x / TSV;
+  const float inv = 1.f / C;
+  float aw[NV], ab[NV], wv[NV];
+#pragma unroll
+  for (int j = 0; j < NV; ++j) {
+    const int c = j * CY + cy;
+    aw[j] = ab[j] = 0.f;
+    wv[j] = c < C ? w.get<T>(c, 1.f) : 0.f;
+  }
+  // consecutive tiles (they share cache lines where rows start anywhere) to one workgroup
+  const int G = gridDim.x, g = xcd_remap(blockIdx.x, G);
+  const int t0 = (int)((long)tiles * g / G), t1 = (int)((long)tiles * (g + 1) / G);
+  for (int t = t0; t < t1; ++t) {
+    const long n = t / per;
+    const long s0 = (long)(t - n * per) * TS + sv * V;
+    const int left = S - s0 >= V ? V : (S - s0 > 0 ? (int)(S - s0) : 0);
+    const long base = n * C * S + s0;
+    uint4 rx[NV], rg[NV];
+#pragma unroll
+    for (int j = 0; j < NV; ++j) {
+      const int c = j * CY + cy;
+      rx[j] = Piece<T>::load(x + base + c * S, c < C ? left : 0);
+      rg[j] = Piece<T>::load(dy + base + c * S, c < C ? left : 0);
+    }
+    float m[V], rs[V], s[2][V];
+#pragma unroll
+    for (int e = 0; e < V; ++e) {
+      m[e] = e < left ? mean[n * S + s0 + e] : 0.f;
+      rs[e] = e < left ? rstd[n * S + s0 + e] : 0.f;
+      s[0][e] = s[1][e] = 0.f;
+    }
+#pragma unroll
+    for (int j = 0; j < NV; ++j) {
+      float u[V], d[V];
+      Chunk<T>::unpack(rx[j], u);
+      Chunk<T>::unpack(rg[j], d);
+#pragma unroll
+      for (int e = 0; e < V; ++e) {
+        u[e] = (u[e] - m[e]) * rs[e];
+        aw[j] += d[e] * u[e];
+        ab[j] += d[e];
+        s[0][e] += d[e] * wv[j];
+        s[1][e] += d[e] * wv[j] * u[e];
+      }
+    }
+    if (dx == nullptr) continue;
+    chan_sum<THREADS, TSV, V, 2>(s, sh);
+#pragma unroll
+    for (int j = 0; j < NV; ++j) {
+      const int c = j * CY + cy;
+      if (c >= C) continue;
+      float u[V], d[V];
+      Chunk<T>::unpack(rx[j], u);
+      Chunk<T>::unpack(rg[j], d);
+#pragma unroll
+      for (int e = 0; e < V; ++e) {
+        u[e] = (u[e] - m[e]) * rs[e];
+        d[e] = rs[e] * (d[e] * wv[j] - s[0][e] * inv - u[e] * (s[1][e] * inv));
+      }
+      Piece<T>::store(dx + base + c * S, d, left);
+    }
+    __syncthreads();                  // the last readers of sh are done
+  }
+  if (part == nullptr) return;
+  float* p = part + (long)g * 2 * C;
+#pragma unroll
+  for (int j = 0; j < NV; ++j) {
+    const int c = j * CY + cy;
+#pragma unroll
+    for (int o = 1; o < TSV; o <<= 1) {
+      aw[j] += __shfl_xor(aw[j], o, 64);
+      ab[j] += __shfl_xor(ab[j], o, 64);
+    }
+    if (sv == 0 && c < C) { p[c] = aw[j]; p[C + c] = ab[j]; }
+  }
+}
+
+// part[G][2][C] -> dw[C], db[C] (either may be absent): 16 columns a workgroup, 16 lanes over the groups, in ascending order each
 template <typename T>
 __global__ __launch_bounds__(256) void ln_dwb_fold(int G, int C, const float* __restrict__ part, void* dw, void* db, int f32) {
-  const int k = blockIdx.x * 256 + threadIdx.x;
-  if (k >= 2 * C) return;
+  __shared__ float sh[16][17];
+  const int col = threadIdx.x & 15, gl = threadIdx.x >> 4;
+  const int k = blockIdx.x * 16 + col;
+  float s = 0.f;
+  if (k < 2 * C)
+    for (int g = gl; g < G; g += 16) s += part[(long)g * 2 * C + k];
+  sh[gl][col] = s;
+  __syncthreads();
+  if (gl != 0 || k >= 2 * C) return;
+#pragma unroll
+  for (int q = 1; q < 16; ++q) s += sh[q][col];
   void* out = k < C ? dw : db;
   if (out == nullptr) return;
-  float s = 0.f;
-  for (int g = 0; g < G; ++g) s += part[(long)g * 2 * C + k];
   const int c = k < C ? k : k - C;
   if (f32) reinterpret_cast<float*>(out)[c] = s;
   else reinterpret_cast<T*>(out)[c] = from_f<T>(s);
@@ -165,20 +532,98 @@ __global__ __launch_bounds__(256) void ln_dwb_fold(int G, int C, const float* __
 
 inline unsigned blocks_for(long n, long most) { return (unsigned)(n < 1 ? 1 : (n < most ? n : most)); }
 
-// groups of the dw / db partial sums
-inline int ln_groups(long rows, int C) {
-  (void)C;
-  const long g = (rows + 63) / 64;
-  return (int)(g < 1 ? 1 : (g > 256 ? 256 : g));
+// How a call is run.  Rows: 8 .. 64 lanes (a wave or a part of it) hold a row in at most 4 pieces each, else a workgroup holds it in at
+// most 4 (fp32: 8); channels: at most 16 pieces a thread; beyond: the three-sweep kernels, which take any length.
+struct LnShape { int lanes, nv, threads, tsv; int groups; long tiles; };
+LnShape ln_rows_shape(int dtype, long R, int C) {
+  LnShape s = {0, 0, 256, 0, 1, 0};
+  const int v = dtype == PXL_F32 ? 4 : 8, pieces = (C + v - 1) / v;
+  if (pieces <= 256) {
+    s.lanes = 8;
+    while (s.lanes < 64 && s.lanes < pieces) s.lanes *= 2;
+    s.nv = pieces <= s.lanes ? 1 : (pieces <= 2 * s.lanes ? 2 : 4);
+  } else if (pieces <= 1024 || (dtype == PXL_F32 && pieces <= 2048)) {
+    s.lanes = 256;
+    s.nv = pieces <= 512 ? 2 : (pieces <= 1024 ? 4 : 8);
+  }
+  if (s.lanes) {
+    const long passes = (R + 256 / s.lanes - 1) / (256 / s.lanes);
+    s.groups = (int)(passes < 1 ? 1 : (passes > 512 ? 512 : passes));
+  } else {
+    const long g = (R + 63) / 64;
+    s.groups = (int)(g < 1 ? 1 : (g > 256 ? 256 : g));
+  }
+  return s;
 }
+LnShape ln_chan_shape(int dtype, long N, int C, long S) {
+  LnShape s = {0, 0, 256, 8, 1, 0};
+  if (C <= 256) {
+    s.nv = C <= 32 ? 1 : (C <= 64 ? 2 : (C <= 128 ? 4 : 8));
+  } else if (C <= 2048) {
+    s.threads = 512;
+    s.tsv = C <= 512 ? 8 : 4;
+    s.nv = C <= 1024 ? 8 : 16;
+  }
+  if (s.nv) {
+    const int ts = s.tsv * (dtype == PXL_F32 ? 4 : 8);
+    s.lanes = s.tsv;
+    s.tiles = N * ((S + ts - 1) / ts);
+    const long most = s.threads == 256 ? 1024 : 512;
+    if (s.tiles >= (1l << 30)) s.lanes = s.nv = 0;
+    s.groups = (int)(s.tiles < 1 ? 1 : (s.tiles > most ? most : s.tiles));
+  }
+  if (!s.nv) {
+    const long g = (N * S + 63) / 64;
+    s.groups = (int)(g < 1 ? 1 : (g > 256 ? 256 : g));
+  }
+  return s;
+}
+inline LnShape ln_shape(int dtype, long R, int C, long S) { return S < 0 ? ln_rows_shape(dtype, R, C) : ln_chan_shape(dtype, S > 0 ? R / S : 0, C, S); }
+
+#define LN_ROWS(KERNEL, BLOCKS, ...)                                                                                   \
+  do {                                                                                                                 \
+    const dim3 grid(BLOCKS);                                                                                           \
+    const int key = s.lanes * 16 + s.nv;                                                                               \
+    if (key == 8 * 16 + 1) hipLaunchKernelGGL((KERNEL<T, 8, 1>), grid, dim3(256), 0, st, __VA_ARGS__);                 \
+    else if (key == 16 * 16 + 1) hipLaunchKernelGGL((KERNEL<T, 16, 1>), grid, dim3(256), 0, st, __VA_ARGS__);          \
+    else if (key == 32 * 16 + 1) hipLaunchKernelGGL((KERNEL<T, 32, 1>), grid, dim3(256), 0, st, __VA_ARGS__);          \
+    else if (key == 64 * 16 + 1) hipLaunchKernelGGL((KERNEL<T, 64, 1>), grid, dim3(256), 0, st, __VA_ARGS__);          \
+    else if (key == 64 * 16 + 2) hipLaunchKernelGGL((KERNEL<T, 64, 2>), grid, dim3(256), 0, st, __VA_ARGS__);          \
+    else if (key == 64 * 16 + 4) hipLaunchKernelGGL((KERNEL<T, 64, 4>), grid, dim3(256), 0, st, __VA_ARGS__);          \
+    else if (key == 256 * 16 + 2) hipLaunchKernelGGL((KERNEL<T, 256, 2>), grid, dim3(256), 0, st, __VA_ARGS__);        \
+    else if (key == 256 * 16 + 4) hipLaunchKernelGGL((KERNEL<T, 256, 4>), grid, dim3(256), 0, st, __VA_ARGS__);        \
+    else if constexpr (sizeof(T) == 4) hipLaunchKernelGGL((KERNEL<T, 256, 8>), grid, dim3(256), 0, st, __VA_ARGS__);   \
+  } while (0)
+#define LN_CHAN(KERNEL, BLOCKS, ...)                                                                                                 \
+  do {                                                                                                                               \
+    const dim3 grid(BLOCKS);                                                                                                         \
+    if (s.threads == 256) {                                                                                                          \
+      if (s.nv == 1) hipLaunchKernelGGL((KERNEL<T, 256, 8, 1>), grid, dim3(256), 0, st, __VA_ARGS__);                                \
+      else if (s.nv == 2) hipLaunchKernelGGL((KERNEL<T, 256, 8, 2>), grid, dim3(256), 0, st, __VA_ARGS__);                           \
+      else if (s.nv == 4) hipLaunchKernelGGL((KERNEL<T, 256, 8, 4>), grid, dim3(256), 0, st, __VA_ARGS__);                           \
+      else hipLaunchKernelGGL((KERNEL<T, 256, 8, 8>), grid, dim3(256), 0, st, __VA_ARGS__);                                          \
+    } else if (s.tsv == 8) hipLaunchKernelGGL((KERNEL<T, 512, 8, 8>), grid, dim3(512), 0, st, __VA_ARGS__);                          \
+    else if (s.nv == 8) hipLaunchKernelGGL((KERNEL<T, 512, 4, 8>), grid, dim3(512), 0, st, __VA_ARGS__);                             \
+    else hipLaunchKernelGGL((KERNEL<T, 512, 4, 16>), grid, dim3(512), 0, st, __VA_ARGS__);                                           \
+  } while (0)
 
 template <typename T>
 int ln_fwd(long R, int C, long S, long xs, const void* x, LnParam w, LnParam b, float eps, void* y, float* mean, float* rstd, hipStream_t st) {
-  if (S < 0)
-    hipLaunchKernelGGL(ln_rows_fwd_loop<T>, dim3(blocks_for(R, 1 << 20)), dim3(256), 0, st, R, C, xs, (const T*)x, w, b, eps, (T*)y, mean, rstd);
-  else
+  const LnShape s = ln_shape(Elem<T>::DTYPE, R, C, S);
+  if (S < 0) {
+    if (s.lanes) {
+      const long passes = (R + 256 / s.lanes - 1) / (256 / s.lanes);
+      LN_ROWS(ln_rows_fwd, blocks_for(passes, 2048), R, C, xs, (const T*)x, w, b, eps, (T*)y, mean, rstd);
+    } else {
+      hipLaunchKernelGGL(ln_rows_fwd_loop<T>, dim3(blocks_for(R, 1 << 20)), dim3(256), 0, st, R, C, xs, (const T*)x, w, b, eps, (T*)y, mean, rstd);
+    }
+  } else if (s.lanes) {
+    const int per = (int)(s.tiles / (R / S));
+    LN_CHAN(ln_chan_fwd, (unsigned)s.tiles, (int)s.tiles, per, C, S, (const T*)x, w, b, eps, (T*)y, mean, rstd);
+  } else {
     hipLaunchKernelGGL(ln_chan_fwd_loop<T>, dim3(blocks_for((R + 255) / 256, 1 << 20)), dim3(256), 0, st, R, C, S, (const T*)x, w, b, eps,
                        (T*)y, mean, rstd);
+  }
   PXL_LAUNCH_CHECK();
   return PXL_OK;
 }
@@ -186,26 +631,45 @@ int ln_fwd(long R, int C, long S, long xs, const void* x, LnParam w, LnParam b, 
 template <typename T>
 int ln_bwd(long R, int C, long S, long xs, const void* x, const void* dy, LnParam w, const float* mean, const float* rstd, void* dx,
            void* dw, void* db, int pf32, float* part, hipStream_t st) {
-  const int G = ln_groups(R, C);
-  if (R > 0 && dx != nullptr) {
-    if (S < 0)
-      hipLaunchKernelGGL(ln_rows_dx_loop<T>, dim3(blocks_for(R, 1 << 20)), dim3(256), 0, st, R, C, xs, (const T*)x, (const T*)dy, w, mean, rstd, (T*)dx);
-    else
-      hipLaunchKernelGGL(ln_chan_dx_loop<T>, dim3(blocks_for((R + 255) / 256, 1 << 20)), dim3(256), 0, st, R, C, S, (const T*)x, (const T*)dy, w,
-                         mean, rstd, (T*)dx);
+  const LnShape s = ln_shape(Elem<T>::DTYPE, R, C, S);
+  const int G = s.groups;
+  const bool params = dw != nullptr || db != nullptr;
+  if (R > 0 && s.lanes && (dx != nullptr || params)) {
+    float* p = params ? part : nullptr;
+    if (S < 0) {
+      LN_ROWS(ln_rows_bwd, (unsigned)G, R, C, xs, (const T*)x, (const T*)dy, w, mean, rstd, (T*)dx, p);
+    } else {
+      const int per = (int)(s.tiles / (R / S));
+      LN_CHAN(ln_chan_bwd, (unsigned)G, (int)s.tiles, per, C, S, (const T*)x, (const T*)dy, w, mean, rstd, (T*)dx, p);
+    }
     PXL_LAUNCH_CHECK();
+  } else if (R > 0) {
+    if (dx != nullptr) {
+      if (S < 0)
+        hipLaunchKernelGGL(ln_rows_dx_loop<T>, dim3(blocks_for(R, 1 << 20)), dim3(256), 0, st, R, C, xs, (const T*)x, (const T*)dy, w, mean, rstd, (T*)dx);
+      else
+        hipLaunchKernelGGL(ln_chan_dx_loop<T>, dim3(blocks_for((R + 255) / 256, 1 << 20)), dim3(256), 0, st, R, C, S, (const T*)x, (const T*)dy, w,
+                           mean, rstd, (T*)dx);
+      PXL_LAUNCH_CHECK();
+    }
+    if (params) {
+      if (S < 0)
+        hipLaunchKernelGGL(ln_rows_dwb_loop<T>, dim3((C + 255) / 256, G), dim3(256), 0, st, R, C, xs, (const T*)x, (const T*)dy, mean, rstd, part);
+      else
+        hipLaunchKernelGGL(ln_chan_dwb_loop<T>, dim3(C, G), dim3(256), 0, st, R, C, S, (const T*)x, (const T*)dy, mean, rstd, part);
+      PXL_LAUNCH_CHECK();
+    }
   }
-  if (dw != nullptr || db != nullptr) {
-    if (S < 0)
-      hipLaunchKernelGGL(ln_rows_dwb_loop<T>, dim3((C + 255) / 256, G), dim3(256), 0, st, R, C, xs, (const T*)x, (const T*)dy, mean, rstd, part);
-    else
-      hipLaunchKernelGGL(ln_chan_dwb_loop<T>, dim3(C, G), dim3(256), 0, st, R, C, S, (const T*)x, (const T*)dy, mean, rstd, part);
-    PXL_LAUNCH_CHECK();
-    hipLaunchKernelGGL(ln_dwb_fold<T>, dim3((2 * C + 255) / 256), dim3(256), 0, st, G, C, part, dw, db, pf32);
+  if (params) {
+    hipLaunchKernelGGL(ln_dwb_fold<T>, dim3((2 * C + 15) / 16), dim3(256), 0, st, R > 0 ? G : 0, C, part, dw, db, pf32);
     PXL_LAUNCH_CHECK();
   }
   return PXL_OK;
 }
+
+// (the workspace queries do not know the type)
+inline int ln_rows_most(long R, int C) { const int a = ln_rows_shape(PXL_F32, R, C).groups, b = ln_rows_shape(PXL_BF16, R, C).groups; return a > b ? a : b; }
+inline int ln_chan_most(long N, int C, long S) { const int a = ln_chan_shape(PXL_F32, N, C, S).groups, b = ln_chan_shape(PXL_BF16, N, C, S).groups; return a > b ? a : b; }
 
 int ln_check(const char* what, int dtype, int pdtype, long R, int C) {
   PXL_REQUIRE(dtype == PXL_F32 || dtype == PXL_BF16, "%s: dtype %d is neither PXL_F32 nor PXL_BF16", what, dtype);
@@ -217,7 +681,7 @@ int ln_check(const char* what, int dtype, int pdtype, long R, int C) {
 }  // namespace
 
 extern "C" size_t pxl_layer_norm_bwd_workspace(long R, int C) {
-  return R < 0 || C < 1 ? 0 : (size_t)ln_groups(R, C) * 2 * C * sizeof(float);
+  return R < 0 || C < 1 ? 0 : (size_t)ln_rows_most(R, C) * 2 * C * sizeof(float);
 }
 
 extern "C" int pxl_layer_norm_fwd(int dtype, int pdtype, long R, int C, long x_stride, const void* x, const void* w, const void* b, float eps,
@@ -260,7 +724,7 @@ extern "C" int pxl_layer_norm_nchw_fwd(int dtype, int pdtype, long N, int C, lon
 }
 
 extern "C" size_t pxl_layer_norm_nchw_bwd_workspace(long N, int C, long S) {
-  return N < 0 || S < 0 || C < 1 ? 0 : (size_t)ln_groups(N * S, C) * 2 * C * sizeof(float);
+  return N < 0 || S < 0 || C < 1 ? 0 : (size_t)ln_chan_most(N, C, S) * 2 * C * sizeof(float);
 }
 
 extern "C" int pxl_layer_norm_nchw_bwd(int dtype, int pdtype, long N, int C, long S, const void* x, const void* dy, const void* w,

@@ -279,11 +279,12 @@ def softmax_channels(x):
 # ---- layer normalisation (csrc/layernorm.hip) ---------------------------------------------------------------------------------
 def _launch(dev, fn, *args):
     """fn(*args, stream) on the current stream of `dev`, which need not be the current device"""
-    if dev.index == torch.cuda.current_device():
-        check(fn(*args, stream_ptr()))
+    index = dev.index
+    if index == torch._C._cuda_getDevice():
+        check(fn(*args, torch._C._cuda_getCurrentRawStream(index)))
     else:
         with torch.cuda.device(dev):
-            check(fn(*args, stream_ptr()))
+            check(fn(*args, torch._C._cuda_getCurrentRawStream(index)))
 
 
 def _row_stride(x):
