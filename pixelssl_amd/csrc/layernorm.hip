@@ -149,33 +149,23 @@ __global__ __launch_bounds__(256) void ln_chan_dwb_loop(long P, int C, long S, c
   }
 }
 
-// ---- 16-byte pieces at any element alignment --------------------------------------------------------------------------------
+// ---- 16-byte pieces at any element alignment.  A piece that would pass the end of its run is moved back to end there: it holds `dup`
+// elements that the piece before it holds too, which count once in sums and are written twice with the same bits ----------------
 template <typename T> struct Piece {
   static constexpr int N = 16 / (int)sizeof(T);
-  // `valid` elements from p on (all N: one unaligned 16-byte access), the others 0
-  static __device__ __forceinline__ uint4 load(const T* p, int valid) {
-    uint4 v = make_uint4(0u, 0u, 0u, 0u);
-    if (valid >= N) {
-      __builtin_memcpy(&v, p, 16);
-    } else if (valid > 0) {
-      T t[N];
-#pragma unroll
-      for (int e = 0; e < N; ++e) t[e] = e < valid ? p[e] : T(0);
-      __builtin_memcpy(&v, t, 16);
-    }
+  static __device__ __forceinline__ uint4 load(const T* p) {
+    uint4 v;
+    __builtin_memcpy(&v, p, 16);
     return v;
   }
-  static __device__ __forceinline__ void store(T* p, const float* f, int valid) {
+  static __device__ __forceinline__ void store(T* p, const float* f) {
     const uint4 v = Chunk<T>::pack(f);
-    if (valid >= N) {
-      __builtin_memcpy(p, &v, 16);
-    } else if (valid > 0) {
-#pragma unroll
-      for (int e = 0; e < N; ++e)
-        if (e < valid) p[e] = from_f<T>(f[e]);
-    }
+    __builtin_memcpy(p, &v, 16);
   }
 };
+
+// makes the compiler take a piece as new: what is unpacked from it after this is unpacked again, not kept in registers from before
+__device__ __forceinline__ void renew(uint4& v) { asm volatile("" : "+v"(v.x), "+v"(v.y), "+v"(v.z), "+v"(v.w)); }
 
 template <int LPR> __device__ __forceinline__ float row_sum(float v, float* sh) {
   if constexpr (LPR == 256) return block_sum<256>(v, sh);
@@ -185,60 +175,76 @@ template <int LPR> __device__ __forceinline__ float row_sum(float v, float* sh) 
 }
 
 // ---- rows that fit into registers: LPR lanes hold a row in NV pieces each, one sweep over memory; weight and bias stay in registers
-// over the rows of a workgroup --------------------------------------------------------------------------------------------------
-template <typename T, int LPR, int NV>
+// over the rows of a workgroup.  TAIL: C is no multiple of a piece --------------------------------------------------------------
+// start of piece j of a lane, moved back where it would pass C; dup: elements it shares with the piece before (N or more: all)
+template <int N, int LPR, bool TAIL> __device__ __forceinline__ int piece_at(int j, int lane, int C, int& dup) {
+  const int c = (j * LPR + lane) * N;
+  if (!TAIL) { dup = c < C ? 0 : N; return c < C ? c : 0; }
+  const int at = c + N <= C ? c : C - N;
+  dup = c - at;
+  return at;
+}
+
+template <typename T, int LPR, int NV, bool TAIL>
 __global__ __launch_bounds__(256) void ln_rows_fwd(long R, int C, long xs, const T* __restrict__ x, LnParam w, LnParam b, float eps,
                                                    T* __restrict__ y, float* __restrict__ mean, float* __restrict__ rstd) {
   constexpr int V = Piece<T>::N, RPB = 256 / LPR;
   __shared__ float sh[4];
   const int lane = threadIdx.x % LPR;
   float wv[NV][V], bv[NV][V];
+  int at[NV], dup[NV];
 #pragma unroll
-  for (int j = 0; j < NV; ++j)
+  for (int j = 0; j < NV; ++j) {
+    at[j] = piece_at<V, LPR, TAIL>(j, lane, C, dup[j]);
 #pragma unroll
     for (int e = 0; e < V; ++e) {
-      const int c = (j * LPR + lane) * V + e;
-      wv[j][e] = c < C ? w.get<T>(c, 1.f) : 0.f;
-      bv[j][e] = c < C ? b.get<T>(c, 0.f) : 0.f;
+      wv[j][e] = w.get<T>(at[j] + e, 1.f);
+      bv[j][e] = b.get<T>(at[j] + e, 0.f);
     }
+  }
   const float inv = 1.f / C;
-  for (long r0 = (long)blockIdx.x * RPB; r0 < R; r0 += (long)gridDim.x * RPB) {
+  const long step = (long)gridDim.x * RPB;
+  uint4 raw[NV];
+  auto fetch = [&](long r) {
+    const T* xr = x + (r < R ? r : R - 1) * xs;            // past the end: the last row again
+#pragma unroll
+    for (int j = 0; j < NV; ++j) raw[j] = Piece<T>::load(xr + at[j]);
+  };
+  fetch((long)blockIdx.x * RPB + threadIdx.x / LPR);
+  for (long r0 = (long)blockIdx.x * RPB; r0 < R; r0 += step) {
     const long r = r0 + threadIdx.x / LPR;
-    const bool live = RPB == 1 || r < R;
     float f[NV][V];
     float s = 0.f;
 #pragma unroll
     for (int j = 0; j < NV; ++j) {
-      const int c = (j * LPR + lane) * V;
-      Chunk<T>::unpack(Piece<T>::load(x + r * xs + c, live ? C - c : 0), f[j]);
+      Chunk<T>::unpack(raw[j], f[j]);
 #pragma unroll
-      for (int e = 0; e < V; ++e) s += f[j][e];
+      for (int e = 0; e < V; ++e) s += e >= dup[j] ? f[j][e] : 0.f;
     }
-    const float m = row_sum<LPR>(s, sh) / C;           // (divided: a row of equal values has its mean exactly)
+    fetch(r + step);                                       // the next row, while this one is reduced
+    const float m = row_sum<LPR>(s, sh) / C;               // (divided: a row of equal values has its mean exactly)
     float q = 0.f;
 #pragma unroll
-    for (int j = 0; j < NV; ++j) {
-      const int left = C - (j * LPR + lane) * V;
+    for (int j = 0; j < NV; ++j)
 #pragma unroll
       for (int e = 0; e < V; ++e) {
         f[j][e] -= m;
-        if (e < left) q += f[j][e] * f[j][e];
+        q += e >= dup[j] ? f[j][e] * f[j][e] : 0.f;
       }
-    }
     const float rs = 1.f / sqrtf(row_sum<LPR>(q, sh) * inv + eps);
+    if (RPB > 1 && r >= R) continue;
 #pragma unroll
     for (int j = 0; j < NV; ++j) {
-      const int c = (j * LPR + lane) * V;
 #pragma unroll
       for (int e = 0; e < V; ++e) f[j][e] = f[j][e] * rs * wv[j][e] + bv[j][e];
-      Piece<T>::store(y + r * C + c, f[j], live ? C - c : 0);
+      if (dup[j] < V) Piece<T>::store(y + r * C + at[j], f[j]);
     }
-    if (mean != nullptr && lane == 0 && live) { mean[r] = m; rstd[r] = rs; }
+    if (mean != nullptr && lane == 0) { mean[r] = m; rstd[r] = rs; }
   }
 }
 
 // dx and, kept in registers over the rows of a workgroup, its share of dw / db -> part[workgroup][2][C]
-template <typename T, int LPR, int NV>
+template <typename T, int LPR, int NV, bool TAIL>
 __global__ __launch_bounds__(256) void ln_rows_bwd(long R, int C, long xs, const T* __restrict__ x, const T* __restrict__ dy, LnParam w,
                                                    const float* __restrict__ mean, const float* __restrict__ rstd, T* __restrict__ dx,
                                                    float* __restrict__ part) {
@@ -246,64 +252,70 @@ __global__ __launch_bounds__(256) void ln_rows_bwd(long R, int C, long xs, const
   __shared__ float sh[4];
   const int lane = threadIdx.x % LPR, sub = threadIdx.x / LPR;
   float wv[NV][V], aw[NV][V], ab[NV][V];
+  int at[NV], dup[NV];
 #pragma unroll
-  for (int j = 0; j < NV; ++j)
+  for (int j = 0; j < NV; ++j) {
+    at[j] = piece_at<V, LPR, TAIL>(j, lane, C, dup[j]);
 #pragma unroll
     for (int e = 0; e < V; ++e) {
-      const int c = (j * LPR + lane) * V + e;
-      wv[j][e] = c < C ? w.get<T>(c, 1.f) : 0.f;
+      wv[j][e] = w.get<T>(at[j] + e, 1.f);
       aw[j][e] = ab[j][e] = 0.f;
     }
+  }
   const float inv = 1.f / C;
   for (long r0 = (long)blockIdx.x * RPB; r0 < R; r0 += (long)gridDim.x * RPB) {
-    const long r = r0 + sub;
-    const bool live = RPB == 1 || r < R;
-    const float m = live ? mean[r] : 0.f, rs = live ? rstd[r] : 0.f;
+    const bool live = RPB == 1 || r0 + sub < R;
+    const long r = live ? r0 + sub : R - 1;                // past the end: the last row again, counted nowhere
+    const float m = mean[r], rs = rstd[r];
     float u[NV][V], g[NV][V];
     float s1 = 0.f, s2 = 0.f;
+    uint4 ru[NV], rg[NV];
 #pragma unroll
     for (int j = 0; j < NV; ++j) {
-      const int c = (j * LPR + lane) * V;
-      Chunk<T>::unpack(Piece<T>::load(x + r * xs + c, live ? C - c : 0), u[j]);
-      Chunk<T>::unpack(Piece<T>::load(dy + r * C + c, live ? C - c : 0), g[j]);
+      ru[j] = Piece<T>::load(x + r * xs + at[j]);
+      rg[j] = Piece<T>::load(dy + r * C + at[j]);
     }
 #pragma unroll
-    for (int j = 0; j < NV; ++j)
+    for (int j = 0; j < NV; ++j) {
+      Chunk<T>::unpack(ru[j], u[j]);
+      Chunk<T>::unpack(rg[j], g[j]);
 #pragma unroll
       for (int e = 0; e < V; ++e) {
         u[j][e] = (u[j][e] - m) * rs;
-        const float d = g[j][e];            // 0 behind the row's end
-        if (part != nullptr) {
+        const float d = g[j][e];
+        if (live) {
           aw[j][e] += d * u[j][e];
           ab[j][e] += d;
         }
         g[j][e] = d * wv[j][e];
-        s1 += g[j][e];
-        s2 += g[j][e] * u[j][e];
+        s1 += e >= dup[j] ? g[j][e] : 0.f;
+        s2 += e >= dup[j] ? g[j][e] * u[j][e] : 0.f;
+        asm volatile("" : "+v"(aw[j][e]), "+v"(ab[j][e]));
       }
+    }
     if (dx == nullptr) continue;
     const float a1 = row_sum<LPR>(s1, sh) * inv, a2 = row_sum<LPR>(s2, sh) * inv;
+    if (!live) continue;
 #pragma unroll
     for (int j = 0; j < NV; ++j) {
-      const int c = (j * LPR + lane) * V;
 #pragma unroll
       for (int e = 0; e < V; ++e) g[j][e] = rs * (g[j][e] - a1 - u[j][e] * a2);
-      Piece<T>::store(dx + r * C + c, g[j], live ? C - c : 0);
+      if (dup[j] < V) Piece<T>::store(dx + r * C + at[j], g[j]);
     }
   }
   if (part == nullptr) return;
+  // a shared column has the same sums in both of its pieces: either is written
   float* p = part + (long)blockIdx.x * 2 * C;
   if constexpr (RPB == 1) {
 #pragma unroll
-    for (int j = 0; j < NV; ++j) {
-      const int c = (j * LPR + lane) * V;
-      Piece<float>::store(p + c, aw[j], C - c);
-      Piece<float>::store(p + C + c, ab[j], C - c);
-      if constexpr (V == 8) {
-        Piece<float>::store(p + c + 4, aw[j] + 4, C - c - 4);
-        Piece<float>::store(p + C + c + 4, ab[j] + 4, C - c - 4);
+    for (int j = 0; j < NV; ++j)
+      if (dup[j] < V) {
+#pragma unroll
+        for (int e = 0; e < V; e += 4) {
+          Piece<float>::store(p + at[j] + e, &aw[j][e]);
+          Piece<float>::store(p + C + at[j] + e, &ab[j][e]);
+        }
       }
-    }
   } else {
     // the row lanes of the workgroup one after the other into one copy
     __shared__ float acc[2][LPR * NV * V];
@@ -313,15 +325,17 @@ __global__ __launch_bounds__(256) void ln_rows_bwd(long R, int C, long xs, const
         for (int j = 0; j < NV; ++j)
 #pragma unroll
           for (int e = 0; e < V; ++e) {
-            const int at = (j * V + e) * LPR + lane;
-            acc[0][at] = k == 0 ? aw[j][e] : acc[0][at] + aw[j][e];
-            acc[1][at] = k == 0 ? ab[j][e] : acc[1][at] + ab[j][e];
+            const int i = (j * V + e) * LPR + lane;
+            acc[0][i] = k == 0 ? aw[j][e] : acc[0][i] + aw[j][e];
+            acc[1][i] = k == 0 ? ab[j][e] : acc[1][i] + ab[j][e];
           }
       }
       __syncthreads();
     }
     for (int c = threadIdx.x; c < C; c += 256) {
-      const int piece = c / V, e = c - piece * V, j = piece / LPR, l = piece - j * LPR;
+      const int piece = c / V, j = piece / LPR, l = piece - j * LPR;
+      int shared;
+      const int e = c - piece_at<V, LPR, TAIL>(j, l, C, shared);
       p[c] = acc[0][(j * V + e) * LPR + l];
       p[C + c] = acc[1][(j * V + e) * LPR + l];
     }
@@ -362,23 +376,30 @@ __device__ __forceinline__ void chan_sum(float (&s)[NS][V], float* sh) {
     for (int e = 0; e < V; ++e) s[k][e] = sh[NW * W + (k * TSV + sv) * V + e];
 }
 
+// addresses: a base per j that the whole workgroup shares, and one 32-bit byte offset per lane (CY * S elements stay below 2^31 bytes)
+template <typename T> __device__ __forceinline__ const T* lane_at(const T* base, unsigned off) {
+  return reinterpret_cast<const T*>(reinterpret_cast<const unsigned char*>(base) + off);
+}
+template <typename T> __device__ __forceinline__ T* lane_at(T* base, unsigned off) {
+  return reinterpret_cast<T*>(reinterpret_cast<unsigned char*>(base) + off);
+}
+
 template <typename T, int THREADS, int TSV, int NV>
-__global__ __launch_bounds__(THREADS) void ln_chan_fwd(int tiles, int per, int C, long S, const T* __restrict__ x, LnParam w, LnParam b, float eps,
+__global__ __launch_bounds__(THREADS) void ln_chan_fwd(int tiles, int per, int C, int S, const T* __restrict__ x, LnParam w, LnParam b, float eps,
                                                        T* __restrict__ y, float* __restrict__ mean, float* __restrict__ rstd) {
   constexpr int V = Piece<T>::N, CY = THREADS / TSV, TS = TSV * V;
   __shared__ float sh[(THREADS / 64 + 1) * TS];
   const int sv = threadIdx.x % TSV, cy = threadIdx.x / TSV;
   const float inv = 1.f / C;
   const int t = xcd_remap(blockIdx.x, tiles);
-  const long n = t / per;
-  const long s0 = (long)(t - n * per) * TS + sv * V;
-  const int left = S - s0 >= V ? V : (S - s0 > 0 ? (int)(S - s0) : 0);
-  const long base = n * C * S + s0;
+  const int n = t / per, s0 = (t - n * per) * TS + sv * V;
+  const int at = s0 + V <= S ? s0 : S - V, dup = s0 - at;
+  const long base = (long)n * C * S, step = (long)CY * S;
   uint4 raw[NV];
 #pragma unroll
   for (int j = 0; j < NV; ++j) {
-    const int c = j * CY + cy;
-    raw[j] = Piece<T>::load(x + base + c * S, c < C ? left : 0);
+    const int b0 = j * CY < C ? j * CY : C - 1, c = b0 + cy < C ? cy : C - 1 - b0;      // past the channels: the last one again
+    raw[j] = Piece<T>::load(lane_at(x + base + (long)b0 * S, (unsigned)(c * S + at) * (unsigned)sizeof(T)));
   }
   float s[1][V];
 #pragma unroll
@@ -387,8 +408,10 @@ __global__ __launch_bounds__(THREADS) void ln_chan_fwd(int tiles, int per, int C
   for (int j = 0; j < NV; ++j) {
     float f[V];
     Chunk<T>::unpack(raw[j], f);
+    if (j * CY + cy < C) {
 #pragma unroll
-    for (int e = 0; e < V; ++e) s[0][e] += f[e];
+      for (int e = 0; e < V; ++e) s[0][e] += f[e];
+    }
   }
   chan_sum<THREADS, TSV, V, 1>(s, sh);
   float m[V];
@@ -397,6 +420,7 @@ __global__ __launch_bounds__(THREADS) void ln_chan_fwd(int tiles, int per, int C
 #pragma unroll
   for (int j = 0; j < NV; ++j) {
     float f[V];
+    renew(raw[j]);
     Chunk<T>::unpack(raw[j], f);
     if (j * CY + cy < C) {
 #pragma unroll
@@ -408,90 +432,104 @@ __global__ __launch_bounds__(THREADS) void ln_chan_fwd(int tiles, int per, int C
   float rs[V];
 #pragma unroll
   for (int e = 0; e < V; ++e) rs[e] = 1.f / sqrtf(s[0][e] * inv + eps);
+  if (dup >= V) return;
 #pragma unroll
   for (int j = 0; j < NV; ++j) {
     const int c = j * CY + cy;
     if (c >= C) continue;
     const float wc = w.get<T>(c, 1.f), bc = b.get<T>(c, 0.f);
     float f[V];
+    renew(raw[j]);
     Chunk<T>::unpack(raw[j], f);
 #pragma unroll
     for (int e = 0; e < V; ++e) f[e] = (f[e] - m[e]) * rs[e] * wc + bc;
-    Piece<T>::store(y + base + c * S, f, left);
+    Piece<T>::store(lane_at(y + base + j * step, (unsigned)(cy * S + at) * (unsigned)sizeof(T)), f);
   }
   if (mean != nullptr && cy == 0) {
 #pragma unroll
-    for (int e = 0; e < V; ++e)
-      if (e < left) { mean[n * S + s0 + e] = m[e]; rstd[n * S + s0 + e] = rs[e]; }
+    for (int e = 0; e < V; ++e) { mean[(long)n * S + at + e] = m[e]; rstd[(long)n * S + at + e] = rs[e]; }
   }
 }
 
 template <typename T, int THREADS, int TSV, int NV>
-__global__ __launch_bounds__(THREADS) void ln_chan_bwd(int tiles, int per, int C, long S, const T* __restrict__ x, const T* __restrict__ dy, LnParam w,
+__global__ __launch_bounds__(THREADS) void ln_chan_bwd(int tiles, int per, int C, int S, const T* __restrict__ x, const T* __restrict__ dy, LnParam w,
                                                        const float* __restrict__ mean, const float* __restrict__ rstd, T* __restrict__ dx,
                                                        float* __restrict__ part) {
   constexpr int V = Piece<T>::N, CY = THREADS / TSV, TS = TSV * V;
   __shared__ float sh[(THREADS / 64 + 1) * 2 * TS];
   const int sv = threadIdx.x % TSV, cy = threadIdx.x / TSV;
   const float inv = 1.f / C;
-  float aw[NV], ab[NV], wv[NV];
+  const long step = (long)CY * S;
+  constexpr bool KEEP = NV <= 8;                           // weights in registers, or read again where they are used
+  float aw[NV], ab[NV], wk[KEEP ? NV : 1];
+  auto weight = [&](int j) { return j * CY + cy < C ? w.get<T>(j * CY + cy, 1.f) : 0.f; };     // (0: a channel past the end adds nothing)
 #pragma unroll
   for (int j = 0; j < NV; ++j) {
-    const int c = j * CY + cy;
     aw[j] = ab[j] = 0.f;
-    wv[j] = c < C ? w.get<T>(c, 1.f) : 0.f;
+    if (KEEP) wk[j] = weight(j);
   }
   // consecutive tiles (they share cache lines where rows start anywhere) to one workgroup
   const int G = gridDim.x, g = xcd_remap(blockIdx.x, G);
   const int t0 = (int)((long)tiles * g / G), t1 = (int)((long)tiles * (g + 1) / G);
   for (int t = t0; t < t1; ++t) {
-    const long n = t / per;
-    const long s0 = (long)(t - n * per) * TS + sv * V;
-    const int left = S - s0 >= V ? V : (S - s0 > 0 ? (int)(S - s0) : 0);
-    const long base = n * C * S + s0;
+    const int n = t / per, s0 = (t - n * per) * TS + sv * V;
+    const int at = s0 + V <= S ? s0 : S - V, dup = s0 - at;
+    const long base = (long)n * C * S;
     uint4 rx[NV], rg[NV];
 #pragma unroll
     for (int j = 0; j < NV; ++j) {
-      const int c = j * CY + cy;
-      rx[j] = Piece<T>::load(x + base + c * S, c < C ? left : 0);
-      rg[j] = Piece<T>::load(dy + base + c * S, c < C ? left : 0);
+      const int b0 = j * CY < C ? j * CY : C - 1, c = b0 + cy < C ? cy : C - 1 - b0;    // past the channels: the last one again
+      const unsigned off = (unsigned)(c * S + at) * (unsigned)sizeof(T);
+      rx[j] = Piece<T>::load(lane_at(x + base + (long)b0 * S, off));
+      rg[j] = Piece<T>::load(lane_at(dy + base + (long)b0 * S, off));
     }
     float m[V], rs[V], s[2][V];
 #pragma unroll
     for (int e = 0; e < V; ++e) {
-      m[e] = e < left ? mean[n * S + s0 + e] : 0.f;
-      rs[e] = e < left ? rstd[n * S + s0 + e] : 0.f;
+      m[e] = mean[(long)n * S + at + e];
+      rs[e] = rstd[(long)n * S + at + e];
       s[0][e] = s[1][e] = 0.f;
     }
 #pragma unroll
     for (int j = 0; j < NV; ++j) {
       float u[V], d[V];
+      const float wj = KEEP ? wk[KEEP ? j : 0] : weight(j);
       Chunk<T>::unpack(rx[j], u);
       Chunk<T>::unpack(rg[j], d);
 #pragma unroll
       for (int e = 0; e < V; ++e) {
         u[e] = (u[e] - m[e]) * rs[e];
-        aw[j] += d[e] * u[e];
-        ab[j] += d[e];
-        s[0][e] += d[e] * wv[j];
-        s[1][e] += d[e] * wv[j] * u[e];
+        const float own = e >= dup ? d[e] : 0.f;          // a position that the piece before holds too counts there
+        aw[j] += e >= dup ? d[e] * u[e] : 0.f;
+        ab[j] += own;
+        s[0][e] += d[e] * wj;
+        s[1][e] += d[e] * wj * u[e];
       }
+      // every sum is taken here: left to the compiler, some sink to the loop's end and keep all pieces unpacked until then (196 registers, 144 so)
+      asm volatile("" : "+v"(aw[j]), "+v"(ab[j]));
+#pragma unroll
+      for (int e = 0; e < V; ++e) asm volatile("" : "+v"(s[0][e]), "+v"(s[1][e]));
     }
     if (dx == nullptr) continue;
     chan_sum<THREADS, TSV, V, 2>(s, sh);
+    if (dup < V) {
 #pragma unroll
-    for (int j = 0; j < NV; ++j) {
-      const int c = j * CY + cy;
-      if (c >= C) continue;
-      float u[V], d[V];
-      Chunk<T>::unpack(rx[j], u);
-      Chunk<T>::unpack(rg[j], d);
+      for (int j = 0; j < NV; ++j) {
+        const int c = j * CY + cy;
+        if (c >= C) continue;
+        float u[V], d[V];
+        const float wj = KEEP ? wk[KEEP ? j : 0] : weight(j);
+        renew(rx[j]);
+        renew(rg[j]);
+        Chunk<T>::unpack(rx[j], u);
+        Chunk<T>::unpack(rg[j], d);
 #pragma unroll
-      for (int e = 0; e < V; ++e) {
-        u[e] = (u[e] - m[e]) * rs[e];
-        d[e] = rs[e] * (d[e] * wv[j] - s[0][e] * inv - u[e] * (s[1][e] * inv));
+        for (int e = 0; e < V; ++e) {
+          u[e] = (u[e] - m[e]) * rs[e];
+          d[e] = rs[e] * (d[e] * wj - s[0][e] * inv - u[e] * (s[1][e] * inv));
+        }
+        Piece<T>::store(lane_at(dx + base + j * step, (unsigned)(cy * S + at) * (unsigned)sizeof(T)), d);
       }
-      Piece<T>::store(dx + base + c * S, d, left);
     }
     __syncthreads();                  // the last readers of sh are done
   }
@@ -509,20 +547,30 @@ __global__ __launch_bounds__(THREADS) void ln_chan_bwd(int tiles, int per, int C
   }
 }
 
-// part[G][2][C] -> dw[C], db[C] (either may be absent): 16 columns a workgroup, 16 lanes over the groups, in ascending order each
+// part[G][2][C] -> dw[C], db[C] (either may be absent): 16 columns a workgroup, 64 lanes over the groups, in ascending order each
 template <typename T>
-__global__ __launch_bounds__(256) void ln_dwb_fold(int G, int C, const float* __restrict__ part, void* dw, void* db, int f32) {
-  __shared__ float sh[16][17];
+__global__ __launch_bounds__(1024) void ln_dwb_fold(int G, int C, const float* __restrict__ part, void* dw, void* db, int f32) {
+  __shared__ float sh[64][17];
   const int col = threadIdx.x & 15, gl = threadIdx.x >> 4;
   const int k = blockIdx.x * 16 + col;
   float s = 0.f;
-  if (k < 2 * C)
-    for (int g = gl; g < G; g += 16) s += part[(long)g * 2 * C + k];
+  if (k < 2 * C) {
+    int g = gl;
+    for (; g + 192 < G; g += 256) {           // four loads in flight
+      float t[4];
+#pragma unroll
+      for (int q = 0; q < 4; ++q) t[q] = part[(long)(g + 64 * q) * 2 * C + k];
+#pragma unroll
+      for (int q = 0; q < 4; ++q) s += t[q];
+    }
+    for (; g < G; g += 64) s += part[(long)g * 2 * C + k];
+  }
   sh[gl][col] = s;
   __syncthreads();
   if (gl != 0 || k >= 2 * C) return;
-#pragma unroll
-  for (int q = 1; q < 16; ++q) s += sh[q][col];
+  s = 0.f;
+#pragma unroll 16
+  for (int q = 0; q < 64; ++q) s += sh[q][col];
   void* out = k < C ? dw : db;
   if (out == nullptr) return;
   const int c = k < C ? k : k - C;
@@ -538,7 +586,9 @@ struct LnShape { int lanes, nv, threads, tsv; int groups; long tiles; };
 LnShape ln_rows_shape(int dtype, long R, int C) {
   LnShape s = {0, 0, 256, 0, 1, 0};
   const int v = dtype == PXL_F32 ? 4 : 8, pieces = (C + v - 1) / v;
-  if (pieces <= 256) {
+  if (C < v) {
+    s.lanes = 0;                          // shorter than a piece
+  } else if (pieces <= 256) {
     s.lanes = 8;
     while (s.lanes < 64 && s.lanes < pieces) s.lanes *= 2;
     s.nv = pieces <= s.lanes ? 1 : (pieces <= 2 * s.lanes ? 2 : 4);
@@ -548,7 +598,8 @@ LnShape ln_rows_shape(int dtype, long R, int C) {
   }
   if (s.lanes) {
     const long passes = (R + 256 / s.lanes - 1) / (256 / s.lanes);
-    s.groups = (int)(passes < 1 ? 1 : (passes > 512 ? 512 : passes));
+    const long each = (passes + 511) / 512;
+    s.groups = (int)(passes < 1 ? 1 : (passes + each - 1) / each);
   } else {
     const long g = (R + 63) / 64;
     s.groups = (int)(g < 1 ? 1 : (g > 256 ? 256 : g));
@@ -556,21 +607,26 @@ LnShape ln_rows_shape(int dtype, long R, int C) {
   return s;
 }
 LnShape ln_chan_shape(int dtype, long N, int C, long S) {
-  LnShape s = {0, 0, 256, 8, 1, 0};
-  if (C <= 256) {
+  LnShape s = {0, 0, 512, 16, 1, 0};
+  const int v = dtype == PXL_F32 ? 4 : 8;
+  if (S < v || S >= (1l << 22)) {
+    s.nv = 0;                             // shorter than a piece; a lane's offsets past 32 bits
+  } else if (C <= 256) {
     s.nv = C <= 32 ? 1 : (C <= 64 ? 2 : (C <= 128 ? 4 : 8));
   } else if (C <= 2048) {
-    s.threads = 512;
     s.tsv = C <= 512 ? 8 : 4;
     s.nv = C <= 1024 ? 8 : 16;
   }
   if (s.nv) {
-    const int ts = s.tsv * (dtype == PXL_F32 ? 4 : 8);
+    const int ts = s.tsv * v;
     s.lanes = s.tsv;
     s.tiles = N * ((S + ts - 1) / ts);
-    const long most = s.threads == 256 ? 1024 : 512;
     if (s.tiles >= (1l << 30)) s.lanes = s.nv = 0;
-    s.groups = (int)(s.tiles < 1 ? 1 : (s.tiles > most ? most : s.tiles));
+    // partial sums of at most 8 MB or 512 workgroups, the tiles spread evenly
+    long most = (1l << 20) / C;
+    if (most < 512) most = 512;
+    const long each = (s.tiles + most - 1) / most;
+    s.groups = (int)(s.tiles < 1 ? 1 : (s.tiles + each - 1) / each);
   }
   if (!s.nv) {
     const long g = (N * S + 63) / 64;
@@ -580,28 +636,33 @@ LnShape ln_chan_shape(int dtype, long N, int C, long S) {
 }
 inline LnShape ln_shape(int dtype, long R, int C, long S) { return S < 0 ? ln_rows_shape(dtype, R, C) : ln_chan_shape(dtype, S > 0 ? R / S : 0, C, S); }
 
+#define LN_ROWS_TAIL(KERNEL, L, N, ...)                                                                                \
+  do {                                                                                                                 \
+    if (C % (16 / (int)sizeof(T))) hipLaunchKernelGGL((KERNEL<T, L, N, true>), grid, dim3(256), 0, st, __VA_ARGS__);   \
+    else hipLaunchKernelGGL((KERNEL<T, L, N, false>), grid, dim3(256), 0, st, __VA_ARGS__);                            \
+  } while (0)
 #define LN_ROWS(KERNEL, BLOCKS, ...)                                                                                   \
   do {                                                                                                                 \
     const dim3 grid(BLOCKS);                                                                                           \
     const int key = s.lanes * 16 + s.nv;                                                                               \
-    if (key == 8 * 16 + 1) hipLaunchKernelGGL((KERNEL<T, 8, 1>), grid, dim3(256), 0, st, __VA_ARGS__);                 \
-    else if (key == 16 * 16 + 1) hipLaunchKernelGGL((KERNEL<T, 16, 1>), grid, dim3(256), 0, st, __VA_ARGS__);          \
-    else if (key == 32 * 16 + 1) hipLaunchKernelGGL((KERNEL<T, 32, 1>), grid, dim3(256), 0, st, __VA_ARGS__);          \
-    else if (key == 64 * 16 + 1) hipLaunchKernelGGL((KERNEL<T, 64, 1>), grid, dim3(256), 0, st, __VA_ARGS__);          \
-    else if (key == 64 * 16 + 2) hipLaunchKernelGGL((KERNEL<T, 64, 2>), grid, dim3(256), 0, st, __VA_ARGS__);          \
-    else if (key == 64 * 16 + 4) hipLaunchKernelGGL((KERNEL<T, 64, 4>), grid, dim3(256), 0, st, __VA_ARGS__);          \
-    else if (key == 256 * 16 + 2) hipLaunchKernelGGL((KERNEL<T, 256, 2>), grid, dim3(256), 0, st, __VA_ARGS__);        \
-    else if (key == 256 * 16 + 4) hipLaunchKernelGGL((KERNEL<T, 256, 4>), grid, dim3(256), 0, st, __VA_ARGS__);        \
-    else if constexpr (sizeof(T) == 4) hipLaunchKernelGGL((KERNEL<T, 256, 8>), grid, dim3(256), 0, st, __VA_ARGS__);   \
+    if (key == 8 * 16 + 1) LN_ROWS_TAIL(KERNEL, 8, 1, __VA_ARGS__);                                                    \
+    else if (key == 16 * 16 + 1) LN_ROWS_TAIL(KERNEL, 16, 1, __VA_ARGS__);                                             \
+    else if (key == 32 * 16 + 1) LN_ROWS_TAIL(KERNEL, 32, 1, __VA_ARGS__);                                             \
+    else if (key == 64 * 16 + 1) LN_ROWS_TAIL(KERNEL, 64, 1, __VA_ARGS__);                                             \
+    else if (key == 64 * 16 + 2) LN_ROWS_TAIL(KERNEL, 64, 2, __VA_ARGS__);                                             \
+    else if (key == 64 * 16 + 4) LN_ROWS_TAIL(KERNEL, 64, 4, __VA_ARGS__);                                             \
+    else if (key == 256 * 16 + 2) LN_ROWS_TAIL(KERNEL, 256, 2, __VA_ARGS__);                                           \
+    else if (key == 256 * 16 + 4) LN_ROWS_TAIL(KERNEL, 256, 4, __VA_ARGS__);                                           \
+    else if constexpr (sizeof(T) == 4) LN_ROWS_TAIL(KERNEL, 256, 8, __VA_ARGS__);                                      \
   } while (0)
 #define LN_CHAN(KERNEL, BLOCKS, ...)                                                                                                 \
   do {                                                                                                                               \
     const dim3 grid(BLOCKS);                                                                                                         \
-    if (s.threads == 256) {                                                                                                          \
-      if (s.nv == 1) hipLaunchKernelGGL((KERNEL<T, 256, 8, 1>), grid, dim3(256), 0, st, __VA_ARGS__);                                \
-      else if (s.nv == 2) hipLaunchKernelGGL((KERNEL<T, 256, 8, 2>), grid, dim3(256), 0, st, __VA_ARGS__);                           \
-      else if (s.nv == 4) hipLaunchKernelGGL((KERNEL<T, 256, 8, 4>), grid, dim3(256), 0, st, __VA_ARGS__);                           \
-      else hipLaunchKernelGGL((KERNEL<T, 256, 8, 8>), grid, dim3(256), 0, st, __VA_ARGS__);                                          \
+    if (s.tsv == 16) {                                                                                                               \
+      if (s.nv == 1) hipLaunchKernelGGL((KERNEL<T, 512, 16, 1>), grid, dim3(512), 0, st, __VA_ARGS__);                               \
+      else if (s.nv == 2) hipLaunchKernelGGL((KERNEL<T, 512, 16, 2>), grid, dim3(512), 0, st, __VA_ARGS__);                          \
+      else if (s.nv == 4) hipLaunchKernelGGL((KERNEL<T, 512, 16, 4>), grid, dim3(512), 0, st, __VA_ARGS__);                          \
+      else hipLaunchKernelGGL((KERNEL<T, 512, 16, 8>), grid, dim3(512), 0, st, __VA_ARGS__);                                         \
     } else if (s.tsv == 8) hipLaunchKernelGGL((KERNEL<T, 512, 8, 8>), grid, dim3(512), 0, st, __VA_ARGS__);                          \
     else if (s.nv == 8) hipLaunchKernelGGL((KERNEL<T, 512, 4, 8>), grid, dim3(512), 0, st, __VA_ARGS__);                             \
     else hipLaunchKernelGGL((KERNEL<T, 512, 4, 16>), grid, dim3(512), 0, st, __VA_ARGS__);                                           \
@@ -612,14 +673,14 @@ int ln_fwd(long R, int C, long S, long xs, const void* x, LnParam w, LnParam b, 
   const LnShape s = ln_shape(Elem<T>::DTYPE, R, C, S);
   if (S < 0) {
     if (s.lanes) {
-      const long passes = (R + 256 / s.lanes - 1) / (256 / s.lanes);
-      LN_ROWS(ln_rows_fwd, blocks_for(passes, 2048), R, C, xs, (const T*)x, w, b, eps, (T*)y, mean, rstd);
+      const long passes = (R + 256 / s.lanes - 1) / (256 / s.lanes), each = (passes + 2047) / 2048;      // evenly over the workgroups
+      LN_ROWS(ln_rows_fwd, blocks_for((passes + each - 1) / each, 2048), R, C, xs, (const T*)x, w, b, eps, (T*)y, mean, rstd);
     } else {
       hipLaunchKernelGGL(ln_rows_fwd_loop<T>, dim3(blocks_for(R, 1 << 20)), dim3(256), 0, st, R, C, xs, (const T*)x, w, b, eps, (T*)y, mean, rstd);
     }
   } else if (s.lanes) {
     const int per = (int)(s.tiles / (R / S));
-    LN_CHAN(ln_chan_fwd, (unsigned)s.tiles, (int)s.tiles, per, C, S, (const T*)x, w, b, eps, (T*)y, mean, rstd);
+    LN_CHAN(ln_chan_fwd, (unsigned)s.tiles, (int)s.tiles, per, C, (int)S, (const T*)x, w, b, eps, (T*)y, mean, rstd);
   } else {
     hipLaunchKernelGGL(ln_chan_fwd_loop<T>, dim3(blocks_for((R + 255) / 256, 1 << 20)), dim3(256), 0, st, R, C, S, (const T*)x, w, b, eps,
                        (T*)y, mean, rstd);
@@ -640,7 +701,7 @@ int ln_bwd(long R, int C, long S, long xs, const void* x, const void* dy, LnPara
       LN_ROWS(ln_rows_bwd, (unsigned)G, R, C, xs, (const T*)x, (const T*)dy, w, mean, rstd, (T*)dx, p);
     } else {
       const int per = (int)(s.tiles / (R / S));
-      LN_CHAN(ln_chan_bwd, (unsigned)G, (int)s.tiles, per, C, S, (const T*)x, (const T*)dy, w, mean, rstd, (T*)dx, p);
+      LN_CHAN(ln_chan_bwd, (unsigned)G, (int)s.tiles, per, C, (int)S, (const T*)x, (const T*)dy, w, mean, rstd, (T*)dx, p);
     }
     PXL_LAUNCH_CHECK();
   } else if (R > 0) {
@@ -661,7 +722,7 @@ int ln_bwd(long R, int C, long S, long xs, const void* x, const void* dy, LnPara
     }
   }
   if (params) {
-    hipLaunchKernelGGL(ln_dwb_fold<T>, dim3((2 * C + 15) / 16), dim3(256), 0, st, R > 0 ? G : 0, C, part, dw, db, pf32);
+    hipLaunchKernelGGL(ln_dwb_fold<T>, dim3((2 * C + 15) / 16), dim3(1024), 0, st, R > 0 ? G : 0, C, part, dw, db, pf32);
     PXL_LAUNCH_CHECK();
   }
   return PXL_OK;
