@@ -39,6 +39,26 @@ constexpr int NS_PARTS = 1024;          // partial sums of squares per matrix at
 // one matrix, in device memory
 struct NsItem { void* p; const void* g; float* mom; float scale; int pad; };
 struct NsTable { NsItem it[NS_TABLE]; };
+// up to 16 of them travel in the kernel arguments of the three kernels that need them: no table launch
+constexpr int NS_INLINE = 16;
+struct NsInline { NsItem it[NS_INLINE]; };
+__device__ __forceinline__ NsItem ns_item(const NsInline& few, const NsItem* table, int i) { return table != nullptr ? table[i] : few.it[i]; }
+
+typedef short s16x4 __attribute__((ext_vector_type(4)));
+typedef __attribute__((address_space(3))) s16x4 lds_s16x4;
+
+// four elements at any element alignment
+__device__ __forceinline__ void load4(const float* p, float* v) { __builtin_memcpy(v, p, 16); }
+__device__ __forceinline__ void load4(const bf16_t* p, float* v) {
+  uint2 w;
+  __builtin_memcpy(&w, p, 8);
+  v[0] = bf_lo(w.x); v[1] = bf_hi(w.x); v[2] = bf_lo(w.y); v[3] = bf_hi(w.y);
+}
+__device__ __forceinline__ void store4(float* p, const float* v) { __builtin_memcpy(p, v, 16); }
+__device__ __forceinline__ void store4(bf16_t* p, const float* v) {
+  const uint2 w = make_uint2(pack_bf2(v[0], v[1]), pack_bf2(v[2], v[3]));
+  __builtin_memcpy(p, &w, 8);
+}
 
 // matrices of one shape, in kernel arguments.  Offsets in bytes from the workspace; the matrices of a class lie `stride` apart.
 struct NsClass {
@@ -46,7 +66,7 @@ struct NsClass {
   int rows, cols, m, n, mp, np;         // mp / np: m / n rounded up (zero padding)
   int start, per;                       // first workgroup and workgroups per matrix of THIS launch
   int chunk, parts;                     // norm pass: elements per workgroup, workgroups per matrix
-  int tn, pad;                          // tiles across (this launch)
+  int tn, ks;                           // tiles across (this launch); split products: K steps of 32 a share
   size_t base, stride;
 };
 struct NsClasses { NsClass c[NS_MAX_CLASSES]; int n; };
@@ -71,16 +91,33 @@ __device__ __forceinline__ float muon_update(float m, float g, const MuonArgs& a
 
 // ---- pass 1: momentum, partial sums of squares (in 64 bits: squares of any fp32 value fit) -----------------------------------
 template <typename T>
-__global__ __launch_bounds__(256) void ns_norm_kernel(NsClasses cs, const NsItem* __restrict__ table, double* __restrict__ part, MuonArgs a) {
+__global__ __launch_bounds__(256) void ns_norm_kernel(NsClasses cs, NsInline few, const NsItem* __restrict__ table, double* __restrict__ part, MuonArgs a) {
   __shared__ double sh[4];
   const int k = find_class(cs, blockIdx.x);
   const NsClass& c = cs.c[k];
   const int local = blockIdx.x - c.start, i = local / c.per, j = local - i * c.per;
-  const NsItem it = table[c.first + i];
+  const NsItem it = ns_item(few, table, c.first + i);
   const long size = (long)c.rows * c.cols, lo = (long)j * c.chunk, hi = lo + c.chunk < size ? lo + c.chunk : size;
   const T* g = reinterpret_cast<const T*>(it.g);
   double s = 0.0;
-  for (long e = lo + threadIdx.x; e < hi; e += 256) {
+  long e = lo + threadIdx.x * 4;
+  for (; e + 4 <= hi; e += 1024) {
+    float u[4];
+    load4(g + e, u);
+    if (it.mom != nullptr) {
+      float m[4];
+      load4(it.mom + e, m);
+#pragma unroll
+      for (int q = 0; q < 4; ++q) {
+        m[q] = muon_momentum(m[q], u[q], a);
+        u[q] = muon_update(m[q], u[q], a);
+      }
+      store4(it.mom + e, m);
+    }
+#pragma unroll
+    for (int q = 0; q < 4; ++q) s += (double)u[q] * u[q];
+  }
+  for (; e < hi; ++e) {                  // the one thread whose four pass the end
     float u = to_f(g[e]);
     if (it.mom != nullptr) {
       const float m = muon_momentum(it.mom[e], u, a);
@@ -96,19 +133,18 @@ __global__ __launch_bounds__(256) void ns_norm_kernel(NsClasses cs, const NsItem
   if (threadIdx.x == 0) part[(long)(c.first + i) * NS_PARTS + j] = (sh[0] + sh[1]) + (sh[2] + sh[3]);
 }
 
-// ---- pass 2: scaled fp16 planes of X in both layouts: Xk [mp][np], Xt [np][mp] ------------------------------------------------
+// ---- pass 2: scaled fp16 planes of X [mp][np] (the smaller side first whatever the matrix is) ---------------------------------
 // residue[i]: what X's entries are still to be multiplied by (1 with two planes)
 template <typename T, int NP>
-__global__ __launch_bounds__(256) void ns_split_kernel(NsClasses cs, const NsItem* __restrict__ table, const double* __restrict__ part,
-                                                       float* __restrict__ residue, unsigned char* __restrict__ ws, size_t off_k, size_t off_t,
-                                                       float eps, float sx, MuonArgs a) {
+__global__ __launch_bounds__(256) void ns_split_kernel(NsClasses cs, NsInline few, const NsItem* __restrict__ table, const double* __restrict__ part,
+                                                       float* __restrict__ residue, unsigned char* __restrict__ ws, float eps, float sx, MuonArgs a) {
   __shared__ double shn[4];
   __shared__ float tile[64][65];
   const int k = find_class(cs, blockIdx.x);
   const NsClass& c = cs.c[k];
   const int local = blockIdx.x - c.start, i = local / c.per, t = local - i * c.per;
   const int tr = t / c.tn, tc = t - tr * c.tn;             // 64 x 64 tile of [mp][np]
-  const NsItem it = table[c.first + i];
+  const NsItem it = ns_item(few, table, c.first + i);
   double s = 0.0;
   for (int e = threadIdx.x; e < c.parts; e += 256) s += part[(long)(c.first + i) * NS_PARTS + e];
 #pragma unroll
@@ -131,68 +167,82 @@ __global__ __launch_bounds__(256) void ns_split_kernel(NsClasses cs, const NsIte
   if (t == 0 && threadIdx.x == 0) residue[c.first + i] = left;
   const T* g = reinterpret_cast<const T*>(it.g);
   const bool tall = c.rows > c.cols;
-  // tile[r][q]: r along m, q along n; read along the memory's rows
-  for (int e = threadIdx.x; e < 4096; e += 256) {
-    const int hi = e >> 6, lo = e & 63;
-    const int r = tall ? lo : hi, q = tall ? hi : lo;
-    const int im = tr * 64 + r, in = tc * 64 + q;
-    float v = 0.f;
-    if (im < c.m && in < c.n) {
-      const long at = tall ? (long)in * c.cols + im : (long)im * c.cols + in;
-      v = to_f(g[at]);
-      if (it.mom != nullptr) v = muon_update(it.mom[at], v, a);
-      v = (float)((double)v * mul);
+  // tile[r][q]: r along m, q along n; read along the memory's rows, four elements a thread
+  const int lines = tall ? c.n : c.m, line0 = tall ? tc * 64 : tr * 64, col0 = tall ? tr * 64 : tc * 64;
+  const int col = col0 + (threadIdx.x & 15) * 4, l0 = threadIdx.x >> 4;
+#pragma unroll
+  for (int q = 0; q < 4; ++q) {
+    const int l = l0 + q * 16, line = line0 + l;
+    float v[4] = {0.f, 0.f, 0.f, 0.f};
+    if (line < lines) {
+      const long at = (long)line * c.cols + col;
+      if (col + 4 <= c.cols) {
+        load4(g + at, v);
+        if (it.mom != nullptr) {
+          float m[4];
+          load4(it.mom + at, m);
+#pragma unroll
+          for (int e = 0; e < 4; ++e) v[e] = muon_update(m[e], v[e], a);
+        }
+      } else {
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+          if (col + e < c.cols) {
+            v[e] = to_f(g[at + e]);
+            if (it.mom != nullptr) v[e] = muon_update(it.mom[at + e], v[e], a);
+          }
+      }
     }
-    tile[r][q] = v;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      const float x = (float)((double)v[e] * mul);
+      if (tall) tile[(threadIdx.x & 15) * 4 + e][l] = x;
+      else tile[l][(threadIdx.x & 15) * 4 + e] = x;
+    }
   }
   __syncthreads();
   unsigned char* base = ws + c.base + (size_t)i * c.stride;
-  const size_t plane = (size_t)c.mp * c.np * 2;
-  for (int e = threadIdx.x; e < 4096; e += 256) {
-    const int hi = e >> 6, lo = e & 63;
-    if (tr * 64 + hi < c.mp && tc * 64 + lo < c.np) {
-      const float v = tile[hi][lo];
-      const _Float16 h = (_Float16)v;
-      _Float16* d = reinterpret_cast<_Float16*>(base + off_k * plane) + (size_t)(tr * 64 + hi) * c.np + tc * 64 + lo;
-      d[0] = h;
-      if (NP == 2) d[plane / 2] = (_Float16)(v - (float)h);
+  const size_t plane = (size_t)c.mp * c.np;
+#pragma unroll
+  for (int q = 0; q < 4; ++q) {
+    const int r = l0 + q * 16, im = tr * 64 + r, in = tc * 64 + (threadIdx.x & 15) * 4;
+    if (im >= c.mp || in >= c.np) continue;
+    f16x4 h, l;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      const float v = tile[r][(threadIdx.x & 15) * 4 + e];
+      h[e] = (_Float16)v;
+      l[e] = (_Float16)(v - (float)h[e]);
     }
-    if (tc * 64 + hi < c.np && tr * 64 + lo < c.mp) {
-      const float v = tile[lo][hi];
-      const _Float16 h = (_Float16)v;
-      _Float16* d = reinterpret_cast<_Float16*>(base + off_t * plane) + (size_t)(tc * 64 + hi) * c.mp + tr * 64 + lo;
-      d[0] = h;
-      if (NP == 2) d[plane / 2] = (_Float16)(v - (float)h);
-    }
+    _Float16* d = reinterpret_cast<_Float16*>(base) + (size_t)im * c.np + in;
+    *reinterpret_cast<f16x4*>(d) = h;
+    if (NP == 2) *reinterpret_cast<f16x4*>(d + plane) = l;
   }
 }
 
-// ---- products: C[i][j] = sum_k a[i][k] b[j][k] over fp16 planes, both operands with k contiguous ------------------------------
-enum { EPI_GRAM = 0, EPI_Q = 1, EPI_MUL = 2, EPI_X = 3, EPI_OUT = 4 };
+// ---- products over fp16 planes ------------------------------------------------------------------------------------------------
+// GRAM, PART, Q, MUL: C[i][j] = sum_k a[i][k] b[j][k], symmetric: tiles on and below the diagonal, mirrored when stored
+// X, OUT:             C[i][j] = sum_k a[i][k] b[k][j]   (a = P, b = X)
+enum { EPI_GRAM = 0, EPI_PART = 1, EPI_Q = 2, EPI_MUL = 3, EPI_X = 4, EPI_OUT = 5 };
 
-// operand / result slots of a matrix's workspace region: X planes first (units of mp * np * 2 bytes), then m x m pairs of planes
-struct NsSlot { int x, mm; };           // x planes, then mm pairs
+// slots of a matrix's workspace region: X planes first (units of mp * np * 2 bytes), then m x m pairs of planes
 __device__ __forceinline__ size_t slot_off(const NsClass& c, int xplanes, int slot) {
   const size_t px = (size_t)c.mp * c.np * 2, pm = (size_t)c.mp * c.mp * 2;
   return slot < xplanes ? (size_t)slot * px : (size_t)xplanes * px + (size_t)(slot - xplanes) * 2 * pm;
 }
 
-struct NsJob { int a, b, out, out2; };  // slots
+struct NsJob { int a, b, out; };        // slots
 struct NsGemm {
-  NsJob job[2];
+  NsJob job;
   int xplanes;                          // X slots of a region
   float unscale, scale;                 // accumulator -> value, value -> planes
   float qa, qb, qc, sa_inv;             // EPI_Q: coefficients, 1 / scale of A's planes
-  int res_pow;                          // EPI_GRAM: value *= residue^2;  EPI_OUT / EPI_X: value *= residue
-  float lr, decay;                      // EPI_OUT of a Muon step
+  int res_pow;                          // GRAM: value *= residue^2;  OUT / X: value *= residue
+  float lr, decay;                      // OUT of a Muon step
   int muon;
+  float* part;                          // PART: [split][tile][T * T] accumulators
+  int splits;                           // PART: shares of K
 };
-
-__device__ __forceinline__ void put_split(_Float16* d, size_t plane, float v) {
-  const _Float16 h = (_Float16)v;
-  d[0] = h;
-  d[plane] = (_Float16)(v - (float)h);
-}
 
 // lower-triangular tile number t -> (row, column), row >= column
 __device__ __forceinline__ void tri_tile(int t, int& r, int& q) {
@@ -202,58 +252,119 @@ __device__ __forceinline__ void tri_tile(int t, int& r, int& q) {
   q = t - r * (r + 1) / 2;
 }
 
-// T x T tile per workgroup of 4 waves (2 x 2), K steps of 32, two LDS buffers; LDS rows of 64 bytes, 16-byte chunk c of row r at
-// c ^ ((r >> 2) & 3): the 16 lanes that read one chunk column in a phase then hit 16 different bank groups
-template <int EPI, int NA, int NB, int T, typename OutT>
-__global__ __launch_bounds__(256) void ns_gemm_kernel(NsClasses cs, NsGemm p, const NsItem* __restrict__ table, const float* __restrict__ residue,
-                                                      unsigned char* __restrict__ ws) {
-  constexpr bool SYM = EPI <= EPI_MUL;
+// accumulators of a symmetric product -> both planes of the result, the tile and its mirror image.  Accumulator element e of a
+// lane: row 8 (e / 4) + 4 (lane / 32) + e % 4, column lane % 32
+template <int EPI, int T>
+__device__ __forceinline__ void ns_store_sym(const NsClass& c, const NsGemm& p, const _Float16* A, _Float16* out, int tr, int tc, float un,
+                                             f32x16 (&acc)[T / 64][T / 64]) {
+  constexpr int W = T / 64;
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, wr = wave >> 1, wc = wave & 1;
+  const size_t pm = (size_t)c.mp * c.mp;
+#pragma unroll
+  for (int u = 0; u < W; ++u)
+#pragma unroll
+    for (int v = 0; v < W; ++v)
+#pragma unroll
+      for (int e4 = 0; e4 < 4; ++e4) {
+        const int r0 = tr * T + wr * (T / 2) + u * 32 + 8 * e4 + 4 * (lane >> 5);
+        const int q = tc * T + wc * (T / 2) + v * 32 + (lane & 31);
+        if (r0 >= c.mp || q >= c.mp) continue;                    // (mp is a multiple of 32)
+        f16x4 h, l;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          float val = acc[u][v][e4 * 4 + e] * un;
+          _Float16* d = out + (size_t)(r0 + e) * c.mp + q;
+          if (EPI == EPI_Q) {
+            const _Float16* am = A + (size_t)(r0 + e) * c.mp + q;
+            val = p.qc * val + p.qb * (((float)am[0] + (float)am[pm]) * p.sa_inv) + (r0 + e == q ? p.qa : 0.f);
+          }
+          const float x = val * p.scale;
+          h[e] = (_Float16)x;
+          l[e] = (_Float16)(x - (float)h[e]);
+          d[0] = h[e];
+          d[pm] = l[e];
+        }
+        if (tr != tc) {
+          _Float16* d = out + (size_t)q * c.mp + r0;
+          *reinterpret_cast<f16x4*>(d) = h;
+          *reinterpret_cast<f16x4*>(d + pm) = l;
+        }
+      }
+}
+
+// One T x T tile per workgroup of 4 waves (2 x 2), K steps of 32.  Global memory -> registers, D steps ahead -> LDS, two buffers, one
+// barrier a step.  LDS images: rows of 32 k (64 bytes), 16-byte chunk ch of row r at ch ^ ((r >> 2) & 3), for a and for b in [j][k]; rows of T
+// columns per k for b in [k][j], 32-byte segment at its number ^ swizzle(k), read with the transposing LDS load (within 16 lanes, lane j
+// receives 16-bit slot j % 4 of lanes j / 4 + 4 e): 4 k of one column.  Both are free of bank conflicts.
+template <int EPI, int NA, int NB, int T, int D, typename OutT>
+__global__ __launch_bounds__(256, 2) void ns_gemm_kernel(NsClasses cs, NsGemm p, NsInline few, const NsItem* __restrict__ table,
+                                                         const float* __restrict__ residue, unsigned char* __restrict__ ws) {
+  constexpr bool SYM = EPI <= EPI_MUL, NN = EPI >= EPI_X;
   constexpr int W = T / 64;                     // 32 x 32 accumulators per wave and direction
   constexpr int PL = T * 64;                    // bytes of one plane's tile
   constexpr int CH = T / 64;                    // 16-byte chunks a thread moves per plane
   __shared__ __attribute__((aligned(16))) unsigned char lds[2][(NA + NB) * PL];
-  const int k = find_class(cs, blockIdx.x);
+  const int bid = xcd_remap(blockIdx.x, gridDim.x);
+  const int k = find_class(cs, bid);
   const NsClass& c = cs.c[k];
-  const int local = blockIdx.x - c.start, i = local / c.per, t = local - i * c.per;
+  const int local = bid - c.start, i = local / c.per, t = local - i * c.per;
   int tr, tc;
   if (SYM) tri_tile(t, tr, tc);
   else { tr = t / c.tn; tc = t - tr * c.tn; }
-  const NsJob job = p.job[blockIdx.z];
   unsigned char* base = ws + c.base + (size_t)i * c.stride;
-  const bool xa = EPI == EPI_GRAM;              // operands: the X planes, or m x m pairs
-  const int K = xa ? c.np : c.mp;
-  const int rowsA = c.mp, rowsB = EPI >= EPI_X ? c.np : c.mp;
-  const size_t plane_a = (size_t)rowsA * K, plane_b = (size_t)rowsB * K;
-  const _Float16* A = reinterpret_cast<const _Float16*>(base + slot_off(c, p.xplanes, job.a));
-  const _Float16* B = reinterpret_cast<const _Float16*>(base + slot_off(c, p.xplanes, job.b));
+  const int K = EPI <= EPI_PART ? c.np : c.mp;
+  const int rowsB = c.mp;
+  const size_t plane_a = (size_t)c.mp * K, plane_b = NN ? (size_t)c.mp * c.np : (size_t)c.mp * K;
+  const _Float16* A = reinterpret_cast<const _Float16*>(base + slot_off(c, p.xplanes, p.job.a));
+  const _Float16* B = reinterpret_cast<const _Float16*>(base + slot_off(c, p.xplanes, p.job.b));
 
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, wr = wave >> 1, wc = wave & 1;
-  u32x4 ra[NA][CH], rb[NB][CH];
-  auto fetch = [&](int k0) {
+  int s0 = 0, steps = K >> 5;
+  if (EPI == EPI_PART) {
+    s0 = blockIdx.y * c.ks;
+    steps = steps - s0 < c.ks ? steps - s0 : c.ks;
+    if (steps <= 0) return;                     // (shapes with fewer shares than the grid has: never read)
+  }
+  // byte offsets of a thread's chunks from the tile's first element, and where they go in LDS
+  unsigned oa[CH], ob[CH];
+  int la[CH], lb[CH];
+#pragma unroll
+  for (int q = 0; q < CH; ++q) {
+    const int e = tid + q * 256, r = e >> 2, ch = e & 3;
+    const int ia = tr * T + r < c.mp ? r : c.mp - 1 - tr * T;      // rows past the matrix: the last one again (never stored; tr * T < mp)
+    oa[q] = (unsigned)(ia * K + ch * 8) * 2u;
+    la[q] = r * 64 + ((ch ^ ((r >> 2) & 3)) << 4);
+    if (NN) {
+      const int kr = e / (T / 8), cc = e % (T / 8);
+      const int col = tc * T + cc * 8 < c.np ? cc * 8 : 0;         // chunks past the matrix: the tile's first again (never stored)
+      ob[q] = (unsigned)(kr * c.np + col) * 2u;
+      const int swz = T == 128 ? kr & 3 : (kr >> 1) & 1;
+      lb[q] = kr * (T * 2) + (((cc >> 1) ^ swz) << 5) + ((cc & 1) << 4);
+    } else {
+      const int ib = tc * T + r < rowsB ? r : rowsB - 1 - tc * T;
+      ob[q] = (unsigned)(ib * K + ch * 8) * 2u;
+      lb[q] = la[q];
+    }
+  }
+  const unsigned char* pa = reinterpret_cast<const unsigned char*>(A + (size_t)tr * T * K + (size_t)s0 * 32);
+  const unsigned char* pb = reinterpret_cast<const unsigned char*>(NN ? B + (size_t)s0 * 32 * c.np + tc * T : B + (size_t)tc * T * K + (size_t)s0 * 32);
+  const size_t step_b = NN ? (size_t)64 * c.np : 64;
+  // (buffer loads: the base that moves stays in scalar registers; offsets below 2^31, a row is at most 2^24 bytes and a tile 128 rows)
+  auto window = [](const unsigned char* at) { return __builtin_amdgcn_make_buffer_rsrc((void*)at, 0, 0x7fffffff, 0x00020000); };
+  u32x4 ra[D][NA][CH], rb[D][NB][CH];
+  int fetched = 0;
+  auto fetch = [&](int slot) {
 #pragma unroll
     for (int q = 0; q < CH; ++q) {
-      const int e = tid + q * 256, r = e >> 2, ch = e & 3;
-      int ia = tr * T + r, ib = tc * T + r;     // rows past the matrix: the last one again (never stored)
-      if (ia >= rowsA) ia = rowsA - 1;
-      if (ib >= rowsB) ib = rowsB - 1;
-      const _Float16* pa = A + (size_t)ia * K + k0 + ch * 8;
-      const _Float16* pb = B + (size_t)ib * K + k0 + ch * 8;
 #pragma unroll
-      for (int z = 0; z < NA; ++z) ra[z][q] = *reinterpret_cast<const u32x4*>(pa + z * plane_a);
+      for (int z = 0; z < NA; ++z) ra[slot][z][q] = __builtin_amdgcn_raw_buffer_load_b128(window(pa + z * plane_a * 2), (int)oa[q], 0, 0);
 #pragma unroll
-      for (int z = 0; z < NB; ++z) rb[z][q] = *reinterpret_cast<const u32x4*>(pb + z * plane_b);
+      for (int z = 0; z < NB; ++z) rb[slot][z][q] = __builtin_amdgcn_raw_buffer_load_b128(window(pb + z * plane_b * 2), (int)ob[q], 0, 0);
     }
-  };
-  auto stash = [&](int buf) {
-#pragma unroll
-    for (int q = 0; q < CH; ++q) {
-      const int e = tid + q * 256, r = e >> 2, ch = e & 3;
-      const int at = r * 64 + ((ch ^ ((r >> 2) & 3)) << 4);
-#pragma unroll
-      for (int z = 0; z < NA; ++z) *reinterpret_cast<u32x4*>(&lds[buf][z * PL + at]) = ra[z][q];
-#pragma unroll
-      for (int z = 0; z < NB; ++z) *reinterpret_cast<u32x4*>(&lds[buf][(NA + z) * PL + at]) = rb[z][q];
-    }
+    // (past the last step: that one again, in bounds and unused -- a fetch under a condition would make every wait one for all loads)
+    const bool more = ++fetched < steps;
+    pa += more ? 64 : 0;
+    pb += more ? step_b : 0;
   };
   f32x16 acc[W][W];
 #pragma unroll
@@ -263,13 +374,22 @@ __global__ __launch_bounds__(256) void ns_gemm_kernel(NsClasses cs, NsGemm p, co
 #pragma unroll
       for (int e = 0; e < 16; ++e) acc[u][v][e] = 0.f;
 
-  fetch(0);
-  stash(0);
-  __syncthreads();
-  const int steps = K >> 5;
-  for (int s = 0; s < steps; ++s) {
-    if (s + 1 < steps) fetch((s + 1) << 5);
-    const unsigned char* buf = lds[s & 1];
+#pragma unroll
+  for (int d = 0; d < D; ++d) {
+    fetch(d);
+    __builtin_amdgcn_sched_barrier(0);          // (in this order: the waits count)
+  }
+  auto step = [&](int s, int slot) {
+    unsigned char* buf = lds[s & 1];
+#pragma unroll
+    for (int q = 0; q < CH; ++q) {
+#pragma unroll
+      for (int z = 0; z < NA; ++z) *reinterpret_cast<u32x4*>(buf + z * PL + la[q]) = ra[slot][z][q];
+#pragma unroll
+      for (int z = 0; z < NB; ++z) *reinterpret_cast<u32x4*>(buf + (NA + z) * PL + lb[q]) = rb[slot][z][q];
+    }
+    fetch(slot);
+    __syncthreads();
 #pragma unroll
     for (int kk = 0; kk < 2; ++kk) {
       f16x8 fa[NA][W], fb[NB][W];
@@ -280,105 +400,207 @@ __global__ __launch_bounds__(256) void ns_gemm_kernel(NsClasses cs, NsGemm p, co
 #pragma unroll
         for (int z = 0; z < NA; ++z) fa[z][u] = *reinterpret_cast<const f16x8*>(buf + z * PL + r * 64 + ((ch ^ ((r >> 2) & 3)) << 4));
 #pragma unroll
-        for (int z = 0; z < NB; ++z) fb[z][u] = *reinterpret_cast<const f16x8*>(buf + (NA + z) * PL + q * 64 + ((ch ^ ((q >> 2) & 3)) << 4));
+        for (int z = 0; z < NB; ++z) {
+          if (NN) {
+            // lanes 0-15 / 16-31: columns 0-15 / 16-31 of this 32, k 0-7; lanes 32-63: the same columns, k 8-15
+            f16x4 half[2];
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+              const int kr = kk * 16 + 8 * (lane >> 5) + 4 * h + ((lane & 15) >> 2);
+              const int seg = (wc * (T / 2) + u * 32) / 16 + ((lane >> 4) & 1);
+              const int swz = T == 128 ? kr & 3 : (kr >> 1) & 1;
+              half[h] = __builtin_bit_cast(f16x4, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)(
+                  buf + (NA + z) * PL + kr * (T * 2) + ((seg ^ swz) << 5) + ((lane & 3) << 3))));
+            }
+            fb[z][u] = __builtin_shufflevector(half[0], half[1], 0, 1, 2, 3, 4, 5, 6, 7);
+          } else {
+            fb[z][u] = *reinterpret_cast<const f16x8*>(buf + (NA + z) * PL + q * 64 + ((ch ^ ((q >> 2) & 3)) << 4));
+          }
+        }
       }
+      // X: the operands the other way round, so that a lane holds four consecutive columns of one row of the result
+#define NS_MFMA(A_, B_, C_) (EPI == EPI_X ? __builtin_amdgcn_mfma_f32_32x32x16_f16(B_, A_, C_, 0, 0, 0) : __builtin_amdgcn_mfma_f32_32x32x16_f16(A_, B_, C_, 0, 0, 0))
 #pragma unroll
       for (int u = 0; u < W; ++u)
 #pragma unroll
         for (int v = 0; v < W; ++v) {
-          if (NB == 2) acc[u][v] = __builtin_amdgcn_mfma_f32_32x32x16_f16(fa[0][u], fb[NB - 1][v], acc[u][v], 0, 0, 0);
-          if (NA == 2) acc[u][v] = __builtin_amdgcn_mfma_f32_32x32x16_f16(fa[NA - 1][u], fb[0][v], acc[u][v], 0, 0, 0);
-          acc[u][v] = __builtin_amdgcn_mfma_f32_32x32x16_f16(fa[0][u], fb[0][v], acc[u][v], 0, 0, 0);
+          if (NB == 2) acc[u][v] = NS_MFMA(fa[0][u], fb[NB - 1][v], acc[u][v]);
+          if (NA == 2) acc[u][v] = NS_MFMA(fa[NA - 1][u], fb[0][v], acc[u][v]);
+          acc[u][v] = NS_MFMA(fa[0][u], fb[0][v], acc[u][v]);
         }
+#undef NS_MFMA
     }
-    if (s + 1 < steps) stash((s + 1) & 1);
-    __syncthreads();
+  };
+  int s = 0;
+  for (; s + D <= steps; s += D) {
+#pragma unroll
+    for (int d = 0; d < D; ++d) step(s + d, d);
   }
+#pragma unroll
+  for (int d = 0; d < D - 1; ++d)
+    if (s + d < steps) step(s + d, d);
 
-  // accumulator element e of lane: row 8 (e / 4) + 4 (lane / 32) + e % 4, column lane % 32
-  const float res = EPI == EPI_Q || EPI == EPI_MUL ? 1.f : (p.res_pow == 0 ? 1.f : (p.res_pow == 2 ? residue[c.first + i] * residue[c.first + i] : residue[c.first + i]));
-  const float un = p.unscale * res;
-  const size_t pm = (size_t)c.mp * c.mp, px = (size_t)c.mp * c.np;
-  _Float16* out = reinterpret_cast<_Float16*>(base + slot_off(c, p.xplanes, job.out));
-  _Float16* out2 = reinterpret_cast<_Float16*>(base + slot_off(c, p.xplanes, job.out2));
-  const NsItem it = table[c.first + i];
-  const bool tall = c.rows > c.cols;
+  if (EPI == EPI_PART) {
+    // accumulators as they lie in the registers: the pass that adds the splits has the same lanes
+    float* o = p.part + ((size_t)blockIdx.y * gridDim.x + bid) * (T * T) + tid;
+#pragma unroll
+    for (int u = 0; u < W; ++u)
+#pragma unroll
+      for (int v = 0; v < W; ++v)
+#pragma unroll
+        for (int e = 0; e < 16; ++e) o[((u * W + v) * 16 + e) * 256] = acc[u][v][e];
+    return;
+  }
+  const float rs = residue[c.first + i];
+  const float un = p.unscale * (p.res_pow == 0 ? 1.f : (p.res_pow == 2 ? rs * rs : rs));
+  _Float16* out = reinterpret_cast<_Float16*>(base + slot_off(c, p.xplanes, p.job.out));
+  if constexpr (SYM) {
+    ns_store_sym<EPI, T>(c, p, A, out, tr, tc, un, acc);
+  } else if constexpr (EPI == EPI_X) {
+    // through LDS, one plane after the other: rows of T columns, 16-byte stores.  Lane: row lane % 32, columns 8 e4 + 4 (lane / 32) + 0 .. 3
+    constexpr int PITCH = T + 8;
+    _Float16* stage = reinterpret_cast<_Float16*>(&lds[0][0]);
+    static_assert(sizeof(lds) >= (size_t)T * PITCH * 2, "a plane's tile fits");
+    const size_t px = (size_t)c.mp * c.np;
+#pragma unroll
+    for (int z = 0; z < NB; ++z) {
+      __syncthreads();
+#pragma unroll
+      for (int u = 0; u < W; ++u)
+#pragma unroll
+        for (int v = 0; v < W; ++v)
+#pragma unroll
+          for (int e4 = 0; e4 < 4; ++e4) {
+            f16x4 h;
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+              const float x = acc[u][v][e4 * 4 + e] * un * p.scale;
+              h[e] = (_Float16)x;
+              if (z == 1) h[e] = (_Float16)(x - (float)h[e]);
+            }
+            *reinterpret_cast<f16x4*>(stage + (wr * (T / 2) + u * 32 + (lane & 31)) * PITCH + wc * (T / 2) + v * 32 + 8 * e4 + 4 * (lane >> 5)) = h;
+          }
+      __syncthreads();
+#pragma unroll
+      for (int q = 0; q < T * T / 8 / 256; ++q) {
+        const int e = tid + q * 256, r = e / (T / 8), cc = e % (T / 8) * 8;
+        if (tr * T + r < c.mp && tc * T + cc < c.np)
+          *reinterpret_cast<u32x4*>(out + z * px + (size_t)(tr * T + r) * c.np + tc * T + cc) = *reinterpret_cast<const u32x4*>(stage + r * PITCH + cc);
+      }
+    }
+  } else {
+    const NsItem it = ns_item(few, table, c.first + i);
+    const bool tall = c.rows > c.cols;
+    const float f = p.muon ? -p.lr * it.scale : 1.f;
+#pragma unroll
+    for (int u = 0; u < W; ++u)
+#pragma unroll
+      for (int v = 0; v < W; ++v)
+#pragma unroll
+        for (int e4 = 0; e4 < 4; ++e4) {
+          const int r0 = tr * T + wr * (T / 2) + u * 32 + 8 * e4 + 4 * (lane >> 5);
+          const int q = tc * T + wc * (T / 2) + v * 32 + (lane & 31);
+          if (r0 >= c.m || q >= c.n) continue;
+          float val[4];
+#pragma unroll
+          for (int e = 0; e < 4; ++e) val[e] = acc[u][v][e4 * 4 + e] * un * f;
+          OutT* o = reinterpret_cast<OutT*>(it.p) + (tall ? (size_t)q * c.cols + r0 : (size_t)r0 * c.cols + q);
+          if (tall && r0 + 4 <= c.m) {
+            float old[4];
+            if (p.muon) {
+              load4(o, old);
+#pragma unroll
+              for (int e = 0; e < 4; ++e) val[e] += old[e] * p.decay;
+            }
+            store4(o, val);
+          } else {
+            const size_t ld = tall ? 1 : c.cols;
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+              if (r0 + e < c.m) o[e * ld] = from_f<OutT>(p.muon ? to_f(o[e * ld]) * p.decay + val[e] : val[e]);
+          }
+        }
+  }
+}
+
+// sums of a split Gram product, in the order of the splits -> A
+template <int T>
+__global__ __launch_bounds__(256) void ns_fold_kernel(NsClasses cs, NsGemm p, const float* __restrict__ residue, unsigned char* __restrict__ ws) {
+  constexpr int W = T / 64;
+  const int bid = blockIdx.x;
+  const int k = find_class(cs, bid);
+  const NsClass& c = cs.c[k];
+  const int local = bid - c.start, i = local / c.per, t = local - i * c.per;
+  int tr, tc;
+  tri_tile(t, tr, tc);
+  f32x16 acc[W][W];
 #pragma unroll
   for (int u = 0; u < W; ++u)
 #pragma unroll
     for (int v = 0; v < W; ++v)
 #pragma unroll
-      for (int e4 = 0; e4 < 4; ++e4) {
-        const int r0 = tr * T + wr * (T / 2) + u * 32 + 8 * e4 + 4 * (lane >> 5);
-        const int q = tc * T + wc * (T / 2) + v * 32 + (lane & 31);
-        float val[4];
+      for (int e = 0; e < 16; ++e) acc[u][v][e] = 0.f;
+  for (int s = 0; s < p.splits && s * c.ks < (c.np >> 5); ++s) {
+    const float* o = p.part + ((size_t)s * gridDim.x + bid) * (T * T) + threadIdx.x;
 #pragma unroll
-        for (int e = 0; e < 4; ++e) val[e] = acc[u][v][e4 * 4 + e] * un;
-        if (EPI == EPI_OUT) {
+    for (int u = 0; u < W; ++u)
 #pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            const int r = r0 + e;
-            if (r >= c.m || q >= c.n) continue;
-            const size_t at = tall ? (size_t)q * c.cols + r : (size_t)r * c.cols + q;
-            OutT* o = reinterpret_cast<OutT*>(it.p) + at;
-            if (p.muon) *o = from_f<OutT>(to_f(*o) * p.decay - p.lr * it.scale * val[e]);
-            else *o = from_f<OutT>(val[e]);
-          }
-          continue;
-        }
-        if (r0 >= c.mp || q >= (EPI == EPI_X ? c.np : c.mp)) continue;      // (mp, np are multiples of 32)
-        if (EPI == EPI_Q) {
+      for (int v = 0; v < W; ++v)
 #pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            const _Float16* am = A + (size_t)(r0 + e) * c.mp + q;
-            val[e] = p.qc * val[e] + p.qb * (((float)am[0] + (float)am[pm]) * p.sa_inv) + (r0 + e == q ? p.qa : 0.f);
-          }
-        }
-        const int ld = EPI == EPI_X ? c.np : c.mp;
-        const size_t pl = EPI == EPI_X ? px : pm;
-        f16x4 h, l;
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          const float x = val[e] * p.scale;
-          h[e] = (_Float16)x;
-          l[e] = (_Float16)(x - (float)h[e]);
-          _Float16* d = out + (size_t)(r0 + e) * ld + q;
-          d[0] = h[e];
-          if (EPI != EPI_X || NB == 2) d[pl] = l[e];
-        }
-        if (EPI == EPI_X || tr != tc) {           // the other layout of X; the mirrored tile of a symmetric product
-          const int ld2 = EPI == EPI_X ? c.mp : c.mp;
-          _Float16* d = (EPI == EPI_X ? out2 : out) + (size_t)q * ld2 + r0;
-          *reinterpret_cast<f16x4*>(d) = h;
-          if (EPI != EPI_X || NB == 2) *reinterpret_cast<f16x4*>(d + pl) = l;
-        }
-      }
+        for (int e = 0; e < 16; ++e) acc[u][v][e] += o[((u * W + v) * 16 + e) * 256];
+  }
+  const float rs = residue[c.first + i];
+  _Float16* out = reinterpret_cast<_Float16*>(ws + c.base + (size_t)i * c.stride + slot_off(c, p.xplanes, p.job.out));
+  ns_store_sym<EPI_GRAM, T>(c, p, nullptr, out, tr, tc, p.unscale * (p.res_pow == 2 ? rs * rs : 1.f), acc);
 }
 
 // ---- host ---------------------------------------------------------------------------------------------------------------------
 struct NsPlan {
-  struct Set { std::vector<NsClass> cls; std::vector<int> order; size_t bytes; int items; };
+  struct Set { std::vector<NsClass> cls; size_t bytes; int items; };
   std::vector<Set> sets;
   int np;                               // planes of X
   int xplanes;
-  size_t head;                          // table + norms + residues, for the largest set
+  size_t head;                          // table + norms + residues, for the largest set; then the shares of split products
   size_t bytes;
 };
 
 inline int round_up(int v, int to) { return (v + to - 1) / to * to; }
 inline size_t round_up_z(size_t v, size_t to) { return (v + to - 1) / to * to; }
 
-// slots of a region: Xk, Xt, Xu (the next Xt), NP planes each, then A, T and three for Q / P
+// Gram products of few tiles are cut along K (n) into shares of at least 8 K steps, about 512 workgroups in all, and added up in order
+struct NsSplit { int tile, splits, tiles; };
+inline int sym_tiles(int mp, int t) { const int k = (mp + t - 1) / t; return k * (k + 1) / 2; }
+NsSplit ns_split_plan(std::vector<NsClass>& cls) {
+  long big = 0, small = 0;
+  for (auto& c : cls) { big += (long)sym_tiles(c.mp, 128) * c.count; small += (long)sym_tiles(c.mp, 64) * c.count; }
+  NsSplit r;
+  r.tile = big >= 256 ? 128 : 64;
+  const long tiles = r.tile == 128 ? big : small;
+  r.tiles = (int)tiles;
+  r.splits = 1;
+  if (tiles < 384) {
+    const long want = (512 + tiles - 1) / tiles;
+    for (auto& c : cls) {
+      const int steps = c.np / 32, even = (int)((steps + want - 1) / want);
+      c.ks = even < 8 ? 8 : even;
+      const int n = (steps + c.ks - 1) / c.ks;
+      if (n > r.splits) r.splits = n;
+    }
+  }
+  return r;
+}
+
+// slots of a region: X and its successor, NP planes each, then A, T and three for Q / P
 int ns_plan(const char* what, int dtype, const pxl_ns_item* items, int n, NsPlan& plan) {
   PXL_REQUIRE(dtype == PXL_F32 || dtype == PXL_BF16, "%s: dtype %d is neither PXL_F32 nor PXL_BF16", what, dtype);
   PXL_REQUIRE(n >= 0 && (n == 0 || items != nullptr), "%s: bad item list", what);
   plan.np = dtype == PXL_F32 ? 2 : 1;
-  plan.xplanes = 3 * plan.np;
+  plan.xplanes = 2 * plan.np;
   std::vector<NsPlan::Set>& sets = plan.sets;
   for (int i = 0; i < n; ++i) {
-    PXL_REQUIRE(items[i].rows >= 1 && items[i].cols >= 1 && items[i].rows <= (1 << 24) && items[i].cols <= (1 << 24) &&
+    PXL_REQUIRE(items[i].rows >= 1 && items[i].cols >= 1 && items[i].rows <= (1 << 23) && items[i].cols <= (1 << 23) &&
                     (items[i].rows < items[i].cols ? items[i].rows : items[i].cols) <= (1 << 15),
-                "%s: item %d is %d x %d (1 .. 2^24, the smaller side at most 32768)", what, i, items[i].rows, items[i].cols);
+                "%s: item %d is %d x %d (1 .. 2^23, the smaller side at most 32768)", what, i, items[i].rows, items[i].cols);
     int sk = -1, ck = -1;
     for (size_t s = 0; s < sets.size() && sk < 0; ++s)
       for (size_t k = 0; k < sets[s].cls.size(); ++k)
@@ -415,7 +637,8 @@ int ns_plan(const char* what, int dtype, const pxl_ns_item* items, int n, NsPlan
     if (head > plan.head) plan.head = head;
   }
   for (auto& s : sets) {
-    size_t at = plan.head;
+    const NsSplit sp = ns_split_plan(s.cls);
+    size_t at = plan.head + (sp.splits > 1 ? (size_t)sp.splits * sp.tiles * sp.tile * sp.tile * sizeof(float) : 0);
     for (auto& c : s.cls) { c.base = at; at += c.stride * c.count; }
     s.bytes = at;
     if (at > plan.bytes) plan.bytes = at;
@@ -466,15 +689,24 @@ inline float plane_scale(double bound) {
 struct NsRun {
   hipStream_t st;
   NsClasses cs;
-  NsItem* table;
+  NsInline few;
+  NsItem* table;                        // NULL: the items are in `few`
   double* part;
   float* residue;
+  float* shares;
   unsigned char* ws;
+  NsSplit split;
 };
 
-template <int EPI, int NA, int NB, typename OutT>
-int ns_gemm(NsRun& r, const NsGemm& g, int jobs) {
-  constexpr int T = 64;
+#define NS_TRY(expr)            \
+  do {                          \
+    const int _rc = (expr);     \
+    if (_rc != PXL_OK) return _rc; \
+  } while (0)
+
+template <int EPI, int NA, int NB, int T, typename OutT>
+int ns_launch(NsRun& r, const NsGemm& g, int splits) {
+  constexpr int D = T == 64 ? 4 : 2;
   int at = 0;
   for (int k = 0; k < r.cs.n; ++k) {
     NsClass& c = r.cs.c[k];
@@ -484,20 +716,34 @@ int ns_gemm(NsRun& r, const NsGemm& g, int jobs) {
     c.start = at;
     at += c.per * c.count;
   }
-  hipLaunchKernelGGL((ns_gemm_kernel<EPI, NA, NB, T, OutT>), dim3(at, 1, jobs), dim3(256), 0, r.st, r.cs, g, r.table, r.residue, r.ws);
+  hipLaunchKernelGGL((ns_gemm_kernel<EPI, NA, NB, T, D, OutT>), dim3(at, splits), dim3(256), 0, r.st, r.cs, g, r.few, r.table, r.residue, r.ws);
   PXL_LAUNCH_CHECK();
+  if (EPI == EPI_PART) {
+    hipLaunchKernelGGL((ns_fold_kernel<T>), dim3(at), dim3(256), 0, r.st, r.cs, g, r.residue, r.ws);
+    PXL_LAUNCH_CHECK();
+  }
   return PXL_OK;
 }
 
-#define NS_TRY(expr)            \
-  do {                          \
-    const int _rc = (expr);     \
-    if (_rc != PXL_OK) return _rc; \
-  } while (0)
+// 128 x 128 tiles where they give every CU one (2048: 136 us a symmetric product with 64 x 64 tiles, see DESIGN), else 64 x 64
+template <int EPI, int NA, int NB, typename OutT>
+int ns_gemm(NsRun& r, const NsGemm& g) {
+  if constexpr (EPI == EPI_GRAM) {
+    if (r.split.splits > 1) return r.split.tile == 128 ? ns_launch<EPI_PART, NA, NB, 128, OutT>(r, g, r.split.splits)
+                                                       : ns_launch<EPI_PART, NA, NB, 64, OutT>(r, g, r.split.splits);
+    return r.split.tile == 128 ? ns_launch<EPI, NA, NB, 128, OutT>(r, g, 1) : ns_launch<EPI, NA, NB, 64, OutT>(r, g, 1);
+  }
+  long big = 0;
+  for (int k = 0; k < r.cs.n; ++k) {
+    const NsClass& c = r.cs.c[k];
+    big += EPI <= EPI_MUL ? (long)sym_tiles(c.mp, 128) * c.count : (long)((c.mp + 127) / 128) * ((c.np + 127) / 128) * c.count;
+  }
+  return big >= 256 ? ns_launch<EPI, NA, NB, 128, OutT>(r, g, 1) : ns_launch<EPI, NA, NB, 64, OutT>(r, g, 1);
+}
 
 template <typename T, int NP>
 int ns_run_set(NsRun& r, const std::vector<NsStep>& steps, float eps, const MuonArgs& ma, int muon) {
-  const int XK = 0, XT = NP, XU = 2 * NP, xplanes = 3 * NP, MA = xplanes, MT = xplanes + 1;
+  const int xplanes = 2 * NP, MA = xplanes, MT = xplanes + 1;
   int blocks = 0;
   for (int k = 0; k < r.cs.n; ++k) {
     NsClass& c = r.cs.c[k];
@@ -505,7 +751,7 @@ int ns_run_set(NsRun& r, const std::vector<NsStep>& steps, float eps, const Muon
     c.start = blocks;
     blocks += c.per * c.count;
   }
-  hipLaunchKernelGGL(ns_norm_kernel<T>, dim3(blocks), dim3(256), 0, r.st, r.cs, r.table, r.part, ma);
+  hipLaunchKernelGGL(ns_norm_kernel<T>, dim3(blocks), dim3(256), 0, r.st, r.cs, r.few, r.table, r.part, ma);
   PXL_LAUNCH_CHECK();
   blocks = 0;
   for (int k = 0; k < r.cs.n; ++k) {
@@ -516,34 +762,37 @@ int ns_run_set(NsRun& r, const std::vector<NsStep>& steps, float eps, const Muon
     blocks += c.per * c.count;
   }
   float sx = plane_scale(1.0);
-  hipLaunchKernelGGL((ns_split_kernel<T, NP>), dim3(blocks), dim3(256), 0, r.st, r.cs, r.table, r.part, r.residue, r.ws, (size_t)XK, (size_t)XT, eps, sx, ma);
+  hipLaunchKernelGGL((ns_split_kernel<T, NP>), dim3(blocks), dim3(256), 0, r.st, r.cs, r.few, r.table, r.part, r.residue, r.ws, eps, sx, ma);
   PXL_LAUNCH_CHECK();
 
   NsGemm g;
   memset(&g, 0, sizeof(g));
   g.xplanes = xplanes;
-  int first = 1, xt = XT, xu = XU;
+  g.part = r.shares;
+  g.splits = r.split.splits;
+  int first = 1, x = 0, x2 = NP;
   size_t s = 0;
   while (s < steps.size()) {
-    double lam = steps[s].lam, pbound = 1.0;
-    float sA = plane_scale(lam), sP = 1.f;
-    g.job[0] = {XK, XK, MA, MA};
+    double pbound = 1.0;
+    float sA = plane_scale(steps[s].lam), sP = 1.f;
+    g.job = {x, x, MA};
     g.unscale = 1.f / (sx * sx);
     g.scale = sA;
     g.res_pow = NP == 1 && first ? 2 : 0;
-    NS_TRY((ns_gemm<EPI_GRAM, NP, NP, T>(r, g, 1)));
+    NS_TRY((ns_gemm<EPI_GRAM, NP, NP, float>(r, g)));
+    g.res_pow = 0;
     int P = -1;
     for (;; ++s) {
       const NsStep& d = steps[s];
       int q = xplanes + 2;
       while (q == P) ++q;
       const float sQ = plane_scale(d.q);
-      g.job[0] = {MA, MA, q, q};
+      g.job = {MA, MA, q};
       g.unscale = 1.f / (sA * sA);
       g.scale = sQ;
       g.qa = (float)d.a; g.qb = (float)d.b; g.qc = (float)d.c;
       g.sa_inv = 1.f / sA;
-      NS_TRY((ns_gemm<EPI_Q, 2, 2, T>(r, g, 1)));
+      NS_TRY((ns_gemm<EPI_Q, 2, 2, float>(r, g)));
       pbound *= d.q;
       const float sP2 = plane_scale(pbound), sT = plane_scale(d.t);
       if (P < 0) {
@@ -552,43 +801,43 @@ int ns_run_set(NsRun& r, const std::vector<NsStep>& steps, float eps, const Muon
       } else {
         int p2 = xplanes + 2;
         while (p2 == P || p2 == q) ++p2;
-        g.job[0] = {q, P, p2, p2};
+        g.job = {q, P, p2};
         g.unscale = 1.f / (sQ * sP);
         g.scale = sP2;
-        NS_TRY((ns_gemm<EPI_MUL, 2, 2, T>(r, g, 1)));
+        NS_TRY((ns_gemm<EPI_MUL, 2, 2, float>(r, g)));
         P = p2;
         sP = sP2;
       }
       if (d.last) break;
-      g.job[0] = {q, MA, MT, MT};
+      g.job = {q, MA, MT};
       g.unscale = 1.f / (sQ * sA);
       g.scale = sT;
-      NS_TRY((ns_gemm<EPI_MUL, 2, 2, T>(r, g, 1)));
+      NS_TRY((ns_gemm<EPI_MUL, 2, 2, float>(r, g)));
       const float sA2 = plane_scale(steps[s + 1].lam);
-      g.job[0] = {q, MT, MA, MA};
+      g.job = {q, MT, MA};
       g.unscale = 1.f / (sQ * sT);
       g.scale = sA2;
-      NS_TRY((ns_gemm<EPI_MUL, 2, 2, T>(r, g, 1)));
+      NS_TRY((ns_gemm<EPI_MUL, 2, 2, float>(r, g)));
       sA = sA2;
     }
     ++s;
     g.unscale = 1.f / (sP * sx);
     g.res_pow = NP == 1 && first ? 1 : 0;
     if (s == steps.size()) {
-      g.job[0] = {P, xt, 0, 0};
+      g.job = {P, x, 0};
       g.muon = muon;
       g.lr = ma.lr;
       g.decay = ma.keep;
-      NS_TRY((ns_gemm<EPI_OUT, 2, NP, T>(r, g, 1)));
+      NS_TRY((ns_gemm<EPI_OUT, 2, NP, T>(r, g)));
     } else {
       const float sx2 = plane_scale(steps[s].sigma);
-      g.job[0] = {P, xt, XK, xu};
+      g.job = {P, x, x2};
       g.scale = sx2;
-      NS_TRY((ns_gemm<EPI_X, 2, NP, T>(r, g, 1)));
+      NS_TRY((ns_gemm<EPI_X, 2, NP, float>(r, g)));
       sx = sx2;
-      const int o = xt;
-      xt = xu;
-      xu = o;
+      const int o = x;
+      x = x2;
+      x2 = o;
       first = 0;
     }
   }
@@ -638,18 +887,26 @@ int ns_run(const char* what, int dtype, const pxl_ns_item* items, int n, int ste
     r.part = reinterpret_cast<double*>(r.ws + round_up_z(set.items * sizeof(NsItem), 256));
     r.residue = reinterpret_cast<float*>(reinterpret_cast<unsigned char*>(r.part) + round_up_z(set.items * sizeof(double) * NS_PARTS, 256));
     r.cs.n = (int)set.cls.size();
+    r.split = ns_split_plan(set.cls);
+    r.shares = reinterpret_cast<float*>(r.ws + plan.head);
     for (int k = 0; k < r.cs.n; ++k) r.cs.c[k] = set.cls[k];
     std::vector<NsItem> list;
     for (auto& c : set.cls)
       for (int i = 0; i < n; ++i)
         if (items[i].rows == c.rows && items[i].cols == c.cols)
           list.push_back(NsItem{items[i].p, items[i].g, muon ? items[i].mom : nullptr, items[i].scale, 0});
-    for (size_t at = 0; at < list.size(); at += NS_TABLE) {
-      NsTable t;
-      const int cnt = (int)(list.size() - at < (size_t)NS_TABLE ? list.size() - at : NS_TABLE);
-      memcpy(t.it, &list[at], cnt * sizeof(NsItem));
-      hipLaunchKernelGGL(ns_table_kernel, dim3(1), dim3(64), 0, r.st, t, cnt, r.table + at);
-      PXL_LAUNCH_CHECK();
+    memset(&r.few, 0, sizeof(r.few));
+    if (list.size() <= (size_t)NS_INLINE) {
+      memcpy(r.few.it, list.data(), list.size() * sizeof(NsItem));
+      r.table = nullptr;
+    } else {
+      for (size_t at = 0; at < list.size(); at += NS_TABLE) {
+        NsTable t;
+        const int cnt = (int)(list.size() - at < (size_t)NS_TABLE ? list.size() - at : NS_TABLE);
+        memcpy(t.it, &list[at], cnt * sizeof(NsItem));
+        hipLaunchKernelGGL(ns_table_kernel, dim3(1), dim3(64), 0, r.st, t, cnt, r.table + at);
+        PXL_LAUNCH_CHECK();
+      }
     }
     if (dtype == PXL_F32) NS_TRY((ns_run_set<float, 2>(r, st, eps, ma, muon)));
     else NS_TRY((ns_run_set<bf16_t, 1>(r, st, eps, ma, muon)));
