@@ -66,7 +66,7 @@ struct NsClass {
   int rows, cols, m, n, mp, np;         // mp / np: m / n rounded up (zero padding)
   int start, per;                       // first workgroup and workgroups per matrix of THIS launch
   int chunk, parts;                     // norm pass: elements per workgroup, workgroups per matrix
-  int tn, ks;                           // tiles across (this launch); split products: K steps of 32 a share
+  int tn, ks;                           // tiles across (this launch); split products: k a share
   size_t base, stride;
 };
 struct NsClasses { NsClass c[NS_MAX_CLASSES]; int n; };
@@ -241,8 +241,13 @@ struct NsGemm {
   float lr, decay;                      // OUT of a Muon step
   int muon;
   float* part;                          // PART: [split][tile][T * T] accumulators
-  int splits;                           // PART: shares of K
 };
+
+__device__ __forceinline__ void put_split(_Float16* d, size_t plane, float v) {
+  const _Float16 h = (_Float16)v;
+  d[0] = h;
+  d[plane] = (_Float16)(v - (float)h);
+}
 
 // lower-triangular tile number t -> (row, column), row >= column
 __device__ __forceinline__ void tri_tile(int t, int& r, int& q) {
@@ -252,58 +257,65 @@ __device__ __forceinline__ void tri_tile(int t, int& r, int& q) {
   q = t - r * (r + 1) / 2;
 }
 
-// accumulators of a symmetric product -> both planes of the result, the tile and its mirror image.  Accumulator element e of a
-// lane: row 8 (e / 4) + 4 (lane / 32) + e % 4, column lane % 32
-template <int EPI, int T>
-__device__ __forceinline__ void ns_store_sym(const NsClass& c, const NsGemm& p, const _Float16* A, _Float16* out, int tr, int tc, float un,
-                                             f32x16 (&acc)[T / 64][T / 64]) {
-  constexpr int W = T / 64;
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, wr = wave >> 1, wc = wave & 1;
+// Where a lane's accumulators of one 32 x 32 block lie: element e at row 8 (e / 4) + 4 (lane / 32) + e % 4, column lane % 32.
+// One block of a symmetric product at (r, q) -> both planes of the result, and its mirror image where it lies below the diagonal tiles
+template <int EPI>
+__device__ __forceinline__ void ns_store_sym(const NsClass& c, const NsGemm& p, const _Float16* A, _Float16* out, int r, int q, bool mirror, float un,
+                                             const f32x16& acc) {
+  const int lane = threadIdx.x & 63;
   const size_t pm = (size_t)c.mp * c.mp;
+  q += lane & 31;
+  r += 4 * (lane >> 5);
 #pragma unroll
-  for (int u = 0; u < W; ++u)
+  for (int e4 = 0; e4 < 4; ++e4) {
+    const int r0 = r + 8 * e4;
+    if (r0 >= c.mp || q >= c.mp) continue;                    // (mp is a multiple of 32)
+    f16x4 h, l;
 #pragma unroll
-    for (int v = 0; v < W; ++v)
-#pragma unroll
-      for (int e4 = 0; e4 < 4; ++e4) {
-        const int r0 = tr * T + wr * (T / 2) + u * 32 + 8 * e4 + 4 * (lane >> 5);
-        const int q = tc * T + wc * (T / 2) + v * 32 + (lane & 31);
-        if (r0 >= c.mp || q >= c.mp) continue;                    // (mp is a multiple of 32)
-        f16x4 h, l;
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          float val = acc[u][v][e4 * 4 + e] * un;
-          _Float16* d = out + (size_t)(r0 + e) * c.mp + q;
-          if (EPI == EPI_Q) {
-            const _Float16* am = A + (size_t)(r0 + e) * c.mp + q;
-            val = p.qc * val + p.qb * (((float)am[0] + (float)am[pm]) * p.sa_inv) + (r0 + e == q ? p.qa : 0.f);
-          }
-          const float x = val * p.scale;
-          h[e] = (_Float16)x;
-          l[e] = (_Float16)(x - (float)h[e]);
-          d[0] = h[e];
-          d[pm] = l[e];
-        }
-        if (tr != tc) {
-          _Float16* d = out + (size_t)q * c.mp + r0;
-          *reinterpret_cast<f16x4*>(d) = h;
-          *reinterpret_cast<f16x4*>(d + pm) = l;
-        }
+    for (int e = 0; e < 4; ++e) {
+      float val = acc[e4 * 4 + e] * un;
+      _Float16* d = out + (size_t)(r0 + e) * c.mp + q;
+      if (EPI == EPI_Q) {
+        const _Float16* am = A + (size_t)(r0 + e) * c.mp + q;
+        val = p.qc * val + p.qb * (((float)am[0] + (float)am[pm]) * p.sa_inv) + (r0 + e == q ? p.qa : 0.f);
       }
+      const float x = val * p.scale;
+      h[e] = (_Float16)x;
+      l[e] = (_Float16)(x - (float)h[e]);
+      d[0] = h[e];
+      d[pm] = l[e];
+    }
+    if (mirror) {
+      _Float16* d = out + (size_t)q * c.mp + r0;
+      *reinterpret_cast<f16x4*>(d) = h;
+      *reinterpret_cast<f16x4*>(d + pm) = l;
+    }
+  }
 }
 
-// One T x T tile per workgroup of 4 waves (2 x 2), K steps of 32.  Global memory -> registers, D steps ahead -> LDS, two buffers, one
-// barrier a step.  LDS images: rows of 32 k (64 bytes), 16-byte chunk ch of row r at ch ^ ((r >> 2) & 3), for a and for b in [j][k]; rows of T
-// columns per k for b in [k][j], 32-byte segment at its number ^ swizzle(k), read with the transposing LDS load (within 16 lanes, lane j
-// receives 16-bit slot j % 4 of lanes j / 4 + 4 e): 4 k of one column.  Both are free of bank conflicts.
-template <int EPI, int NA, int NB, int T, int D, typename OutT>
+// One T x T tile per workgroup of 4 waves.  T = 128: K steps of 32, the waves 2 x 2 on the tile.  T = 64 (few tiles): K steps of 64, each wave
+// takes 16 of them for the WHOLE tile and the four sums are added at the end in order: an LDS read feeds as many matrix instructions as with
+// T = 128 (32 x 32 a wave would be bound by LDS reads), and a barrier stands between 12 of them instead of 6.
+// Global memory -> registers, D steps ahead -> LDS, two buffers, one barrier a step.  LDS images: rows of one K step for a, and for b in [j][k],
+// 16-byte chunks permuted within the row; rows of T columns per k for b in [k][j], 32-byte segments permuted, read with the transposing LDS load
+// (within 16 lanes, lane j receives 16-bit slot j % 4 of lanes j / 4 + 4 e): 4 k of one column.  The permutations keep every group of lanes that
+// is served at once on different banks.
+template <int T> __device__ __forceinline__ int chunk_at(int r, int ch) {          // byte of chunk ch of row r
+  return T == 128 ? r * 64 + ((ch ^ ((r >> 2) & 3)) << 4) : r * 128 + ((ch ^ ((r >> 1) & 7)) << 4);
+}
+template <int T> __device__ __forceinline__ int segment_at(int k, int seg) {       // byte of 32-byte segment seg of row k
+  return T == 128 ? k * 256 + ((seg ^ ((k & 3) << 1)) << 5) : k * 128 + ((seg ^ (k & 2)) << 5);
+}
+template <int EPI, int NA, int NB, int T, typename OutT>
 __global__ __launch_bounds__(256, 2) void ns_gemm_kernel(NsClasses cs, NsGemm p, NsInline few, const NsItem* __restrict__ table,
                                                          const float* __restrict__ residue, unsigned char* __restrict__ ws) {
   constexpr bool SYM = EPI <= EPI_MUL, NN = EPI >= EPI_X;
-  constexpr int W = T / 64;                     // 32 x 32 accumulators per wave and direction
-  constexpr int PL = T * 64;                    // bytes of one plane's tile
-  constexpr int CH = T / 64;                    // 16-byte chunks a thread moves per plane
-  __shared__ __attribute__((aligned(16))) unsigned char lds[2][(NA + NB) * PL];
+  constexpr int KS = T == 128 ? 32 : 64;        // k a step
+  constexpr int D = 2;                          // (3 with T = 64: 16 registers spilled)
+  constexpr int PL = T * KS * 2;                // bytes of one plane's tile
+  constexpr int BUF = (NA + NB) * PL;
+  constexpr int WB = T == 128 ? 1 : 2;          // blocks of 32 x 32 a wave ends up with: 4 / 1
+  __shared__ __attribute__((aligned(16))) unsigned char lds[T == 64 && 2 * BUF < 65536 ? 65536 : 2 * BUF];
   const int bid = xcd_remap(blockIdx.x, gridDim.x);
   const int k = find_class(cs, bid);
   const NsClass& c = cs.c[k];
@@ -313,64 +325,72 @@ __global__ __launch_bounds__(256, 2) void ns_gemm_kernel(NsClasses cs, NsGemm p,
   else { tr = t / c.tn; tc = t - tr * c.tn; }
   unsigned char* base = ws + c.base + (size_t)i * c.stride;
   const int K = EPI <= EPI_PART ? c.np : c.mp;
-  const int rowsB = c.mp;
   const size_t plane_a = (size_t)c.mp * K, plane_b = NN ? (size_t)c.mp * c.np : (size_t)c.mp * K;
   const _Float16* A = reinterpret_cast<const _Float16*>(base + slot_off(c, p.xplanes, p.job.a));
   const _Float16* B = reinterpret_cast<const _Float16*>(base + slot_off(c, p.xplanes, p.job.b));
 
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, wr = wave >> 1, wc = wave & 1;
-  int s0 = 0, steps = K >> 5;
+  int k0 = 0, k1 = K;
   if (EPI == EPI_PART) {
-    s0 = blockIdx.y * c.ks;
-    steps = steps - s0 < c.ks ? steps - s0 : c.ks;
-    if (steps <= 0) return;                     // (shapes with fewer shares than the grid has: never read)
+    k0 = blockIdx.y * c.ks;
+    k1 = k0 + c.ks < K ? k0 + c.ks : K;
+    if (k0 >= k1) return;                       // (shapes with fewer shares than the grid has: never read)
   }
+  const int steps = (k1 - k0 + KS - 1) / KS;
   // byte offsets of a thread's chunks from the tile's first element, and where they go in LDS
-  unsigned oa[CH], ob[CH];
-  int la[CH], lb[CH];
+  constexpr int RC = KS / 8;                    // chunks a row
+  unsigned oa[2], ob[2];
+  int la[2], lb[2];
 #pragma unroll
-  for (int q = 0; q < CH; ++q) {
-    const int e = tid + q * 256, r = e >> 2, ch = e & 3;
+  for (int q = 0; q < 2; ++q) {
+    const int e = tid + q * 256, r = e / RC, ch = e % RC;
     const int ia = tr * T + r < c.mp ? r : c.mp - 1 - tr * T;      // rows past the matrix: the last one again (never stored; tr * T < mp)
     oa[q] = (unsigned)(ia * K + ch * 8) * 2u;
-    la[q] = r * 64 + ((ch ^ ((r >> 2) & 3)) << 4);
+    la[q] = chunk_at<T>(r, ch);
     if (NN) {
       const int kr = e / (T / 8), cc = e % (T / 8);
       const int col = tc * T + cc * 8 < c.np ? cc * 8 : 0;         // chunks past the matrix: the tile's first again (never stored)
       ob[q] = (unsigned)(kr * c.np + col) * 2u;
-      const int swz = T == 128 ? kr & 3 : (kr >> 1) & 1;
-      lb[q] = kr * (T * 2) + (((cc >> 1) ^ swz) << 5) + ((cc & 1) << 4);
+      lb[q] = segment_at<T>(kr, cc >> 1) + ((cc & 1) << 4);
     } else {
-      const int ib = tc * T + r < rowsB ? r : rowsB - 1 - tc * T;
+      const int ib = tc * T + r < c.mp ? r : c.mp - 1 - tc * T;
       ob[q] = (unsigned)(ib * K + ch * 8) * 2u;
       lb[q] = la[q];
     }
   }
-  const unsigned char* pa = reinterpret_cast<const unsigned char*>(A + (size_t)tr * T * K + (size_t)s0 * 32);
-  const unsigned char* pb = reinterpret_cast<const unsigned char*>(NN ? B + (size_t)s0 * 32 * c.np + tc * T : B + (size_t)tc * T * K + (size_t)s0 * 32);
-  const size_t step_b = NN ? (size_t)64 * c.np : 64;
-  // (buffer loads: the base that moves stays in scalar registers; offsets below 2^31, a row is at most 2^24 bytes and a tile 128 rows)
-  auto window = [](const unsigned char* at) { return __builtin_amdgcn_make_buffer_rsrc((void*)at, 0, 0x7fffffff, 0x00020000); };
-  u32x4 ra[D][NA][CH], rb[D][NB][CH];
+  // Buffer loads: the moving base stays in scalar registers, and what lies past the end of a plane reads as zero (the last step of 64 where K is
+  // an odd multiple of 32: what else it reads there is not used).  Offsets within a window stay below 2^31.
+  size_t pa = ((size_t)tr * T * K + k0) * 2, pb = (NN ? (size_t)k0 * c.np + tc * T : (size_t)tc * T * K + k0) * 2;
+  const size_t step_b = NN ? (size_t)KS * 2 * c.np : KS * 2;
+  auto window = [](const _Float16* plane, size_t at, size_t bytes) {
+    const size_t left = bytes - at;
+    return __builtin_amdgcn_make_buffer_rsrc((void*)(reinterpret_cast<const unsigned char*>(plane) + at), 0, (int)(left < 0x7fffffff ? left : 0x7fffffff), 0x00020000);
+  };
+  u32x4 ra[D][NA][2], rb[D][NB][2];
   int fetched = 0;
   auto fetch = [&](int slot) {
 #pragma unroll
-    for (int q = 0; q < CH; ++q) {
+    for (int z = 0; z < NA; ++z) {
+      const auto w = window(A + z * plane_a, pa, plane_a * 2);
 #pragma unroll
-      for (int z = 0; z < NA; ++z) ra[slot][z][q] = __builtin_amdgcn_raw_buffer_load_b128(window(pa + z * plane_a * 2), (int)oa[q], 0, 0);
+      for (int q = 0; q < 2; ++q) ra[slot][z][q] = __builtin_amdgcn_raw_buffer_load_b128(w, (int)oa[q], 0, 0);
+    }
 #pragma unroll
-      for (int z = 0; z < NB; ++z) rb[slot][z][q] = __builtin_amdgcn_raw_buffer_load_b128(window(pb + z * plane_b * 2), (int)ob[q], 0, 0);
+    for (int z = 0; z < NB; ++z) {
+      const auto w = window(B + z * plane_b, pb, plane_b * 2);
+#pragma unroll
+      for (int q = 0; q < 2; ++q) rb[slot][z][q] = __builtin_amdgcn_raw_buffer_load_b128(w, (int)ob[q], 0, 0);
     }
     // (past the last step: that one again, in bounds and unused -- a fetch under a condition would make every wait one for all loads)
     const bool more = ++fetched < steps;
-    pa += more ? 64 : 0;
+    pa += more ? KS * 2 : 0;
     pb += more ? step_b : 0;
   };
-  f32x16 acc[W][W];
+  f32x16 acc[2][2];
 #pragma unroll
-  for (int u = 0; u < W; ++u)
+  for (int u = 0; u < 2; ++u)
 #pragma unroll
-    for (int v = 0; v < W; ++v)
+    for (int v = 0; v < 2; ++v)
 #pragma unroll
       for (int e = 0; e < 16; ++e) acc[u][v][e] = 0.f;
 
@@ -379,10 +399,47 @@ __global__ __launch_bounds__(256, 2) void ns_gemm_kernel(NsClasses cs, NsGemm p,
     fetch(d);
     __builtin_amdgcn_sched_barrier(0);          // (in this order: the waits count)
   }
-  auto step = [&](int s, int slot) {
-    unsigned char* buf = lds[s & 1];
+  auto multiply = [&](const unsigned char* buf, int kk) {           // k 16 kk .. 16 kk + 15 of the step
+    f16x8 fa[NA][2], fb[NB][2];
+    const int ro = T == 128 ? wr * 64 : 0, qo = T == 128 ? wc * 64 : 0, ch = kk * 2 + (lane >> 5);
 #pragma unroll
-    for (int q = 0; q < CH; ++q) {
+    for (int u = 0; u < 2; ++u) {
+      const int r = ro + u * 32 + (lane & 31), q = qo + u * 32 + (lane & 31);
+#pragma unroll
+      for (int z = 0; z < NA; ++z) fa[z][u] = *reinterpret_cast<const f16x8*>(buf + z * PL + chunk_at<T>(r, ch));
+#pragma unroll
+      for (int z = 0; z < NB; ++z) {
+        if (NN) {
+          // lanes 0-15 / 16-31: columns 0-15 / 16-31 of these 32, k 0-7; lanes 32-63: the same columns, k 8-15
+          f16x4 half[2];
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {
+            const int kr = kk * 16 + 8 * (lane >> 5) + 4 * h + ((lane & 15) >> 2);
+            half[h] = __builtin_bit_cast(f16x4, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)(
+                buf + (NA + z) * PL + segment_at<T>(kr, (qo + u * 32) / 16 + ((lane >> 4) & 1)) + ((lane & 3) << 3))));
+          }
+          fb[z][u] = __builtin_shufflevector(half[0], half[1], 0, 1, 2, 3, 4, 5, 6, 7);
+        } else {
+          fb[z][u] = *reinterpret_cast<const f16x8*>(buf + (NA + z) * PL + chunk_at<T>(q, ch));
+        }
+      }
+    }
+    // X: the operands the other way round, so that a lane holds four consecutive columns of one row of the result
+#define NS_MFMA(A_, B_, C_) (EPI == EPI_X ? __builtin_amdgcn_mfma_f32_32x32x16_f16(B_, A_, C_, 0, 0, 0) : __builtin_amdgcn_mfma_f32_32x32x16_f16(A_, B_, C_, 0, 0, 0))
+#pragma unroll
+    for (int u = 0; u < 2; ++u)
+#pragma unroll
+      for (int v = 0; v < 2; ++v) {
+        if (NB == 2) acc[u][v] = NS_MFMA(fa[0][u], fb[NB - 1][v], acc[u][v]);
+        if (NA == 2) acc[u][v] = NS_MFMA(fa[NA - 1][u], fb[0][v], acc[u][v]);
+        acc[u][v] = NS_MFMA(fa[0][u], fb[0][v], acc[u][v]);
+      }
+#undef NS_MFMA
+  };
+  auto step = [&](int s, int slot) {
+    unsigned char* buf = lds + (s & 1) * BUF;
+#pragma unroll
+    for (int q = 0; q < 2; ++q) {
 #pragma unroll
       for (int z = 0; z < NA; ++z) *reinterpret_cast<u32x4*>(buf + z * PL + la[q]) = ra[slot][z][q];
 #pragma unroll
@@ -390,45 +447,11 @@ __global__ __launch_bounds__(256, 2) void ns_gemm_kernel(NsClasses cs, NsGemm p,
     }
     fetch(slot);
     __syncthreads();
-#pragma unroll
-    for (int kk = 0; kk < 2; ++kk) {
-      f16x8 fa[NA][W], fb[NB][W];
-#pragma unroll
-      for (int u = 0; u < W; ++u) {
-        const int r = wr * (T / 2) + u * 32 + (lane & 31), ch = kk * 2 + (lane >> 5);
-        const int q = wc * (T / 2) + u * 32 + (lane & 31);
-#pragma unroll
-        for (int z = 0; z < NA; ++z) fa[z][u] = *reinterpret_cast<const f16x8*>(buf + z * PL + r * 64 + ((ch ^ ((r >> 2) & 3)) << 4));
-#pragma unroll
-        for (int z = 0; z < NB; ++z) {
-          if (NN) {
-            // lanes 0-15 / 16-31: columns 0-15 / 16-31 of this 32, k 0-7; lanes 32-63: the same columns, k 8-15
-            f16x4 half[2];
-#pragma unroll
-            for (int h = 0; h < 2; ++h) {
-              const int kr = kk * 16 + 8 * (lane >> 5) + 4 * h + ((lane & 15) >> 2);
-              const int seg = (wc * (T / 2) + u * 32) / 16 + ((lane >> 4) & 1);
-              const int swz = T == 128 ? kr & 3 : (kr >> 1) & 1;
-              half[h] = __builtin_bit_cast(f16x4, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)(
-                  buf + (NA + z) * PL + kr * (T * 2) + ((seg ^ swz) << 5) + ((lane & 3) << 3))));
-            }
-            fb[z][u] = __builtin_shufflevector(half[0], half[1], 0, 1, 2, 3, 4, 5, 6, 7);
-          } else {
-            fb[z][u] = *reinterpret_cast<const f16x8*>(buf + (NA + z) * PL + q * 64 + ((ch ^ ((q >> 2) & 3)) << 4));
-          }
-        }
-      }
-      // X: the operands the other way round, so that a lane holds four consecutive columns of one row of the result
-#define NS_MFMA(A_, B_, C_) (EPI == EPI_X ? __builtin_amdgcn_mfma_f32_32x32x16_f16(B_, A_, C_, 0, 0, 0) : __builtin_amdgcn_mfma_f32_32x32x16_f16(A_, B_, C_, 0, 0, 0))
-#pragma unroll
-      for (int u = 0; u < W; ++u)
-#pragma unroll
-        for (int v = 0; v < W; ++v) {
-          if (NB == 2) acc[u][v] = NS_MFMA(fa[0][u], fb[NB - 1][v], acc[u][v]);
-          if (NA == 2) acc[u][v] = NS_MFMA(fa[NA - 1][u], fb[0][v], acc[u][v]);
-          acc[u][v] = NS_MFMA(fa[0][u], fb[0][v], acc[u][v]);
-        }
-#undef NS_MFMA
+    if (T == 128) {
+      multiply(buf, 0);
+      multiply(buf, 1);
+    } else if (k0 + s * KS + wave * 16 < k1) {
+      multiply(buf, wave);
     }
   };
   int s = 0;
@@ -440,46 +463,79 @@ __global__ __launch_bounds__(256, 2) void ns_gemm_kernel(NsClasses cs, NsGemm p,
   for (int d = 0; d < D - 1; ++d)
     if (s + d < steps) step(s + d, d);
 
-  if (EPI == EPI_PART) {
-    // accumulators as they lie in the registers: the pass that adds the splits has the same lanes
-    float* o = p.part + ((size_t)blockIdx.y * gridDim.x + bid) * (T * T) + tid;
+  // T = 64: the waves' sums through LDS; wave w goes on with block (w / 2, w % 2)
+  f32x16 sum;
+  if constexpr (T == 64) {
+    __syncthreads();
+    float4* x = reinterpret_cast<float4*>(lds);
 #pragma unroll
-    for (int u = 0; u < W; ++u)
+    for (int u = 0; u < 2; ++u)
 #pragma unroll
-      for (int v = 0; v < W; ++v)
+      for (int v = 0; v < 2; ++v)
 #pragma unroll
-        for (int e = 0; e < 16; ++e) o[((u * W + v) * 16 + e) * 256] = acc[u][v][e];
+        for (int e4 = 0; e4 < 4; ++e4)
+          x[((wave * 4 + u * 2 + v) * 4 + e4) * 64 + lane] = make_float4(acc[u][v][e4 * 4], acc[u][v][e4 * 4 + 1], acc[u][v][e4 * 4 + 2], acc[u][v][e4 * 4 + 3]);
+    __syncthreads();
+#pragma unroll
+    for (int e4 = 0; e4 < 4; ++e4) {
+      float4 a = x[(wave * 4 + e4) * 64 + lane];
+#pragma unroll
+      for (int w = 1; w < 4; ++w) {
+        const float4 b = x[((w * 4 + wave) * 4 + e4) * 64 + lane];
+        a.x += b.x; a.y += b.y; a.z += b.z; a.w += b.w;
+      }
+      sum[e4 * 4] = a.x; sum[e4 * 4 + 1] = a.y; sum[e4 * 4 + 2] = a.z; sum[e4 * 4 + 3] = a.w;
+    }
+    __syncthreads();
+  }
+  // blocks of this wave: (number, row, column, accumulators)
+  auto blocks = [&](auto&& f) {
+    if constexpr (T == 64) {
+      f(wave, tr * 64 + wr * 32, tc * 64 + wc * 32, sum);
+    } else {
+#pragma unroll
+      for (int u = 0; u < 2; ++u)
+#pragma unroll
+        for (int v = 0; v < 2; ++v) f(wave * 4 + u * 2 + v, tr * 128 + wr * 64 + u * 32, tc * 128 + wc * 64 + v * 32, acc[u][v]);
+    }
+  };
+
+  if constexpr (EPI == EPI_PART) {
+    // [share][tile][block][e / 4][lane] float4: the pass that adds the shares has the same lanes
+    blocks([&](int n, int, int, const f32x16& a) {
+      float4* o = reinterpret_cast<float4*>(p.part) + (((size_t)blockIdx.y * gridDim.x + bid) * (T * T / 1024) + n) * 256 + lane;
+#pragma unroll
+      for (int e4 = 0; e4 < 4; ++e4) o[e4 * 64] = make_float4(a[e4 * 4], a[e4 * 4 + 1], a[e4 * 4 + 2], a[e4 * 4 + 3]);
+    });
     return;
   }
   const float rs = residue[c.first + i];
   const float un = p.unscale * (p.res_pow == 0 ? 1.f : (p.res_pow == 2 ? rs * rs : rs));
   _Float16* out = reinterpret_cast<_Float16*>(base + slot_off(c, p.xplanes, p.job.out));
   if constexpr (SYM) {
-    ns_store_sym<EPI, T>(c, p, A, out, tr, tc, un, acc);
+    blocks([&](int, int r, int q, const f32x16& a) { ns_store_sym<EPI>(c, p, A, out, r, q, tr != tc, un, a); });
   } else if constexpr (EPI == EPI_X) {
     // through LDS, one plane after the other: rows of T columns, 16-byte stores.  Lane: row lane % 32, columns 8 e4 + 4 (lane / 32) + 0 .. 3
     constexpr int PITCH = T + 8;
-    _Float16* stage = reinterpret_cast<_Float16*>(&lds[0][0]);
+    _Float16* stage = reinterpret_cast<_Float16*>(lds);
     static_assert(sizeof(lds) >= (size_t)T * PITCH * 2, "a plane's tile fits");
     const size_t px = (size_t)c.mp * c.np;
 #pragma unroll
     for (int z = 0; z < NB; ++z) {
       __syncthreads();
+      blocks([&](int, int r, int q, const f32x16& a) {
 #pragma unroll
-      for (int u = 0; u < W; ++u)
+        for (int e4 = 0; e4 < 4; ++e4) {
+          f16x4 h;
 #pragma unroll
-        for (int v = 0; v < W; ++v)
-#pragma unroll
-          for (int e4 = 0; e4 < 4; ++e4) {
-            f16x4 h;
-#pragma unroll
-            for (int e = 0; e < 4; ++e) {
-              const float x = acc[u][v][e4 * 4 + e] * un * p.scale;
-              h[e] = (_Float16)x;
-              if (z == 1) h[e] = (_Float16)(x - (float)h[e]);
-            }
-            *reinterpret_cast<f16x4*>(stage + (wr * (T / 2) + u * 32 + (lane & 31)) * PITCH + wc * (T / 2) + v * 32 + 8 * e4 + 4 * (lane >> 5)) = h;
+          for (int e = 0; e < 4; ++e) {
+            const float x = a[e4 * 4 + e] * un * p.scale;
+            h[e] = (_Float16)x;
+            if (z == 1) h[e] = (_Float16)(x - (float)h[e]);
           }
+          *reinterpret_cast<f16x4*>(stage + (r - tr * T + (lane & 31)) * PITCH + q - tc * T + 8 * e4 + 4 * (lane >> 5)) = h;
+        }
+      });
       __syncthreads();
 #pragma unroll
       for (int q = 0; q < T * T / 8 / 256; ++q) {
@@ -492,66 +548,209 @@ __global__ __launch_bounds__(256, 2) void ns_gemm_kernel(NsClasses cs, NsGemm p,
     const NsItem it = ns_item(few, table, c.first + i);
     const bool tall = c.rows > c.cols;
     const float f = p.muon ? -p.lr * it.scale : 1.f;
+    blocks([&](int, int r, int qb, const f32x16& a) {
 #pragma unroll
-    for (int u = 0; u < W; ++u)
+      for (int e4 = 0; e4 < 4; ++e4) {
+        const int r0 = r + 8 * e4 + 4 * (lane >> 5), q = qb + (lane & 31);
+        if (r0 >= c.m || q >= c.n) continue;
+        float val[4];
 #pragma unroll
-      for (int v = 0; v < W; ++v)
+        for (int e = 0; e < 4; ++e) val[e] = a[e4 * 4 + e] * un * f;
+        OutT* o = reinterpret_cast<OutT*>(it.p) + (tall ? (size_t)q * c.cols + r0 : (size_t)r0 * c.cols + q);
+        if (tall && r0 + 4 <= c.m) {
+          float old[4];
+          if (p.muon) {
+            load4(o, old);
 #pragma unroll
-        for (int e4 = 0; e4 < 4; ++e4) {
-          const int r0 = tr * T + wr * (T / 2) + u * 32 + 8 * e4 + 4 * (lane >> 5);
-          const int q = tc * T + wc * (T / 2) + v * 32 + (lane & 31);
-          if (r0 >= c.m || q >= c.n) continue;
-          float val[4];
-#pragma unroll
-          for (int e = 0; e < 4; ++e) val[e] = acc[u][v][e4 * 4 + e] * un * f;
-          OutT* o = reinterpret_cast<OutT*>(it.p) + (tall ? (size_t)q * c.cols + r0 : (size_t)r0 * c.cols + q);
-          if (tall && r0 + 4 <= c.m) {
-            float old[4];
-            if (p.muon) {
-              load4(o, old);
-#pragma unroll
-              for (int e = 0; e < 4; ++e) val[e] += old[e] * p.decay;
-            }
-            store4(o, val);
-          } else {
-            const size_t ld = tall ? 1 : c.cols;
-#pragma unroll
-            for (int e = 0; e < 4; ++e)
-              if (r0 + e < c.m) o[e * ld] = from_f<OutT>(p.muon ? to_f(o[e * ld]) * p.decay + val[e] : val[e]);
+            for (int e = 0; e < 4; ++e) val[e] += old[e] * p.decay;
           }
+          store4(o, val);
+        } else {
+          const size_t ld = tall ? 1 : c.cols;
+#pragma unroll
+          for (int e = 0; e < 4; ++e)
+            if (r0 + e < c.m) o[e * ld] = from_f<OutT>(p.muon ? to_f(o[e * ld]) * p.decay + val[e] : val[e]);
         }
+      }
+    });
   }
 }
 
-// sums of a split Gram product, in the order of the splits -> A
+// number of shares of a class's Gram product
+__device__ __forceinline__ int ns_shares(const NsClass& c) { return (c.np + c.ks - 1) / c.ks; }
+
+// one block's share sums, in the order of the shares
+template <int UNROLL> __device__ __forceinline__ f32x16 ns_share_sum(const float* part, int shares, size_t per_share, size_t at) {
+  f32x16 a;
+#pragma unroll
+  for (int e = 0; e < 16; ++e) a[e] = 0.f;
+  const float4* x = reinterpret_cast<const float4*>(part) + at * 256 + (threadIdx.x & 63);
+#pragma unroll UNROLL
+  for (int s = 0; s < shares; ++s) {
+#pragma unroll
+    for (int e4 = 0; e4 < 4; ++e4) {
+      const float4 v = x[(size_t)s * per_share * 256 + e4 * 64];
+      a[e4 * 4] += v.x; a[e4 * 4 + 1] += v.y; a[e4 * 4 + 2] += v.z; a[e4 * 4 + 3] += v.w;
+    }
+  }
+  return a;
+}
+
+// a split Gram product's shares -> A; one wave a block of 32 x 32
 template <int T>
-__global__ __launch_bounds__(256) void ns_fold_kernel(NsClasses cs, NsGemm p, const float* __restrict__ residue, unsigned char* __restrict__ ws) {
-  constexpr int W = T / 64;
-  const int bid = blockIdx.x;
+__global__ __launch_bounds__(64) void ns_fold_kernel(NsClasses cs, NsGemm p, int tiles, const float* __restrict__ residue, unsigned char* __restrict__ ws) {
+  constexpr int NBL = T * T / 1024, SIDE = T / 32;
+  const int bid = blockIdx.x / NBL, n = blockIdx.x % NBL;
   const int k = find_class(cs, bid);
   const NsClass& c = cs.c[k];
   const int local = bid - c.start, i = local / c.per, t = local - i * c.per;
   int tr, tc;
   tri_tile(t, tr, tc);
-  f32x16 acc[W][W];
-#pragma unroll
-  for (int u = 0; u < W; ++u)
-#pragma unroll
-    for (int v = 0; v < W; ++v)
-#pragma unroll
-      for (int e = 0; e < 16; ++e) acc[u][v][e] = 0.f;
-  for (int s = 0; s < p.splits && s * c.ks < (c.np >> 5); ++s) {
-    const float* o = p.part + ((size_t)s * gridDim.x + bid) * (T * T) + threadIdx.x;
-#pragma unroll
-    for (int u = 0; u < W; ++u)
-#pragma unroll
-      for (int v = 0; v < W; ++v)
-#pragma unroll
-        for (int e = 0; e < 16; ++e) acc[u][v][e] += o[((u * W + v) * 16 + e) * 256];
-  }
+  // block n of a tile, as the product numbers them
+  const int br = T == 64 ? n >> 1 : (n >> 3) * 2 + ((n >> 1) & 1), bc = T == 64 ? n & 1 : ((n >> 2) & 1) * 2 + (n & 1);
+  static_assert(SIDE * SIDE == NBL, "blocks of a tile");
+  const f32x16 a = ns_share_sum<4>(p.part, ns_shares(c), (size_t)tiles * NBL, (size_t)bid * NBL + n);
   const float rs = residue[c.first + i];
   _Float16* out = reinterpret_cast<_Float16*>(ws + c.base + (size_t)i * c.stride + slot_off(c, p.xplanes, p.job.out));
-  ns_store_sym<EPI_GRAM, T>(c, p, nullptr, out, tr, tc, p.unscale * (p.res_pow == 2 ? rs * rs : 1.f), acc);
+  ns_store_sym<EPI_GRAM>(c, p, nullptr, out, tr * T + br * 32, tc * T + bc * 32, tr != tc, p.unscale * (p.res_pow == 2 ? rs * rs : 1.f), a);
+}
+
+// ---- a whole segment's recursion for matrices of at most 32 MT rows: one workgroup of MT^2 waves a matrix, everything on the CU ----------
+// Wave (I, J) holds its 32 x 32 block of A, P and what it multiplies next in registers; LDS holds the two operands of the product at
+// hand (both symmetric: C[i][j] = sum_k x[i][k] y[j][k]).  In place of 3 to 5 launches a step of some 4 us each.
+struct NsRec {
+  int steps, xplanes, out;              // of this segment; slot of P
+  float unscale;                        // share sums -> A
+  int res_pow;
+  float sA[NS_MAX_STEPS], sQ[NS_MAX_STEPS], sT[NS_MAX_STEPS], sP[NS_MAX_STEPS];      // plane scales
+  float a[NS_MAX_STEPS], b[NS_MAX_STEPS], c[NS_MAX_STEPS];
+  const float* part;
+};
+template <int MT>
+__global__ __launch_bounds__(MT * MT * 64) void ns_rec_kernel(NsClasses cs, NsRec p, int tiles, const float* __restrict__ residue, unsigned char* __restrict__ ws) {
+  constexpr int M = 32 * MT, ROW = M * 2, PL = M * ROW;             // bytes
+  __shared__ __attribute__((aligned(16))) unsigned char lds[2][2 * PL];
+  const int k = find_class(cs, blockIdx.x);
+  const NsClass& c = cs.c[k];
+  const int i = blockIdx.x - c.start;
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, I = wave / MT, J = wave % MT;
+  const bool inside = I * 32 < c.mp && J * 32 < c.mp;               // mp is a multiple of 32
+  // 16-byte chunk ch of row r
+  auto at = [](int r, int ch) { return r * ROW + ((MT == 2 ? ch ^ ((r >> 1) & 7) : ch ^ (r & 15)) << 4); };
+  auto elem = [&](int r, int q) { return at(r, q >> 3) + (q & 7) * 2; };
+  auto put = [&](int slot, const f32x16& v, float s, bool mirror) {
+#pragma unroll
+    for (int e4 = 0; e4 < 4; ++e4) {
+      f16x4 h, l;
+      const int r0 = I * 32 + 8 * e4 + 4 * (lane >> 5), q = J * 32 + (lane & 31);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const float x = v[e4 * 4 + e] * s;
+        h[e] = (_Float16)x;
+        l[e] = (_Float16)(x - (float)h[e]);
+        if (!mirror || I == J) {
+          *reinterpret_cast<_Float16*>(&lds[slot][elem(r0 + e, q)]) = h[e];
+          *reinterpret_cast<_Float16*>(&lds[slot][PL + elem(r0 + e, q)]) = l[e];
+        }
+      }
+      if (mirror && I != J) {           // row q, columns r0 .. r0 + 3, and the block itself
+        *reinterpret_cast<f16x4*>(&lds[slot][elem(q, r0)]) = h;
+        *reinterpret_cast<f16x4*>(&lds[slot][PL + elem(q, r0)]) = l;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          *reinterpret_cast<_Float16*>(&lds[slot][elem(r0 + e, q)]) = h[e];
+          *reinterpret_cast<_Float16*>(&lds[slot][PL + elem(r0 + e, q)]) = l[e];
+        }
+      }
+    }
+  };
+  auto product = [&](int x, int y) {
+    f32x16 acc;
+#pragma unroll
+    for (int e = 0; e < 16; ++e) acc[e] = 0.f;
+#pragma unroll 2
+    for (int kk = 0; kk < 2 * MT && kk * 16 < c.mp; ++kk) {
+      const int ch = kk * 2 + (lane >> 5), r = I * 32 + (lane & 31), q = J * 32 + (lane & 31);
+      const f16x8 xh = *reinterpret_cast<const f16x8*>(&lds[x][at(r, ch)]), xl = *reinterpret_cast<const f16x8*>(&lds[x][PL + at(r, ch)]);
+      const f16x8 yh = *reinterpret_cast<const f16x8*>(&lds[y][at(q, ch)]), yl = *reinterpret_cast<const f16x8*>(&lds[y][PL + at(q, ch)]);
+      acc = __builtin_amdgcn_mfma_f32_32x32x16_f16(xh, yl, acc, 0, 0, 0);
+      acc = __builtin_amdgcn_mfma_f32_32x32x16_f16(xl, yh, acc, 0, 0, 0);
+      acc = __builtin_amdgcn_mfma_f32_32x32x16_f16(xh, yh, acc, 0, 0, 0);
+    }
+    return acc;
+  };
+  const float rs = residue[c.first + i];
+  const float un = p.unscale * (p.res_pow == 2 ? rs * rs : 1.f);
+  f32x16 P, V;
+#pragma unroll
+  for (int e = 0; e < 16; ++e) P[e] = V[e] = 0.f;
+  // A from the shares of the 64 x 64 tiles on and below the diagonal; blocks above it by mirroring
+  if (inside && (I >> 1) >= (J >> 1)) {
+    const int t = (I >> 1) * ((I >> 1) + 1) / 2 + (J >> 1);
+    V = ns_share_sum<MT == 2 ? 4 : 2>(p.part, ns_shares(c), (size_t)tiles * 4, ((size_t)c.tn + (size_t)i * c.per + t) * 4 + (I & 1) * 2 + (J & 1));
+#pragma unroll
+    for (int e = 0; e < 16; ++e) V[e] *= un;
+    if (I >= J) put(0, V, p.sA[0], true);
+  }
+  __syncthreads();
+  for (int s = 0; s < p.steps; ++s) {
+    if (inside) {
+      const f32x16 acc = product(0, 0);
+      const float g = p.c[s] / (p.sA[s] * p.sA[s]), ia = p.b[s] / p.sA[s];
+#pragma unroll
+      for (int e = 0; e < 16; ++e) {
+        const int r = I * 32 + 8 * (e >> 2) + 4 * (lane >> 5) + (e & 3), q = J * 32 + (lane & 31), o = elem(r, q);
+        const float am = (float)*reinterpret_cast<const _Float16*>(&lds[0][o]) + (float)*reinterpret_cast<const _Float16*>(&lds[0][PL + o]);
+        V[e] = g * acc[e] + ia * am + (r == q ? p.a[s] : 0.f);
+      }
+    }
+    // (slot 1 is free: its last readers have passed a barrier since)
+    if (inside) put(1, V, p.sQ[s], false);
+    __syncthreads();
+    const bool last = s + 1 == p.steps;
+    f32x16 tq;
+#pragma unroll
+    for (int e = 0; e < 16; ++e) tq[e] = 0.f;
+    if (!last && inside) tq = product(1, 0);            // Q A
+    if (s == 0) {
+      P = V;
+    } else {
+      __syncthreads();
+      if (inside) put(0, P, p.sP[s - 1], false);
+      __syncthreads();
+      if (inside) {
+        P = product(1, 0);
+        const float f = 1.f / (p.sQ[s] * p.sP[s - 1]);
+#pragma unroll
+        for (int e = 0; e < 16; ++e) P[e] *= f;
+      }
+    }
+    if (last) break;
+    __syncthreads();
+    if (inside) {
+      const float f = 1.f / (p.sQ[s] * p.sA[s]);
+#pragma unroll
+      for (int e = 0; e < 16; ++e) tq[e] *= f;
+      put(0, tq, p.sT[s], false);
+    }
+    __syncthreads();
+    if (inside) {
+      V = product(1, 0);                                 // Q (Q A)
+      const float f = 1.f / (p.sQ[s] * p.sT[s]);
+#pragma unroll
+      for (int e = 0; e < 16; ++e) V[e] *= f;
+    }
+    __syncthreads();
+    if (inside && I >= J) put(0, V, p.sA[s + 1], true);
+    __syncthreads();
+  }
+  if (!inside) return;
+  _Float16* out = reinterpret_cast<_Float16*>(ws + c.base + (size_t)i * c.stride + slot_off(c, p.xplanes, p.out));
+  const size_t pm = (size_t)c.mp * c.mp;
+  const float sp = p.sP[p.steps - 1];
+#pragma unroll
+  for (int e = 0; e < 16; ++e)
+    put_split(out + (size_t)(I * 32 + 8 * (e >> 2) + 4 * (lane >> 5) + (e & 3)) * c.mp + J * 32 + (lane & 31), pm, P[e] * sp);
 }
 
 // ---- host ---------------------------------------------------------------------------------------------------------------------
@@ -564,28 +763,35 @@ struct NsPlan {
   size_t bytes;
 };
 
+// 128 x 128 tiles or four times as many of 64 x 64: rounds over the 256 CUs, a small tile at 0.3 of a large one's time
+inline bool ns_big_tiles(long big, long few) { return (big + 255) / 256 * 10 <= (few + 255) / 256 * 3 && big >= 128; }
+
 inline int round_up(int v, int to) { return (v + to - 1) / to * to; }
 inline size_t round_up_z(size_t v, size_t to) { return (v + to - 1) / to * to; }
 
-// Gram products of few tiles are cut along K (n) into shares of at least 8 K steps, about 512 workgroups in all, and added up in order
-struct NsSplit { int tile, splits, tiles; };
+// How the matrices of one set run.  small: all have at most 128 on their smaller side, their recursion runs on one CU each.
+// Gram products of few tiles (all of a small set's) are cut along K (n) into shares of at least 256, about 512 workgroups in all, and
+// added up in order.
+struct NsSplit { int tile, shares, tiles, small, mt; };
 inline int sym_tiles(int mp, int t) { const int k = (mp + t - 1) / t; return k * (k + 1) / 2; }
 NsSplit ns_split_plan(std::vector<NsClass>& cls) {
-  long big = 0, small = 0;
-  for (auto& c : cls) { big += (long)sym_tiles(c.mp, 128) * c.count; small += (long)sym_tiles(c.mp, 64) * c.count; }
-  NsSplit r;
-  r.tile = big >= 256 ? 128 : 64;
-  const long tiles = r.tile == 128 ? big : small;
+  long big = 0, few = 0;
+  NsSplit r = {64, 1, 0, 1, 2};
+  for (auto& c : cls) {
+    big += (long)sym_tiles(c.mp, 128) * c.count;
+    few += (long)sym_tiles(c.mp, 64) * c.count;
+    if (c.mp > 64) r.mt = 4;
+    if (c.mp > 128) r.small = 0;
+  }
+  if (!r.small && ns_big_tiles(big, few)) r.tile = 128;
+  const long tiles = r.tile == 128 ? big : few;
   r.tiles = (int)tiles;
-  r.splits = 1;
-  if (tiles < 384) {
-    const long want = (512 + tiles - 1) / tiles;
-    for (auto& c : cls) {
-      const int steps = c.np / 32, even = (int)((steps + want - 1) / want);
-      c.ks = even < 8 ? 8 : even;
-      const int n = (steps + c.ks - 1) / c.ks;
-      if (n > r.splits) r.splits = n;
-    }
+  const long want = tiles < 384 ? (512 + tiles - 1) / tiles : 1;
+  for (auto& c : cls) {
+    const long even = ((c.np + want - 1) / want + 63) / 64 * 64;
+    c.ks = want == 1 ? c.np : (int)(even < 256 ? 256 : even);
+    const int n = (c.np + c.ks - 1) / c.ks;
+    if (n > r.shares) r.shares = n;
   }
   return r;
 }
@@ -606,7 +812,6 @@ int ns_plan(const char* what, int dtype, const pxl_ns_item* items, int n, NsPlan
       for (size_t k = 0; k < sets[s].cls.size(); ++k)
         if (sets[s].cls[k].rows == items[i].rows && sets[s].cls[k].cols == items[i].cols) { sk = (int)s; ck = (int)k; break; }
     if (sk < 0) {
-      if (sets.empty() || sets.back().cls.size() == (size_t)NS_MAX_CLASSES) sets.emplace_back();
       NsClass c;
       memset(&c, 0, sizeof(c));
       c.rows = items[i].rows;
@@ -622,9 +827,16 @@ int ns_plan(const char* what, int dtype, const pxl_ns_item* items, int n, NsPlan
       c.chunk = (int)chunk;
       c.parts = (int)((size + chunk - 1) / chunk);
       c.stride = round_up_z((size_t)plan.xplanes * c.mp * c.np * 2 + (size_t)5 * 2 * c.mp * c.mp * 2, 256);
-      sets.back().cls.push_back(c);
-      sk = (int)sets.size() - 1;
-      ck = (int)sets.back().cls.size() - 1;
+      // matrices whose recursion runs on one CU, by its two sizes, and the others: in sets of their own
+      auto kind = [](const NsClass& x) { return x.mp <= 64 ? 0 : (x.mp <= 128 ? 1 : 2); };
+      for (size_t q = 0; q < sets.size(); ++q)
+        if (kind(sets[q].cls[0]) == kind(c) && sets[q].cls.size() < (size_t)NS_MAX_CLASSES) sk = (int)q;
+      if (sk < 0) {
+        sets.emplace_back();
+        sk = (int)sets.size() - 1;
+      }
+      sets[sk].cls.push_back(c);
+      ck = (int)sets[sk].cls.size() - 1;
     }
     sets[sk].cls[ck].count++;
   }
@@ -638,7 +850,7 @@ int ns_plan(const char* what, int dtype, const pxl_ns_item* items, int n, NsPlan
   }
   for (auto& s : sets) {
     const NsSplit sp = ns_split_plan(s.cls);
-    size_t at = plan.head + (sp.splits > 1 ? (size_t)sp.splits * sp.tiles * sp.tile * sp.tile * sizeof(float) : 0);
+    size_t at = plan.head + (sp.shares > 1 || sp.small ? (size_t)sp.shares * sp.tiles * sp.tile * sp.tile * sizeof(float) : 0);
     for (auto& c : s.cls) { c.base = at; at += c.stride * c.count; }
     s.bytes = at;
     if (at > plan.bytes) plan.bytes = at;
@@ -705,8 +917,7 @@ struct NsRun {
   } while (0)
 
 template <int EPI, int NA, int NB, int T, typename OutT>
-int ns_launch(NsRun& r, const NsGemm& g, int splits) {
-  constexpr int D = T == 64 ? 4 : 2;
+int ns_launch(NsRun& r, const NsGemm& g) {
   int at = 0;
   for (int k = 0; k < r.cs.n; ++k) {
     NsClass& c = r.cs.c[k];
@@ -716,29 +927,63 @@ int ns_launch(NsRun& r, const NsGemm& g, int splits) {
     c.start = at;
     at += c.per * c.count;
   }
-  hipLaunchKernelGGL((ns_gemm_kernel<EPI, NA, NB, T, D, OutT>), dim3(at, splits), dim3(256), 0, r.st, r.cs, g, r.few, r.table, r.residue, r.ws);
+  hipLaunchKernelGGL((ns_gemm_kernel<EPI, NA, NB, T, OutT>), dim3(at, EPI == EPI_PART ? r.split.shares : 1), dim3(256), 0, r.st, r.cs, g, r.few, r.table,
+                     r.residue, r.ws);
   PXL_LAUNCH_CHECK();
-  if (EPI == EPI_PART) {
-    hipLaunchKernelGGL((ns_fold_kernel<T>), dim3(at), dim3(256), 0, r.st, r.cs, g, r.residue, r.ws);
+  if (EPI == EPI_PART && !r.split.small) {
+    hipLaunchKernelGGL((ns_fold_kernel<T>), dim3(at * (T * T / 1024)), dim3(64), 0, r.st, r.cs, g, at, r.residue, r.ws);
     PXL_LAUNCH_CHECK();
   }
   return PXL_OK;
 }
 
-// 128 x 128 tiles where they give every CU one (2048: 136 us a symmetric product with 64 x 64 tiles, see DESIGN), else 64 x 64
 template <int EPI, int NA, int NB, typename OutT>
 int ns_gemm(NsRun& r, const NsGemm& g) {
   if constexpr (EPI == EPI_GRAM) {
-    if (r.split.splits > 1) return r.split.tile == 128 ? ns_launch<EPI_PART, NA, NB, 128, OutT>(r, g, r.split.splits)
-                                                       : ns_launch<EPI_PART, NA, NB, 64, OutT>(r, g, r.split.splits);
-    return r.split.tile == 128 ? ns_launch<EPI, NA, NB, 128, OutT>(r, g, 1) : ns_launch<EPI, NA, NB, 64, OutT>(r, g, 1);
+    if (r.split.shares > 1 || r.split.small)
+      return r.split.tile == 128 ? ns_launch<EPI_PART, NA, NB, 128, OutT>(r, g) : ns_launch<EPI_PART, NA, NB, 64, OutT>(r, g);
+    return r.split.tile == 128 ? ns_launch<EPI, NA, NB, 128, OutT>(r, g) : ns_launch<EPI, NA, NB, 64, OutT>(r, g);
   }
-  long big = 0;
+  long big = 0, few = 0;
   for (int k = 0; k < r.cs.n; ++k) {
     const NsClass& c = r.cs.c[k];
     big += EPI <= EPI_MUL ? (long)sym_tiles(c.mp, 128) * c.count : (long)((c.mp + 127) / 128) * ((c.np + 127) / 128) * c.count;
+    few += EPI <= EPI_MUL ? (long)sym_tiles(c.mp, 64) * c.count : (long)((c.mp + 63) / 64) * ((c.np + 63) / 64) * c.count;
   }
-  return big >= 256 ? ns_launch<EPI, NA, NB, 128, OutT>(r, g, 1) : ns_launch<EPI, NA, NB, 64, OutT>(r, g, 1);
+  return ns_big_tiles(big, few) ? ns_launch<EPI, NA, NB, 128, OutT>(r, g) : ns_launch<EPI, NA, NB, 64, OutT>(r, g);
+}
+
+// the recursion of steps [s, e) of a small set: shares -> P in slot `out`; -> the scale of P's planes
+int ns_rec(NsRun& r, const std::vector<NsStep>& steps, size_t s, size_t e, float unscale, int res_pow, int xplanes, int out, float* sP) {
+  NsRec q;
+  memset(&q, 0, sizeof(q));
+  q.steps = (int)(e - s);
+  q.xplanes = xplanes;
+  q.out = out;
+  q.unscale = unscale;
+  q.res_pow = res_pow;
+  q.part = r.shares;
+  double pbound = 1.0;
+  for (size_t k = s; k < e; ++k) {
+    const NsStep& d = steps[k];
+    pbound *= d.q;
+    q.sA[k - s] = plane_scale(d.lam); q.sQ[k - s] = plane_scale(d.q); q.sT[k - s] = plane_scale(d.t); q.sP[k - s] = plane_scale(pbound);
+    q.a[k - s] = (float)d.a; q.b[k - s] = (float)d.b; q.c[k - s] = (float)d.c;
+  }
+  *sP = q.sP[q.steps - 1];
+  int at = 0, tiles = 0;
+  for (int k = 0; k < r.cs.n; ++k) {
+    NsClass& c = r.cs.c[k];
+    c.per = sym_tiles(c.mp, 64);
+    c.tn = tiles;                       // first tile of the class among the product's
+    c.start = at;
+    at += c.count;
+    tiles += c.per * c.count;
+  }
+  if (r.split.mt == 2) hipLaunchKernelGGL((ns_rec_kernel<2>), dim3(at), dim3(256), 0, r.st, r.cs, q, tiles, r.residue, r.ws);
+  else hipLaunchKernelGGL((ns_rec_kernel<4>), dim3(at), dim3(1024), 0, r.st, r.cs, q, tiles, r.residue, r.ws);
+  PXL_LAUNCH_CHECK();
+  return PXL_OK;
 }
 
 template <typename T, int NP>
@@ -769,7 +1014,6 @@ int ns_run_set(NsRun& r, const std::vector<NsStep>& steps, float eps, const Muon
   memset(&g, 0, sizeof(g));
   g.xplanes = xplanes;
   g.part = r.shares;
-  g.splits = r.split.splits;
   int first = 1, x = 0, x2 = NP;
   size_t s = 0;
   while (s < steps.size()) {
@@ -780,9 +1024,16 @@ int ns_run_set(NsRun& r, const std::vector<NsStep>& steps, float eps, const Muon
     g.scale = sA;
     g.res_pow = NP == 1 && first ? 2 : 0;
     NS_TRY((ns_gemm<EPI_GRAM, NP, NP, float>(r, g)));
-    g.res_pow = 0;
     int P = -1;
-    for (;; ++s) {
+    if (r.split.small) {
+      size_t e = s;
+      while (!steps[e].last) ++e;
+      P = xplanes + 2;
+      NS_TRY(ns_rec(r, steps, s, e + 1, g.unscale, g.res_pow, xplanes, P, &sP));
+      s = e;
+    }
+    g.res_pow = 0;
+    for (; !r.split.small; ++s) {
       const NsStep& d = steps[s];
       int q = xplanes + 2;
       while (q == P) ++q;
