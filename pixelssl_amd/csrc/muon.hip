@@ -33,7 +33,7 @@ typedef unsigned u32x4 __attribute__((ext_vector_type(4)));
 constexpr int NS_MAX_CLASSES = 12;      // shapes per set of launches (kernel arguments); more shapes: further sets, one after the other
 constexpr int NS_MAX_STEPS = 16;
 constexpr int NS_TABLE = 64;            // items per table-writing launch
-constexpr int NS_CHUNK = 8192;          // elements a workgroup of the norm pass takes at least
+constexpr int NS_CHUNK = 2048;          // elements a workgroup of the norm pass takes at least
 constexpr int NS_PARTS = 1024;          // partial sums of squares per matrix at most
 
 // one matrix, in device memory
@@ -145,6 +145,37 @@ __global__ __launch_bounds__(256) void ns_split_kernel(NsClasses cs, NsInline fe
   const int local = blockIdx.x - c.start, i = local / c.per, t = local - i * c.per;
   const int tr = t / c.tn, tc = t - tr * c.tn;             // 64 x 64 tile of [mp][np]
   const NsItem it = ns_item(few, table, c.first + i);
+  const T* g = reinterpret_cast<const T*>(it.g);
+  const bool tall = c.rows > c.cols;
+  // tile[r][q]: r along m, q along n; read along the memory's rows, four elements a thread -- before the norm is there
+  const int lines = tall ? c.n : c.m, line0 = tall ? tc * 64 : tr * 64, col0 = tall ? tr * 64 : tc * 64;
+  const int col = col0 + (threadIdx.x & 15) * 4, l0 = threadIdx.x >> 4;
+  float u[4][4];
+#pragma unroll
+  for (int q = 0; q < 4; ++q) {
+    const int line = line0 + l0 + q * 16;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) u[q][e] = 0.f;
+    if (line < lines) {
+      const long at = (long)line * c.cols + col;
+      if (col + 4 <= c.cols) {
+        load4(g + at, u[q]);
+        if (it.mom != nullptr) {
+          float m[4];
+          load4(it.mom + at, m);
+#pragma unroll
+          for (int e = 0; e < 4; ++e) u[q][e] = muon_update(m[e], u[q][e], a);
+        }
+      } else {
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+          if (col + e < c.cols) {
+            u[q][e] = to_f(g[at + e]);
+            if (it.mom != nullptr) u[q][e] = muon_update(it.mom[at + e], u[q][e], a);
+          }
+      }
+    }
+  }
   double s = 0.0;
   for (int e = threadIdx.x; e < c.parts; e += 256) s += part[(long)(c.first + i) * NS_PARTS + e];
 #pragma unroll
@@ -165,41 +196,14 @@ __global__ __launch_bounds__(256) void ns_split_kernel(NsClasses cs, NsInline fe
   }
   if (!(square < HUGE_VAL)) mul = nan("");                 // a NaN or an infinity in the matrix: all of its result is NaN
   if (t == 0 && threadIdx.x == 0) residue[c.first + i] = left;
-  const T* g = reinterpret_cast<const T*>(it.g);
-  const bool tall = c.rows > c.cols;
-  // tile[r][q]: r along m, q along n; read along the memory's rows, four elements a thread
-  const int lines = tall ? c.n : c.m, line0 = tall ? tc * 64 : tr * 64, col0 = tall ? tr * 64 : tc * 64;
-  const int col = col0 + (threadIdx.x & 15) * 4, l0 = threadIdx.x >> 4;
 #pragma unroll
-  for (int q = 0; q < 4; ++q) {
-    const int l = l0 + q * 16, line = line0 + l;
-    float v[4] = {0.f, 0.f, 0.f, 0.f};
-    if (line < lines) {
-      const long at = (long)line * c.cols + col;
-      if (col + 4 <= c.cols) {
-        load4(g + at, v);
-        if (it.mom != nullptr) {
-          float m[4];
-          load4(it.mom + at, m);
-#pragma unroll
-          for (int e = 0; e < 4; ++e) v[e] = muon_update(m[e], v[e], a);
-        }
-      } else {
-#pragma unroll
-        for (int e = 0; e < 4; ++e)
-          if (col + e < c.cols) {
-            v[e] = to_f(g[at + e]);
-            if (it.mom != nullptr) v[e] = muon_update(it.mom[at + e], v[e], a);
-          }
-      }
-    }
+  for (int q = 0; q < 4; ++q)
 #pragma unroll
     for (int e = 0; e < 4; ++e) {
-      const float x = (float)((double)v[e] * mul);
-      if (tall) tile[(threadIdx.x & 15) * 4 + e][l] = x;
-      else tile[l][(threadIdx.x & 15) * 4 + e] = x;
+      const float x = (float)((double)u[q][e] * mul);
+      if (tall) tile[(threadIdx.x & 15) * 4 + e][l0 + q * 16] = x;
+      else tile[l0 + q * 16][(threadIdx.x & 15) * 4 + e] = x;
     }
-  }
   __syncthreads();
   unsigned char* base = ws + c.base + (size_t)i * c.stride;
   const size_t plane = (size_t)c.mp * c.np;
@@ -243,12 +247,6 @@ struct NsGemm {
   float* part;                          // PART: [split][tile][T * T] accumulators
 };
 
-__device__ __forceinline__ void put_split(_Float16* d, size_t plane, float v) {
-  const _Float16 h = (_Float16)v;
-  d[0] = h;
-  d[plane] = (_Float16)(v - (float)h);
-}
-
 // lower-triangular tile number t -> (row, column), row >= column
 __device__ __forceinline__ void tri_tile(int t, int& r, int& q) {
   r = (int)((sqrtf(8.f * t + 1.f) - 1.f) * 0.5f);
@@ -258,18 +256,19 @@ __device__ __forceinline__ void tri_tile(int t, int& r, int& q) {
 }
 
 // Where a lane's accumulators of one 32 x 32 block lie: element e at row 8 (e / 4) + 4 (lane / 32) + e % 4, column lane % 32.
-// One block of a symmetric product at (r, q) -> both planes of the result, and its mirror image where it lies below the diagonal tiles
+// One block of a symmetric product at (r, q) -> both planes of the result: what lies on or below the diagonal, and its mirror image.  EXACTLY
+// symmetric matrices are what keeps the recursion one of commuting factors: with the two halves rounded apart, an error across strong and
+// weak directions grows by a^2 a step where a symmetric one does not grow at all (one strong direction over 1e-3: 15 % off after 5 steps).
 template <int EPI>
-__device__ __forceinline__ void ns_store_sym(const NsClass& c, const NsGemm& p, const _Float16* A, _Float16* out, int r, int q, bool mirror, float un,
-                                             const f32x16& acc) {
+__device__ __forceinline__ void ns_store_sym(const NsClass& c, const NsGemm& p, const _Float16* A, _Float16* out, int r, int q, float un, const f32x16& acc) {
   const int lane = threadIdx.x & 63;
+  if (r >= c.mp || q >= c.mp || r < q) return;                // (blocks are 32 wide, mp is a multiple of 32; a block above the diagonal)
   const size_t pm = (size_t)c.mp * c.mp;
   q += lane & 31;
   r += 4 * (lane >> 5);
 #pragma unroll
   for (int e4 = 0; e4 < 4; ++e4) {
     const int r0 = r + 8 * e4;
-    if (r0 >= c.mp || q >= c.mp) continue;                    // (mp is a multiple of 32)
     f16x4 h, l;
 #pragma unroll
     for (int e = 0; e < 4; ++e) {
@@ -282,13 +281,22 @@ __device__ __forceinline__ void ns_store_sym(const NsClass& c, const NsGemm& p, 
       const float x = val * p.scale;
       h[e] = (_Float16)x;
       l[e] = (_Float16)(x - (float)h[e]);
-      d[0] = h[e];
-      d[pm] = l[e];
+      if (r0 + e >= q) {
+        d[0] = h[e];
+        d[pm] = l[e];
+      }
     }
-    if (mirror) {
-      _Float16* d = out + (size_t)q * c.mp + r0;
+    _Float16* d = out + (size_t)q * c.mp + r0;
+    if (r0 > q) {
       *reinterpret_cast<f16x4*>(d) = h;
       *reinterpret_cast<f16x4*>(d + pm) = l;
+    } else {
+#pragma unroll
+      for (int e = 1; e < 4; ++e)
+        if (r0 + e > q) {
+          d[e] = h[e];
+          d[pm + e] = l[e];
+        }
     }
   }
 }
@@ -513,7 +521,7 @@ __global__ __launch_bounds__(256, 2) void ns_gemm_kernel(NsClasses cs, NsGemm p,
   const float un = p.unscale * (p.res_pow == 0 ? 1.f : (p.res_pow == 2 ? rs * rs : rs));
   _Float16* out = reinterpret_cast<_Float16*>(base + slot_off(c, p.xplanes, p.job.out));
   if constexpr (SYM) {
-    blocks([&](int, int r, int q, const f32x16& a) { ns_store_sym<EPI>(c, p, A, out, r, q, tr != tc, un, a); });
+    blocks([&](int, int r, int q, const f32x16& a) { ns_store_sym<EPI>(c, p, A, out, r, q, un, a); });
   } else if constexpr (EPI == EPI_X) {
     // through LDS, one plane after the other: rows of T columns, 16-byte stores.  Lane: row lane % 32, columns 8 e4 + 4 (lane / 32) + 0 .. 3
     constexpr int PITCH = T + 8;
@@ -548,28 +556,44 @@ __global__ __launch_bounds__(256, 2) void ns_gemm_kernel(NsClasses cs, NsGemm p,
     const NsItem it = ns_item(few, table, c.first + i);
     const bool tall = c.rows > c.cols;
     const float f = p.muon ? -p.lr * it.scale : 1.f;
-    blocks([&](int, int r, int qb, const f32x16& a) {
+    OutT* o = reinterpret_cast<OutT*>(it.p);
+    // element (r, q) of [m][n]; four consecutive r of a lane are consecutive in memory where the matrix is tall
+    auto place = [&](int r, int q) { return tall ? (size_t)q * c.cols + r : (size_t)r * c.cols + q; };
+    // a Muon step's parameters are read before any is written: one wait for all of them (interleaved: 53 us in place of 37 for 3 x 512 x 4608)
+    f32x16 old[T == 64 ? 1 : 4];
+    if (p.muon) {
+      blocks([&](int n, int r, int qb, const f32x16&) {
+        f32x16& w = old[T == 64 ? 0 : n & 3];
+#pragma unroll
+        for (int e4 = 0; e4 < 4; ++e4) {
+          const int r0 = r + 8 * e4 + 4 * (lane >> 5), q = qb + (lane & 31);
+          if (tall && r0 + 4 <= c.m && q < c.n) {
+            float v[4];
+            load4(o + place(r0, q), v);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) w[e4 * 4 + e] = v[e];
+          } else {
+#pragma unroll
+            for (int e = 0; e < 4; ++e) w[e4 * 4 + e] = r0 + e < c.m && q < c.n ? to_f(o[place(r0 + e, q)]) : 0.f;
+          }
+        }
+      });
+    }
+    blocks([&](int n, int r, int qb, const f32x16& a) {
+      const f32x16& w = old[T == 64 ? 0 : n & 3];
 #pragma unroll
       for (int e4 = 0; e4 < 4; ++e4) {
         const int r0 = r + 8 * e4 + 4 * (lane >> 5), q = qb + (lane & 31);
         if (r0 >= c.m || q >= c.n) continue;
         float val[4];
 #pragma unroll
-        for (int e = 0; e < 4; ++e) val[e] = a[e4 * 4 + e] * un * f;
-        OutT* o = reinterpret_cast<OutT*>(it.p) + (tall ? (size_t)q * c.cols + r0 : (size_t)r0 * c.cols + q);
+        for (int e = 0; e < 4; ++e) val[e] = a[e4 * 4 + e] * un * f + (p.muon ? w[e4 * 4 + e] * p.decay : 0.f);
         if (tall && r0 + 4 <= c.m) {
-          float old[4];
-          if (p.muon) {
-            load4(o, old);
-#pragma unroll
-            for (int e = 0; e < 4; ++e) val[e] += old[e] * p.decay;
-          }
-          store4(o, val);
+          store4(o + place(r0, q), val);
         } else {
-          const size_t ld = tall ? 1 : c.cols;
 #pragma unroll
           for (int e = 0; e < 4; ++e)
-            if (r0 + e < c.m) o[e * ld] = from_f<OutT>(p.muon ? to_f(o[e * ld]) * p.decay + val[e] : val[e]);
+            if (r0 + e < c.m) o[place(r0 + e, q)] = from_f<OutT>(val[e]);
         }
       }
     });
@@ -612,7 +636,7 @@ __global__ __launch_bounds__(64) void ns_fold_kernel(NsClasses cs, NsGemm p, int
   const f32x16 a = ns_share_sum<4>(p.part, ns_shares(c), (size_t)tiles * NBL, (size_t)bid * NBL + n);
   const float rs = residue[c.first + i];
   _Float16* out = reinterpret_cast<_Float16*>(ws + c.base + (size_t)i * c.stride + slot_off(c, p.xplanes, p.job.out));
-  ns_store_sym<EPI_GRAM>(c, p, nullptr, out, tr * T + br * 32, tc * T + bc * 32, tr != tc, p.unscale * (p.res_pow == 2 ? rs * rs : 1.f), a);
+  ns_store_sym<EPI_GRAM>(c, p, nullptr, out, tr * T + br * 32, tc * T + bc * 32, p.unscale * (p.res_pow == 2 ? rs * rs : 1.f), a);
 }
 
 // ---- a whole segment's recursion for matrices of at most 32 MT rows: one workgroup of MT^2 waves a matrix, everything on the CU ----------
@@ -634,33 +658,36 @@ __global__ __launch_bounds__(MT * MT * 64) void ns_rec_kernel(NsClasses cs, NsRe
   const NsClass& c = cs.c[k];
   const int i = blockIdx.x - c.start;
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, I = wave / MT, J = wave % MT;
-  const bool inside = I * 32 < c.mp && J * 32 < c.mp;               // mp is a multiple of 32
+  const bool inside = I * 32 < c.mp && J <= I;                      // (mp is a multiple of 32); waves above the diagonal only wait
   // 16-byte chunk ch of row r
   auto at = [](int r, int ch) { return r * ROW + ((MT == 2 ? ch ^ ((r >> 1) & 7) : ch ^ (r & 15)) << 4); };
   auto elem = [&](int r, int q) { return at(r, q >> 3) + (q & 7) * 2; };
-  auto put = [&](int slot, const f32x16& v, float s, bool mirror) {
+  // a block on or below the diagonal and its mirror image (ns_store_sym says why): elements (r0 .. r0 + 3, q) are one 8-byte access there
+  auto put = [&](int slot, const f32x16& v, float s) {
 #pragma unroll
     for (int e4 = 0; e4 < 4; ++e4) {
-      f16x4 h, l;
       const int r0 = I * 32 + 8 * e4 + 4 * (lane >> 5), q = J * 32 + (lane & 31);
+      f16x4 h, l;
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
         const float x = v[e4 * 4 + e] * s;
         h[e] = (_Float16)x;
         l[e] = (_Float16)(x - (float)h[e]);
-        if (!mirror || I == J) {
+        if (r0 + e >= q) {
           *reinterpret_cast<_Float16*>(&lds[slot][elem(r0 + e, q)]) = h[e];
           *reinterpret_cast<_Float16*>(&lds[slot][PL + elem(r0 + e, q)]) = l[e];
         }
       }
-      if (mirror && I != J) {           // row q, columns r0 .. r0 + 3, and the block itself
+      if (r0 > q) {
         *reinterpret_cast<f16x4*>(&lds[slot][elem(q, r0)]) = h;
         *reinterpret_cast<f16x4*>(&lds[slot][PL + elem(q, r0)]) = l;
+      } else {
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          *reinterpret_cast<_Float16*>(&lds[slot][elem(r0 + e, q)]) = h[e];
-          *reinterpret_cast<_Float16*>(&lds[slot][PL + elem(r0 + e, q)]) = l[e];
-        }
+        for (int e = 1; e < 4; ++e)
+          if (r0 + e > q) {
+            *reinterpret_cast<_Float16*>(&lds[slot][elem(q, r0 + e)]) = h[e];
+            *reinterpret_cast<_Float16*>(&lds[slot][PL + elem(q, r0 + e)]) = l[e];
+          }
       }
     }
   };
@@ -684,13 +711,12 @@ __global__ __launch_bounds__(MT * MT * 64) void ns_rec_kernel(NsClasses cs, NsRe
   f32x16 P, V;
 #pragma unroll
   for (int e = 0; e < 16; ++e) P[e] = V[e] = 0.f;
-  // A from the shares of the 64 x 64 tiles on and below the diagonal; blocks above it by mirroring
-  if (inside && (I >> 1) >= (J >> 1)) {
+  if (inside) {                         // A from the shares of the 64 x 64 tiles on and below the diagonal
     const int t = (I >> 1) * ((I >> 1) + 1) / 2 + (J >> 1);
     V = ns_share_sum<MT == 2 ? 4 : 2>(p.part, ns_shares(c), (size_t)tiles * 4, ((size_t)c.tn + (size_t)i * c.per + t) * 4 + (I & 1) * 2 + (J & 1));
 #pragma unroll
     for (int e = 0; e < 16; ++e) V[e] *= un;
-    if (I >= J) put(0, V, p.sA[0], true);
+    put(0, V, p.sA[0]);
   }
   __syncthreads();
   for (int s = 0; s < p.steps; ++s) {
@@ -698,14 +724,18 @@ __global__ __launch_bounds__(MT * MT * 64) void ns_rec_kernel(NsClasses cs, NsRe
       const f32x16 acc = product(0, 0);
       const float g = p.c[s] / (p.sA[s] * p.sA[s]), ia = p.b[s] / p.sA[s];
 #pragma unroll
-      for (int e = 0; e < 16; ++e) {
-        const int r = I * 32 + 8 * (e >> 2) + 4 * (lane >> 5) + (e & 3), q = J * 32 + (lane & 31), o = elem(r, q);
-        const float am = (float)*reinterpret_cast<const _Float16*>(&lds[0][o]) + (float)*reinterpret_cast<const _Float16*>(&lds[0][PL + o]);
-        V[e] = g * acc[e] + ia * am + (r == q ? p.a[s] : 0.f);
+      for (int e4 = 0; e4 < 4; ++e4) {
+        const int o = elem(J * 32 + (lane & 31), I * 32 + 8 * e4 + 4 * (lane >> 5));          // (the mirror image: one access)
+        const f16x4 h = *reinterpret_cast<const f16x4*>(&lds[0][o]), l = *reinterpret_cast<const f16x4*>(&lds[0][PL + o]);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const int r = I * 32 + 8 * e4 + 4 * (lane >> 5) + e, q = J * 32 + (lane & 31);
+          V[e4 * 4 + e] = g * acc[e4 * 4 + e] + ia * ((float)h[e] + (float)l[e]) + (r == q ? p.a[s] : 0.f);
+        }
       }
     }
     // (slot 1 is free: its last readers have passed a barrier since)
-    if (inside) put(1, V, p.sQ[s], false);
+    if (inside) put(1, V, p.sQ[s]);
     __syncthreads();
     const bool last = s + 1 == p.steps;
     f32x16 tq;
@@ -716,7 +746,7 @@ __global__ __launch_bounds__(MT * MT * 64) void ns_rec_kernel(NsClasses cs, NsRe
       P = V;
     } else {
       __syncthreads();
-      if (inside) put(0, P, p.sP[s - 1], false);
+      if (inside) put(0, P, p.sP[s - 1]);
       __syncthreads();
       if (inside) {
         P = product(1, 0);
@@ -731,7 +761,7 @@ __global__ __launch_bounds__(MT * MT * 64) void ns_rec_kernel(NsClasses cs, NsRe
       const float f = 1.f / (p.sQ[s] * p.sA[s]);
 #pragma unroll
       for (int e = 0; e < 16; ++e) tq[e] *= f;
-      put(0, tq, p.sT[s], false);
+      put(0, tq, p.sT[s]);
     }
     __syncthreads();
     if (inside) {
@@ -741,16 +771,14 @@ __global__ __launch_bounds__(MT * MT * 64) void ns_rec_kernel(NsClasses cs, NsRe
       for (int e = 0; e < 16; ++e) V[e] *= f;
     }
     __syncthreads();
-    if (inside && I >= J) put(0, V, p.sA[s + 1], true);
+    if (inside) put(0, V, p.sA[s + 1]);
     __syncthreads();
   }
   if (!inside) return;
   _Float16* out = reinterpret_cast<_Float16*>(ws + c.base + (size_t)i * c.stride + slot_off(c, p.xplanes, p.out));
-  const size_t pm = (size_t)c.mp * c.mp;
-  const float sp = p.sP[p.steps - 1];
-#pragma unroll
-  for (int e = 0; e < 16; ++e)
-    put_split(out + (size_t)(I * 32 + 8 * (e >> 2) + 4 * (lane >> 5) + (e & 3)) * c.mp + J * 32 + (lane & 31), pm, P[e] * sp);
+  NsGemm g;                             // (P as a product of the other kernels would be stored)
+  g.scale = p.sP[p.steps - 1];
+  ns_store_sym<EPI_MUL>(c, g, nullptr, out, I * 32, J * 32, 1.f, P);
 }
 
 // ---- host ---------------------------------------------------------------------------------------------------------------------
@@ -763,8 +791,9 @@ struct NsPlan {
   size_t bytes;
 };
 
-// 128 x 128 tiles or four times as many of 64 x 64: rounds over the 256 CUs, a small tile at 0.3 of a large one's time
-inline bool ns_big_tiles(long big, long few) { return (big + 255) / 256 * 10 <= (few + 255) / 256 * 3 && big >= 128; }
+// 128 x 128 tiles or about four times as many of 64 x 64, by rounds over the 256 CUs: a small tile takes 0.4 of a large one's time (23 x P X of
+// 256 x 2304: 39 us in 828 large, 51 us in 3312 small tiles; 2 products of 2048^3, symmetric: 105 us in 272 large, 106 us in 1056 small)
+inline bool ns_big_tiles(long big, long few) { return (big + 255) / 256 * 10 <= (few + 255) / 256 * 4 && big >= 128; }
 
 inline int round_up(int v, int to) { return (v + to - 1) / to * to; }
 inline size_t round_up_z(size_t v, size_t to) { return (v + to - 1) / to * to; }
@@ -783,7 +812,7 @@ NsSplit ns_split_plan(std::vector<NsClass>& cls) {
     if (c.mp > 64) r.mt = 4;
     if (c.mp > 128) r.small = 0;
   }
-  if (!r.small && ns_big_tiles(big, few)) r.tile = 128;
+  if (!r.small && big * 10 <= few * 4) r.tile = 128;       // (shares fill the chip: the work alone counts)
   const long tiles = r.tile == 128 ? big : few;
   r.tiles = (int)tiles;
   const long want = tiles < 384 ? (512 + tiles - 1) / tiles : 1;
