@@ -71,11 +71,16 @@ struct NsClass {
 };
 struct NsClasses { NsClass c[NS_MAX_CLASSES]; int n; };
 
-__device__ __forceinline__ int find_class(const NsClasses& cs, int b) {
-  int k = 0;
+// the class of workgroup b, by value: the first one's fields are fetched together with the other arguments (one shape: no further round trip)
+__device__ __forceinline__ NsClass find_class(const NsClasses& cs, int b) {
+  NsClass c = cs.c[0];
+  if (cs.n > 1 && b >= cs.c[1].start) {
+    int k = 1;
 #pragma unroll 1
-  while (k + 1 < cs.n && b >= cs.c[k + 1].start) ++k;
-  return k;
+    while (k + 1 < cs.n && b >= cs.c[k + 1].start) ++k;
+    c = cs.c[k];
+  }
+  return c;
 }
 
 __global__ void ns_table_kernel(NsTable t, int n, NsItem* __restrict__ dst) {
@@ -93,8 +98,7 @@ __device__ __forceinline__ float muon_update(float m, float g, const MuonArgs& a
 template <typename T>
 __global__ __launch_bounds__(256) void ns_norm_kernel(NsClasses cs, NsInline few, const NsItem* __restrict__ table, double* __restrict__ part, MuonArgs a) {
   __shared__ double sh[4];
-  const int k = find_class(cs, blockIdx.x);
-  const NsClass& c = cs.c[k];
+  const NsClass c = find_class(cs, blockIdx.x);
   const int local = blockIdx.x - c.start, i = local / c.per, j = local - i * c.per;
   const NsItem it = ns_item(few, table, c.first + i);
   const long size = (long)c.rows * c.cols, lo = (long)j * c.chunk, hi = lo + c.chunk < size ? lo + c.chunk : size;
@@ -140,8 +144,7 @@ __global__ __launch_bounds__(256) void ns_split_kernel(NsClasses cs, NsInline fe
                                                        float* __restrict__ residue, unsigned char* __restrict__ ws, float eps, float sx, MuonArgs a) {
   __shared__ double shn[4];
   __shared__ float tile[64][65];
-  const int k = find_class(cs, blockIdx.x);
-  const NsClass& c = cs.c[k];
+  const NsClass c = find_class(cs, blockIdx.x);
   const int local = blockIdx.x - c.start, i = local / c.per, t = local - i * c.per;
   const int tr = t / c.tn, tc = t - tr * c.tn;             // 64 x 64 tile of [mp][np]
   const NsItem it = ns_item(few, table, c.first + i);
@@ -259,8 +262,27 @@ __device__ __forceinline__ void tri_tile(int t, int& r, int& q) {
 // One block of a symmetric product at (r, q) -> both planes of the result: what lies on or below the diagonal, and its mirror image.  EXACTLY
 // symmetric matrices are what keeps the recursion one of commuting factors: with the two halves rounded apart, an error across strong and
 // weak directions grows by a^2 a step where a symmetric one does not grow at all (one strong direction over 1e-3: 15 % off after 5 steps).
+// (A's elements of the block, EPI_Q, come from there too: four at a time)
+struct NsOld { f16x4 h[4], l[4]; };
+__device__ __forceinline__ NsOld ns_load_sym(const NsClass& c, const _Float16* A, int r, int q) {
+  const int lane = threadIdx.x & 63;
+  const size_t pm = (size_t)c.mp * c.mp;
+  NsOld o;
+  if (r >= c.mp || q >= c.mp || r < q) {
+#pragma unroll
+    for (int e4 = 0; e4 < 4; ++e4) o.h[e4] = o.l[e4] = f16x4{0, 0, 0, 0};
+    return o;
+  }
+  const _Float16* a = A + (size_t)(q + (lane & 31)) * c.mp + r + 4 * (lane >> 5);
+#pragma unroll
+  for (int e4 = 0; e4 < 4; ++e4) {
+    o.h[e4] = *reinterpret_cast<const f16x4*>(a + 8 * e4);
+    o.l[e4] = *reinterpret_cast<const f16x4*>(a + pm + 8 * e4);
+  }
+  return o;
+}
 template <int EPI>
-__device__ __forceinline__ void ns_store_sym(const NsClass& c, const NsGemm& p, const _Float16* A, _Float16* out, int r, int q, float un, const f32x16& acc) {
+__device__ __forceinline__ void ns_store_sym(const NsClass& c, const NsGemm& p, const NsOld& old, _Float16* out, int r, int q, float un, const f32x16& acc) {
   const int lane = threadIdx.x & 63;
   if (r >= c.mp || q >= c.mp || r < q) return;                // (blocks are 32 wide, mp is a multiple of 32; a block above the diagonal)
   const size_t pm = (size_t)c.mp * c.mp;
@@ -274,10 +296,7 @@ __device__ __forceinline__ void ns_store_sym(const NsClass& c, const NsGemm& p, 
     for (int e = 0; e < 4; ++e) {
       float val = acc[e4 * 4 + e] * un;
       _Float16* d = out + (size_t)(r0 + e) * c.mp + q;
-      if (EPI == EPI_Q) {
-        const _Float16* am = A + (size_t)(r0 + e) * c.mp + q;
-        val = p.qc * val + p.qb * (((float)am[0] + (float)am[pm]) * p.sa_inv) + (r0 + e == q ? p.qa : 0.f);
-      }
+      if (EPI == EPI_Q) val = p.qc * val + p.qb * (((float)old.h[e4][e] + (float)old.l[e4][e]) * p.sa_inv) + (r0 + e == q ? p.qa : 0.f);
       const float x = val * p.scale;
       h[e] = (_Float16)x;
       l[e] = (_Float16)(x - (float)h[e]);
@@ -304,7 +323,7 @@ __device__ __forceinline__ void ns_store_sym(const NsClass& c, const NsGemm& p, 
 // One T x T tile per workgroup of 4 waves.  T = 128: K steps of 32, the waves 2 x 2 on the tile.  T = 64 (few tiles): K steps of 64, each wave
 // takes 16 of them for the WHOLE tile and the four sums are added at the end in order: an LDS read feeds as many matrix instructions as with
 // T = 128 (32 x 32 a wave would be bound by LDS reads), and a barrier stands between 12 of them instead of 6.
-// Global memory -> registers, D steps ahead -> LDS, two buffers, one barrier a step.  LDS images: rows of one K step for a, and for b in [j][k],
+// Global memory -> registers, D steps ahead (2; 4 in launches of at most a workgroup per CU, which then have all registers) -> LDS, two buffers, one barrier a step.  LDS images: rows of one K step for a, and for b in [j][k],
 // 16-byte chunks permuted within the row; rows of T columns per k for b in [k][j], 32-byte segments permuted, read with the transposing LDS load
 // (within 16 lanes, lane j receives 16-bit slot j % 4 of lanes j / 4 + 4 e): 4 k of one column.  The permutations keep every group of lanes that
 // is served at once on different banks.
@@ -314,19 +333,17 @@ template <int T> __device__ __forceinline__ int chunk_at(int r, int ch) {       
 template <int T> __device__ __forceinline__ int segment_at(int k, int seg) {       // byte of 32-byte segment seg of row k
   return T == 128 ? k * 256 + ((seg ^ ((k & 3) << 1)) << 5) : k * 128 + ((seg ^ (k & 2)) << 5);
 }
-template <int EPI, int NA, int NB, int T, typename OutT>
-__global__ __launch_bounds__(256, 2) void ns_gemm_kernel(NsClasses cs, NsGemm p, NsInline few, const NsItem* __restrict__ table,
+template <int EPI, int NA, int NB, int T, int D, typename OutT>
+__global__ __launch_bounds__(256, D == 2 ? 2 : 1) void ns_gemm_kernel(NsClasses cs, NsGemm p, NsInline few, const NsItem* __restrict__ table,
                                                          const float* __restrict__ residue, unsigned char* __restrict__ ws) {
   constexpr bool SYM = EPI <= EPI_MUL, NN = EPI >= EPI_X;
   constexpr int KS = T == 128 ? 32 : 64;        // k a step
-  constexpr int D = 2;                          // (3 with T = 64: 16 registers spilled)
   constexpr int PL = T * KS * 2;                // bytes of one plane's tile
   constexpr int BUF = (NA + NB) * PL;
   constexpr int WB = T == 128 ? 1 : 2;          // blocks of 32 x 32 a wave ends up with: 4 / 1
   __shared__ __attribute__((aligned(16))) unsigned char lds[T == 64 && 2 * BUF < 65536 ? 65536 : 2 * BUF];
   const int bid = xcd_remap(blockIdx.x, gridDim.x);
-  const int k = find_class(cs, bid);
-  const NsClass& c = cs.c[k];
+  const NsClass c = find_class(cs, bid);
   const int local = bid - c.start, i = local / c.per, t = local - i * c.per;
   int tr, tc;
   if (SYM) tri_tile(t, tr, tc);
@@ -407,6 +424,8 @@ __global__ __launch_bounds__(256, 2) void ns_gemm_kernel(NsClasses cs, NsGemm p,
     fetch(d);
     __builtin_amdgcn_sched_barrier(0);          // (in this order: the waits count)
   }
+  NsOld old[EPI == EPI_Q && T == 128 ? 4 : 1];
+  if (EPI == EPI_Q && T == 64) old[0] = ns_load_sym(c, A, tr * 64 + wr * 32, tc * 64 + wc * 32);
   auto multiply = [&](const unsigned char* buf, int kk) {           // k 16 kk .. 16 kk + 15 of the step
     f16x8 fa[NA][2], fb[NB][2];
     const int ro = T == 128 ? wr * 64 : 0, qo = T == 128 ? wc * 64 : 0, ch = kk * 2 + (lane >> 5);
@@ -517,11 +536,15 @@ __global__ __launch_bounds__(256, 2) void ns_gemm_kernel(NsClasses cs, NsGemm p,
     });
     return;
   }
-  const float rs = residue[c.first + i];
-  const float un = p.unscale * (p.res_pow == 0 ? 1.f : (p.res_pow == 2 ? rs * rs : rs));
+  float un = p.unscale;
+  if (EPI != EPI_Q && EPI != EPI_MUL && p.res_pow) {
+    const float rs = residue[c.first + i];
+    un *= p.res_pow == 2 ? rs * rs : rs;
+  }
   _Float16* out = reinterpret_cast<_Float16*>(base + slot_off(c, p.xplanes, p.job.out));
   if constexpr (SYM) {
-    blocks([&](int, int r, int q, const f32x16& a) { ns_store_sym<EPI>(c, p, A, out, r, q, un, a); });
+    if (EPI == EPI_Q && T == 128) blocks([&](int n, int r, int q, const f32x16&) { old[EPI == EPI_Q && T == 128 ? n & 3 : 0] = ns_load_sym(c, A, r, q); });
+    blocks([&](int n, int r, int q, const f32x16& a) { ns_store_sym<EPI>(c, p, old[EPI == EPI_Q && T == 128 ? n & 3 : 0], out, r, q, un, a); });
   } else if constexpr (EPI == EPI_X) {
     // through LDS, one plane after the other: rows of T columns, 16-byte stores.  Lane: row lane % 32, columns 8 e4 + 4 (lane / 32) + 0 .. 3
     constexpr int PITCH = T + 8;
@@ -560,10 +583,10 @@ __global__ __launch_bounds__(256, 2) void ns_gemm_kernel(NsClasses cs, NsGemm p,
     // element (r, q) of [m][n]; four consecutive r of a lane are consecutive in memory where the matrix is tall
     auto place = [&](int r, int q) { return tall ? (size_t)q * c.cols + r : (size_t)r * c.cols + q; };
     // a Muon step's parameters are read before any is written: one wait for all of them (interleaved: 53 us in place of 37 for 3 x 512 x 4608)
-    f32x16 old[T == 64 ? 1 : 4];
+    f32x16 was[T == 64 ? 1 : 4];
     if (p.muon) {
       blocks([&](int n, int r, int qb, const f32x16&) {
-        f32x16& w = old[T == 64 ? 0 : n & 3];
+        f32x16& w = was[T == 64 ? 0 : n & 3];
 #pragma unroll
         for (int e4 = 0; e4 < 4; ++e4) {
           const int r0 = r + 8 * e4 + 4 * (lane >> 5), q = qb + (lane & 31);
@@ -580,7 +603,7 @@ __global__ __launch_bounds__(256, 2) void ns_gemm_kernel(NsClasses cs, NsGemm p,
       });
     }
     blocks([&](int n, int r, int qb, const f32x16& a) {
-      const f32x16& w = old[T == 64 ? 0 : n & 3];
+      const f32x16& w = was[T == 64 ? 0 : n & 3];
 #pragma unroll
       for (int e4 = 0; e4 < 4; ++e4) {
         const int r0 = r + 8 * e4 + 4 * (lane >> 5), q = qb + (lane & 31);
@@ -625,8 +648,7 @@ template <int T>
 __global__ __launch_bounds__(64) void ns_fold_kernel(NsClasses cs, NsGemm p, int tiles, const float* __restrict__ residue, unsigned char* __restrict__ ws) {
   constexpr int NBL = T * T / 1024, SIDE = T / 32;
   const int bid = blockIdx.x / NBL, n = blockIdx.x % NBL;
-  const int k = find_class(cs, bid);
-  const NsClass& c = cs.c[k];
+  const NsClass c = find_class(cs, bid);
   const int local = bid - c.start, i = local / c.per, t = local - i * c.per;
   int tr, tc;
   tri_tile(t, tr, tc);
@@ -636,7 +658,7 @@ __global__ __launch_bounds__(64) void ns_fold_kernel(NsClasses cs, NsGemm p, int
   const f32x16 a = ns_share_sum<4>(p.part, ns_shares(c), (size_t)tiles * NBL, (size_t)bid * NBL + n);
   const float rs = residue[c.first + i];
   _Float16* out = reinterpret_cast<_Float16*>(ws + c.base + (size_t)i * c.stride + slot_off(c, p.xplanes, p.job.out));
-  ns_store_sym<EPI_GRAM>(c, p, nullptr, out, tr * T + br * 32, tc * T + bc * 32, p.unscale * (p.res_pow == 2 ? rs * rs : 1.f), a);
+  ns_store_sym<EPI_GRAM>(c, p, NsOld(), out, tr * T + br * 32, tc * T + bc * 32, p.unscale * (p.res_pow == 2 ? rs * rs : 1.f), a);
 }
 
 // ---- a whole segment's recursion for matrices of at most 32 MT rows: one workgroup of MT^2 waves a matrix, everything on the CU ----------
@@ -653,17 +675,20 @@ struct NsRec {
 template <int MT>
 __global__ __launch_bounds__(MT * MT * 64) void ns_rec_kernel(NsClasses cs, NsRec p, int tiles, const float* __restrict__ residue, unsigned char* __restrict__ ws) {
   constexpr int M = 32 * MT, ROW = M * 2, PL = M * ROW;             // bytes
-  __shared__ __attribute__((aligned(16))) unsigned char lds[2][2 * PL];
-  const int k = find_class(cs, blockIdx.x);
-  const NsClass& c = cs.c[k];
+  constexpr int SLOT = 2 * PL + 16;                                 // both planes, and the place nobody reads
+  __shared__ __attribute__((aligned(16))) unsigned char lds[2 * SLOT];
+  const NsClass c = find_class(cs, blockIdx.x);
   const int i = blockIdx.x - c.start;
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, I = wave / MT, J = wave % MT;
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), I = wave / MT, J = wave % MT;
   const bool inside = I * 32 < c.mp && J <= I;                      // (mp is a multiple of 32); waves above the diagonal only wait
   // 16-byte chunk ch of row r
   auto at = [](int r, int ch) { return r * ROW + ((MT == 2 ? ch ^ ((r >> 1) & 7) : ch ^ (r & 15)) << 4); };
   auto elem = [&](int r, int q) { return at(r, q >> 3) + (q & 7) * 2; };
   // a block on or below the diagonal and its mirror image (ns_store_sym says why): elements (r0 .. r0 + 3, q) are one 8-byte access there
+  // (on the diagonal what the other triangle holds goes to a place nobody reads: two writes in place of two branches an element)
+  const int nowhere = 2 * PL;
   auto put = [&](int slot, const f32x16& v, float s) {
+    unsigned char* at0 = lds + slot * SLOT;
 #pragma unroll
     for (int e4 = 0; e4 < 4; ++e4) {
       const int r0 = I * 32 + 8 * e4 + 4 * (lane >> 5), q = J * 32 + (lane & 31);
@@ -673,36 +698,44 @@ __global__ __launch_bounds__(MT * MT * 64) void ns_rec_kernel(NsClasses cs, NsRe
         const float x = v[e4 * 4 + e] * s;
         h[e] = (_Float16)x;
         l[e] = (_Float16)(x - (float)h[e]);
-        if (r0 + e >= q) {
-          *reinterpret_cast<_Float16*>(&lds[slot][elem(r0 + e, q)]) = h[e];
-          *reinterpret_cast<_Float16*>(&lds[slot][PL + elem(r0 + e, q)]) = l[e];
-        }
       }
-      if (r0 > q) {
-        *reinterpret_cast<f16x4*>(&lds[slot][elem(q, r0)]) = h;
-        *reinterpret_cast<f16x4*>(&lds[slot][PL + elem(q, r0)]) = l;
+      if (I != J) {
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          *reinterpret_cast<_Float16*>(at0 + elem(r0 + e, q)) = h[e];
+          *reinterpret_cast<_Float16*>(at0 + PL + elem(r0 + e, q)) = l[e];
+        }
+        *reinterpret_cast<f16x4*>(at0 + elem(q, r0)) = h;
+        *reinterpret_cast<f16x4*>(at0 + PL + elem(q, r0)) = l;
       } else {
 #pragma unroll
-        for (int e = 1; e < 4; ++e)
-          if (r0 + e > q) {
-            *reinterpret_cast<_Float16*>(&lds[slot][elem(q, r0 + e)]) = h[e];
-            *reinterpret_cast<_Float16*>(&lds[slot][PL + elem(q, r0 + e)]) = l[e];
-          }
+        for (int e = 0; e < 4; ++e) {
+          const int o1 = r0 + e >= q ? elem(r0 + e, q) : nowhere, o2 = r0 + e > q ? elem(q, r0 + e) : nowhere;
+          const int low = PL;
+          *reinterpret_cast<_Float16*>(at0 + o1) = h[e];
+          *reinterpret_cast<_Float16*>(at0 + o2) = h[e];
+          *reinterpret_cast<_Float16*>(at0 + (r0 + e >= q ? o1 + low : nowhere)) = l[e];
+          *reinterpret_cast<_Float16*>(at0 + (r0 + e > q ? o2 + low : nowhere)) = l[e];
+        }
       }
     }
   };
   auto product = [&](int x, int y) {
+    const unsigned char *px = lds + x * SLOT, *py = lds + y * SLOT;
     f32x16 acc;
 #pragma unroll
     for (int e = 0; e < 16; ++e) acc[e] = 0.f;
-#pragma unroll 2
-    for (int kk = 0; kk < 2 * MT && kk * 16 < c.mp; ++kk) {
+    auto slice = [&](int kk) {
       const int ch = kk * 2 + (lane >> 5), r = I * 32 + (lane & 31), q = J * 32 + (lane & 31);
-      const f16x8 xh = *reinterpret_cast<const f16x8*>(&lds[x][at(r, ch)]), xl = *reinterpret_cast<const f16x8*>(&lds[x][PL + at(r, ch)]);
-      const f16x8 yh = *reinterpret_cast<const f16x8*>(&lds[y][at(q, ch)]), yl = *reinterpret_cast<const f16x8*>(&lds[y][PL + at(q, ch)]);
+      const f16x8 xh = *reinterpret_cast<const f16x8*>(px + at(r, ch)), xl = *reinterpret_cast<const f16x8*>(px + PL + at(r, ch));
+      const f16x8 yh = *reinterpret_cast<const f16x8*>(py + at(q, ch)), yl = *reinterpret_cast<const f16x8*>(py + PL + at(q, ch));
       acc = __builtin_amdgcn_mfma_f32_32x32x16_f16(xh, yl, acc, 0, 0, 0);
       acc = __builtin_amdgcn_mfma_f32_32x32x16_f16(xl, yh, acc, 0, 0, 0);
       acc = __builtin_amdgcn_mfma_f32_32x32x16_f16(xh, yh, acc, 0, 0, 0);
+    };
+    for (int k2 = 0; k2 < c.mp; k2 += 32) {             // (mp is a multiple of 32)
+      slice(k2 / 16);
+      slice(k2 / 16 + 1);
     }
     return acc;
   };
@@ -726,7 +759,7 @@ __global__ __launch_bounds__(MT * MT * 64) void ns_rec_kernel(NsClasses cs, NsRe
 #pragma unroll
       for (int e4 = 0; e4 < 4; ++e4) {
         const int o = elem(J * 32 + (lane & 31), I * 32 + 8 * e4 + 4 * (lane >> 5));          // (the mirror image: one access)
-        const f16x4 h = *reinterpret_cast<const f16x4*>(&lds[0][o]), l = *reinterpret_cast<const f16x4*>(&lds[0][PL + o]);
+        const f16x4 h = *reinterpret_cast<const f16x4*>(lds + o), l = *reinterpret_cast<const f16x4*>(lds + PL + o);
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
           const int r = I * 32 + 8 * e4 + 4 * (lane >> 5) + e, q = J * 32 + (lane & 31);
@@ -778,7 +811,7 @@ __global__ __launch_bounds__(MT * MT * 64) void ns_rec_kernel(NsClasses cs, NsRe
   _Float16* out = reinterpret_cast<_Float16*>(ws + c.base + (size_t)i * c.stride + slot_off(c, p.xplanes, p.out));
   NsGemm g;                             // (P as a product of the other kernels would be stored)
   g.scale = p.sP[p.steps - 1];
-  ns_store_sym<EPI_MUL>(c, g, nullptr, out, I * 32, J * 32, 1.f, P);
+  ns_store_sym<EPI_MUL>(c, g, NsOld(), out, I * 32, J * 32, 1.f, P);
 }
 
 // ---- host ---------------------------------------------------------------------------------------------------------------------
@@ -956,8 +989,12 @@ int ns_launch(NsRun& r, const NsGemm& g) {
     c.start = at;
     at += c.per * c.count;
   }
-  hipLaunchKernelGGL((ns_gemm_kernel<EPI, NA, NB, T, OutT>), dim3(at, EPI == EPI_PART ? r.split.shares : 1), dim3(256), 0, r.st, r.cs, g, r.few, r.table,
-                     r.residue, r.ws);
+  const dim3 grid(at, EPI == EPI_PART ? r.split.shares : 1);
+  if (T == 64 && at <= 256 && (EPI == EPI_Q || EPI == EPI_MUL))
+    hipLaunchKernelGGL((ns_gemm_kernel<EPI, NA, NB, T, T == 64 && (EPI == EPI_Q || EPI == EPI_MUL) ? 4 : 2, OutT>), grid, dim3(256), 0, r.st, r.cs, g, r.few,
+                       r.table, r.residue, r.ws);
+  else
+    hipLaunchKernelGGL((ns_gemm_kernel<EPI, NA, NB, T, 2, OutT>), grid, dim3(256), 0, r.st, r.cs, g, r.few, r.table, r.residue, r.ws);
   PXL_LAUNCH_CHECK();
   if (EPI == EPI_PART && !r.split.small) {
     hipLaunchKernelGGL((ns_fold_kernel<T>), dim3(at * (T * T / 1024)), dim3(64), 0, r.st, r.cs, g, at, r.residue, r.ws);
