@@ -39,8 +39,8 @@ constexpr int NS_PARTS = 1024;          // partial sums of squares per matrix at
 // one matrix, in device memory
 struct NsItem { void* p; const void* g; float* mom; float scale; int pad; };
 struct NsTable { NsItem it[NS_TABLE]; };
-// up to 16 of them travel in the kernel arguments of the three kernels that need them: no table launch
-constexpr int NS_INLINE = 16;
+// up to 32 of them travel in the kernel arguments of the three kernels that need them: no table launch
+constexpr int NS_INLINE = 32;
 struct NsInline { NsItem it[NS_INLINE]; };
 __device__ __forceinline__ NsItem ns_item(const NsInline& few, const NsItem* table, int i) { return table != nullptr ? table[i] : few.it[i]; }
 
@@ -240,9 +240,9 @@ __device__ __forceinline__ size_t slot_off(const NsClass& c, int xplanes, int sl
 
 struct NsJob { int a, b, out; };        // slots
 struct NsGemm {
-  NsJob job;
+  NsJob job[2];                         // MUL may do two products of one kind in a launch (blockIdx.z)
   int xplanes;                          // X slots of a region
-  float unscale, scale;                 // accumulator -> value, value -> planes
+  float unscale[2], scale[2];           // accumulator -> value, value -> planes
   float qa, qb, qc, sa_inv;             // EPI_Q: coefficients, 1 / scale of A's planes
   int res_pow;                          // GRAM: value *= residue^2;  OUT / X: value *= residue
   float lr, decay;                      // OUT of a Muon step
@@ -282,7 +282,7 @@ __device__ __forceinline__ NsOld ns_load_sym(const NsClass& c, const _Float16* A
   return o;
 }
 template <int EPI>
-__device__ __forceinline__ void ns_store_sym(const NsClass& c, const NsGemm& p, const NsOld& old, _Float16* out, int r, int q, float un, const f32x16& acc) {
+__device__ __forceinline__ void ns_store_sym(const NsClass& c, const NsGemm& p, const NsOld& old, _Float16* out, int r, int q, float un, float scale, const f32x16& acc) {
   const int lane = threadIdx.x & 63;
   if (r >= c.mp || q >= c.mp || r < q) return;                // (blocks are 32 wide, mp is a multiple of 32; a block above the diagonal)
   const size_t pm = (size_t)c.mp * c.mp;
@@ -297,7 +297,7 @@ __device__ __forceinline__ void ns_store_sym(const NsClass& c, const NsGemm& p, 
       float val = acc[e4 * 4 + e] * un;
       _Float16* d = out + (size_t)(r0 + e) * c.mp + q;
       if (EPI == EPI_Q) val = p.qc * val + p.qb * (((float)old.h[e4][e] + (float)old.l[e4][e]) * p.sa_inv) + (r0 + e == q ? p.qa : 0.f);
-      const float x = val * p.scale;
+      const float x = val * scale;
       h[e] = (_Float16)x;
       l[e] = (_Float16)(x - (float)h[e]);
       if (r0 + e >= q) {
@@ -351,8 +351,10 @@ __global__ __launch_bounds__(256, D == 2 ? 2 : 1) void ns_gemm_kernel(NsClasses 
   unsigned char* base = ws + c.base + (size_t)i * c.stride;
   const int K = EPI <= EPI_PART ? c.np : c.mp;
   const size_t plane_a = (size_t)c.mp * K, plane_b = NN ? (size_t)c.mp * c.np : (size_t)c.mp * K;
-  const _Float16* A = reinterpret_cast<const _Float16*>(base + slot_off(c, p.xplanes, p.job.a));
-  const _Float16* B = reinterpret_cast<const _Float16*>(base + slot_off(c, p.xplanes, p.job.b));
+  const int z = EPI == EPI_MUL ? blockIdx.z : 0;
+  const NsJob job = p.job[z];
+  const _Float16* A = reinterpret_cast<const _Float16*>(base + slot_off(c, p.xplanes, job.a));
+  const _Float16* B = reinterpret_cast<const _Float16*>(base + slot_off(c, p.xplanes, job.b));
 
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, wr = wave >> 1, wc = wave & 1;
   int k0 = 0, k1 = K;
@@ -536,15 +538,16 @@ __global__ __launch_bounds__(256, D == 2 ? 2 : 1) void ns_gemm_kernel(NsClasses 
     });
     return;
   }
-  float un = p.unscale;
+  const float scale = p.scale[z];
+  float un = p.unscale[z];
   if (EPI != EPI_Q && EPI != EPI_MUL && p.res_pow) {
     const float rs = residue[c.first + i];
     un *= p.res_pow == 2 ? rs * rs : rs;
   }
-  _Float16* out = reinterpret_cast<_Float16*>(base + slot_off(c, p.xplanes, p.job.out));
+  _Float16* out = reinterpret_cast<_Float16*>(base + slot_off(c, p.xplanes, job.out));
   if constexpr (SYM) {
     if (EPI == EPI_Q && T == 128) blocks([&](int n, int r, int q, const f32x16&) { old[EPI == EPI_Q && T == 128 ? n & 3 : 0] = ns_load_sym(c, A, r, q); });
-    blocks([&](int n, int r, int q, const f32x16& a) { ns_store_sym<EPI>(c, p, old[EPI == EPI_Q && T == 128 ? n & 3 : 0], out, r, q, un, a); });
+    blocks([&](int n, int r, int q, const f32x16& a) { ns_store_sym<EPI>(c, p, old[EPI == EPI_Q && T == 128 ? n & 3 : 0], out, r, q, un, scale, a); });
   } else if constexpr (EPI == EPI_X) {
     // through LDS, one plane after the other: rows of T columns, 16-byte stores.  Lane: row lane % 32, columns 8 e4 + 4 (lane / 32) + 0 .. 3
     constexpr int PITCH = T + 8;
@@ -560,7 +563,7 @@ __global__ __launch_bounds__(256, D == 2 ? 2 : 1) void ns_gemm_kernel(NsClasses 
           f16x4 h;
 #pragma unroll
           for (int e = 0; e < 4; ++e) {
-            const float x = a[e4 * 4 + e] * un * p.scale;
+            const float x = a[e4 * 4 + e] * un * scale;
             h[e] = (_Float16)x;
             if (z == 1) h[e] = (_Float16)(x - (float)h[e]);
           }
@@ -657,11 +660,11 @@ __global__ __launch_bounds__(64) void ns_fold_kernel(NsClasses cs, NsGemm p, int
   static_assert(SIDE * SIDE == NBL, "blocks of a tile");
   const f32x16 a = ns_share_sum<4>(p.part, ns_shares(c), (size_t)tiles * NBL, (size_t)bid * NBL + n);
   const float rs = residue[c.first + i];
-  _Float16* out = reinterpret_cast<_Float16*>(ws + c.base + (size_t)i * c.stride + slot_off(c, p.xplanes, p.job.out));
-  ns_store_sym<EPI_GRAM>(c, p, NsOld(), out, tr * T + br * 32, tc * T + bc * 32, p.unscale * (p.res_pow == 2 ? rs * rs : 1.f), a);
+  _Float16* out = reinterpret_cast<_Float16*>(ws + c.base + (size_t)i * c.stride + slot_off(c, p.xplanes, p.job[0].out));
+  ns_store_sym<EPI_GRAM>(c, p, NsOld(), out, tr * T + br * 32, tc * T + bc * 32, p.unscale[0] * (p.res_pow == 2 ? rs * rs : 1.f), p.scale[0], a);
 }
 
-// ---- a whole segment's recursion for matrices of at most 32 MT rows: one workgroup of MT^2 waves a matrix, everything on the CU ----------
+// ---- a whole segment's recursion for matrices of at most 32 MT rows: one workgroup a matrix, everything on the CU -----------------------
 // Wave (I, J) holds its 32 x 32 block of A, P and what it multiplies next in registers; LDS holds the two operands of the product at
 // hand (both symmetric: C[i][j] = sum_k x[i][k] y[j][k]).  In place of 3 to 5 launches a step of some 4 us each.
 struct NsRec {
@@ -673,14 +676,14 @@ struct NsRec {
   const float* part;
 };
 template <int MT>
-__global__ __launch_bounds__(MT * MT * 64) void ns_rec_kernel(NsClasses cs, NsRec p, int tiles, const float* __restrict__ residue, unsigned char* __restrict__ ws) {
+__global__ __launch_bounds__(MT == 2 ? 512 : 1024) void ns_rec_kernel(NsClasses cs, NsRec p, int tiles, const float* __restrict__ residue, unsigned char* __restrict__ ws) {
   constexpr int M = 32 * MT, ROW = M * 2, PL = M * ROW;             // bytes
   constexpr int SLOT = 2 * PL + 16;                                 // both planes, and the place nobody reads
   __shared__ __attribute__((aligned(16))) unsigned char lds[2 * SLOT];
   const NsClass c = find_class(cs, blockIdx.x);
   const int i = blockIdx.x - c.start;
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), I = wave / MT, J = wave % MT;
-  const bool inside = I * 32 < c.mp && J <= I;                      // (mp is a multiple of 32); waves above the diagonal only wait
+  const bool inside = I < MT && I * 32 < c.mp && J <= I;            // (mp is a multiple of 32); the other waves only wait
   // 16-byte chunk ch of row r
   auto at = [](int r, int ch) { return r * ROW + ((MT == 2 ? ch ^ ((r >> 1) & 7) : ch ^ (r & 15)) << 4); };
   auto elem = [&](int r, int q) { return at(r, q >> 3) + (q & 7) * 2; };
@@ -744,9 +747,33 @@ __global__ __launch_bounds__(MT * MT * 64) void ns_rec_kernel(NsClasses cs, NsRe
   f32x16 P, V;
 #pragma unroll
   for (int e = 0; e < 16; ++e) P[e] = V[e] = 0.f;
-  if (inside) {                         // A from the shares of the 64 x 64 tiles on and below the diagonal
+  if (MT == 2) {
+    // one tile, often many shares: waves 0 .. 3 add the first half of their block's, waves 4 .. 7 the second half
+    const int n = ns_shares(c), half = (n + 1) / 2, from = wave < 4 ? 0 : half;
+    const size_t per_share = (size_t)tiles * 4, first = ((size_t)c.tn + (size_t)i * c.per) * 4 + (wave & 3);
+    V = ns_share_sum<8>(p.part + (size_t)from * per_share * 1024, wave < 4 ? half : n - half, per_share, first);
+    float4* x = reinterpret_cast<float4*>(lds) + (wave & 3) * 256 + lane;
+    if (wave >= 4) {
+#pragma unroll
+      for (int e4 = 0; e4 < 4; ++e4) x[e4 * 64] = make_float4(V[e4 * 4], V[e4 * 4 + 1], V[e4 * 4 + 2], V[e4 * 4 + 3]);
+    }
+    __syncthreads();
+    if (inside) {
+#pragma unroll
+      for (int e4 = 0; e4 < 4; ++e4) {
+        const float4 v = x[e4 * 64];
+        V[e4 * 4] += v.x; V[e4 * 4 + 1] += v.y; V[e4 * 4 + 2] += v.z; V[e4 * 4 + 3] += v.w;
+      }
+    }
+    __syncthreads();
+    if (inside) {
+#pragma unroll
+      for (int e = 0; e < 16; ++e) V[e] *= un;
+      put(0, V, p.sA[0]);
+    }
+  } else if (inside) {                  // A from the shares of the 64 x 64 tiles on and below the diagonal
     const int t = (I >> 1) * ((I >> 1) + 1) / 2 + (J >> 1);
-    V = ns_share_sum<MT == 2 ? 4 : 2>(p.part, ns_shares(c), (size_t)tiles * 4, ((size_t)c.tn + (size_t)i * c.per + t) * 4 + (I & 1) * 2 + (J & 1));
+    V = ns_share_sum<2>(p.part, ns_shares(c), (size_t)tiles * 4, ((size_t)c.tn + (size_t)i * c.per + t) * 4 + (I & 1) * 2 + (J & 1));
 #pragma unroll
     for (int e = 0; e < 16; ++e) V[e] *= un;
     put(0, V, p.sA[0]);
@@ -809,9 +836,7 @@ __global__ __launch_bounds__(MT * MT * 64) void ns_rec_kernel(NsClasses cs, NsRe
   }
   if (!inside) return;
   _Float16* out = reinterpret_cast<_Float16*>(ws + c.base + (size_t)i * c.stride + slot_off(c, p.xplanes, p.out));
-  NsGemm g;                             // (P as a product of the other kernels would be stored)
-  g.scale = p.sP[p.steps - 1];
-  ns_store_sym<EPI_MUL>(c, g, NsOld(), out, I * 32, J * 32, 1.f, P);
+  ns_store_sym<EPI_MUL>(c, NsGemm(), NsOld(), out, I * 32, J * 32, 1.f, p.sP[p.steps - 1], P);
 }
 
 // ---- host ---------------------------------------------------------------------------------------------------------------------
@@ -831,29 +856,43 @@ inline bool ns_big_tiles(long big, long few) { return (big + 255) / 256 * 10 <= 
 inline int round_up(int v, int to) { return (v + to - 1) / to * to; }
 inline size_t round_up_z(size_t v, size_t to) { return (v + to - 1) / to * to; }
 
-// How the matrices of one set run.  small: all have at most 128 on their smaller side, their recursion runs on one CU each.
-// Gram products of few tiles (all of a small set's) are cut along K (n) into shares of at least 256, about 512 workgroups in all, and
-// added up in order.
-struct NsSplit { int tile, shares, tiles, small, mt; };
 inline int sym_tiles(int mp, int t) { const int k = (mp + t - 1) / t; return k * (k + 1) / 2; }
+
+// How the matrices of one set run.  small: all have at most 128 on their smaller side, their recursion runs on one CU each.
+// Gram products may be cut along K (n) into shares that are added up in order; tile and share (K a workgroup takes) by a model of their
+// time: rounds of workgroups over the 256 CUs, 0.82 us a K step of 32 of a large tile and 0.66 us a K step of 64 of a small one (measured, whether
+// one or two workgroups are on a CU), shares written and read at 5 TB/s and 4 us for the launch that adds them.  23 x 256 x 2304: 230 small
+// tiles in one share 24 us (model) against 34 measured for 8 shares of 69 large ones; 3 x 512 x 4608: 8 shares of 30 large tiles.
+struct NsSplit { int tile, shares, tiles, small, mt; };
 NsSplit ns_split_plan(std::vector<NsClass>& cls) {
-  long big = 0, few = 0;
   NsSplit r = {64, 1, 0, 1, 2};
+  int longest = 0;
   for (auto& c : cls) {
-    big += (long)sym_tiles(c.mp, 128) * c.count;
-    few += (long)sym_tiles(c.mp, 64) * c.count;
     if (c.mp > 64) r.mt = 4;
     if (c.mp > 128) r.small = 0;
+    longest = c.np > longest ? c.np : longest;
   }
-  if (!r.small && big * 10 <= few * 4) r.tile = 128;       // (shares fill the chip: the work alone counts)
-  const long tiles = r.tile == 128 ? big : few;
-  r.tiles = (int)tiles;
-  const long want = tiles < 384 ? (512 + tiles - 1) / tiles : 1;
+  double best = 1e30;
+  int ks = 0;
+  for (int t = 64; t <= (r.small ? 64 : 128); t *= 2)
+    for (int s = 1; s <= 128 && (s == 1 || longest / s >= 128); ++s) {
+      const int k = ((longest + s - 1) / s + 63) / 64 * 64;
+      long wg = 0;
+      double bytes = 0.0;
+      for (auto& c : cls) {
+        const long n = (long)sym_tiles(c.mp, t) * c.count * ((c.np + k - 1) / k);
+        wg += n;
+        bytes += (double)n * t * t * 8.0;
+      }
+      const int rounds = (int)((wg + 255) / 256);
+      const double time = rounds * (t == 128 ? k / 32 * 0.82 : k / 64 * 0.66) + (s > 1 || r.small ? bytes / 5e6 : 0.0) + (s > 1 && !r.small ? 4.0 : 0.0);
+      if (time < best) { best = time; r.tile = t; ks = k; }
+    }
   for (auto& c : cls) {
-    const long even = ((c.np + want - 1) / want + 63) / 64 * 64;
-    c.ks = want == 1 ? c.np : (int)(even < 256 ? 256 : even);
-    const int n = (c.np + c.ks - 1) / c.ks;
+    c.ks = ks;
+    const int n = (c.np + ks - 1) / ks;
     if (n > r.shares) r.shares = n;
+    r.tiles += sym_tiles(c.mp, r.tile) * c.count;
   }
   return r;
 }
@@ -934,8 +973,8 @@ int ns_schedule(const char* what, int steps, const float* coef, int np, std::vec
     d.lam = sigma * sigma;
     double next = 0.0;
     d.q = d.t = 0.0;
-    for (int e = 0; e <= 4096; ++e) {
-      const double x = sigma * e / 4096, l = x * x, q = fabs(d.a + l * (d.b + d.c * l));
+    for (int e = 0; e <= 256; ++e) {                       // (smooth: the maxima to 2e-4, under the 1 % added below)
+      const double x = sigma * e / 256, l = x * x, q = fabs(d.a + l * (d.b + d.c * l));
       next = fmax(next, x * q);
       d.q = fmax(d.q, q);
       d.t = fmax(d.t, l * q);
@@ -979,7 +1018,7 @@ struct NsRun {
   } while (0)
 
 template <int EPI, int NA, int NB, int T, typename OutT>
-int ns_launch(NsRun& r, const NsGemm& g) {
+int ns_launch(NsRun& r, const NsGemm& g, int jobs = 1) {
   int at = 0;
   for (int k = 0; k < r.cs.n; ++k) {
     NsClass& c = r.cs.c[k];
@@ -989,8 +1028,8 @@ int ns_launch(NsRun& r, const NsGemm& g) {
     c.start = at;
     at += c.per * c.count;
   }
-  const dim3 grid(at, EPI == EPI_PART ? r.split.shares : 1);
-  if (T == 64 && at <= 256 && (EPI == EPI_Q || EPI == EPI_MUL))
+  const dim3 grid(at, EPI == EPI_PART ? r.split.shares : 1, jobs);
+  if (T == 64 && at * jobs <= 256 && (EPI == EPI_Q || EPI == EPI_MUL))
     hipLaunchKernelGGL((ns_gemm_kernel<EPI, NA, NB, T, T == 64 && (EPI == EPI_Q || EPI == EPI_MUL) ? 4 : 2, OutT>), grid, dim3(256), 0, r.st, r.cs, g, r.few,
                        r.table, r.residue, r.ws);
   else
@@ -1004,7 +1043,7 @@ int ns_launch(NsRun& r, const NsGemm& g) {
 }
 
 template <int EPI, int NA, int NB, typename OutT>
-int ns_gemm(NsRun& r, const NsGemm& g) {
+int ns_gemm(NsRun& r, const NsGemm& g, int jobs = 1) {
   if constexpr (EPI == EPI_GRAM) {
     if (r.split.shares > 1 || r.split.small)
       return r.split.tile == 128 ? ns_launch<EPI_PART, NA, NB, 128, OutT>(r, g) : ns_launch<EPI_PART, NA, NB, 64, OutT>(r, g);
@@ -1016,7 +1055,7 @@ int ns_gemm(NsRun& r, const NsGemm& g) {
     big += EPI <= EPI_MUL ? (long)sym_tiles(c.mp, 128) * c.count : (long)((c.mp + 127) / 128) * ((c.np + 127) / 128) * c.count;
     few += EPI <= EPI_MUL ? (long)sym_tiles(c.mp, 64) * c.count : (long)((c.mp + 63) / 64) * ((c.np + 63) / 64) * c.count;
   }
-  return ns_big_tiles(big, few) ? ns_launch<EPI, NA, NB, 128, OutT>(r, g) : ns_launch<EPI, NA, NB, 64, OutT>(r, g);
+  return ns_big_tiles(big * jobs, few * jobs) ? ns_launch<EPI, NA, NB, 128, OutT>(r, g, jobs) : ns_launch<EPI, NA, NB, 64, OutT>(r, g, jobs);
 }
 
 // the recursion of steps [s, e) of a small set: shares -> P in slot `out`; -> the scale of P's planes
@@ -1046,7 +1085,7 @@ int ns_rec(NsRun& r, const std::vector<NsStep>& steps, size_t s, size_t e, float
     at += c.count;
     tiles += c.per * c.count;
   }
-  if (r.split.mt == 2) hipLaunchKernelGGL((ns_rec_kernel<2>), dim3(at), dim3(256), 0, r.st, r.cs, q, tiles, r.residue, r.ws);
+  if (r.split.mt == 2) hipLaunchKernelGGL((ns_rec_kernel<2>), dim3(at), dim3(512), 0, r.st, r.cs, q, tiles, r.residue, r.ws);
   else hipLaunchKernelGGL((ns_rec_kernel<4>), dim3(at), dim3(1024), 0, r.st, r.cs, q, tiles, r.residue, r.ws);
   PXL_LAUNCH_CHECK();
   return PXL_OK;
@@ -1085,9 +1124,9 @@ int ns_run_set(NsRun& r, const std::vector<NsStep>& steps, float eps, const Muon
   while (s < steps.size()) {
     double pbound = 1.0;
     float sA = plane_scale(steps[s].lam), sP = 1.f;
-    g.job = {x, x, MA};
-    g.unscale = 1.f / (sx * sx);
-    g.scale = sA;
+    g.job[0] = {x, x, MA};
+    g.unscale[0] = 1.f / (sx * sx);
+    g.scale[0] = sA;
     g.res_pow = NP == 1 && first ? 2 : 0;
     NS_TRY((ns_gemm<EPI_GRAM, NP, NP, float>(r, g)));
     int P = -1;
@@ -1095,7 +1134,7 @@ int ns_run_set(NsRun& r, const std::vector<NsStep>& steps, float eps, const Muon
       size_t e = s;
       while (!steps[e].last) ++e;
       P = xplanes + 2;
-      NS_TRY(ns_rec(r, steps, s, e + 1, g.unscale, g.res_pow, xplanes, P, &sP));
+      NS_TRY(ns_rec(r, steps, s, e + 1, g.unscale[0], g.res_pow, xplanes, P, &sP));
       s = e;
     }
     g.res_pow = 0;
@@ -1104,52 +1143,56 @@ int ns_run_set(NsRun& r, const std::vector<NsStep>& steps, float eps, const Muon
       int q = xplanes + 2;
       while (q == P) ++q;
       const float sQ = plane_scale(d.q);
-      g.job = {MA, MA, q};
-      g.unscale = 1.f / (sA * sA);
-      g.scale = sQ;
+      g.job[0] = {MA, MA, q};
+      g.unscale[0] = 1.f / (sA * sA);
+      g.scale[0] = sQ;
       g.qa = (float)d.a; g.qb = (float)d.b; g.qc = (float)d.c;
       g.sa_inv = 1.f / sA;
       NS_TRY((ns_gemm<EPI_Q, 2, 2, float>(r, g)));
       pbound *= d.q;
       const float sP2 = plane_scale(pbound), sT = plane_scale(d.t);
+      // P <- Q P and T = Q A, in one launch where there are both
+      int jobs = 0;
       if (P < 0) {
         P = q;
         sP = sQ;
       } else {
         int p2 = xplanes + 2;
         while (p2 == P || p2 == q) ++p2;
-        g.job = {q, P, p2};
-        g.unscale = 1.f / (sQ * sP);
-        g.scale = sP2;
-        NS_TRY((ns_gemm<EPI_MUL, 2, 2, float>(r, g)));
+        g.job[0] = {q, P, p2};
+        g.unscale[0] = 1.f / (sQ * sP);
+        g.scale[0] = sP2;
+        jobs = 1;
         P = p2;
         sP = sP2;
       }
+      if (!d.last) {
+        g.job[jobs] = {q, MA, MT};
+        g.unscale[jobs] = 1.f / (sQ * sA);
+        g.scale[jobs++] = sT;
+      }
+      if (jobs) NS_TRY((ns_gemm<EPI_MUL, 2, 2, float>(r, g, jobs)));
       if (d.last) break;
-      g.job = {q, MA, MT};
-      g.unscale = 1.f / (sQ * sA);
-      g.scale = sT;
-      NS_TRY((ns_gemm<EPI_MUL, 2, 2, float>(r, g)));
       const float sA2 = plane_scale(steps[s + 1].lam);
-      g.job = {q, MT, MA};
-      g.unscale = 1.f / (sQ * sT);
-      g.scale = sA2;
+      g.job[0] = {q, MT, MA};
+      g.unscale[0] = 1.f / (sQ * sT);
+      g.scale[0] = sA2;
       NS_TRY((ns_gemm<EPI_MUL, 2, 2, float>(r, g)));
       sA = sA2;
     }
     ++s;
-    g.unscale = 1.f / (sP * sx);
+    g.unscale[0] = 1.f / (sP * sx);
     g.res_pow = NP == 1 && first ? 1 : 0;
     if (s == steps.size()) {
-      g.job = {P, x, 0};
+      g.job[0] = {P, x, 0};
       g.muon = muon;
       g.lr = ma.lr;
       g.decay = ma.keep;
       NS_TRY((ns_gemm<EPI_OUT, 2, NP, T>(r, g)));
     } else {
       const float sx2 = plane_scale(steps[s].sigma);
-      g.job = {P, x, x2};
-      g.scale = sx2;
+      g.job[0] = {P, x, x2};
+      g.scale[0] = sx2;
       NS_TRY((ns_gemm<EPI_X, 2, NP, float>(r, g)));
       sx = sx2;
       const int o = x;
