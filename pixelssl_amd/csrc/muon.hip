@@ -678,23 +678,25 @@ struct NsRec {
 template <int MT>
 __global__ __launch_bounds__(MT == 2 ? 512 : 1024) void ns_rec_kernel(NsClasses cs, NsRec p, int tiles, const float* __restrict__ residue, unsigned char* __restrict__ ws) {
   constexpr int M = 32 * MT, ROW = M * 2, PL = M * ROW;             // bytes
-  constexpr int SLOT = 2 * PL + 16;                                 // both planes, and the place nobody reads
+  constexpr int SLOT = 2 * PL;                                      // both planes
   __shared__ __attribute__((aligned(16))) unsigned char lds[2 * SLOT];
   const NsClass c = find_class(cs, blockIdx.x);
   const int i = blockIdx.x - c.start;
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), I = wave / MT, J = wave % MT;
-  const bool inside = I < MT && I * 32 < c.mp && J <= I;            // (mp is a multiple of 32); the other waves only wait
+  const bool inside = I < MT && I * 32 < c.mp && J * 32 < c.mp, lower = inside && J <= I;      // (mp is a multiple of 32); other waves only wait
   // 16-byte chunk ch of row r
   auto at = [](int r, int ch) { return r * ROW + ((MT == 2 ? ch ^ ((r >> 1) & 7) : ch ^ (r & 15)) << 4); };
   auto elem = [&](int r, int q) { return at(r, q >> 3) + (q & 7) * 2; };
-  // a block on or below the diagonal and its mirror image (ns_store_sym says why): elements (r0 .. r0 + 3, q) are one 8-byte access there
-  // (on the diagonal what the other triangle holds goes to a place nobody reads: two writes in place of two branches an element)
-  const int nowhere = 2 * PL;
+  // The matrices are kept EXACTLY symmetric (ns_store_sym says why).  Blocks (I, J) and (J, I) are the same sums in the same order with the
+  // operands of the matrix instructions exchanged, a block on the diagonal is the mean of its product and the exchanged one: so every wave
+  // writes its block alone, four elements (r0 .. r0 + 3, q) as one access at row q, columns r0 .. r0 + 3.
+  int mine[4];
+#pragma unroll
+  for (int e4 = 0; e4 < 4; ++e4) mine[e4] = elem(J * 32 + (lane & 31), I * 32 + 8 * e4 + 4 * (lane >> 5));
   auto put = [&](int slot, const f32x16& v, float s) {
     unsigned char* at0 = lds + slot * SLOT;
 #pragma unroll
     for (int e4 = 0; e4 < 4; ++e4) {
-      const int r0 = I * 32 + 8 * e4 + 4 * (lane >> 5), q = J * 32 + (lane & 31);
       f16x4 h, l;
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
@@ -702,45 +704,61 @@ __global__ __launch_bounds__(MT == 2 ? 512 : 1024) void ns_rec_kernel(NsClasses 
         h[e] = (_Float16)x;
         l[e] = (_Float16)(x - (float)h[e]);
       }
-      if (I != J) {
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          *reinterpret_cast<_Float16*>(at0 + elem(r0 + e, q)) = h[e];
-          *reinterpret_cast<_Float16*>(at0 + PL + elem(r0 + e, q)) = l[e];
-        }
-        *reinterpret_cast<f16x4*>(at0 + elem(q, r0)) = h;
-        *reinterpret_cast<f16x4*>(at0 + PL + elem(q, r0)) = l;
-      } else {
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          const int o1 = r0 + e >= q ? elem(r0 + e, q) : nowhere, o2 = r0 + e > q ? elem(q, r0 + e) : nowhere;
-          const int low = PL;
-          *reinterpret_cast<_Float16*>(at0 + o1) = h[e];
-          *reinterpret_cast<_Float16*>(at0 + o2) = h[e];
-          *reinterpret_cast<_Float16*>(at0 + (r0 + e >= q ? o1 + low : nowhere)) = l[e];
-          *reinterpret_cast<_Float16*>(at0 + (r0 + e > q ? o2 + low : nowhere)) = l[e];
-        }
-      }
+      *reinterpret_cast<f16x4*>(at0 + mine[e4]) = h;
+      *reinterpret_cast<f16x4*>(at0 + PL + mine[e4]) = l;
     }
   };
   auto product = [&](int x, int y) {
-    const unsigned char *px = lds + x * SLOT, *py = lds + y * SLOT;
+    const unsigned char *pa = lds + (I < J ? y : x) * SLOT, *pb = lds + (I < J ? x : y) * SLOT;
+    const int r = I * 32 + (lane & 31), q = J * 32 + (lane & 31), hi = lane >> 5;
     f32x16 acc;
 #pragma unroll
     for (int e = 0; e < 16; ++e) acc[e] = 0.f;
-    auto slice = [&](int kk) {
-      const int ch = kk * 2 + (lane >> 5), r = I * 32 + (lane & 31), q = J * 32 + (lane & 31);
-      const f16x8 xh = *reinterpret_cast<const f16x8*>(px + at(r, ch)), xl = *reinterpret_cast<const f16x8*>(px + PL + at(r, ch));
-      const f16x8 yh = *reinterpret_cast<const f16x8*>(py + at(q, ch)), yl = *reinterpret_cast<const f16x8*>(py + PL + at(q, ch));
-      acc = __builtin_amdgcn_mfma_f32_32x32x16_f16(xh, yl, acc, 0, 0, 0);
-      acc = __builtin_amdgcn_mfma_f32_32x32x16_f16(xl, yh, acc, 0, 0, 0);
-      acc = __builtin_amdgcn_mfma_f32_32x32x16_f16(xh, yh, acc, 0, 0, 0);
-    };
-    for (int k2 = 0; k2 < c.mp; k2 += 32) {             // (mp is a multiple of 32)
-      slice(k2 / 16);
-      slice(k2 / 16 + 1);
+    if (I != J) {
+      // above the diagonal the lows come in the other order: the same sum as its mirror image
+      const unsigned char *pa1 = I < J ? pa + PL : pa, *pa2 = I < J ? pa : pa + PL, *pb1 = I < J ? pb : pb + PL, *pb2 = I < J ? pb + PL : pb;
+#pragma unroll 2
+      for (int k2 = 0; k2 < c.mp; k2 += 16) {
+        const int oa = at(r, (k2 >> 3) + hi), ob = at(q, (k2 >> 3) + hi);
+        const f16x8 a1 = *reinterpret_cast<const f16x8*>(pa1 + oa), b1 = *reinterpret_cast<const f16x8*>(pb1 + ob);
+        const f16x8 a2 = *reinterpret_cast<const f16x8*>(pa2 + oa), b2 = *reinterpret_cast<const f16x8*>(pb2 + ob);
+        acc = __builtin_amdgcn_mfma_f32_32x32x16_f16(a1, b1, acc, 0, 0, 0);
+        acc = __builtin_amdgcn_mfma_f32_32x32x16_f16(a2, b2, acc, 0, 0, 0);
+        acc = I < J ? __builtin_amdgcn_mfma_f32_32x32x16_f16(a2, b1, acc, 0, 0, 0) : __builtin_amdgcn_mfma_f32_32x32x16_f16(a1, b2, acc, 0, 0, 0);
+      }
+    } else {
+      f32x16 turned = acc;
+#pragma unroll 2
+      for (int k2 = 0; k2 < c.mp; k2 += 16) {
+        const int o = at(r, (k2 >> 3) + hi);
+        const f16x8 ah = *reinterpret_cast<const f16x8*>(pa + o), al = *reinterpret_cast<const f16x8*>(pa + PL + o);
+        const f16x8 bh = *reinterpret_cast<const f16x8*>(pb + o), bl = *reinterpret_cast<const f16x8*>(pb + PL + o);
+        acc = __builtin_amdgcn_mfma_f32_32x32x16_f16(ah, bl, acc, 0, 0, 0);
+        turned = __builtin_amdgcn_mfma_f32_32x32x16_f16(bl, ah, turned, 0, 0, 0);
+        acc = __builtin_amdgcn_mfma_f32_32x32x16_f16(al, bh, acc, 0, 0, 0);
+        turned = __builtin_amdgcn_mfma_f32_32x32x16_f16(bh, al, turned, 0, 0, 0);
+        acc = __builtin_amdgcn_mfma_f32_32x32x16_f16(ah, bh, acc, 0, 0, 0);
+        turned = __builtin_amdgcn_mfma_f32_32x32x16_f16(bh, ah, turned, 0, 0, 0);
+      }
+#pragma unroll
+      for (int e = 0; e < 16; ++e) acc[e] = 0.5f * (acc[e] + turned[e]);
     }
     return acc;
+  };
+  // the Gram product's blocks come below and on the diagonal: each with its mirror image, on the diagonal what lies above it from below
+  auto put_gram = [&](const f32x16& v, float s) {
+#pragma unroll
+    for (int e = 0; e < 16; ++e) {
+      const int r = I * 32 + 8 * (e >> 2) + 4 * (lane >> 5) + (e & 3), q = J * 32 + (lane & 31);
+      const float x = v[e] * s;
+      const _Float16 h = (_Float16)x, l = (_Float16)(x - (float)h);
+      if (r >= q) {
+        *reinterpret_cast<_Float16*>(lds + elem(r, q)) = h;
+        *reinterpret_cast<_Float16*>(lds + PL + elem(r, q)) = l;
+        *reinterpret_cast<_Float16*>(lds + elem(q, r)) = h;
+        *reinterpret_cast<_Float16*>(lds + PL + elem(q, r)) = l;
+      }
+    }
   };
   const float rs = residue[c.first + i];
   const float un = p.unscale * (p.res_pow == 2 ? rs * rs : 1.f);
@@ -758,7 +776,7 @@ __global__ __launch_bounds__(MT == 2 ? 512 : 1024) void ns_rec_kernel(NsClasses 
       for (int e4 = 0; e4 < 4; ++e4) x[e4 * 64] = make_float4(V[e4 * 4], V[e4 * 4 + 1], V[e4 * 4 + 2], V[e4 * 4 + 3]);
     }
     __syncthreads();
-    if (inside) {
+    if (lower) {
 #pragma unroll
       for (int e4 = 0; e4 < 4; ++e4) {
         const float4 v = x[e4 * 64];
@@ -766,17 +784,17 @@ __global__ __launch_bounds__(MT == 2 ? 512 : 1024) void ns_rec_kernel(NsClasses 
       }
     }
     __syncthreads();
-    if (inside) {
+    if (lower) {
 #pragma unroll
       for (int e = 0; e < 16; ++e) V[e] *= un;
-      put(0, V, p.sA[0]);
+      put_gram(V, p.sA[0]);
     }
-  } else if (inside) {                  // A from the shares of the 64 x 64 tiles on and below the diagonal
+  } else if (lower) {                  // A from the shares of the 64 x 64 tiles on and below the diagonal
     const int t = (I >> 1) * ((I >> 1) + 1) / 2 + (J >> 1);
     V = ns_share_sum<2>(p.part, ns_shares(c), (size_t)tiles * 4, ((size_t)c.tn + (size_t)i * c.per + t) * 4 + (I & 1) * 2 + (J & 1));
 #pragma unroll
     for (int e = 0; e < 16; ++e) V[e] *= un;
-    put(0, V, p.sA[0]);
+    put_gram(V, p.sA[0]);
   }
   __syncthreads();
   for (int s = 0; s < p.steps; ++s) {
@@ -785,8 +803,7 @@ __global__ __launch_bounds__(MT == 2 ? 512 : 1024) void ns_rec_kernel(NsClasses 
       const float g = p.c[s] / (p.sA[s] * p.sA[s]), ia = p.b[s] / p.sA[s];
 #pragma unroll
       for (int e4 = 0; e4 < 4; ++e4) {
-        const int o = elem(J * 32 + (lane & 31), I * 32 + 8 * e4 + 4 * (lane >> 5));          // (the mirror image: one access)
-        const f16x4 h = *reinterpret_cast<const f16x4*>(lds + o), l = *reinterpret_cast<const f16x4*>(lds + PL + o);
+        const f16x4 h = *reinterpret_cast<const f16x4*>(lds + mine[e4]), l = *reinterpret_cast<const f16x4*>(lds + PL + mine[e4]);
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
           const int r = I * 32 + 8 * e4 + 4 * (lane >> 5) + e, q = J * 32 + (lane & 31);
@@ -836,7 +853,21 @@ __global__ __launch_bounds__(MT == 2 ? 512 : 1024) void ns_rec_kernel(NsClasses 
   }
   if (!inside) return;
   _Float16* out = reinterpret_cast<_Float16*>(ws + c.base + (size_t)i * c.stride + slot_off(c, p.xplanes, p.out));
-  ns_store_sym<EPI_MUL>(c, NsGemm(), NsOld(), out, I * 32, J * 32, 1.f, p.sP[p.steps - 1], P);
+  const size_t pm = (size_t)c.mp * c.mp;
+  const float sp = p.sP[p.steps - 1];
+#pragma unroll
+  for (int e4 = 0; e4 < 4; ++e4) {
+    f16x4 h, l;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      const float x = P[e4 * 4 + e] * sp;
+      h[e] = (_Float16)x;
+      l[e] = (_Float16)(x - (float)h[e]);
+    }
+    _Float16* d = out + (size_t)(J * 32 + (lane & 31)) * c.mp + I * 32 + 8 * e4 + 4 * (lane >> 5);
+    *reinterpret_cast<f16x4*>(d) = h;
+    *reinterpret_cast<f16x4*>(d + pm) = l;
+  }
 }
 
 // ---- host ---------------------------------------------------------------------------------------------------------------------
@@ -861,7 +892,8 @@ inline int sym_tiles(int mp, int t) { const int k = (mp + t - 1) / t; return k *
 // How the matrices of one set run.  small: all have at most 128 on their smaller side, their recursion runs on one CU each.
 // Gram products may be cut along K (n) into shares that are added up in order; tile and share (K a workgroup takes) by a model of their
 // time: rounds of workgroups over the 256 CUs, 0.82 us a K step of 32 of a large tile and 0.66 us a K step of 64 of a small one (measured, whether
-// one or two workgroups are on a CU), shares written and read at 5 TB/s and 4 us for the launch that adds them.  23 x 256 x 2304: 230 small
+// one or two workgroups are on a CU), shares written and read at 5 TB/s and 4 us for the launch that adds them
+// (small: 1.2 us for every 16 of them in the recursion's workgroup).  23 x 256 x 2304: 230 small
 // tiles in one share 24 us (model) against 34 measured for 8 shares of 69 large ones; 3 x 512 x 4608: 8 shares of 30 large tiles.
 struct NsSplit { int tile, shares, tiles, small, mt; };
 NsSplit ns_split_plan(std::vector<NsClass>& cls) {
@@ -885,7 +917,7 @@ NsSplit ns_split_plan(std::vector<NsClass>& cls) {
         bytes += (double)n * t * t * 8.0;
       }
       const int rounds = (int)((wg + 255) / 256);
-      const double time = rounds * (t == 128 ? k / 32 * 0.82 : k / 64 * 0.66) + (s > 1 || r.small ? bytes / 5e6 : 0.0) + (s > 1 && !r.small ? 4.0 : 0.0);
+      const double time = rounds * (t == 128 ? k / 32 * 0.82 : k / 64 * 0.66) + (s > 1 || r.small ? bytes / 5e6 : 0.0) + (s > 1 && !r.small ? 4.0 : 0.0) + (r.small ? (s + 15) / 16 * 1.2 : 0.0);
       if (time < best) { best = time; r.tile = t; ks = k; }
     }
   for (auto& c : cls) {
