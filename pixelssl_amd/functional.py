@@ -277,14 +277,15 @@ def softmax_channels(x):
 
 
 # ---- layer normalisation (csrc/layernorm.hip) ---------------------------------------------------------------------------------
-def _launch(dev, fn, *args):
-    """fn(*args, stream) on the current stream of `dev`, which need not be the current device"""
-    index = dev.index
+def _launch(index, fn, *args):
+    """fn(*args, stream) on the current stream of device `index`, which need not be the current device"""
     if index == torch._C._cuda_getDevice():
-        check(fn(*args, torch._C._cuda_getCurrentRawStream(index)))
+        rc = fn(*args, torch._C._cuda_getCurrentRawStream(index))
     else:
-        with torch.cuda.device(dev):
-            check(fn(*args, torch._C._cuda_getCurrentRawStream(index)))
+        with torch.cuda.device(index):
+            rc = fn(*args, torch._C._cuda_getCurrentRawStream(index))
+    if rc:
+        check(rc)
 
 
 def _row_stride(x):
@@ -309,9 +310,10 @@ def _row_stride(x):
 
 
 def _ln_forward(x, weight, bias, eps, channels, keep):
-    """-> (x as the kernel read it, geometry, y, mean, rstd); mean / rstd None unless `keep`"""
-    code = dtype_code(x.dtype)
-    pcode = code if weight is None and bias is None else dtype_code((bias if weight is None else weight).dtype)
+    """-> (x as the kernel read it, geometry, y, statistics): mean and 1 / deviation of every row, None unless `keep`"""
+    code = 0 if x.dtype is torch.float32 else 1                     # PXL_F32 / PXL_BF16
+    p = bias if weight is None else weight
+    pcode = code if p is None or p.dtype is x.dtype else 0
     if channels:
         x = x.contiguous()
         N, C = x.shape[0], x.shape[1]
@@ -321,72 +323,86 @@ def _ln_forward(x, weight, bias, eps, channels, keep):
         y = torch.empty_like(x)
     else:
         C = x.shape[-1]
-        stride = C if x.is_contiguous() else _row_stride(x)
-        if stride is None:
-            x, stride = x.contiguous(), C
+        if x.is_contiguous():
+            stride, y = C, torch.empty_like(x)
+        else:
+            stride = _row_stride(x)
+            if stride is None:
+                x, stride = x.contiguous(), C
+            y = torch.empty(x.shape, device=x.device, dtype=x.dtype)
         rows = x.numel() // C
         geo = (code, pcode, rows, C, stride)
         fn = lib().pxl_layer_norm_fwd
-        y = torch.empty(x.shape, device=x.device, dtype=x.dtype)
-    stats = torch.empty(2, rows, device=x.device, dtype=torch.float32) if keep else None
-    mean = stats.data_ptr() if keep else None
-    _launch(x.device, fn, *geo, ptr(x), ptr(weight), ptr(bias), eps, ptr(y), mean, mean + 4 * rows if keep else None)
+    stats = mean = rstd = None
+    if keep:
+        stats = torch.empty(2 * rows, device=x.device, dtype=torch.float32)
+        mean = stats.data_ptr()
+        rstd = mean + 4 * rows
+    _launch(x.device.index, fn, *geo, x.data_ptr(), ptr(weight), ptr(bias), eps, y.data_ptr(), mean, rstd)
     return x, geo, y, stats
 
 
 class _LayerNorm(torch.autograd.Function):
+    # (the engine runs backward on a thread of its own, where everything takes two to three times as long: little is done there)
     @staticmethod
     def forward(ctx, x, weight, bias, eps, channels):
-        x, ctx.geo, y, stats = _ln_forward(x, weight, bias, eps, channels, True)
+        x, geo, y, stats = _ln_forward(x, weight, bias, eps, channels, True)
         ctx.save_for_backward(x, weight, stats)
-        ctx.channels, ctx.pdtype = channels, None if weight is None and bias is None else (bias if weight is None else weight).dtype
+        h = lib()
+        p = bias if weight is None else weight
+        rows = stats.shape[0] // 2
+        ctx.plan = (geo, h.pxl_layer_norm_nchw_bwd if channels else h.pxl_layer_norm_bwd, None if p is None else p.dtype, 4 * rows,
+                    h.pxl_layer_norm_nchw_bwd_workspace(geo[2], geo[3], geo[4]) if channels else h.pxl_layer_norm_bwd_workspace(rows, geo[3]))
         return y
 
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, dy):
         x, weight, stats = ctx.saved_tensors
+        geo, fn, pdtype, second, nbytes = ctx.plan
         dy = dy.contiguous()
-        geo, C = ctx.geo, ctx.geo[3]
-        rows = stats.shape[1]
-        need_x, need_w, need_b = ctx.needs_input_grad[:3]
         dev = x.device
-        dx = torch.empty(x.shape, device=dev, dtype=x.dtype) if need_x else None
-        dw = torch.empty(C, device=dev, dtype=ctx.pdtype) if need_w else None
-        db = torch.empty(C, device=dev, dtype=ctx.pdtype) if need_b else None
-        h = lib()
-        ws, nbytes = None, 0
+        need_x, need_w, need_b = ctx.needs_input_grad[:3]
+        dx = dw = db = ws = None
+        if need_x:
+            dx = torch.empty(x.shape, device=dev, dtype=x.dtype)
+        if need_w:
+            dw = torch.empty(geo[3], device=dev, dtype=pdtype)
+        if need_b:
+            db = torch.empty(geo[3], device=dev, dtype=pdtype)
         if need_w or need_b:
-            nbytes = h.pxl_layer_norm_nchw_bwd_workspace(geo[2], C, geo[4]) if ctx.channels else h.pxl_layer_norm_bwd_workspace(rows, C)
             ws = torch.empty(nbytes, device=dev, dtype=torch.uint8)
         mean = stats.data_ptr()
-        _launch(dev, h.pxl_layer_norm_nchw_bwd if ctx.channels else h.pxl_layer_norm_bwd, *geo, ptr(x), ptr(dy), ptr(weight), mean,
-                mean + 4 * rows, ptr(dx), ptr(dw), ptr(db), ptr(ws), nbytes)
+        _launch(dev.index, fn, *geo, x.data_ptr(), dy.data_ptr(), ptr(weight), mean, mean + second, ptr(dx), ptr(dw), ptr(db), ptr(ws), nbytes)
         return dx, dw, db, None, None
 
 
 def _layer_norm(name, x, weight, bias, eps, channels):
-    axis = 1 if channels else -1
-    if x.dim() < (2 if channels else 1) or x.shape[axis] == 0:
+    dtype = x.dtype
+    if dtype is not torch.float32 and dtype is not torch.bfloat16:
+        raise ValueError("%s: float32 or bfloat16, got %s" % (name, dtype))
+    if x.dim() < (2 if channels else 1) or x.shape[1 if channels else -1] == 0:
         raise ValueError("%s: no features to normalise over in %s" % (name, tuple(x.shape)))
-    C = x.shape[axis]
+    C = x.shape[1 if channels else -1]
+    grad = x.requires_grad
     for what, t in (("weight", weight), ("bias", bias)):
         if t is None:
             continue
         if t.dim() != 1 or t.shape[0] != C:
             raise ValueError("%s: %s %s for %d features" % (name, what, tuple(t.shape), C))
-        if t.dtype not in (torch.float32, x.dtype) or (weight is not None and t.dtype != weight.dtype):
-            raise ValueError("%s: weight and bias are both float32 or both of the type of x (%s), got %s" % (name, x.dtype, t.dtype))
+        if (t.dtype is not torch.float32 and t.dtype is not dtype) or (weight is not None and t.dtype is not weight.dtype):
+            raise ValueError("%s: weight and bias are both float32 or both of the type of x (%s), got %s" % (name, dtype, t.dtype))
         if t.device != x.device:
             raise ValueError("%s: %s on %s, x on %s" % (name, what, t.device, x.device))
-    if x.dtype not in (torch.float32, torch.bfloat16):
-        raise ValueError("%s: float32 or bfloat16, got %s" % (name, x.dtype))
+        grad = grad or t.requires_grad
     if not eps >= 0:
         raise ValueError("%s: eps %r" % (name, eps))
     _gpu(x)
-    weight = weight.contiguous() if weight is not None else None
-    bias = bias.contiguous() if bias is not None else None
-    if torch.is_grad_enabled() and (x.requires_grad or (weight is not None and weight.requires_grad) or (bias is not None and bias.requires_grad)):
+    if weight is not None and not weight.is_contiguous():
+        weight = weight.contiguous()
+    if bias is not None and not bias.is_contiguous():
+        bias = bias.contiguous()
+    if grad and torch.is_grad_enabled():
         return _LayerNorm.apply(x, weight, bias, float(eps), channels)
     return _ln_forward(x, weight, bias, float(eps), channels, False)[2]
 
@@ -457,7 +473,7 @@ def _run_ns(fn, dev, code, items, n, steps, coef, eps, *scalars):
     if nbytes == 0:
         raise _lib.PixelHipError("libpixelhip: %s" % lib().pxl_last_error().decode())
     ws = torch.empty(nbytes, device=dev, dtype=torch.uint8)
-    _launch(dev, fn, code, items, n, int(steps), coef, float(eps), *scalars, ptr(ws), nbytes)
+    _launch(dev.index, fn, code, items, n, int(steps), coef, float(eps), *scalars, ptr(ws), nbytes)
 
 
 def _dense_strides(t):
@@ -558,6 +574,6 @@ def adam_update(params, grads, exp_avgs, exp_avg_sqs, lr, betas=(0.9, 0.999), ep
         work.setdefault((p.device, p.dtype), []).append((p.data_ptr(), g.data_ptr(), m.data_ptr(), v.data_ptr(), p.numel()))
         touched += [p, m, v]
     for (dev, dtype), entries in work.items():
-        _launch(dev, lib().pxl_adam_list, dtype_code(dtype), (_lib.AdamItem * len(entries))(*entries), len(entries), float(lr), b1, b2, float(eps),
+        _launch(dev.index, lib().pxl_adam_list, dtype_code(dtype), (_lib.AdamItem * len(entries))(*entries), len(entries), float(lr), b1, b2, float(eps),
                 int(step))
     torch.autograd.graph.increment_version(touched)
