@@ -1,4 +1,5 @@
-"""Build libpixelhip.so (HIP kernels + C-ABI + network executor) for gfx950, in-tree.
+"""Build libpixelhip.so (HIP kernels + C-ABI + network executor) for gfx950 and _pxlnode.so (its autograd nodes: host C++
+against torch's headers), in-tree.
 
     python -m pixelssl_amd.build            # incremental
     python -m pixelssl_amd.build --force
@@ -48,11 +49,37 @@ def _compile(src, force):
     return obj, False
 
 
+NODE_SRC = os.path.join(HERE, "node", "layer_norm_node.cpp")
+NODE_LIB = os.path.join(HERE, "_pxlnode.so")
+
+
+def _build_node(force):
+    """host code only: the kernels are reached through addresses that functional.py hands over, so libpixelhip.so is loaded once"""
+    if not force and not _stale(NODE_LIB, [NODE_SRC] + HEADERS):
+        return False
+    import sysconfig
+    import torch
+    from torch.utils import cpp_extension
+    libdir = os.path.join(os.path.dirname(torch.__file__), "lib")
+    cmd = [os.environ.get("CXX", "g++"), "-O2", "-std=c++17", "-fPIC", "-shared", "-D__HIP_PLATFORM_AMD__=1", "-DUSE_ROCM=1",
+           "-D_GLIBCXX_USE_CXX11_ABI=%d" % torch._C._GLIBCXX_USE_CXX11_ABI, NODE_SRC, "-o", NODE_LIB]
+    for d in cpp_extension.include_paths() + [sysconfig.get_paths()["include"], "/opt/rocm/include"]:
+        cmd += ["-isystem", d]
+    cmd += ["-L" + libdir] + ["-l" + n for n in ("c10", "torch_cpu", "torch_python", "c10_hip", "torch_hip")]
+    r = subprocess.run(cmd, capture_output=True, text=True)
+    if r.returncode != 0:
+        raise RuntimeError("compiling %s failed:\n%s\n%s" % (NODE_SRC, r.stdout, r.stderr))
+    return True
+
+
 def build(force=False, verbose=True):
     os.makedirs(OBJDIR, exist_ok=True)
     srcs = sources()
-    with ThreadPoolExecutor(max_workers=min(8, len(srcs))) as ex:
+    with ThreadPoolExecutor(max_workers=min(8, len(srcs) + 1)) as ex:
+        node = ex.submit(_build_node, force)
         results = list(ex.map(lambda s: _compile(s, force), srcs))
+        if node.result() and verbose:
+            print("built", NODE_LIB)
     objs = [o for o, _ in results]
     if force or any(c for _, c in results) or _stale(LIB, objs):
         cmd = [HIPCC, "--offload-arch=" + ARCH, "-shared", "-fPIC", "-o", LIB] + objs

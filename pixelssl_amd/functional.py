@@ -288,93 +288,24 @@ def _launch(index, fn, *args):
         check(rc)
 
 
-def _row_stride(x):
-    """elements between the rows of a tensor whose last axis is contiguous and whose leading axes form one evenly spaced run
-    without overlap; None where they do not"""
-    C = x.shape[-1]
-    if x.stride(-1) != 1 and C > 1:
-        return None
-    step, span = None, 1
-    for k in range(x.dim() - 2, -1, -1):
-        n = x.shape[k]
-        if n == 1:
-            continue
-        if step is None:
-            step = x.stride(k)
-        elif x.stride(k) != step * span:
-            return None
-        span *= n
-    if step is None:
-        return C
-    return step if step >= C else None
+_pxlnode = None
 
 
-def _ln_forward(x, weight, bias, eps, channels, keep):
-    """-> (x as the kernel read it, geometry, y, statistics): mean and 1 / deviation of every row, None unless `keep`"""
-    code = 0 if x.dtype is torch.float32 else 1                     # PXL_F32 / PXL_BF16
-    p = bias if weight is None else weight
-    pcode = code if p is None or p.dtype is x.dtype else 0
-    if channels:
-        x = x.contiguous()
-        N, C = x.shape[0], x.shape[1]
-        S = x.numel() // (N * C) if x.numel() else 0
-        geo = (code, pcode, N, C, S)
-        rows, fn = N * S, lib().pxl_layer_norm_nchw_fwd
-        y = torch.empty_like(x)
-    else:
-        C = x.shape[-1]
-        if x.is_contiguous():
-            stride, y = C, torch.empty_like(x)
-        else:
-            stride = _row_stride(x)
-            if stride is None:
-                x, stride = x.contiguous(), C
-            y = torch.empty(x.shape, device=x.device, dtype=x.dtype)
-        rows = x.numel() // C
-        geo = (code, pcode, rows, C, stride)
-        fn = lib().pxl_layer_norm_fwd
-    stats = mean = rstd = None
-    if keep:
-        stats = torch.empty(2 * rows, device=x.device, dtype=torch.float32)
-        mean = stats.data_ptr()
-        rstd = mean + 4 * rows
-    _launch(x.device.index, fn, *geo, x.data_ptr(), ptr(weight), ptr(bias), eps, y.data_ptr(), mean, rstd)
-    return x, geo, y, stats
-
-
-class _LayerNorm(torch.autograd.Function):
-    # (the engine runs backward on a thread of its own, where everything takes two to three times as long: little is done there)
-    @staticmethod
-    def forward(ctx, x, weight, bias, eps, channels):
-        x, geo, y, stats = _ln_forward(x, weight, bias, eps, channels, True)
-        ctx.save_for_backward(x, weight, stats)
-        h = lib()
-        p = bias if weight is None else weight
-        rows = stats.shape[0] // 2
-        ctx.plan = (geo, h.pxl_layer_norm_nchw_bwd if channels else h.pxl_layer_norm_bwd, None if p is None else p.dtype, 4 * rows,
-                    h.pxl_layer_norm_nchw_bwd_workspace(geo[2], geo[3], geo[4]) if channels else h.pxl_layer_norm_bwd_workspace(rows, geo[3]))
-        return y
-
-    @staticmethod
-    @torch.autograd.function.once_differentiable
-    def backward(ctx, dy):
-        x, weight, stats = ctx.saved_tensors
-        geo, fn, pdtype, second, nbytes = ctx.plan
-        dy = dy.contiguous()
-        dev = x.device
-        need_x, need_w, need_b = ctx.needs_input_grad[:3]
-        dx = dw = db = ws = None
-        if need_x:
-            dx = torch.empty(x.shape, device=dev, dtype=x.dtype)
-        if need_w:
-            dw = torch.empty(geo[3], device=dev, dtype=pdtype)
-        if need_b:
-            db = torch.empty(geo[3], device=dev, dtype=pdtype)
-        if need_w or need_b:
-            ws = torch.empty(nbytes, device=dev, dtype=torch.uint8)
-        mean = stats.data_ptr()
-        _launch(dev.index, fn, *geo, x.data_ptr(), dy.data_ptr(), ptr(weight), mean, mean + second, ptr(dx), ptr(dw), ptr(db), ptr(ws), nbytes)
-        return dx, dw, db, None, None
+def _node():
+    """the compiled autograd nodes (pixelssl_amd/node), bound to the loaded libpixelhip.so"""
+    global _pxlnode
+    if _pxlnode is None:
+        try:
+            from . import _pxlnode as module
+        except ImportError as e:
+            raise _lib.PixelHipError("_pxlnode.so is missing or does not load (%s). Build it with `python -m pixelssl_amd.build`; there is "
+                                     "no other path." % e)
+        raw = ctypes.CDLL(_lib.LIB_PATH)          # (the same loaded library as lib(): its addresses)
+        module.bind([ctypes.cast(getattr(raw, name), ctypes.c_void_p).value for name in (
+            "pxl_layer_norm_fwd", "pxl_layer_norm_bwd", "pxl_layer_norm_bwd_workspace", "pxl_layer_norm_nchw_fwd", "pxl_layer_norm_nchw_bwd",
+            "pxl_layer_norm_nchw_bwd_workspace", "pxl_last_error")])
+        _pxlnode = module
+    return _pxlnode
 
 
 def _layer_norm(name, x, weight, bias, eps, channels):
@@ -384,7 +315,6 @@ def _layer_norm(name, x, weight, bias, eps, channels):
     if x.dim() < (2 if channels else 1) or x.shape[1 if channels else -1] == 0:
         raise ValueError("%s: no features to normalise over in %s" % (name, tuple(x.shape)))
     C = x.shape[1 if channels else -1]
-    grad = x.requires_grad
     for what, t in (("weight", weight), ("bias", bias)):
         if t is None:
             continue
@@ -394,17 +324,10 @@ def _layer_norm(name, x, weight, bias, eps, channels):
             raise ValueError("%s: weight and bias are both float32 or both of the type of x (%s), got %s" % (name, dtype, t.dtype))
         if t.device != x.device:
             raise ValueError("%s: %s on %s, x on %s" % (name, what, t.device, x.device))
-        grad = grad or t.requires_grad
     if not eps >= 0:
         raise ValueError("%s: eps %r" % (name, eps))
     _gpu(x)
-    if weight is not None and not weight.is_contiguous():
-        weight = weight.contiguous()
-    if bias is not None and not bias.is_contiguous():
-        bias = bias.contiguous()
-    if grad and torch.is_grad_enabled():
-        return _LayerNorm.apply(x, weight, bias, float(eps), channels)
-    return _ln_forward(x, weight, bias, float(eps), channels, False)[2]
+    return (_pxlnode or _node()).layer_norm(x, weight, bias, eps, channels)
 
 
 def layer_norm(x, weight=None, bias=None, eps=1e-5):

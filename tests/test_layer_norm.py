@@ -301,6 +301,29 @@ def test_other_stream_and_second_use_of_a_leaf():
 
 
 @pytest.mark.gpu
+def test_gradients_of_gradients_are_refused_and_kept_graphs_run_again():
+    from pixelssl_amd import functional as PF
+    x, w, b, dy = make((30, 70), 70, torch.float32, torch.float32, 16)
+    want = run(x, w, b, dy, False)
+    for which in ((True, True, True), (True, False, False), (False, True, False)):
+        leaves = [t.detach().requires_grad_(g) for t, g in zip((x, w, b), which)]
+        has = [t for t in leaves if t.requires_grad]
+        y = PF.layer_norm(*leaves)
+        first = torch.autograd.grad(y, has, dy, retain_graph=True)
+        again = torch.autograd.grad(y, has, dy, create_graph=True)
+        for a, c, d in zip(first, again, [v for v, g in zip(want[1:], which) if g]):
+            assert torch.equal(a, c) and torch.equal(a, d)
+        with pytest.raises(RuntimeError, match="differentiable once"):
+            sum(g.sum() for g in again).backward()
+    with torch.autograd.set_multithreading_enabled(False):
+        assert all(torch.equal(a, c) for a, c in zip(want, run(x, w, b, dy, False)))
+    y = PF.layer_norm(x, w.clone().requires_grad_(True), b)
+    assert y.requires_grad
+    with torch.no_grad():
+        assert not PF.layer_norm(x, w.clone().requires_grad_(True), b).requires_grad
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("channels", [False, True], ids=["rows", "channels"])
 def test_captured_forward_and_backward(channels):
     """two graphs of forward + backward, replayed in turn with eager work between: each replay equals the eager result"""
@@ -421,7 +444,8 @@ def test_formula_against_autograd_in_64_bits():
 
 
 def test_row_strides():
-    from pixelssl_amd.functional import _row_stride
+    from pixelssl_amd.functional import _node
+    _row_stride = lambda t: None if _node().row_stride(t) < 0 else _node().row_stride(t)
     t = torch.zeros(4, 6, 20)
     assert _row_stride(t) == 20 and _row_stride(t[:, :, 3:9]) == 20 and _row_stride(t[:, ::2]) == 40
     assert _row_stride(t[:, ::2, :5]) == 40 and _row_stride(t[:, :5]) is None and _row_stride(t[::2, 1]) == 240
