@@ -664,92 +664,113 @@ __global__ __launch_bounds__(64) void ns_fold_kernel(NsClasses cs, NsGemm p, int
   ns_store_sym<EPI_GRAM>(c, p, NsOld(), out, tr * T + br * 32, tc * T + bc * 32, p.unscale[0] * (p.res_pow == 2 ? rs * rs : 1.f), p.scale[0], a);
 }
 
-// ---- a whole segment's recursion for matrices of at most 32 MT rows: one workgroup a matrix, everything on the CU -----------------------
-// Wave (I, J) holds its 32 x 32 block of A, P and what it multiplies next in registers; LDS holds the two operands of the product at
-// hand (both symmetric: C[i][j] = sum_k x[i][k] y[j][k]).  In place of 3 to 5 launches a step of some 4 us each.
+// ---- the recursion of a whole segment on one CU, for matrices of at most 32 MT rows ---------------------------------------------------
+// Wave (I, J) = (wave / MT, wave % MT) holds its 32 x 32 block of A, P and what it multiplies next in registers; LDS holds the planes of
+// the two operands of the product at hand (all symmetric: C[i][j] = sum_k x[i][k] y[j][k]).  In place of 3 to 5 launches a step.
+// The matrices are kept EXACTLY symmetric (ns_store_sym says why).  Blocks (I, J) and (J, I) are the same sums in the same order with the
+// operands of the matrix instructions exchanged, a block on the diagonal is the mean of its product and the exchanged one: so every wave
+// writes its block alone, four elements (r0 .. r0 + 3, q) as one access at row q, columns r0 .. r0 + 3.
+struct NsRecStep {                      // one step: factors from a product's sums to what is stored, plane scales (powers of two) in them
+  float g, ia, a;                       // Q = g (A A)' + ia A' + a
+  float fP, fT, fA;                     // P = fP (Q P)',  T = fT (Q A)',  next A = fA (Q T)'
+  float sP, pad;                        // planes of P where it is the segment's last step
+};
 struct NsRec {
   int steps, xplanes, out;              // of this segment; slot of P
   float unscale;                        // share sums -> A
   int res_pow;
-  float sA[NS_MAX_STEPS], sQ[NS_MAX_STEPS], sT[NS_MAX_STEPS], sP[NS_MAX_STEPS];      // plane scales
-  float a[NS_MAX_STEPS], b[NS_MAX_STEPS], c[NS_MAX_STEPS];
   const float* part;
+  float sA[NS_MAX_STEPS];               // planes of A where a segment begins
+  NsRecStep step[NS_MAX_STEPS];
 };
-template <int MT>
-__global__ __launch_bounds__(MT == 2 ? 512 : 1024) void ns_rec_kernel(NsClasses cs, NsRec p, int tiles, const float* __restrict__ residue, unsigned char* __restrict__ ws) {
-  constexpr int M = 32 * MT, ROW = M * 2, PL = M * ROW;             // bytes
-  constexpr int SLOT = 2 * PL;                                      // both planes
-  __shared__ __attribute__((aligned(16))) unsigned char lds[2 * SLOT];
-  const NsClass c = find_class(cs, blockIdx.x);
-  const int i = blockIdx.x - c.start;
-  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), I = wave / MT, J = wave % MT;
-  const bool inside = I < MT && I * 32 < c.mp && J * 32 < c.mp, lower = inside && J <= I;      // (mp is a multiple of 32); other waves only wait
-  // 16-byte chunk ch of row r
-  auto at = [](int r, int ch) { return r * ROW + ((MT == 2 ? ch ^ ((r >> 1) & 7) : ch ^ (r & 15)) << 4); };
-  auto elem = [&](int r, int q) { return at(r, q >> 3) + (q & 7) * 2; };
-  // The matrices are kept EXACTLY symmetric (ns_store_sym says why).  Blocks (I, J) and (J, I) are the same sums in the same order with the
-  // operands of the matrix instructions exchanged, a block on the diagonal is the mean of its product and the exchanged one: so every wave
-  // writes its block alone, four elements (r0 .. r0 + 3, q) as one access at row q, columns r0 .. r0 + 3.
+template <int MT> struct NsOnCu {
+  static constexpr int ROW = 64 * MT, PL = 32 * MT * ROW, SLOT = 2 * PL;      // bytes of a row, a plane, both planes
+  unsigned char* lds;                   // two slots
+  int mp, lane, I, J;
+  bool inside;                          // this wave has a block (mp is a multiple of 32); the others only wait
   int mine[4];
+  // 16-byte chunk ch of row r
+  static __device__ __forceinline__ int at(int r, int ch) { return r * ROW + ((MT == 2 ? ch ^ ((r >> 1) & 7) : ch ^ (r & 15)) << 4); }
+  static __device__ __forceinline__ int elem(int r, int q) { return at(r, q >> 3) + (q & 7) * 2; }
+  __device__ __forceinline__ NsOnCu(unsigned char* lds_, int mp_, int wave, int lane_) : lds(lds_), mp(mp_), lane(lane_), I(wave / MT), J(wave % MT) {
+    inside = I < MT && I * 32 < mp && J * 32 < mp;
 #pragma unroll
-  for (int e4 = 0; e4 < 4; ++e4) mine[e4] = elem(J * 32 + (lane & 31), I * 32 + 8 * e4 + 4 * (lane >> 5));
-  auto put = [&](int slot, const f32x16& v, float s) {
+    for (int e4 = 0; e4 < 4; ++e4) mine[e4] = elem(J * 32 + (lane & 31), (I < MT ? I : 0) * 32 + 8 * e4 + 4 * (lane >> 5));
+  }
+  __device__ __forceinline__ void put(int slot, const f32x16& v) {
     unsigned char* at0 = lds + slot * SLOT;
 #pragma unroll
     for (int e4 = 0; e4 < 4; ++e4) {
       f16x4 h, l;
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
-        const float x = v[e4 * 4 + e] * s;
-        h[e] = (_Float16)x;
-        l[e] = (_Float16)(x - (float)h[e]);
+        h[e] = (_Float16)v[e4 * 4 + e];
+        l[e] = (_Float16)(v[e4 * 4 + e] - (float)h[e]);
       }
       *reinterpret_cast<f16x4*>(at0 + mine[e4]) = h;
       *reinterpret_cast<f16x4*>(at0 + PL + mine[e4]) = l;
     }
-  };
-  auto product = [&](int x, int y) {
-    const unsigned char *pa = lds + (I < J ? y : x) * SLOT, *pb = lds + (I < J ? x : y) * SLOT;
-    const int r = I * 32 + (lane & 31), q = J * 32 + (lane & 31), hi = lane >> 5;
+  }
+  // Products, KT times 16 along k: WHERE 0 a block on the diagonal, 1 below, 2 above it.  hi lo, lo hi, hi hi; above the
+  // diagonal with the operands exchanged -- the same sum in the same order as its mirror image's.  On the diagonal: the sum of the product
+  // and of the exchanged one (2 C: f below makes up for it).
+  template <int WHERE, int KT, typename X, typename Y> static __device__ __forceinline__ f32x16 sums(const X& x, const Y& y) {
     f32x16 acc;
 #pragma unroll
     for (int e = 0; e < 16; ++e) acc[e] = 0.f;
-    if (I != J) {
-      // above the diagonal the lows come in the other order: the same sum as its mirror image
-      const unsigned char *pa1 = I < J ? pa + PL : pa, *pa2 = I < J ? pa : pa + PL, *pb1 = I < J ? pb : pb + PL, *pb2 = I < J ? pb + PL : pb;
-#pragma unroll 2
-      for (int k2 = 0; k2 < c.mp; k2 += 16) {
-        const int oa = at(r, (k2 >> 3) + hi), ob = at(q, (k2 >> 3) + hi);
-        const f16x8 a1 = *reinterpret_cast<const f16x8*>(pa1 + oa), b1 = *reinterpret_cast<const f16x8*>(pb1 + ob);
-        const f16x8 a2 = *reinterpret_cast<const f16x8*>(pa2 + oa), b2 = *reinterpret_cast<const f16x8*>(pb2 + ob);
-        acc = __builtin_amdgcn_mfma_f32_32x32x16_f16(a1, b1, acc, 0, 0, 0);
-        acc = __builtin_amdgcn_mfma_f32_32x32x16_f16(a2, b2, acc, 0, 0, 0);
-        acc = I < J ? __builtin_amdgcn_mfma_f32_32x32x16_f16(a2, b1, acc, 0, 0, 0) : __builtin_amdgcn_mfma_f32_32x32x16_f16(a1, b2, acc, 0, 0, 0);
+    f32x16 turned = acc;
+#pragma unroll(MT == 2 ? KT : 2)
+    for (int k = 0; k < KT; ++k) {
+      const f16x8 xh = x.hi(k), xl = x.lo(k), yh = y.hi(k), yl = y.lo(k);
+      if (WHERE == 2) {
+        acc = __builtin_amdgcn_mfma_f32_32x32x16_f16(yl, xh, acc, 0, 0, 0);
+        acc = __builtin_amdgcn_mfma_f32_32x32x16_f16(yh, xl, acc, 0, 0, 0);
+        acc = __builtin_amdgcn_mfma_f32_32x32x16_f16(yh, xh, acc, 0, 0, 0);
+        continue;
       }
-    } else {
-      f32x16 turned = acc;
-#pragma unroll 2
-      for (int k2 = 0; k2 < c.mp; k2 += 16) {
-        const int o = at(r, (k2 >> 3) + hi);
-        const f16x8 ah = *reinterpret_cast<const f16x8*>(pa + o), al = *reinterpret_cast<const f16x8*>(pa + PL + o);
-        const f16x8 bh = *reinterpret_cast<const f16x8*>(pb + o), bl = *reinterpret_cast<const f16x8*>(pb + PL + o);
-        acc = __builtin_amdgcn_mfma_f32_32x32x16_f16(ah, bl, acc, 0, 0, 0);
-        turned = __builtin_amdgcn_mfma_f32_32x32x16_f16(bl, ah, turned, 0, 0, 0);
-        acc = __builtin_amdgcn_mfma_f32_32x32x16_f16(al, bh, acc, 0, 0, 0);
-        turned = __builtin_amdgcn_mfma_f32_32x32x16_f16(bh, al, turned, 0, 0, 0);
-        acc = __builtin_amdgcn_mfma_f32_32x32x16_f16(ah, bh, acc, 0, 0, 0);
-        turned = __builtin_amdgcn_mfma_f32_32x32x16_f16(bh, ah, turned, 0, 0, 0);
-      }
+      acc = __builtin_amdgcn_mfma_f32_32x32x16_f16(xh, yl, acc, 0, 0, 0);
+      if (WHERE == 0) turned = __builtin_amdgcn_mfma_f32_32x32x16_f16(yl, xh, turned, 0, 0, 0);
+      acc = __builtin_amdgcn_mfma_f32_32x32x16_f16(xl, yh, acc, 0, 0, 0);
+      if (WHERE == 0) turned = __builtin_amdgcn_mfma_f32_32x32x16_f16(yh, xl, turned, 0, 0, 0);
+      acc = __builtin_amdgcn_mfma_f32_32x32x16_f16(xh, yh, acc, 0, 0, 0);
+      if (WHERE == 0) turned = __builtin_amdgcn_mfma_f32_32x32x16_f16(yh, xh, turned, 0, 0, 0);
+    }
+    if (WHERE == 0) {
 #pragma unroll
-      for (int e = 0; e < 16; ++e) acc[e] = 0.5f * (acc[e] + turned[e]);
+      for (int e = 0; e < 16; ++e) acc[e] += turned[e];
     }
     return acc;
+  }
+  // fragments of 32 rows of an operand: in LDS, or in registers (what several products share is read once)
+  struct Lds {
+    const unsigned char* x;
+    int row, half;
+    __device__ __forceinline__ f16x8 hi(int k) const { return *reinterpret_cast<const f16x8*>(x + at(row, 2 * k + half)); }
+    __device__ __forceinline__ f16x8 lo(int k) const { return *reinterpret_cast<const f16x8*>(x + PL + at(row, 2 * k + half)); }
   };
-  // the Gram product's blocks come below and on the diagonal: each with its mirror image, on the diagonal what lies above it from below
-  auto put_gram = [&](const f32x16& v, float s) {
+  template <int KT> struct Regs {
+    f16x8 h[KT], l[KT];
+    __device__ __forceinline__ f16x8 hi(int k) const { return h[k]; }
+    __device__ __forceinline__ f16x8 lo(int k) const { return l[k]; }
+  };
+  __device__ __forceinline__ Lds rows_of(int slot, int u) const { return Lds{lds + slot * SLOT, u * 32 + (lane & 31), lane >> 5}; }
+  // this wave's block of x y, times f: from the rows max(I, J) of x and min(I, J) of y
+  template <int KT, typename X> __device__ __forceinline__ f32x16 product(const X& x, int y, float f) const {
+    const Lds l = rows_of(y, I < J ? I : J);
+    f32x16 r;
+    if (I == J) r = sums<0, KT>(x, l);
+    else if (I > J) r = sums<1, KT>(x, l);
+    else r = sums<2, KT>(x, l);
+    if (I == J) f *= 0.5f;
+#pragma unroll
+    for (int e = 0; e < 16; ++e) r[e] *= f;
+    return r;
+  }
+  // block (bi, bj) of a Gram product, on or below the diagonal, with its mirror image -> slot 0; on the diagonal what lies above it from below
+  __device__ __forceinline__ void put_gram(const f32x16& v, float s, int bi, int bj) {
 #pragma unroll
     for (int e = 0; e < 16; ++e) {
-      const int r = I * 32 + 8 * (e >> 2) + 4 * (lane >> 5) + (e & 3), q = J * 32 + (lane & 31);
+      const int r = bi * 32 + 8 * (e >> 2) + 4 * (lane >> 5) + (e & 3), q = bj * 32 + (lane & 31);
       const float x = v[e] * s;
       const _Float16 h = (_Float16)x, l = (_Float16)(x - (float)h);
       if (r >= q) {
@@ -759,12 +780,73 @@ __global__ __launch_bounds__(MT == 2 ? 512 : 1024) void ns_rec_kernel(NsClasses 
         *reinterpret_cast<_Float16*>(lds + PL + elem(q, r)) = l;
       }
     }
-  };
+  }
+  // steps first .. last from A in slot 0 (a barrier has been passed since it was written) -> this wave's block of P, times its planes'
+  // scale.  Every thread of the workgroup calls it.  Slot 1 is read until its end.
+  __device__ __forceinline__ f32x16 run(const NsRec& p, int first, int last) {
+    return mp == 32 * MT ? run_k<2 * MT>(p, first, last) : run_k<2 * MT - 2>(p, first, last);
+  }
+  template <int KT> __device__ __forceinline__ f32x16 run_k(const NsRec& p, int first, int last) {
+    const int u = I < J ? J : I;
+    f32x16 P, V, tq;
+    for (int s = first; s <= last; ++s) {
+      const NsRecStep d = p.step[s];                     // (fetched at once, ahead of the products)
+      if (inside) {
+        V = product<KT>(rows_of(0, u), 0, d.g);
+#pragma unroll
+        for (int e4 = 0; e4 < 4; ++e4) {
+          const f16x4 h = *reinterpret_cast<const f16x4*>(lds + mine[e4]), l = *reinterpret_cast<const f16x4*>(lds + PL + mine[e4]);
+#pragma unroll
+          for (int e = 0; e < 4; ++e) V[e4 * 4 + e] = __fmaf_rn(d.ia, (float)h[e], __fmaf_rn(d.ia, (float)l[e], V[e4 * 4 + e]));
+        }
+        if (I == J) {
+#pragma unroll
+          for (int e = 0; e < 16; ++e) V[e] += 8 * (e >> 2) + 4 * (lane >> 5) + (e & 3) == (lane & 31) ? d.a : 0.f;
+        }
+        put(1, V);                      // (slot 1 is free: its last readers have passed a barrier since)
+      }
+      __syncthreads();
+      const Lds ql = rows_of(1, u);
+      Regs<KT> qr;                      // (16 waves have no registers for it)
+      if (MT == 2 && inside) {
+#pragma unroll
+        for (int k = 0; k < KT; ++k) { qr.h[k] = ql.hi(k); qr.l[k] = ql.lo(k); }
+      }
+      auto with_q = [&](float f) { return MT == 2 ? product<KT>(qr, 0, f) : product<KT>(ql, 0, f); };
+      if (s < last && inside) tq = with_q(d.fT);         // Q A
+      if (s == first) {
+        P = V;
+      } else {
+        __syncthreads();
+        if (inside) put(0, P);
+        __syncthreads();
+        if (inside) P = with_q(d.fP);
+      }
+      if (s == last) break;
+      __syncthreads();
+      if (inside) put(0, tq);
+      __syncthreads();
+      if (inside) V = with_q(d.fA);                      // Q (Q A)
+      __syncthreads();
+      if (inside) put(0, V);
+      __syncthreads();
+    }
+    return P;
+  }
+};
+
+template <int MT>
+__global__ __launch_bounds__(MT == 2 ? 512 : 1024) void ns_rec_kernel(NsClasses cs, NsRec p, int tiles, const float* __restrict__ residue, unsigned char* __restrict__ ws) {
+  __shared__ __attribute__((aligned(16))) unsigned char lds[2 * NsOnCu<MT>::SLOT];
+  const NsClass c = find_class(cs, blockIdx.x);
+  const int i = blockIdx.x - c.start;
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  NsOnCu<MT> m(lds, c.mp, wave, lane);
+  const int I = m.I, J = m.J;
+  const bool lower = m.inside && J <= I;
   const float rs = residue[c.first + i];
   const float un = p.unscale * (p.res_pow == 2 ? rs * rs : 1.f);
-  f32x16 P, V;
-#pragma unroll
-  for (int e = 0; e < 16; ++e) P[e] = V[e] = 0.f;
+  f32x16 V;
   if (MT == 2) {
     // one tile, often many shares: waves 0 .. 3 add the first half of their block's, waves 4 .. 7 the second half
     const int n = ns_shares(c), half = (n + 1) / 2, from = wave < 4 ? 0 : half;
@@ -784,89 +866,274 @@ __global__ __launch_bounds__(MT == 2 ? 512 : 1024) void ns_rec_kernel(NsClasses 
       }
     }
     __syncthreads();
-    if (lower) {
-#pragma unroll
-      for (int e = 0; e < 16; ++e) V[e] *= un;
-      put_gram(V, p.sA[0]);
-    }
   } else if (lower) {                  // A from the shares of the 64 x 64 tiles on and below the diagonal
     const int t = (I >> 1) * ((I >> 1) + 1) / 2 + (J >> 1);
     V = ns_share_sum<2>(p.part, ns_shares(c), (size_t)tiles * 4, ((size_t)c.tn + (size_t)i * c.per + t) * 4 + (I & 1) * 2 + (J & 1));
+  }
+  if (lower) {
 #pragma unroll
     for (int e = 0; e < 16; ++e) V[e] *= un;
-    put_gram(V, p.sA[0]);
+    m.put_gram(V, p.sA[0], I, J);
   }
   __syncthreads();
-  for (int s = 0; s < p.steps; ++s) {
-    if (inside) {
-      const f32x16 acc = product(0, 0);
-      const float g = p.c[s] / (p.sA[s] * p.sA[s]), ia = p.b[s] / p.sA[s];
-#pragma unroll
-      for (int e4 = 0; e4 < 4; ++e4) {
-        const f16x4 h = *reinterpret_cast<const f16x4*>(lds + mine[e4]), l = *reinterpret_cast<const f16x4*>(lds + PL + mine[e4]);
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          const int r = I * 32 + 8 * e4 + 4 * (lane >> 5) + e, q = J * 32 + (lane & 31);
-          V[e4 * 4 + e] = g * acc[e4 * 4 + e] + ia * ((float)h[e] + (float)l[e]) + (r == q ? p.a[s] : 0.f);
-        }
-      }
-    }
-    // (slot 1 is free: its last readers have passed a barrier since)
-    if (inside) put(1, V, p.sQ[s]);
-    __syncthreads();
-    const bool last = s + 1 == p.steps;
-    f32x16 tq;
-#pragma unroll
-    for (int e = 0; e < 16; ++e) tq[e] = 0.f;
-    if (!last && inside) tq = product(1, 0);            // Q A
-    if (s == 0) {
-      P = V;
-    } else {
-      __syncthreads();
-      if (inside) put(0, P, p.sP[s - 1]);
-      __syncthreads();
-      if (inside) {
-        P = product(1, 0);
-        const float f = 1.f / (p.sQ[s] * p.sP[s - 1]);
-#pragma unroll
-        for (int e = 0; e < 16; ++e) P[e] *= f;
-      }
-    }
-    if (last) break;
-    __syncthreads();
-    if (inside) {
-      const float f = 1.f / (p.sQ[s] * p.sA[s]);
-#pragma unroll
-      for (int e = 0; e < 16; ++e) tq[e] *= f;
-      put(0, tq, p.sT[s]);
-    }
-    __syncthreads();
-    if (inside) {
-      V = product(1, 0);                                 // Q (Q A)
-      const float f = 1.f / (p.sQ[s] * p.sT[s]);
-#pragma unroll
-      for (int e = 0; e < 16; ++e) V[e] *= f;
-    }
-    __syncthreads();
-    if (inside) put(0, V, p.sA[s + 1]);
-    __syncthreads();
-  }
-  if (!inside) return;
+  const f32x16 P = m.run(p, 0, p.steps - 1);
+  if (!m.inside) return;
   _Float16* out = reinterpret_cast<_Float16*>(ws + c.base + (size_t)i * c.stride + slot_off(c, p.xplanes, p.out));
   const size_t pm = (size_t)c.mp * c.mp;
-  const float sp = p.sP[p.steps - 1];
 #pragma unroll
   for (int e4 = 0; e4 < 4; ++e4) {
     f16x4 h, l;
 #pragma unroll
     for (int e = 0; e < 4; ++e) {
-      const float x = P[e4 * 4 + e] * sp;
+      const float x = P[e4 * 4 + e];
       h[e] = (_Float16)x;
       l[e] = (_Float16)(x - (float)h[e]);
     }
     _Float16* d = out + (size_t)(J * 32 + (lane & 31)) * c.mp + I * 32 + 8 * e4 + 4 * (lane >> 5);
     *reinterpret_cast<f16x4*>(d) = h;
     *reinterpret_cast<f16x4*>(d + pm) = l;
+  }
+}
+
+// ---- matrices that fit one CU's LDS whole: norm, all steps and the update in ONE launch, a workgroup of 8 waves a matrix ----------------------
+// At most 64 on the smaller side, 384 (bf16: 256) on the other.  X lives in LDS as planes [mp][pitch]: 16-byte chunk ch of row r at
+// ch ^ ((r >> 2) & 3), a pitch of an odd number of 64 bytes -- 16 rows of one chunk, and the four rows of a transposing read, lie on different
+// banks.  The products are the ones of the larger matrices; only what is moved differs.
+// Measured, this against the launches of the larger ones (5 steps, us): fp32 16 x 27 24 / 56, 64 x 147 37 / 69, 64 x 256 47 / 69,
+// 64 x 448 66 / 71; bf16 64 x 64 33 / 44, 64 x 256 44 / 46, 64 x 320 48 / 46: the limits.  What bounds it is one CU's chain of small products
+// (1 us each: 24 matrix instructions of 32 cycles on the diagonal, 512 cycles of LDS reads, the split into planes, two barriers).
+template <int NP> constexpr int NS_TINY_N = NP == 2 ? 384 : 256;
+__host__ __device__ inline int ns_tiny_pitch(int np) { return np * 2 + (np & 32 ? 0 : 64); }
+struct NsTiny {
+  NsRec rec;                            // scales and coefficients of all steps
+  unsigned ends;                        // bit s: step s ends a segment
+  float sx[NS_MAX_STEPS + 1];           // scale of X's planes where a segment begins with step s
+  float eps, lr, decay;
+  int muon;
+};
+template <typename T, int NP>
+__global__ __launch_bounds__(512) void ns_tiny_kernel(NsClasses cs, NsTiny p, NsInline few, const NsItem* __restrict__ table, MuonArgs ma) {
+  constexpr int XB = 64 * (NS_TINY_N<NP> * 2 + 64);             // bytes of one plane of X at most
+  constexpr int GROUPS = 64 * NS_TINY_N<NP> / 4 / 512;          // fours of elements a thread holds at most
+  __shared__ __attribute__((aligned(16))) unsigned char x[NP * XB];
+  __shared__ __attribute__((aligned(16))) unsigned char lds[2 * NsOnCu<2>::SLOT];
+  __shared__ double sh[8];
+  const NsClass c = find_class(cs, blockIdx.x);
+  const int i = blockIdx.x - c.start;
+  const NsItem it = ns_item(few, table, c.first + i);
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int pitch = ns_tiny_pitch(c.np), plane = c.mp * pitch;
+  auto xat = [&](int r, int q) { return r * pitch + (((q >> 3) ^ ((r >> 2) & 3)) << 4) + (q & 7) * 2; };
+  const T* g = reinterpret_cast<const T*>(it.g);
+  const bool tall = c.rows > c.cols;
+
+  // momentum, update and its norm; the update stays in registers
+  const int per_line = (c.cols + 3) >> 2, groups = c.rows * per_line;
+  float u[GROUPS][4];
+  double s = 0.0;
+#pragma unroll
+  for (int k = 0; k < GROUPS; ++k) {
+#pragma unroll
+    for (int e = 0; e < 4; ++e) u[k][e] = 0.f;
+    const int n = tid + k * 512;
+    if (n < groups) {
+      const int line = n / per_line, col = (n - line * per_line) * 4;
+      const long at = (long)line * c.cols + col;
+      if (col + 4 <= c.cols) {
+        load4(g + at, u[k]);
+        if (it.mom != nullptr) {
+          float m[4];
+          load4(it.mom + at, m);
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            m[e] = muon_momentum(m[e], u[k][e], ma);
+            u[k][e] = muon_update(m[e], u[k][e], ma);
+          }
+          store4(it.mom + at, m);
+        }
+      } else {
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+          if (col + e < c.cols) {
+            float v = to_f(g[at + e]);
+            if (it.mom != nullptr) {
+              const float m = muon_momentum(it.mom[at + e], v, ma);
+              it.mom[at + e] = m;
+              v = muon_update(m, v, ma);
+            }
+            u[k][e] = v;
+          }
+      }
+#pragma unroll
+      for (int e = 0; e < 4; ++e) s += (double)u[k][e] * u[k][e];
+    }
+  }
+#pragma unroll
+  for (int o = 32; o > 0; o >>= 1) s += __shfl_xor(s, o, 64);
+  if (lane == 0) sh[wave] = s;
+  for (int e = tid * 16; e < NP * plane; e += 512 * 16) *reinterpret_cast<uint4*>(x + e) = make_uint4(0u, 0u, 0u, 0u);     // the padding
+  __syncthreads();
+  double square = 0.0;
+#pragma unroll
+  for (int w = 0; w < 8; ++w) square += sh[w];
+  const double norm = fmax(sqrt(square), (double)p.eps);
+  double mul;
+  float left = 1.f;
+  if (NP == 2) {
+    mul = (double)p.sx[0] / norm;
+  } else {
+    int e;
+    frexp(norm, &e);
+    mul = ldexp((double)p.sx[0], -e);
+    left = (float)(ldexp(1.0, e) / norm);
+  }
+  if (!(square < HUGE_VAL)) mul = nan("");                  // a NaN or an infinity in the matrix: all of its result is NaN
+#pragma unroll
+  for (int k = 0; k < GROUPS; ++k) {
+    const int n = tid + k * 512;
+    if (n < groups) {
+      const int line = n / per_line, col = (n - line * per_line) * 4;
+      f16x4 h, l;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const float v = (float)((double)u[k][e] * mul);     // (0 behind a line's end: padding)
+        h[e] = (_Float16)v;
+        l[e] = (_Float16)(v - (float)h[e]);
+      }
+      if (!tall) {
+        *reinterpret_cast<f16x4*>(x + xat(line, col)) = h;
+        if (NP == 2) *reinterpret_cast<f16x4*>(x + plane + xat(line, col)) = l;
+      } else {
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          *reinterpret_cast<_Float16*>(x + xat(col + e, line)) = h[e];
+          if (NP == 2) *reinterpret_cast<_Float16*>(x + plane + xat(col + e, line)) = l[e];
+        }
+      }
+    }
+  }
+  __syncthreads();
+
+  NsOnCu<2> m(lds, c.mp, wave, lane);
+  const int steps = p.rec.steps, hi = lane >> 5;
+  int s0 = 0;
+  while (true) {
+    int s1 = s0;
+    while (!(p.ends >> s1 & 1)) ++s1;
+    const float sx = p.sx[s0], res = s0 == 0 ? left : 1.f;
+    // A = X X': wave w has block w % nb of the nb on and below the diagonal, and every (8 / nb)-th 16 of K from w / nb on
+    const int nb = c.mp > 32 ? 3 : 1, parts = 8 / nb, blk = wave % nb, part = wave / nb;
+    const int bi = blk > 0, bj = blk == 2;
+    f32x16 a;
+#pragma unroll
+    for (int e = 0; e < 16; ++e) a[e] = 0.f;
+    if (part < parts) {
+      for (int k = part * 16; k < c.np; k += parts * 16) {
+        const int oa = xat(bi * 32 + (lane & 31), k + 8 * hi), ob = xat(bj * 32 + (lane & 31), k + 8 * hi);
+        const f16x8 ah = *reinterpret_cast<const f16x8*>(x + oa), bh = *reinterpret_cast<const f16x8*>(x + ob);
+        if (NP == 2) {
+          const f16x8 al = *reinterpret_cast<const f16x8*>(x + plane + oa), bl = *reinterpret_cast<const f16x8*>(x + plane + ob);
+          a = __builtin_amdgcn_mfma_f32_32x32x16_f16(ah, bl, a, 0, 0, 0);
+          a = __builtin_amdgcn_mfma_f32_32x32x16_f16(al, bh, a, 0, 0, 0);
+        }
+        a = __builtin_amdgcn_mfma_f32_32x32x16_f16(ah, bh, a, 0, 0, 0);
+      }
+      if (part > 0) {
+        float4* o = reinterpret_cast<float4*>(lds) + ((part - 1) * nb + blk) * 256 + lane;          // at most 7 blocks of 4 KB
+#pragma unroll
+        for (int e4 = 0; e4 < 4; ++e4) o[e4 * 64] = make_float4(a[e4 * 4], a[e4 * 4 + 1], a[e4 * 4 + 2], a[e4 * 4 + 3]);
+      }
+    }
+    __syncthreads();
+    if (part == 0) {
+      for (int q = 1; q < parts; ++q) {
+        const float4* o = reinterpret_cast<const float4*>(lds) + ((q - 1) * nb + blk) * 256 + lane;
+#pragma unroll
+        for (int e4 = 0; e4 < 4; ++e4) {
+          const float4 v = o[e4 * 64];
+          a[e4 * 4] += v.x; a[e4 * 4 + 1] += v.y; a[e4 * 4 + 2] += v.z; a[e4 * 4 + 3] += v.w;
+        }
+      }
+    }
+    __syncthreads();
+    if (part == 0) {
+      const float un = res * res / (sx * sx);
+#pragma unroll
+      for (int e = 0; e < 16; ++e) a[e] *= un;
+      m.put_gram(a, p.rec.sA[s0], bi, bj);
+    }
+    __syncthreads();
+    const f32x16 P = m.run(p.rec, s0, s1);
+    __syncthreads();
+    if (m.inside) m.put(0, P);
+    __syncthreads();
+    // X <- P X in place: a wave takes blocks of 32 columns, all rows of them (nobody else reads those columns)
+    const bool done = s1 == steps - 1;
+    const float un = res / (p.rec.step[s1].sP * sx), to = p.sx[s1 + 1];
+    for (int nblk = wave; nblk * 32 < c.np; nblk += 8) {
+      f32x16 y[2];
+#pragma unroll
+      for (int v = 0; v < 2; ++v)
+#pragma unroll
+        for (int e = 0; e < 16; ++e) y[v][e] = 0.f;
+      for (int k = 0; k < c.mp; k += 16) {
+        // columns of X as rows of the first operand: 4 k of one column a lane and read
+        f16x8 xf[NP];
+#pragma unroll
+        for (int z = 0; z < NP; ++z) {
+          f16x4 half[2];
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {
+            const int kr = k + 8 * hi + 4 * h + ((lane & 15) >> 2), col = nblk * 32 + ((lane >> 4) & 1) * 16 + (lane & 3) * 4;
+            half[h] = __builtin_bit_cast(f16x4, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)(x + z * plane + xat(kr, col))));
+          }
+          xf[z] = __builtin_shufflevector(half[0], half[1], 0, 1, 2, 3, 4, 5, 6, 7);
+        }
+#pragma unroll
+        for (int v = 0; v < 2; ++v) {
+          if (v * 32 >= c.mp) continue;
+          const int o = NsOnCu<2>::at(v * 32 + (lane & 31), (k >> 3) + hi);
+          const f16x8 ph = *reinterpret_cast<const f16x8*>(lds + o), pl = *reinterpret_cast<const f16x8*>(lds + NsOnCu<2>::PL + o);
+          if (NP == 2) y[v] = __builtin_amdgcn_mfma_f32_32x32x16_f16(xf[NP - 1], ph, y[v], 0, 0, 0);
+          y[v] = __builtin_amdgcn_mfma_f32_32x32x16_f16(xf[0], pl, y[v], 0, 0, 0);
+          y[v] = __builtin_amdgcn_mfma_f32_32x32x16_f16(xf[0], ph, y[v], 0, 0, 0);
+        }
+      }
+      // a lane: row 32 v + lane % 32, columns 32 nblk + 8 e4 + 4 (lane / 32) + 0 .. 3
+#pragma unroll
+      for (int v = 0; v < 2; ++v) {
+        if (v * 32 >= c.mp) continue;
+        const int r = v * 32 + (lane & 31);
+#pragma unroll
+        for (int e4 = 0; e4 < 4; ++e4) {
+          const int q = nblk * 32 + 8 * e4 + 4 * hi;
+          if (!done) {
+            f16x4 h, l;
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+              const float w = y[v][e4 * 4 + e] * un * to;
+              h[e] = (_Float16)w;
+              l[e] = (_Float16)(w - (float)h[e]);
+            }
+            *reinterpret_cast<f16x4*>(x + xat(r, q)) = h;
+            if (NP == 2) *reinterpret_cast<f16x4*>(x + plane + xat(r, q)) = l;
+          } else if (r < c.m) {
+            T* o = reinterpret_cast<T*>(it.p);
+            const float f = p.muon ? -p.lr * it.scale : 1.f;
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+              if (q + e < c.n) {
+                const size_t at = tall ? (size_t)(q + e) * c.cols + r : (size_t)r * c.cols + q + e;
+                const float w = y[v][e4 * 4 + e] * un * f;
+                o[at] = from_f<T>(p.muon ? to_f(o[at]) * p.decay + w : w);
+              }
+          }
+        }
+      }
+    }
+    if (done) break;
+    __syncthreads();
+    s0 = s1 + 1;
   }
 }
 
@@ -895,9 +1162,14 @@ inline int sym_tiles(int mp, int t) { const int k = (mp + t - 1) / t; return k *
 // one or two workgroups are on a CU), shares written and read at 5 TB/s and 4 us for the launch that adds them
 // (small: 1.2 us for every 16 of them in the recursion's workgroup).  23 x 256 x 2304: 230 small
 // tiles in one share 24 us (model) against 34 measured for 8 shares of 69 large ones; 3 x 512 x 4608: 8 shares of 30 large tiles.
-struct NsSplit { int tile, shares, tiles, small, mt; };
-NsSplit ns_split_plan(std::vector<NsClass>& cls) {
-  NsSplit r = {64, 1, 0, 1, 2};
+struct NsSplit { int tile, shares, tiles, small, mt, tiny; };
+inline bool ns_is_tiny(const NsClass& c, int planes) { return c.mp <= 64 && c.np <= (planes == 2 ? NS_TINY_N<2> : NS_TINY_N<1>); }
+NsSplit ns_split_plan(std::vector<NsClass>& cls, int planes) {
+  NsSplit r = {64, 1, 0, 1, 2, 0};
+  if (ns_is_tiny(cls[0], planes)) {               // (and with it all of the set)
+    r.tiny = 1;
+    return r;
+  }
   int longest = 0;
   for (auto& c : cls) {
     if (c.mp > 64) r.mt = 4;
@@ -960,8 +1232,9 @@ int ns_plan(const char* what, int dtype, const pxl_ns_item* items, int n, NsPlan
       c.chunk = (int)chunk;
       c.parts = (int)((size + chunk - 1) / chunk);
       c.stride = round_up_z((size_t)plan.xplanes * c.mp * c.np * 2 + (size_t)5 * 2 * c.mp * c.mp * 2, 256);
-      // matrices whose recursion runs on one CU, by its two sizes, and the others: in sets of their own
-      auto kind = [](const NsClass& x) { return x.mp <= 64 ? 0 : (x.mp <= 128 ? 1 : 2); };
+      // matrices that run on one CU whole, those whose recursion does, by its two sizes, and the others: in sets of their own
+      auto kind = [&](const NsClass& x) { return ns_is_tiny(x, plan.np) ? 0 : (x.mp <= 64 ? 1 : (x.mp <= 128 ? 2 : 3)); };
+      if (ns_is_tiny(c, plan.np)) c.stride = 0;
       for (size_t q = 0; q < sets.size(); ++q)
         if (kind(sets[q].cls[0]) == kind(c) && sets[q].cls.size() < (size_t)NS_MAX_CLASSES) sk = (int)q;
       if (sk < 0) {
@@ -982,8 +1255,8 @@ int ns_plan(const char* what, int dtype, const pxl_ns_item* items, int n, NsPlan
     if (head > plan.head) plan.head = head;
   }
   for (auto& s : sets) {
-    const NsSplit sp = ns_split_plan(s.cls);
-    size_t at = plan.head + (sp.shares > 1 || sp.small ? (size_t)sp.shares * sp.tiles * sp.tile * sp.tile * sizeof(float) : 0);
+    const NsSplit sp = ns_split_plan(s.cls, plan.np);
+    size_t at = plan.head + (!sp.tiny && (sp.shares > 1 || sp.small) ? (size_t)sp.shares * sp.tiles * sp.tile * sp.tile * sizeof(float) : 0);
     for (auto& c : s.cls) { c.base = at; at += c.stride * c.count; }
     s.bytes = at;
     if (at > plan.bytes) plan.bytes = at;
@@ -1090,6 +1363,26 @@ int ns_gemm(NsRun& r, const NsGemm& g, int jobs = 1) {
   return ns_big_tiles(big * jobs, few * jobs) ? ns_launch<EPI, NA, NB, 128, OutT>(r, g, jobs) : ns_launch<EPI, NA, NB, 64, OutT>(r, g, jobs);
 }
 
+// coefficients and plane scales of steps [s, e), one segment, at places [at, ...)
+void ns_rec_scales(NsRec& q, const std::vector<NsStep>& steps, size_t s, size_t e, size_t at) {
+  double pbound = 1.0;
+  float sP = 1.f;
+  q.sA[at] = plane_scale(steps[s].lam);
+  for (size_t k = s; k < e; ++k) {
+    const NsStep& d = steps[k];
+    NsRecStep& o = q.step[at + k - s];
+    const float sA = plane_scale(d.lam), sQ = plane_scale(d.q), sT = plane_scale(d.t), before = sP;
+    pbound *= d.q;
+    o.sP = sP = plane_scale(pbound);                     // (the first step's P is Q: the same scale)
+    o.g = (float)d.c * sQ / (sA * sA);
+    o.ia = (float)d.b * sQ / sA;
+    o.a = (float)d.a * sQ;
+    o.fP = sP / (sQ * before);
+    o.fT = sT / (sQ * sA);
+    o.fA = (k + 1 < e ? plane_scale(steps[k + 1].lam) : 1.f) / (sQ * sT);
+  }
+}
+
 // the recursion of steps [s, e) of a small set: shares -> P in slot `out`; -> the scale of P's planes
 int ns_rec(NsRun& r, const std::vector<NsStep>& steps, size_t s, size_t e, float unscale, int res_pow, int xplanes, int out, float* sP) {
   NsRec q;
@@ -1100,14 +1393,8 @@ int ns_rec(NsRun& r, const std::vector<NsStep>& steps, size_t s, size_t e, float
   q.unscale = unscale;
   q.res_pow = res_pow;
   q.part = r.shares;
-  double pbound = 1.0;
-  for (size_t k = s; k < e; ++k) {
-    const NsStep& d = steps[k];
-    pbound *= d.q;
-    q.sA[k - s] = plane_scale(d.lam); q.sQ[k - s] = plane_scale(d.q); q.sT[k - s] = plane_scale(d.t); q.sP[k - s] = plane_scale(pbound);
-    q.a[k - s] = (float)d.a; q.b[k - s] = (float)d.b; q.c[k - s] = (float)d.c;
-  }
-  *sP = q.sP[q.steps - 1];
+  ns_rec_scales(q, steps, s, e, 0);
+  *sP = q.step[q.steps - 1].sP;
   int at = 0, tiles = 0;
   for (int k = 0; k < r.cs.n; ++k) {
     NsClass& c = r.cs.c[k];
@@ -1124,7 +1411,35 @@ int ns_rec(NsRun& r, const std::vector<NsStep>& steps, size_t s, size_t e, float
 }
 
 template <typename T, int NP>
+int ns_run_tiny(NsRun& r, const std::vector<NsStep>& steps, float eps, const MuonArgs& ma, int muon) {
+  NsTiny q;
+  memset(&q, 0, sizeof(q));
+  q.rec.steps = (int)steps.size();
+  for (size_t s = 0; s < steps.size();) {
+    size_t e = s;
+    while (!steps[e].last) ++e;
+    ns_rec_scales(q.rec, steps, s, e + 1, s);
+    q.ends |= 1u << e;
+    q.sx[s] = plane_scale(s == 0 ? 1.0 : steps[s].sigma);
+    s = e + 1;
+  }
+  q.eps = eps;
+  q.muon = muon;
+  q.lr = ma.lr;
+  q.decay = ma.keep;
+  int at = 0;
+  for (int k = 0; k < r.cs.n; ++k) {
+    r.cs.c[k].start = at;
+    at += r.cs.c[k].count;
+  }
+  hipLaunchKernelGGL((ns_tiny_kernel<T, NP>), dim3(at), dim3(512), 0, r.st, r.cs, q, r.few, r.table, ma);
+  PXL_LAUNCH_CHECK();
+  return PXL_OK;
+}
+
+template <typename T, int NP>
 int ns_run_set(NsRun& r, const std::vector<NsStep>& steps, float eps, const MuonArgs& ma, int muon) {
+  if (r.split.tiny) return ns_run_tiny<T, NP>(r, steps, eps, ma, muon);
   const int xplanes = 2 * NP, MA = xplanes, MT = xplanes + 1;
   int blocks = 0;
   for (int k = 0; k < r.cs.n; ++k) {
@@ -1279,7 +1594,7 @@ int ns_run(const char* what, int dtype, const pxl_ns_item* items, int n, int ste
     r.part = reinterpret_cast<double*>(r.ws + round_up_z(set.items * sizeof(NsItem), 256));
     r.residue = reinterpret_cast<float*>(reinterpret_cast<unsigned char*>(r.part) + round_up_z(set.items * sizeof(double) * NS_PARTS, 256));
     r.cs.n = (int)set.cls.size();
-    r.split = ns_split_plan(set.cls);
+    r.split = ns_split_plan(set.cls, plan.np);
     r.shares = reinterpret_cast<float*>(r.ws + plan.head);
     for (int k = 0; k < r.cs.n; ++k) r.cs.c[k] = set.cls[k];
     std::vector<NsItem> list;

@@ -52,7 +52,7 @@ def gradient(shape, seed, dtype=torch.float32, rank=4):
 
 
 SHAPES = [(1, 1), (1, 64), (70, 1), (3, 5), (31, 33), (2, 32, 32), (64, 147), (147, 64), (5, 40, 70), (129, 257), (256, 256), (3, 200, 640), (300, 128),
-          (21, 4608), (2304, 96), (513, 640), (2, 3, 16, 24), (65, 65)]
+          (21, 4608), (2304, 96), (513, 640), (2, 3, 16, 24), (65, 65), (64, 384), (384, 63), (64, 385), (33, 256), (257, 64), (2, 32, 417), (300, 1, 5)]
 
 
 @pytest.mark.gpu
@@ -83,7 +83,7 @@ def spectrum(m, n, kind, seed):
 def test_spectra(kind, dtype):
     """from one strong direction to singular values over six decades: where rounding of A next to zero would grow"""
     from pixelssl_amd import functional as PF
-    for m, n in ((96, 160), (160, 160)):
+    for m, n in ((60, 130), (96, 160), (160, 160)):
         x = spectrum(m, n, kind, 3).to(dtype)
         for y in (x, x.t().contiguous()):
             close(PF.orthogonalize(y.cuda()), exact(y), dtype, what="%s %s" % (kind, tuple(y.shape)))
@@ -208,6 +208,18 @@ def test_muon_update_of_mixed_shapes(nesterov, wd):
         PF.muon_update([a[0]], [a[1]], [a[2]], lr=0.02, nesterov=nesterov, weight_decay=wd)
         muon_close(a[0], a[2], want[k], torch.float32, "alone, %s" % (MIX[k],))
         assert torch.equal(a[2], m)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("rows,step", [(20, 3), (40, 30), (100, 11)])
+def test_muon_update_of_many_shapes(rows, step):
+    """15 shapes that run alike: more than the arguments of one launch hold"""
+    from pixelssl_amd import functional as PF
+    trip = [make((rows, 24 + step * k) if k % 2 else (24 + step * k, rows), k) for k in range(15)]
+    want = [muon_exact(p, g, m, 0.01) for p, g, m in trip]
+    PF.muon_update(*zip(*trip), lr=0.01)
+    for (p, g, m), w in zip(trip, want):
+        muon_close(p, m, w, torch.float32, str(tuple(p.shape)))
 
 
 @pytest.mark.gpu
