@@ -376,7 +376,7 @@ __device__ __forceinline__ void chan_sum(float (&s)[NS][V], float* sh) {
     for (int e = 0; e < V; ++e) s[k][e] = sh[NW * W + (k * TSV + sv) * V + e];
 }
 
-// addresses: a base per j that the whole workgroup shares, and one 32-bit byte offset per lane (CY * S elements stay below 2^31 bytes)
+// addresses: a base per j that the whole workgroup shares, and one 32-bit byte offset per lane (CY S <= 2^8 2^22 elements of 4 bytes)
 template <typename T> __device__ __forceinline__ const T* lane_at(const T* base, unsigned off) {
   return reinterpret_cast<const T*>(reinterpret_cast<const unsigned char*>(base) + off);
 }
@@ -659,7 +659,9 @@ inline LnShape ln_shape(int dtype, long R, int C, long S) { return S < 0 ? ln_ro
     else if (key == 256 * 16 + 4) LN_ROWS_TAIL(KERNEL, 256, 4, __VA_ARGS__);                                           \
     else if constexpr (sizeof(T) == 4) LN_ROWS_TAIL(KERNEL, 256, 8, __VA_ARGS__);                                      \
   } while (0)
-#define LN_CHAN(KERNEL, BLOCKS, ...)                                                                                                 \
+// more than 1024 channels: a piece of MANY channels a thread.  16 of them over 512 threads (two workgroups a CU) forward, 87 us for
+// 8 x 2048 x 65 x 65 bf16 (8 over 1024 threads 104); backward holds x and dy, one workgroup a CU either way: 8 over 1024 threads, 183 us (194)
+#define LN_CHAN(KERNEL, MANY, BLOCKS, ...)                                                                                           \
   do {                                                                                                                               \
     const dim3 grid(BLOCKS);                                                                                                         \
     if (s.threads == 256 && s.tsv == 8) {                                                                                            \
@@ -669,7 +671,7 @@ inline LnShape ln_shape(int dtype, long R, int C, long S) { return S < 0 ? ln_ro
       else hipLaunchKernelGGL((KERNEL<T, 256, 8, 8>), grid, dim3(256), 0, st, __VA_ARGS__);                                          \
     } else if (s.threads == 256) hipLaunchKernelGGL((KERNEL<T, 256, 4, 8>), grid, dim3(256), 0, st, __VA_ARGS__);                    \
     else if (s.nv == 8) hipLaunchKernelGGL((KERNEL<T, 512, 4, 8>), grid, dim3(512), 0, st, __VA_ARGS__);                             \
-    else hipLaunchKernelGGL((KERNEL<T, 512, 4, 16>), grid, dim3(512), 0, st, __VA_ARGS__);                                           \
+    else hipLaunchKernelGGL((KERNEL<T, 8192 / MANY, 4, MANY>), grid, dim3(8192 / MANY), 0, st, __VA_ARGS__);                         \
   } while (0)
 
 template <typename T>
@@ -685,7 +687,7 @@ int ln_fwd(long R, int C, long S, long xs, const void* x, LnParam w, LnParam b, 
     }
   } else if (s.lanes) {
     const int per = (int)(s.tiles / (R / S));
-    LN_CHAN(ln_chan_fwd, (unsigned)s.tiles, (int)s.tiles, per, C, (int)S, (const T*)x, w, b, eps, (T*)y, mean, rstd);
+    LN_CHAN(ln_chan_fwd, 16, (unsigned)s.tiles, (int)s.tiles, per, C, (int)S, (const T*)x, w, b, eps, (T*)y, mean, rstd);
   } else {
     hipLaunchKernelGGL(ln_chan_fwd_loop<T>, dim3(blocks_for((R + 255) / 256, 1 << 20)), dim3(256), 0, st, R, C, S, (const T*)x, w, b, eps,
                        (T*)y, mean, rstd);
@@ -706,7 +708,7 @@ int ln_bwd(long R, int C, long S, long xs, const void* x, const void* dy, LnPara
       LN_ROWS(ln_rows_bwd, (unsigned)G, R, C, xs, (const T*)x, (const T*)dy, w, mean, rstd, (T*)dx, p);
     } else {
       const int per = (int)(s.tiles / (R / S));
-      LN_CHAN(ln_chan_bwd, (unsigned)G, (int)s.tiles, per, C, (int)S, (const T*)x, (const T*)dy, w, mean, rstd, (T*)dx, p);
+      LN_CHAN(ln_chan_bwd, 8, (unsigned)G, (int)s.tiles, per, C, (int)S, (const T*)x, (const T*)dy, w, mean, rstd, (T*)dx, p);
     }
     PXL_LAUNCH_CHECK();
   } else if (R > 0) {
