@@ -247,7 +247,8 @@ struct NsGemm {
   int res_pow;                          // GRAM: value *= residue^2;  OUT / X: value *= residue
   float lr, decay;                      // OUT of a Muon step
   int muon;
-  float* part;                          // PART: [split][tile][T * T] accumulators
+  float* part;                          // PART: [share][tile][T * T] accumulators;  cut tiles: [job][tile][share][T * T]
+  int full, cut;                        // symmetric products in 128 x 128 tiles: tiles from `full` on run in `cut` shares of K each (1: none do)
 };
 
 // lower-triangular tile number t -> (row, column), row >= column
@@ -333,6 +334,8 @@ template <int T> __device__ __forceinline__ int chunk_at(int r, int ch) {       
 template <int T> __device__ __forceinline__ int segment_at(int k, int seg) {       // byte of 32-byte segment seg of row k
   return T == 128 ? k * 256 + ((seg ^ ((k & 3) << 1)) << 5) : k * 128 + ((seg ^ (k & 2)) << 5);
 }
+// k of a share of a cut tile
+__host__ __device__ inline int ns_cut(int K, int cut) { return (K / 32 + cut - 1) / cut * 32; }
 template <int EPI, int NA, int NB, int T, int D, typename OutT>
 __global__ __launch_bounds__(256, D == 2 ? 2 : 1) void ns_gemm_kernel(NsClasses cs, NsGemm p, NsInline few, const NsItem* __restrict__ table,
                                                          const float* __restrict__ residue, unsigned char* __restrict__ ws) {
@@ -342,14 +345,16 @@ __global__ __launch_bounds__(256, D == 2 ? 2 : 1) void ns_gemm_kernel(NsClasses 
   constexpr int BUF = (NA + NB) * PL;
   constexpr int WB = T == 128 ? 1 : 2;          // blocks of 32 x 32 a wave ends up with: 4 / 1
   __shared__ __attribute__((aligned(16))) unsigned char lds[T == 64 && 2 * BUF < 65536 ? 65536 : 2 * BUF];
-  const int bid = xcd_remap(blockIdx.x, gridDim.x);
+  constexpr bool CUTS = T == 128 && SYM && EPI != EPI_PART;
+  const bool cut = CUTS && (int)blockIdx.x >= p.full;
+  const int bid = !CUTS ? xcd_remap(blockIdx.x, gridDim.x) : (cut ? p.full + (int)(blockIdx.x - p.full) / p.cut : xcd_remap(blockIdx.x, p.full));
   const NsClass c = find_class(cs, bid);
   const int local = bid - c.start, i = local / c.per, t = local - i * c.per;
   int tr, tc;
   if (SYM) tri_tile(t, tr, tc);
   else { tr = t / c.tn; tc = t - tr * c.tn; }
   unsigned char* base = ws + c.base + (size_t)i * c.stride;
-  const int K = EPI <= EPI_PART ? c.np : c.mp;
+  const int K = EPI <= EPI_PART ? c.np : c.mp;          // (a multiple of 32)
   const size_t plane_a = (size_t)c.mp * K, plane_b = NN ? (size_t)c.mp * c.np : (size_t)c.mp * K;
   const int z = EPI == EPI_MUL ? blockIdx.z : 0;
   const NsJob job = p.job[z];
@@ -362,6 +367,13 @@ __global__ __launch_bounds__(256, D == 2 ? 2 : 1) void ns_gemm_kernel(NsClasses 
     k0 = blockIdx.y * c.ks;
     k1 = k0 + c.ks < K ? k0 + c.ks : K;
     if (k0 >= k1) return;                       // (shapes with fewer shares than the grid has: never read)
+  }
+  const int share = cut ? (int)(blockIdx.x - p.full) % p.cut : 0;
+  if (cut) {
+    const int ks = ns_cut(K, p.cut);
+    k0 = share * ks;
+    k1 = k0 + ks < K ? k0 + ks : K;
+    if (k0 >= k1) return;                       // (never read)
   }
   const int steps = (k1 - k0 + KS - 1) / KS;
   // byte offsets of a thread's chunks from the tile's first element, and where they go in LDS
@@ -428,14 +440,15 @@ __global__ __launch_bounds__(256, D == 2 ? 2 : 1) void ns_gemm_kernel(NsClasses 
   }
   NsOld old[EPI == EPI_Q && T == 128 ? 4 : 1];
   if (EPI == EPI_Q && T == 64) old[0] = ns_load_sym(c, A, tr * 64 + wr * 32, tc * 64 + wc * 32);
-  auto multiply = [&](const unsigned char* buf, int kk) {           // k 16 kk .. 16 kk + 15 of the step
-    f16x8 fa[NA][2], fb[NB][2];
+  // fragments of k 16 kk .. 16 kk + 15 of a step
+  struct Frags { f16x8 a[NA][2], b[NB][2]; };
+  auto read = [&](Frags& f, const unsigned char* buf, int kk) {
     const int ro = T == 128 ? wr * 64 : 0, qo = T == 128 ? wc * 64 : 0, ch = kk * 2 + (lane >> 5);
 #pragma unroll
     for (int u = 0; u < 2; ++u) {
       const int r = ro + u * 32 + (lane & 31), q = qo + u * 32 + (lane & 31);
 #pragma unroll
-      for (int z = 0; z < NA; ++z) fa[z][u] = *reinterpret_cast<const f16x8*>(buf + z * PL + chunk_at<T>(r, ch));
+      for (int z = 0; z < NA; ++z) f.a[z][u] = *reinterpret_cast<const f16x8*>(buf + z * PL + chunk_at<T>(r, ch));
 #pragma unroll
       for (int z = 0; z < NB; ++z) {
         if (NN) {
@@ -447,25 +460,27 @@ __global__ __launch_bounds__(256, D == 2 ? 2 : 1) void ns_gemm_kernel(NsClasses 
             half[h] = __builtin_bit_cast(f16x4, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)(
                 buf + (NA + z) * PL + segment_at<T>(kr, (qo + u * 32) / 16 + ((lane >> 4) & 1)) + ((lane & 3) << 3))));
           }
-          fb[z][u] = __builtin_shufflevector(half[0], half[1], 0, 1, 2, 3, 4, 5, 6, 7);
+          f.b[z][u] = __builtin_shufflevector(half[0], half[1], 0, 1, 2, 3, 4, 5, 6, 7);
         } else {
-          fb[z][u] = *reinterpret_cast<const f16x8*>(buf + (NA + z) * PL + chunk_at<T>(q, ch));
+          f.b[z][u] = *reinterpret_cast<const f16x8*>(buf + (NA + z) * PL + chunk_at<T>(q, ch));
         }
       }
     }
+  };
+  auto multiply = [&](const Frags& f) {
     // X: the operands the other way round, so that a lane holds four consecutive columns of one row of the result
 #define NS_MFMA(A_, B_, C_) (EPI == EPI_X ? __builtin_amdgcn_mfma_f32_32x32x16_f16(B_, A_, C_, 0, 0, 0) : __builtin_amdgcn_mfma_f32_32x32x16_f16(A_, B_, C_, 0, 0, 0))
 #pragma unroll
     for (int u = 0; u < 2; ++u)
 #pragma unroll
       for (int v = 0; v < 2; ++v) {
-        if (NB == 2) acc[u][v] = NS_MFMA(fa[0][u], fb[NB - 1][v], acc[u][v]);
-        if (NA == 2) acc[u][v] = NS_MFMA(fa[NA - 1][u], fb[0][v], acc[u][v]);
-        acc[u][v] = NS_MFMA(fa[0][u], fb[0][v], acc[u][v]);
+        if (NB == 2) acc[u][v] = NS_MFMA(f.a[0][u], f.b[NB - 1][v], acc[u][v]);
+        if (NA == 2) acc[u][v] = NS_MFMA(f.a[NA - 1][u], f.b[0][v], acc[u][v]);
+        acc[u][v] = NS_MFMA(f.a[0][u], f.b[0][v], acc[u][v]);
       }
 #undef NS_MFMA
   };
-  auto step = [&](int s, int slot) {
+  auto put = [&](int s, int slot) {
     unsigned char* buf = lds + (s & 1) * BUF;
 #pragma unroll
     for (int q = 0; q < 2; ++q) {
@@ -475,22 +490,49 @@ __global__ __launch_bounds__(256, D == 2 ? 2 : 1) void ns_gemm_kernel(NsClasses 
       for (int z = 0; z < NB; ++z) *reinterpret_cast<u32x4*>(buf + (NA + z) * PL + lb[q]) = rb[slot][z][q];
     }
     fetch(slot);
-    __syncthreads();
-    if (T == 128) {
-      multiply(buf, 0);
-      multiply(buf, 1);
-    } else if (k0 + s * KS + wave * 16 < k1) {
-      multiply(buf, wave);
-    }
   };
-  int s = 0;
-  for (; s + D <= steps; s += D) {
+  if constexpr (T == 128) {
+    // LDS is read ahead of the matrix instructions by half a step: while those of one half run, the other half's operands arrive and the next
+    // step's tiles are written.  (The last step writes and reads on, in bounds and unused.)
+    static_assert(D == 2, "slots by the parity of the step");
+    Frags f0, f1;
+    auto step = [&](int s, int next) {
+      const unsigned char *buf = lds + (s & 1) * BUF, *then = lds + ((s + 1) & 1) * BUF;
+      read(f1, buf, 1);
+      multiply(f0);
+      put(s + 1, next);
+      __syncthreads();
+      read(f0, then, 0);
+      multiply(f1);
+    };
+    put(0, 0);
+    __syncthreads();
+    read(f0, lds, 0);
+    int s = 0;
+    for (; s + 2 <= steps; s += 2) {
+      step(s, 1);
+      step(s + 1, 0);
+    }
+    if (s < steps) step(s, 1);
+  } else {
+    auto step = [&](int s, int slot) {
+      put(s, slot);
+      __syncthreads();
+      if (k0 + s * KS + wave * 16 < k1) {
+        Frags f;
+        read(f, lds + (s & 1) * BUF, wave);
+        multiply(f);
+      }
+    };
+    int s = 0;
+    for (; s + D <= steps; s += D) {
 #pragma unroll
-    for (int d = 0; d < D; ++d) step(s + d, d);
+      for (int d = 0; d < D; ++d) step(s + d, d);
+    }
+#pragma unroll
+    for (int d = 0; d < D - 1; ++d)
+      if (s + d < steps) step(s + d, d);
   }
-#pragma unroll
-  for (int d = 0; d < D - 1; ++d)
-    if (s + d < steps) step(s + d, d);
 
   // T = 64: the waves' sums through LDS; wave w goes on with block (w / 2, w % 2)
   f32x16 sum;
@@ -537,6 +579,17 @@ __global__ __launch_bounds__(256, D == 2 ? 2 : 1) void ns_gemm_kernel(NsClasses 
       for (int e4 = 0; e4 < 4; ++e4) o[e4 * 64] = make_float4(a[e4 * 4], a[e4 * 4 + 1], a[e4 * 4 + 2], a[e4 * 4 + 3]);
     });
     return;
+  }
+  if constexpr (CUTS) {
+    if (cut) {
+      const size_t tile = ((size_t)z * ((gridDim.x - p.full) / p.cut) + (bid - p.full)) * p.cut + share;
+      blocks([&](int n, int, int, const f32x16& a) {
+        float4* o = reinterpret_cast<float4*>(p.part) + (tile * 16 + n) * 256 + lane;
+#pragma unroll
+        for (int e4 = 0; e4 < 4; ++e4) o[e4 * 64] = make_float4(a[e4 * 4], a[e4 * 4 + 1], a[e4 * 4 + 2], a[e4 * 4 + 3]);
+      });
+      return;
+    }
   }
   const float scale = p.scale[z];
   float un = p.unscale[z];
@@ -662,6 +715,25 @@ __global__ __launch_bounds__(64) void ns_fold_kernel(NsClasses cs, NsGemm p, int
   const float rs = residue[c.first + i];
   _Float16* out = reinterpret_cast<_Float16*>(ws + c.base + (size_t)i * c.stride + slot_off(c, p.xplanes, p.job[0].out));
   ns_store_sym<EPI_GRAM>(c, p, NsOld(), out, tr * T + br * 32, tc * T + bc * 32, p.unscale[0] * (p.res_pow == 2 ? rs * rs : 1.f), p.scale[0], a);
+}
+
+// the shares of a product's cut tiles -> its result; one wave a block of 32 x 32
+template <int EPI>
+__global__ __launch_bounds__(64) void ns_cut_fold_kernel(NsClasses cs, NsGemm p, const float* __restrict__ residue, unsigned char* __restrict__ ws) {
+  const int j = blockIdx.x >> 4, n = blockIdx.x & 15, bid = p.full + j, z = blockIdx.z;
+  const NsClass c = find_class(cs, bid);
+  const int local = bid - c.start, i = local / c.per, t = local - i * c.per;
+  int tr, tc;
+  tri_tile(t, tr, tc);
+  const int r = tr * 128 + ((n >> 3) * 2 + ((n >> 1) & 1)) * 32, q = tc * 128 + (((n >> 2) & 1) * 2 + (n & 1)) * 32;
+  const int K = EPI == EPI_GRAM ? c.np : c.mp, ks = ns_cut(K, p.cut);
+  unsigned char* base = ws + c.base + (size_t)i * c.stride;
+  NsOld old;
+  if (EPI == EPI_Q) old = ns_load_sym(c, reinterpret_cast<const _Float16*>(base + slot_off(c, p.xplanes, p.job[z].a)), r, q);
+  const f32x16 a = ns_share_sum<4>(p.part, (K + ks - 1) / ks, 16, ((size_t)z * (gridDim.x >> 4) + j) * p.cut * 16 + n);
+  float un = p.unscale[z];
+  if (EPI == EPI_GRAM && p.res_pow) un *= residue[c.first + i] * residue[c.first + i];
+  ns_store_sym<EPI>(c, p, old, reinterpret_cast<_Float16*>(base + slot_off(c, p.xplanes, p.job[z].out)), r, q, un, p.scale[z], a);
 }
 
 // ---- the recursion of a whole segment on one CU, for matrices of at most 32 MT rows ---------------------------------------------------
@@ -1147,14 +1219,38 @@ struct NsPlan {
   size_t bytes;
 };
 
-// 128 x 128 tiles or about four times as many of 64 x 64, by rounds over the 256 CUs: a small tile takes 0.4 of a large one's time (23 x P X of
-// 256 x 2304: 39 us in 828 large, 51 us in 3312 small tiles; 2 products of 2048^3, symmetric: 105 us in 272 large, 106 us in 1056 small)
+inline int sym_tiles(int mp, int t) { const int k = (mp + t - 1) / t; return k * (k + 1) / 2; }
+
+// A symmetric product of `jobs` times the classes' matrices.  Tile: 128 x 128, or about four times as many of 64 x 64, by rounds over the 256 CUs
+// of 0.82 us a K step of 32 of a large tile; a small one takes 0.4 of its time.  full / cut: large tiles that pass a multiple of 256 run last, in
+// `cut` shares of K over the whole card, which a pass of their own adds up: 65 KB written and read a share at 5 TB/s, 4 us for the launch.
+// (2 products of 2048 x 2048 x 2048 in 272 tiles: 105 us as two rounds, 106 us in 1056 small tiles, 84 + 8 us with 16 tiles in 8 shares)
+struct NsTiling { int tile, full, cut; double time; };
+NsTiling ns_sym_tiling(const NsClass* c, int n, bool gram, int jobs) {
+  long big = 0, few = 0;
+  int K = 0;
+  for (int k = 0; k < n; ++k) {
+    big += (long)sym_tiles(c[k].mp, 128) * c[k].count;
+    few += (long)sym_tiles(c[k].mp, 64) * c[k].count;
+    const int kk = gram ? c[k].np : c[k].mp;
+    K = kk > K ? kk : K;
+  }
+  const double round = K / 32 * 0.82, small = (jobs * few + 255) / 256 * 0.4 * round;
+  NsTiling r = {128, (int)big, 1, (jobs * big + 255) / 256 * round};
+  const long full = big / 256 * 256, rest = big - full;
+  if (full > 0 && rest > 0)
+    for (int s = 2; s <= 16 && s * rest <= 256; ++s) {
+      const double time = jobs * (full / 256 * round + round / s + s * rest * 131072 / 5e6) + 4.0;
+      if (time < r.time) { r.time = time; r.full = (int)full; r.cut = s; }
+    }
+  if (jobs * big < 128 || small < r.time) r = {64, 0, 1, small};
+  return r;
+}
+// other products: 23 x P X of 256 x 2304 39 us in 828 large, 51 us in 3312 small tiles
 inline bool ns_big_tiles(long big, long few) { return (big + 255) / 256 * 10 <= (few + 255) / 256 * 4 && big >= 128; }
 
 inline int round_up(int v, int to) { return (v + to - 1) / to * to; }
 inline size_t round_up_z(size_t v, size_t to) { return (v + to - 1) / to * to; }
-
-inline int sym_tiles(int mp, int t) { const int k = (mp + t - 1) / t; return k * (k + 1) / 2; }
 
 // How the matrices of one set run.  small: all have at most 128 on their smaller side, their recursion runs on one CU each.
 // Gram products may be cut along K (n) into shares that are added up in order; tile and share (K a workgroup takes) by a model of their
@@ -1162,10 +1258,10 @@ inline int sym_tiles(int mp, int t) { const int k = (mp + t - 1) / t; return k *
 // one or two workgroups are on a CU), shares written and read at 5 TB/s and 4 us for the launch that adds them
 // (small: 1.2 us for every 16 of them in the recursion's workgroup).  23 x 256 x 2304: 230 small
 // tiles in one share 24 us (model) against 34 measured for 8 shares of 69 large ones; 3 x 512 x 4608: 8 shares of 30 large tiles.
-struct NsSplit { int tile, shares, tiles, small, mt, tiny; };
+struct NsSplit { int tile, shares, tiles, small, mt, tiny, full, cut; size_t bytes; };      // bytes: of all shares, cut tiles' too
 inline bool ns_is_tiny(const NsClass& c, int planes) { return c.mp <= 64 && c.np <= (planes == 2 ? NS_TINY_N<2> : NS_TINY_N<1>); }
 NsSplit ns_split_plan(std::vector<NsClass>& cls, int planes) {
-  NsSplit r = {64, 1, 0, 1, 2, 0};
+  NsSplit r = {64, 1, 0, 1, 2, 0, 0, 1, 0};
   if (ns_is_tiny(cls[0], planes)) {               // (and with it all of the set)
     r.tiny = 1;
     return r;
@@ -1192,11 +1288,26 @@ NsSplit ns_split_plan(std::vector<NsClass>& cls, int planes) {
       const double time = rounds * (t == 128 ? k / 32 * 0.82 : k / 64 * 0.66) + (s > 1 || r.small ? bytes / 5e6 : 0.0) + (s > 1 && !r.small ? 4.0 : 0.0) + (r.small ? (s + 15) / 16 * 1.2 : 0.0);
       if (time < best) { best = time; r.tile = t; ks = k; }
     }
+  NsTiling cut = {0, 0, 1, 0.0};
+  if (!r.small) {
+    cut = ns_sym_tiling(cls.data(), (int)cls.size(), true, 1);
+    if (cut.cut > 1 && cut.time < best) { r.tile = 128; ks = (longest + 63) / 64 * 64; }
+    else cut.cut = 1;
+  }
   for (auto& c : cls) {
     c.ks = ks;
     const int n = (c.np + ks - 1) / ks;
     if (n > r.shares) r.shares = n;
     r.tiles += sym_tiles(c.mp, r.tile) * c.count;
+  }
+  r.full = cut.cut > 1 ? cut.full : r.tiles;
+  r.cut = cut.cut;
+  if (r.shares > 1 || r.small) r.bytes = (size_t)r.shares * r.tiles * r.tile * r.tile * sizeof(float);
+  // cut tiles of any of the set's products: at most 256 a job
+  if (!r.small) {
+    const int n = (int)cls.size();
+    const bool any = cut.cut > 1 || ns_sym_tiling(cls.data(), n, false, 1).cut > 1 || ns_sym_tiling(cls.data(), n, false, 2).cut > 1;
+    if (any) r.bytes = std::max(r.bytes, (size_t)2 * 256 * 128 * 128 * sizeof(float));
   }
   return r;
 }
@@ -1256,7 +1367,7 @@ int ns_plan(const char* what, int dtype, const pxl_ns_item* items, int n, NsPlan
   }
   for (auto& s : sets) {
     const NsSplit sp = ns_split_plan(s.cls, plan.np);
-    size_t at = plan.head + (!sp.tiny && (sp.shares > 1 || sp.small) ? (size_t)sp.shares * sp.tiles * sp.tile * sp.tile * sizeof(float) : 0);
+    size_t at = plan.head + sp.bytes;
     for (auto& c : s.cls) { c.base = at; at += c.stride * c.count; }
     s.bytes = at;
     if (at > plan.bytes) plan.bytes = at;
@@ -1323,7 +1434,7 @@ struct NsRun {
   } while (0)
 
 template <int EPI, int NA, int NB, int T, typename OutT>
-int ns_launch(NsRun& r, const NsGemm& g, int jobs = 1) {
+int ns_launch(NsRun& r, NsGemm& g, int jobs = 1, int full = 0, int cut = 1) {
   int at = 0;
   for (int k = 0; k < r.cs.n; ++k) {
     NsClass& c = r.cs.c[k];
@@ -1333,13 +1444,22 @@ int ns_launch(NsRun& r, const NsGemm& g, int jobs = 1) {
     c.start = at;
     at += c.per * c.count;
   }
-  const dim3 grid(at, EPI == EPI_PART ? r.split.shares : 1, jobs);
+  g.full = cut > 1 ? full : at;
+  g.cut = cut;
+  const int rest = at - g.full;
+  const dim3 grid(g.full + rest * cut, EPI == EPI_PART ? r.split.shares : 1, jobs);
   if (T == 64 && at * jobs <= 256 && (EPI == EPI_Q || EPI == EPI_MUL))
     hipLaunchKernelGGL((ns_gemm_kernel<EPI, NA, NB, T, T == 64 && (EPI == EPI_Q || EPI == EPI_MUL) ? 4 : 2, OutT>), grid, dim3(256), 0, r.st, r.cs, g, r.few,
                        r.table, r.residue, r.ws);
   else
     hipLaunchKernelGGL((ns_gemm_kernel<EPI, NA, NB, T, 2, OutT>), grid, dim3(256), 0, r.st, r.cs, g, r.few, r.table, r.residue, r.ws);
   PXL_LAUNCH_CHECK();
+  if constexpr (T == 128 && (EPI == EPI_GRAM || EPI == EPI_Q || EPI == EPI_MUL)) {
+    if (rest > 0) {
+      hipLaunchKernelGGL((ns_cut_fold_kernel<EPI>), dim3(rest * 16, 1, jobs), dim3(64), 0, r.st, r.cs, g, r.residue, r.ws);
+      PXL_LAUNCH_CHECK();
+    }
+  }
   if (EPI == EPI_PART && !r.split.small) {
     hipLaunchKernelGGL((ns_fold_kernel<T>), dim3(at * (T * T / 1024)), dim3(64), 0, r.st, r.cs, g, at, r.residue, r.ws);
     PXL_LAUNCH_CHECK();
@@ -1348,19 +1468,23 @@ int ns_launch(NsRun& r, const NsGemm& g, int jobs = 1) {
 }
 
 template <int EPI, int NA, int NB, typename OutT>
-int ns_gemm(NsRun& r, const NsGemm& g, int jobs = 1) {
+int ns_gemm(NsRun& r, NsGemm& g, int jobs = 1) {
   if constexpr (EPI == EPI_GRAM) {
     if (r.split.shares > 1 || r.split.small)
       return r.split.tile == 128 ? ns_launch<EPI_PART, NA, NB, 128, OutT>(r, g) : ns_launch<EPI_PART, NA, NB, 64, OutT>(r, g);
-    return r.split.tile == 128 ? ns_launch<EPI, NA, NB, 128, OutT>(r, g) : ns_launch<EPI, NA, NB, 64, OutT>(r, g);
+    return r.split.tile == 128 ? ns_launch<EPI, NA, NB, 128, OutT>(r, g, 1, r.split.full, r.split.cut) : ns_launch<EPI, NA, NB, 64, OutT>(r, g);
+  } else if constexpr (EPI <= EPI_MUL) {
+    const NsTiling t = ns_sym_tiling(r.cs.c, r.cs.n, false, jobs);
+    return t.tile == 128 ? ns_launch<EPI, NA, NB, 128, OutT>(r, g, jobs, t.full, t.cut) : ns_launch<EPI, NA, NB, 64, OutT>(r, g, jobs);
+  } else {
+    long big = 0, few = 0;
+    for (int k = 0; k < r.cs.n; ++k) {
+      const NsClass& c = r.cs.c[k];
+      big += (long)((c.mp + 127) / 128) * ((c.np + 127) / 128) * c.count;
+      few += (long)((c.mp + 63) / 64) * ((c.np + 63) / 64) * c.count;
+    }
+    return ns_big_tiles(big, few) ? ns_launch<EPI, NA, NB, 128, OutT>(r, g) : ns_launch<EPI, NA, NB, 64, OutT>(r, g);
   }
-  long big = 0, few = 0;
-  for (int k = 0; k < r.cs.n; ++k) {
-    const NsClass& c = r.cs.c[k];
-    big += EPI <= EPI_MUL ? (long)sym_tiles(c.mp, 128) * c.count : (long)((c.mp + 127) / 128) * ((c.np + 127) / 128) * c.count;
-    few += EPI <= EPI_MUL ? (long)sym_tiles(c.mp, 64) * c.count : (long)((c.mp + 63) / 64) * ((c.np + 63) / 64) * c.count;
-  }
-  return ns_big_tiles(big * jobs, few * jobs) ? ns_launch<EPI, NA, NB, 128, OutT>(r, g, jobs) : ns_launch<EPI, NA, NB, 64, OutT>(r, g, jobs);
 }
 
 // coefficients and plane scales of steps [s, e), one segment, at places [at, ...)

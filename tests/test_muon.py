@@ -68,6 +68,19 @@ def test_orthogonalize(shape, dtype):
     close(got, exact(x), dtype, what=str(shape))
 
 
+@pytest.mark.gpu
+@pytest.mark.parametrize("shape,dtype", [((8, 1000, 1056), torch.float32), ((8, 2100, 1024), torch.float32), ((8, 1024, 1024), torch.bfloat16),
+                                         ((5, 2, 900, 1700), torch.float32), ((1, 2930, 2940), torch.bfloat16)],
+                         ids=lambda v: "x".join(map(str, v)) if isinstance(v, tuple) else str(v)[6:])
+def test_more_tiles_than_compute_units(shape, dtype):
+    """the tiles of the last round run in shares (the 64-bit products on the GPU: the plain formula all the same)"""
+    from pixelssl_amd import functional as PF
+    x = gradient(shape, 7, dtype).cuda()
+    got = PF.orthogonalize(x)
+    close(got, exact(x).cpu(), dtype, what=str(shape))
+    assert torch.equal(got, PF.orthogonalize(x))
+
+
 def spectrum(m, n, kind, seed):
     g = torch.Generator().manual_seed(seed)
     u, _, vh = torch.linalg.svd(torch.randn(m, n, generator=g, dtype=torch.float64), full_matrices=False)
@@ -216,6 +229,17 @@ def test_muon_update_of_many_shapes(rows, step):
     """15 shapes that run alike: more than the arguments of one launch hold"""
     from pixelssl_amd import functional as PF
     trip = [make((rows, 24 + step * k) if k % 2 else (24 + step * k, rows), k) for k in range(15)]
+    want = [muon_exact(p, g, m, 0.01) for p, g, m in trip]
+    PF.muon_update(*zip(*trip), lr=0.01)
+    for (p, g, m), w in zip(trip, want):
+        muon_close(p, m, w, torch.float32, str(tuple(p.shape)))
+
+
+@pytest.mark.gpu
+def test_muon_update_of_large_matrices_of_two_shapes():
+    """more tiles than compute units, of two shapes, the last round's of the second one"""
+    from pixelssl_amd import functional as PF
+    trip = [make((1000, 1024) if k < 4 else (900, 1300), k) for k in range(9)]
     want = [muon_exact(p, g, m, 0.01) for p, g, m in trip]
     PF.muon_update(*zip(*trip), lr=0.01)
     for (p, g, m), w in zip(trip, want):
