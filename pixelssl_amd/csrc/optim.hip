@@ -4,6 +4,9 @@
 //   * EMA teacher update (ssl_mt.py:359-363)
 #include <cmath>
 
+#include <algorithm>
+#include <vector>
+
 #include "common.h"
 
 namespace {
@@ -286,12 +289,40 @@ extern "C" int pxl_adam_step_wd(long n, float* p, const float* g, float* exp_avg
   return PXL_OK;
 }
 
+// what is written (parameters, moments) overlaps nothing else of the call: two grid rows would race
+static int adam_overlap(int dtype, const pxl_adam_item* items, int n) {
+  struct Span { uintptr_t lo, hi; bool written; };
+  std::vector<Span> v;
+  v.reserve(4 * (size_t)n);
+  for (int k = 0; k < n; ++k) {
+    const uintptr_t size = (uintptr_t)items[k].n, bytes = size * (dtype == PXL_F32 ? 4 : 2);
+    v.push_back({(uintptr_t)items[k].p, (uintptr_t)items[k].p + bytes, true});
+    v.push_back({(uintptr_t)items[k].g, (uintptr_t)items[k].g + bytes, false});
+    v.push_back({(uintptr_t)items[k].exp_avg, (uintptr_t)items[k].exp_avg + size * 4, true});
+    v.push_back({(uintptr_t)items[k].exp_avg_sq, (uintptr_t)items[k].exp_avg_sq + size * 4, true});
+  }
+  std::sort(v.begin(), v.end(), [](const Span& a, const Span& b) { return a.lo < b.lo; });
+  uintptr_t written = 0, any = 0;
+  for (const Span& s : v) {
+    PXL_REQUIRE(s.lo >= (s.written ? any : written), "adam_list: the same memory appears twice (at %p)", (void*)s.lo);
+    if (s.written) written = std::max(written, s.hi);
+    any = std::max(any, s.hi);
+  }
+  return PXL_OK;
+}
+
 extern "C" int pxl_adam_list(int dtype, const pxl_adam_item* items, int n, double lr, double beta1, double beta2, double eps, int step, void* stream) {
   PXL_REQUIRE(dtype == PXL_F32 || dtype == PXL_BF16, "adam_list: dtype %d is neither PXL_F32 nor PXL_BF16", dtype);
   PXL_REQUIRE(n >= 0 && (n == 0 || items != nullptr) && step >= 1 && beta1 >= 0 && beta1 < 1 && beta2 >= 0 && beta2 < 1 && eps > 0,
               "adam_list: bad argument (step counts from 1)");
   for (int k = 0; k < n; ++k)
     PXL_REQUIRE(items[k].p && items[k].g && items[k].exp_avg && items[k].exp_avg_sq && items[k].n >= 1, "adam_list: item %d: null pointer or no elements", k);
+  try {
+    const int rc = adam_overlap(dtype, items, n);
+    if (rc != PXL_OK) return rc;
+  } catch (...) {
+    return pxl_set_error(PXL_ERR_ARG, "adam_list: out of host memory");
+  }
   const double bc1 = 1.0 - pow(beta1, step), bc2 = 1.0 - pow(beta2, step);
   for (int at = 0; at < n; at += 40) {
     AdamList list;

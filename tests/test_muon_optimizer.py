@@ -303,6 +303,8 @@ def test_refusals():
         PF.adam_update([v], [v], [v], [v], lr=0.1, step=0)
     with pytest.raises(ValueError, match="shapes"):
         PF.adam_update([v], [v[:2]], [v], [v], lr=0.1)
+    with pytest.raises(ValueError, match="moments"):
+        PF.adam_update([v, v], [v, v], [v], [v, v], lr=0.1)
     with pytest.raises(ValueError, match="moments float32"):
         PF.adam_update([v], [v], [v.double()], [v], lr=0.1)
     assert "muon" not in popt.VALID_OPTIMIZER
@@ -328,3 +330,21 @@ def test_factory_defaults_and_formulas():
         ref.step()
         q, m, v = adam_exact(q, p.grad, m, v, 0.1, (0.8, 0.9), 1e-8, step)
         assert torch.allclose(q, p.detach(), rtol=1e-12)
+
+
+@pytest.mark.gpu
+def test_adam_update_refuses_memory_that_appears_twice():
+    """the same vector, or a piece of it, twice in a call: two of its workgroups would race"""
+    from pixelssl_amd import _lib, functional as PF
+    new = lambda: torch.ones(40, device="cuda")
+    p, q = new(), new()
+    a, b = p[:24], p[20:]
+    for lists in (([p, p], [new(), new()], [new(), new()], [new(), new()]), ([p], [p], [new()], [new()]), ([a, b], [new()[:24], new()[:20]], [new()[:24], new()[:20]],
+                  [new()[:24], new()[:20]]), ([p, new()], [q, new()], [new(), q], [new(), new()])):
+        with pytest.raises(_lib.PixelHipError, match="twice"):
+            PF.adam_update(*lists, lr=0.1)
+    m = new()
+    with pytest.raises(_lib.PixelHipError, match="twice"):
+        PF.adam_update([p], [q], [m], [m], lr=0.1)
+    assert torch.equal(p, new()) and torch.equal(q, new()) and torch.equal(m, new())
+    PF.adam_update([p, new()], [q, q], [new(), new()], [new(), new()], lr=0.1)          # (one gradient of two parameters is only read)
