@@ -1315,7 +1315,7 @@ NsSplit ns_split_plan(std::vector<NsClass>& cls, int planes) {
 // slots of a region: X and its successor, NP planes each, then A, T and three for Q / P
 int ns_plan(const char* what, int dtype, const pxl_ns_item* items, int n, NsPlan& plan) {
   PXL_REQUIRE(dtype == PXL_F32 || dtype == PXL_BF16, "%s: dtype %d is neither PXL_F32 nor PXL_BF16", what, dtype);
-  PXL_REQUIRE(n >= 0 && (n == 0 || items != nullptr), "%s: bad item list", what);
+  PXL_REQUIRE(n >= 0 && n <= (1 << 22) && (n == 0 || items != nullptr), "%s: bad item list (%d matrices, at most 2^22)", what, n);
   plan.np = dtype == PXL_F32 ? 2 : 1;
   plan.xplanes = 2 * plan.np;
   std::vector<NsPlan::Set>& sets = plan.sets;
@@ -1362,7 +1362,8 @@ int ns_plan(const char* what, int dtype, const pxl_ns_item* items, int n, NsPlan
     int first = 0;
     for (auto& c : s.cls) { c.first = first; first += c.count; }
     s.items = first;
-    const size_t head = round_up_z(first * sizeof(NsItem), 256) + round_up_z(first * sizeof(double) * NS_PARTS, 256) + round_up_z(first * sizeof(float), 256);
+    const size_t table = round_up_z(first * sizeof(NsItem), 256);
+    const size_t head = ns_is_tiny(s.cls[0], plan.np) ? table : table + round_up_z(first * sizeof(double) * NS_PARTS, 256) + round_up_z(first * sizeof(float), 256);
     if (head > plan.head) plan.head = head;
   }
   for (auto& s : sets) {
