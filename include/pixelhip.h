@@ -875,7 +875,7 @@ int pxl_elt_pair_end(void);
 /* u = (x - mean) / sqrt(var + eps), y = u * w + b; mean / var over the C features of a row, in fp32.
  * dtype: type of x, y, dy, dx; pdtype: type of w, b, dw, db -- PXL_F32 or dtype; w / b NULL: 1 / 0.
  * rows form: x [R] rows of C contiguous features, x_stride elements apart (>= C); y, dy, dx are [R][C] without gaps.
- * nchw form: x [N][C][S] without gaps, normalised over C at each of the N * S positions.
+ * nchw form: x [N][C][S] without gaps, normalised over C at each of the N * S positions.  At most 2^24 features.
  * mean, rstd: fp32, one per row / position, written by _fwd (both NULL: not kept) and read by _bwd.
  * _bwd: dx, dw, db may each be NULL (not wanted); ws: *_bwd_workspace bytes when dw or db is wanted.  R == 0 / N * S == 0: dw and
  * db are zero, nothing else is touched.  Sums have one order: equal inputs give equal bits.  No atomics, capturable. */
@@ -903,7 +903,7 @@ typedef struct pxl_ns_item {
   float scale;
   int32_t reserved;
 } pxl_ns_item;
-/* items: HOST array; n matrices of any mix of shapes, none of which overlap (p of one against anything of another); p == g is allowed
+/* items: HOST array; n <= 2^22 matrices of any mix of shapes, none of which overlap (p of one against anything of another); p == g is allowed
  * in pxl_orthogonalize.  coef: HOST array [steps][3], 1 .. 16 steps;
  *   X = G / max(|G|_F, eps);  per step  X <- a X + (b L + c L^2) X,  L = X X'  (of the transposed matrix when rows > cols)
  * fp32 results: every product to 22 bits and more, sums in fp32;  bf16: the result rounded once.  Coefficients that let singular values in
@@ -919,7 +919,7 @@ int pxl_muon_step(int dtype, const pxl_ns_item* items, int n, int steps, const f
                   double weight_decay, void* ws, size_t ws_bytes, void* stream);
 
 /* pxl_adam_step without weight decay on n tensors, 40 to a launch: the vectors that the Muon optimizer leaves to Adam.  items: HOST array,
- * copied at the call; p / g of type dtype, moments fp32; the tensors may not overlap. */
+ * copied at the call; p / g of type dtype, moments fp32; p and moments of one may overlap nothing of the call. */
 typedef struct pxl_adam_item {
   void* p;
   const void* g;

@@ -742,7 +742,7 @@ inline int ln_chan_most(long N, int C, long S) { const int a = ln_chan_shape(PXL
 int ln_check(const char* what, int dtype, int pdtype, long R, int C) {
   PXL_REQUIRE(dtype == PXL_F32 || dtype == PXL_BF16, "%s: dtype %d is neither PXL_F32 nor PXL_BF16", what, dtype);
   PXL_REQUIRE(pdtype == PXL_F32 || pdtype == dtype, "%s: weight and bias are 32-bit or of the type of x", what);
-  PXL_REQUIRE(R >= 0 && C >= 1 && C <= (1 << 30), "%s: bad sizes (rows %ld, features %d)", what, R, C);
+  PXL_REQUIRE(R >= 0 && C >= 1 && C <= (1 << 24), "%s: bad sizes (rows %ld, features %d: 1 .. 2^24)", what, R, C);
   return PXL_OK;
 }
 

@@ -315,6 +315,8 @@ def _layer_norm(name, x, weight, bias, eps, channels):
     if x.dim() < (2 if channels else 1) or x.shape[1 if channels else -1] == 0:
         raise ValueError("%s: no features to normalise over in %s" % (name, tuple(x.shape)))
     C = x.shape[1 if channels else -1]
+    if C > 1 << 24:
+        raise ValueError("%s: %d features (at most 2^24)" % (name, C))
     for what, t in (("weight", weight), ("bias", bias)):
         if t is None:
             continue
@@ -473,7 +475,10 @@ def muon_update(params, grads, momenta, lr, momentum=0.95, nesterov=True, weight
 def adam_update(params, grads, exp_avgs, exp_avg_sqs, lr, betas=(0.9, 0.999), eps=1e-8, step=1):
     """torch.optim.Adam's update without weight decay (FusedAdam's arithmetic) on lists of tensors, in place, many in one launch: the
     vectors beside muon_update's matrices.  params / grads fp32 or bf16, exp_avgs / exp_avg_sqs fp32, all four of an entry dense and
-    alike in memory (a gradient may lie otherwise).  step counts from 1."""
+    alike in memory (a gradient may lie otherwise).  Parameters and moments may overlap nothing.  step counts from 1."""
+    params, grads, exp_avgs, exp_avg_sqs = list(params), list(grads), list(exp_avgs), list(exp_avg_sqs)
+    if not len(params) == len(grads) == len(exp_avgs) == len(exp_avg_sqs):
+        raise ValueError("adam_update: %d parameters, %d gradients, %d and %d moments" % (len(params), len(grads), len(exp_avgs), len(exp_avg_sqs)))
     b1, b2 = float(betas[0]), float(betas[1])
     if not (0 <= b1 < 1 and 0 <= b2 < 1 and eps > 0 and int(step) >= 1):
         raise ValueError("adam_update: betas %r, eps %r, step %r" % (betas, eps, step))

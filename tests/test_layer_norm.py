@@ -379,6 +379,43 @@ def test_module():
 
 
 # ---- refusals: no kernel is reached, so they run without a GPU -----------------------------------------------------------------
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("shape,channels", [((2 ** 20 + 9, 2051), False), ((3, 701, 1023, 1021), True)], ids=["rows", "channels"])
+def test_more_elements_than_32_bits_count(shape, channels):
+    """the rows / positions at the end of a bf16 tensor of more than 2^31 elements are those of the same call on them alone, bit for bit"""
+    from pixelssl_amd import functional as PF
+    f = PF.layer_norm_channels if channels else PF.layer_norm
+    C = shape[1]
+    gen = torch.Generator(device="cuda").manual_seed(5)
+    few = lambda t: t[-1:, :, -9:, :] if channels else t[-9:]
+    x = torch.empty(shape, device="cuda", dtype=torch.bfloat16)
+    dy = torch.empty_like(x)
+    for t in (x, dy):
+        t.fill_(0.25)
+        few(t).normal_(generator=gen)
+    w, b = (torch.randn(C, device="cuda", generator=gen) for _ in range(2))
+
+    def run(x, dy):
+        x, wl, bl = x.detach().requires_grad_(), w.clone().requires_grad_(), b.clone().requires_grad_()
+        y = f(x, wl, bl)
+        return (y.detach(),) + torch.autograd.grad(y, (x, wl, bl), dy)
+
+    y, dx, dw, db = run(x, dy)
+    assert x.numel() > 2 ** 31
+    y1, dx1, dw1, db1 = run(few(x).contiguous(), few(dy).contiguous())
+    assert torch.equal(few(y), y1) and torch.equal(few(dx), dx1)
+    # equal values have their mean exactly: y = b there, their u is 0 -- dw is the last rows' alone, db theirs and 0.25 a row (exact in
+    # 32 bits).  In other orders: under 64 additions with something to round, half a step of the largest sum each: 2^-24 2^6
+    rows = x.numel() // C - few(x).numel() // C
+    other = y[0, :, 0, 0] if channels else y[0]
+    assert torch.equal(other, b.to(torch.bfloat16))
+    scale = few(dy).float().pow(2).sum().sqrt()
+    assert ((dw - dw1).abs() <= 2.0 ** -18 * scale).all()
+    assert ((db - db1 - 0.25 * rows).abs() <= 2.0 ** -18 * (0.25 * rows + scale)).all()
+
+
 def test_refusals():
     import pixelssl_amd as P
     from pixelssl_amd import _lib, functional as PF
@@ -402,6 +439,8 @@ def test_refusals():
             f(x, eps=float("nan"))
         with pytest.raises(ValueError, match="no features"):
             f(torch.randn(4, 0))
+        with pytest.raises(ValueError, match="at most"):           # (2^32 + 8 would be 8 to a 32-bit count)
+            f(torch.zeros(1).expand(1, 2 ** 32 + 8))
     with pytest.raises(ValueError, match="no features"):
         PF.layer_norm_channels(torch.randn(4))
     with pytest.raises(ValueError):
@@ -415,6 +454,7 @@ def test_c_entry_points_refuse_bad_arguments():
     assert h.pxl_layer_norm_fwd(0, 1, 4, 8, 8, 1, 1, 1, 1e-5, 1, None, None, None) == -1 and b"type of x" in h.pxl_last_error()
     assert h.pxl_layer_norm_fwd(0, 0, 4, 8, 7, 1, 1, 1, 1e-5, 1, None, None, None) == -1            # rows overlap
     assert h.pxl_layer_norm_fwd(0, 0, 4, 0, 8, 1, 1, 1, 1e-5, 1, None, None, None) == -1
+    assert h.pxl_layer_norm_fwd(0, 0, 4, 2 ** 24 + 1, 2 ** 25, 1, 1, 1, 1e-5, 1, None, None, None) == -1 and b"2^24" in h.pxl_last_error()
     assert h.pxl_layer_norm_fwd(0, 0, -1, 8, 8, 1, 1, 1, 1e-5, 1, None, None, None) == -1
     assert h.pxl_layer_norm_fwd(0, 0, 4, 8, 8, None, 1, 1, 1e-5, 1, None, None, None) == -1
     assert h.pxl_layer_norm_fwd(0, 0, 4, 8, 8, 1, 1, 1, 1e-5, 1, 1, None, None) == -1               # mean without rstd
