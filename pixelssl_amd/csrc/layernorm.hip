@@ -625,10 +625,10 @@ LnShape ln_chan_shape(int dtype, long N, int C, long S) {
     s.lanes = s.tsv;
     s.tiles = N * ((S + ts - 1) / ts);
     if (s.tiles >= (1l << 30)) s.lanes = s.nv = 0;
-    // partial sums of at most 8 MB or 512 workgroups, the tiles spread evenly
-    long most = (1l << 20) / C;
-    if (most < 768) most = 768;
-    if (s.threads == 512) most = 256;     // (one workgroup of them fits a CU)
+    // backward: as many workgroups as are resident at once (of 1024 threads 1 a CU, of 512 2, of 256 5), the tiles evenly over them: fewer partial
+    // sums too (8 x 64 x 257 x 257 fp32 108 us + 5 to add 1175 of them, a workgroup for every 4 tiles 106 + 20)
+    const int threads = s.nv >= 8 ? 2 * s.threads : s.threads;
+    const long most = threads == 1024 ? 256 : (threads == 512 ? 512 : 1280);
     const long each = (s.tiles + most - 1) / most;
     s.groups = (int)(s.tiles < 1 ? 1 : (s.tiles + each - 1) / each);
   }
@@ -659,19 +659,19 @@ inline LnShape ln_shape(int dtype, long R, int C, long S) { return S < 0 ? ln_ro
     else if (key == 256 * 16 + 4) LN_ROWS_TAIL(KERNEL, 256, 4, __VA_ARGS__);                                           \
     else if constexpr (sizeof(T) == 4) LN_ROWS_TAIL(KERNEL, 256, 8, __VA_ARGS__);                                      \
   } while (0)
-// more than 1024 channels: a piece of MANY channels a thread.  16 of them over 512 threads (two workgroups a CU) forward, 87 us for
-// 8 x 2048 x 65 x 65 bf16 (8 over 1024 threads 104); backward holds x and dy, one workgroup a CU either way: 8 over 1024 threads, 183 us (194)
-#define LN_CHAN(KERNEL, MANY, BLOCKS, ...)                                                                                           \
+// Backward (H = 2), which holds x and dy: 8 channels a thread and more go to twice the threads with half of them each (8 x 256 x 129 x 129 fp32
+// 100 us, with 8 a thread 109; 8 x 2048 x 65 x 65 bf16 180 us, with 16 a thread 194; forward the other way round, 87 with 16 and 104 with 8)
+#define LN_CHAN(KERNEL, H, BLOCKS, ...)                                                                                              \
   do {                                                                                                                               \
     const dim3 grid(BLOCKS);                                                                                                         \
-    if (s.threads == 256 && s.tsv == 8) {                                                                                            \
+    if (s.tsv == 8) {                                                                                                                \
       if (s.nv == 1) hipLaunchKernelGGL((KERNEL<T, 256, 8, 1>), grid, dim3(256), 0, st, __VA_ARGS__);                                \
       else if (s.nv == 2) hipLaunchKernelGGL((KERNEL<T, 256, 8, 2>), grid, dim3(256), 0, st, __VA_ARGS__);                           \
       else if (s.nv == 4) hipLaunchKernelGGL((KERNEL<T, 256, 8, 4>), grid, dim3(256), 0, st, __VA_ARGS__);                           \
-      else hipLaunchKernelGGL((KERNEL<T, 256, 8, 8>), grid, dim3(256), 0, st, __VA_ARGS__);                                          \
-    } else if (s.threads == 256) hipLaunchKernelGGL((KERNEL<T, 256, 4, 8>), grid, dim3(256), 0, st, __VA_ARGS__);                    \
-    else if (s.nv == 8) hipLaunchKernelGGL((KERNEL<T, 512, 4, 8>), grid, dim3(512), 0, st, __VA_ARGS__);                             \
-    else hipLaunchKernelGGL((KERNEL<T, 8192 / MANY, 4, MANY>), grid, dim3(8192 / MANY), 0, st, __VA_ARGS__);                         \
+      else hipLaunchKernelGGL((KERNEL<T, 256 * H, 8, 8 / H>), grid, dim3(256 * H), 0, st, __VA_ARGS__);                              \
+    } else if (s.threads == 256) hipLaunchKernelGGL((KERNEL<T, 256 * H, 4, 8 / H>), grid, dim3(256 * H), 0, st, __VA_ARGS__);        \
+    else if (s.nv == 8) hipLaunchKernelGGL((KERNEL<T, 512 * H, 4, 8 / H>), grid, dim3(512 * H), 0, st, __VA_ARGS__);                 \
+    else hipLaunchKernelGGL((KERNEL<T, 512 * H, 4, 16 / H>), grid, dim3(512 * H), 0, st, __VA_ARGS__);                               \
   } while (0)
 
 template <typename T>
@@ -687,7 +687,7 @@ int ln_fwd(long R, int C, long S, long xs, const void* x, LnParam w, LnParam b, 
     }
   } else if (s.lanes) {
     const int per = (int)(s.tiles / (R / S));
-    LN_CHAN(ln_chan_fwd, 16, (unsigned)s.tiles, (int)s.tiles, per, C, (int)S, (const T*)x, w, b, eps, (T*)y, mean, rstd);
+    LN_CHAN(ln_chan_fwd, 1, (unsigned)s.tiles, (int)s.tiles, per, C, (int)S, (const T*)x, w, b, eps, (T*)y, mean, rstd);
   } else {
     hipLaunchKernelGGL(ln_chan_fwd_loop<T>, dim3(blocks_for((R + 255) / 256, 1 << 20)), dim3(256), 0, st, R, C, S, (const T*)x, w, b, eps,
                        (T*)y, mean, rstd);
@@ -708,7 +708,7 @@ int ln_bwd(long R, int C, long S, long xs, const void* x, const void* dy, LnPara
       LN_ROWS(ln_rows_bwd, (unsigned)G, R, C, xs, (const T*)x, (const T*)dy, w, mean, rstd, (T*)dx, p);
     } else {
       const int per = (int)(s.tiles / (R / S));
-      LN_CHAN(ln_chan_bwd, 8, (unsigned)G, (int)s.tiles, per, C, (int)S, (const T*)x, (const T*)dy, w, mean, rstd, (T*)dx, p);
+      LN_CHAN(ln_chan_bwd, 2, (unsigned)G, (int)s.tiles, per, C, (int)S, (const T*)x, (const T*)dy, w, mean, rstd, (T*)dx, p);
     }
     PXL_LAUNCH_CHECK();
   } else if (R > 0) {
