@@ -6,6 +6,12 @@
 // Statistics, sums and the parameter gradients are held in 32 bits whatever the type of x; the variance is taken around the
 // mean in a second sweep (sum x^2 - C mean^2 cancels where the mean is large against the deviation).  No atomics: every sum has
 // one order, so two calls on the same inputs agree bit for bit.  y and dx are rounded once.
+//
+// Bound by memory: forward moves x and y once, backward x, dy and dx once (rows and channels live in registers between the sweeps), at
+// 5.1 TB/s of a large copy.  Measured, us (rate): 33800 x 2048 bf16 forward 62 (4.5 TB/s), backward 90 (4.6); 8 x 256 x 129 x 129 fp32 64 (4.3)
+// and 100 (4.1); 8 x 2048 x 65 x 65 bf16 87 (3.2) and 180 (2.3) -- rows of 8450 bytes, so pieces lie across cache lines, and one workgroup a CU
+// that loads, sums and stores in turn.  Partial dw / db: under 5 us to write and to add.  Small calls are bound by the launches (5 us a
+// kernel) and, forward + backward, by the host: 67 us, of which an engine pass with a trivial node takes 47.
 #include "common.h"
 
 namespace {
@@ -176,6 +182,7 @@ template <int LPR> __device__ __forceinline__ float row_sum(float v, float* sh) 
 
 // ---- rows that fit into registers: LPR lanes hold a row in NV pieces each, one sweep over memory; weight and bias stay in registers
 // over the rows of a workgroup.  TAIL: C is no multiple of a piece --------------------------------------------------------------
+// (Three sweeps over memory by a workgroup a row: 503 us forward + backward of 33800 x 2048 bf16, this 157.)
 // start of piece j of a lane, moved back where it would pass C; dup: elements it shares with the piece before (N or more: all)
 template <int N, int LPR, bool TAIL> __device__ __forceinline__ int piece_at(int j, int lane, int C, int& dup) {
   const int c = (j * LPR + lane) * N;
