@@ -924,22 +924,24 @@ __global__ __launch_bounds__(MT == 2 ? 512 : 1024) void ns_rec_kernel(NsClasses 
   const float un = p.unscale * (p.res_pow == 2 ? rs * rs : 1.f);
   f32x16 V;
   if (MT == 2) {
-    // one tile, often many shares: waves 0 .. 3 add the first half of their block's, waves 4 .. 7 the second half
-    const int n = ns_shares(c), half = (n + 1) / 2, from = wave < 4 ? 0 : half;
-    const size_t per_share = (size_t)tiles * 4, first = ((size_t)c.tn + (size_t)i * c.per) * 4 + (wave & 3);
-    V = ns_share_sum<8>(p.part + (size_t)from * per_share * 1024, wave < 4 ? half : n - half, per_share, first);
-    float4* x = reinterpret_cast<float4*>(lds) + (wave & 3) * 256 + lane;
-    if (wave >= 4) {
+    // one tile, often many shares: two groups of waves add a part of their block's each; of 32 rows, which have one block, all eight
+    const int nb = c.mp > 32 ? 4 : 1, groups = 8 / nb, blk = wave % nb, group = wave / nb;
+    const int n = ns_shares(c), each = (n + groups - 1) / groups, from = group * each;
+    const size_t per_share = (size_t)tiles * 4, first = ((size_t)c.tn + (size_t)i * c.per) * 4 + blk;
+    V = ns_share_sum<8>(p.part + (size_t)from * per_share * 1024, n - from < each ? n - from : each, per_share, first);
+    float4* x = reinterpret_cast<float4*>(lds) + blk * 256 + lane;
+    if (group > 0) {
 #pragma unroll
-      for (int e4 = 0; e4 < 4; ++e4) x[e4 * 64] = make_float4(V[e4 * 4], V[e4 * 4 + 1], V[e4 * 4 + 2], V[e4 * 4 + 3]);
+      for (int e4 = 0; e4 < 4; ++e4) x[(group - 1) * nb * 256 + e4 * 64] = make_float4(V[e4 * 4], V[e4 * 4 + 1], V[e4 * 4 + 2], V[e4 * 4 + 3]);
     }
     __syncthreads();
     if (lower) {
+      for (int q = 0; q < groups - 1; ++q)
 #pragma unroll
-      for (int e4 = 0; e4 < 4; ++e4) {
-        const float4 v = x[e4 * 64];
-        V[e4 * 4] += v.x; V[e4 * 4 + 1] += v.y; V[e4 * 4 + 2] += v.z; V[e4 * 4 + 3] += v.w;
-      }
+        for (int e4 = 0; e4 < 4; ++e4) {
+          const float4 v = x[q * nb * 256 + e4 * 64];
+          V[e4 * 4] += v.x; V[e4 * 4 + 1] += v.y; V[e4 * 4 + 2] += v.z; V[e4 * 4 + 3] += v.w;
+        }
     }
     __syncthreads();
   } else if (lower) {                  // A from the shares of the 64 x 64 tiles on and below the diagonal
@@ -969,6 +971,217 @@ __global__ __launch_bounds__(MT == 2 ? 512 : 1024) void ns_rec_kernel(NsClasses 
     *reinterpret_cast<f16x4*>(d) = h;
     *reinterpret_cast<f16x4*>(d + pm) = l;
   }
+}
+
+// ---- P X for matrices of at most 64 rows: X's planes, and the shares of the NEXT segment's Gram product; or the result ----------------------
+// A wave takes all rows of 64 columns at a time, in LDS of its own (no barrier): [row][64] per plane, chunks permuted as in the products (chunk_at).
+// P's fragments stay in registers, X's come through the transposing LDS load, the result goes back in place, from there to memory in rows of 128
+// bytes and, K being columns now, into the Gram product's sums: a launch less a segment, and no tiles of 64 rows for matrices of 32.  5 steps of
+// 4 x 21 x 18432 fp32 121 -> 78 us, of 32 x 2304 x 64 110 -> 102, of 1 x 64 x 576 64 either way.
+struct NsSlim {
+  int xplanes, p, x, out;               // slots
+  float unscale, scale;                 // sums -> value;  value -> planes
+  int use_res;                          // value *= residue
+  float lr, decay;
+  int muon;
+  float* part;                          // [share][matrix][4 blocks][1024]
+  int matrices;
+};
+template <int NP> constexpr int NS_SLIM_X = 4 * NP * 64 * 128;      // bytes of LDS: columns of four waves
+constexpr int NS_SLIM_P = 2 * 64 * 128;                              // P
+template <int NP, int MT, bool LAST, typename T>
+__device__ __forceinline__ void ns_slim_rows(const NsClass& c, const NsSlim& p, const NsItem& it, const float* __restrict__ residue, unsigned char* __restrict__ ws,
+                                             unsigned char* lds, int i, int share) {
+  constexpr int PL = 64 * 128;          // a plane of a wave's columns
+  constexpr int mp = 32 * MT;
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), hi = lane >> 5;
+  unsigned char *base = ws + c.base + (size_t)i * c.stride, *x = lds + wave * NP * PL, *lp = lds + NS_SLIM_X<NP>;
+  const size_t px = (size_t)mp * c.np, pm = (size_t)mp * mp;
+  const _Float16* X = reinterpret_cast<const _Float16*>(base + slot_off(c, p.xplanes, p.x));
+  const _Float16* P = reinterpret_cast<const _Float16*>(base + slot_off(c, p.xplanes, p.p));
+  _Float16* out = reinterpret_cast<_Float16*>(base + slot_off(c, p.xplanes, p.out));
+  const float un = p.unscale * (p.use_res ? residue[c.first + i] : 1.f);
+  const bool tall = c.rows > c.cols;
+
+  // P -> LDS, both planes: 16-byte chunks
+#pragma unroll
+  for (int e = 0; e < MT * MT; ++e) {
+    const int n = threadIdx.x + e * 256, z = n / (mp * mp / 8), r = n % (mp * mp / 8) / (mp / 8), ch = n % (mp / 8);
+    *reinterpret_cast<u32x4*>(lp + z * PL + chunk_at<64>(r, ch)) = *reinterpret_cast<const u32x4*>(P + z * pm + (size_t)r * mp + ch * 8);
+  }
+  __syncthreads();
+  f32x16 gram[MT == 2 ? 3 : 1];
+#pragma unroll
+  for (int b = 0; b < (MT == 2 ? 3 : 1); ++b)
+#pragma unroll
+    for (int e = 0; e < 16; ++e) gram[b][e] = 0.f;
+
+  const int end = (share + 1) * c.ks < c.np ? (share + 1) * c.ks : c.np;
+  for (int col = share * c.ks + wave * 64; col < end; col += 256) {
+    // columns -> LDS; eight rows of 128 bytes at a time, zero behind the last column (np is a multiple of 32)
+    const int lr = lane >> 3, ch = lane & 7;
+    const bool in = col + ch * 8 < c.np;
+    u32x4 g[NP][4 * MT];
+#pragma unroll
+    for (int z = 0; z < NP; ++z)
+#pragma unroll
+      for (int k = 0; k < 4 * MT; ++k) {
+        g[z][k] = u32x4{0u, 0u, 0u, 0u};
+        if (in) g[z][k] = *reinterpret_cast<const u32x4*>(X + z * px + (size_t)(k * 8 + lr) * c.np + col + ch * 8);
+      }
+#pragma unroll
+    for (int z = 0; z < NP; ++z)
+#pragma unroll
+      for (int k = 0; k < 4 * MT; ++k)
+        *reinterpret_cast<u32x4*>(x + z * PL + chunk_at<64>(k * 8 + lr, ch)) = g[z][k];
+#pragma unroll
+    for (int cb = 0; cb < 2; ++cb) {
+      f32x16 y[MT];
+#pragma unroll
+      for (int v = 0; v < MT; ++v)
+#pragma unroll
+        for (int e = 0; e < 16; ++e) y[v][e] = 0.f;
+#pragma unroll
+      for (int k = 0; k < 2 * MT; ++k) {
+        f16x8 xf[NP];
+#pragma unroll
+        for (int z = 0; z < NP; ++z) {
+          f16x4 half[2];
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {
+            const int kr = k * 16 + 8 * hi + 4 * h + ((lane & 15) >> 2), q = cb * 32 + ((lane >> 4) & 1) * 16 + (lane & 3) * 4;
+            half[h] = __builtin_bit_cast(f16x4, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)(x + z * PL + chunk_at<64>(kr, q >> 3) + (q & 7) * 2)));
+          }
+          xf[z] = __builtin_shufflevector(half[0], half[1], 0, 1, 2, 3, 4, 5, 6, 7);
+        }
+#pragma unroll
+        for (int v = 0; v < MT; ++v) {
+          const int o = chunk_at<64>(v * 32 + (lane & 31), 2 * k + hi);
+          const f16x8 ph = *reinterpret_cast<const f16x8*>(lp + o), pl = *reinterpret_cast<const f16x8*>(lp + PL + o);
+          if (NP == 2) y[v] = __builtin_amdgcn_mfma_f32_32x32x16_f16(xf[NP - 1], ph, y[v], 0, 0, 0);
+          y[v] = __builtin_amdgcn_mfma_f32_32x32x16_f16(xf[0], pl, y[v], 0, 0, 0);
+          y[v] = __builtin_amdgcn_mfma_f32_32x32x16_f16(xf[0], ph, y[v], 0, 0, 0);
+        }
+      }
+      // a lane: row 32 v + lane % 32, columns 32 cb + 8 e4 + 4 (lane / 32) + 0 .. 3
+      if constexpr (!LAST) {
+#pragma unroll
+        for (int v = 0; v < MT; ++v) {
+#pragma unroll
+          for (int e4 = 0; e4 < 4; ++e4) {
+            f16x4 h, l;
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+              const float w = y[v][e4 * 4 + e] * un * p.scale;
+              h[e] = (_Float16)w;
+              l[e] = (_Float16)(w - (float)h[e]);
+            }
+            const int q = cb * 32 + 8 * e4 + 4 * hi, o = chunk_at<64>(v * 32 + (lane & 31), q >> 3) + (q & 7) * 2;
+            *reinterpret_cast<f16x4*>(x + o) = h;
+            if (NP == 2) *reinterpret_cast<f16x4*>(x + PL + o) = l;
+          }
+        }
+      } else {
+        T* o = reinterpret_cast<T*>(it.p);
+        const float f = p.muon ? -p.lr * it.scale : 1.f;
+        auto place = [&](int r, int q) { return tall ? (size_t)q * c.cols + r : (size_t)r * c.cols + q; };
+        float was[MT][16];               // a Muon step's parameters: all read before any is written
+#pragma unroll
+        for (int v = 0; v < MT; ++v)
+#pragma unroll
+          for (int e4 = 0; e4 < 4; ++e4) {
+            const int r = v * 32 + (lane & 31), q = col + cb * 32 + 8 * e4 + 4 * hi;
+#pragma unroll
+            for (int e = 0; e < 4; ++e) was[v][e4 * 4 + e] = 0.f;
+            if (!p.muon || r >= c.m || q >= c.n) continue;
+            if (!tall && q + 4 <= c.n) {
+              load4(o + place(r, q), &was[v][e4 * 4]);
+            } else {
+#pragma unroll
+              for (int e = 0; e < 4; ++e)
+                if (q + e < c.n) was[v][e4 * 4 + e] = to_f(o[place(r, q + e)]);
+            }
+          }
+#pragma unroll
+        for (int v = 0; v < MT; ++v)
+#pragma unroll
+          for (int e4 = 0; e4 < 4; ++e4) {
+            const int r = v * 32 + (lane & 31), q = col + cb * 32 + 8 * e4 + 4 * hi;
+            if (r >= c.m || q >= c.n) continue;
+            float w[4];
+#pragma unroll
+            for (int e = 0; e < 4; ++e) w[e] = y[v][e4 * 4 + e] * un * f + (p.muon ? was[v][e4 * 4 + e] * p.decay : 0.f);
+            if (!tall && q + 4 <= c.n) {
+              store4(o + place(r, q), w);
+            } else {
+#pragma unroll
+              for (int e = 0; e < 4; ++e)
+                if (q + e < c.n) o[place(r, q + e)] = from_f<T>(w[e]);
+            }
+          }
+      }
+    }
+    if constexpr (!LAST) {
+#pragma unroll
+      for (int z = 0; z < NP; ++z)
+#pragma unroll
+        for (int k = 0; k < 4 * MT; ++k)
+          if (in)
+            *reinterpret_cast<u32x4*>(out + z * px + (size_t)(k * 8 + lr) * c.np + col + ch * 8) = *reinterpret_cast<const u32x4*>(x + z * PL + chunk_at<64>(k * 8 + lr, ch));
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {      // 64 columns
+        f16x8 r[MT][NP];
+#pragma unroll
+        for (int v = 0; v < MT; ++v)
+#pragma unroll
+          for (int z = 0; z < NP; ++z)
+            r[v][z] = *reinterpret_cast<const f16x8*>(x + z * PL + chunk_at<64>(v * 32 + (lane & 31), 2 * k + hi));
+#pragma unroll
+        for (int b = 0; b < (MT == 2 ? 3 : 1); ++b) {
+          const int bi = b > 0, bj = b == 2;
+          if (NP == 2) {
+            gram[b] = __builtin_amdgcn_mfma_f32_32x32x16_f16(r[bi][0], r[bj][NP - 1], gram[b], 0, 0, 0);
+            gram[b] = __builtin_amdgcn_mfma_f32_32x32x16_f16(r[bi][NP - 1], r[bj][0], gram[b], 0, 0, 0);
+          }
+          gram[b] = __builtin_amdgcn_mfma_f32_32x32x16_f16(r[bi][0], r[bj][0], gram[b], 0, 0, 0);
+        }
+      }
+    }
+  }
+  if constexpr (!LAST) {
+    // the waves' sums, in order; wave w the blocks (0, 0), (1, 0), (1, 1)
+    __syncthreads();
+    float4* sum = reinterpret_cast<float4*>(lds);
+#pragma unroll
+    for (int b = 0; b < (MT == 2 ? 3 : 1); ++b)
+#pragma unroll
+      for (int e4 = 0; e4 < 4; ++e4) sum[((wave * 3 + b) * 4 + e4) * 64 + lane] = make_float4(gram[b][e4 * 4], gram[b][e4 * 4 + 1], gram[b][e4 * 4 + 2], gram[b][e4 * 4 + 3]);
+    __syncthreads();
+    if (wave < (MT == 2 ? 3 : 1)) {
+      float4* o = reinterpret_cast<float4*>(p.part) + (((size_t)share * p.matrices + c.first + i) * 4 + (wave == 0 ? 0 : wave + 1)) * 256 + lane;
+#pragma unroll
+      for (int e4 = 0; e4 < 4; ++e4) {
+        float4 a = sum[(wave * 4 + e4) * 64 + lane];
+#pragma unroll
+        for (int w = 1; w < 4; ++w) {
+          const float4 b = sum[((w * 3 + wave) * 4 + e4) * 64 + lane];
+          a.x += b.x; a.y += b.y; a.z += b.z; a.w += b.w;
+        }
+        o[e4 * 64] = a;
+      }
+    }
+  }
+}
+template <int NP, bool LAST, typename T>
+__global__ __launch_bounds__(256, 2) void ns_slim_kernel(NsClasses cs, NsSlim p, NsInline few, const NsItem* __restrict__ table,
+                                                         const float* __restrict__ residue, unsigned char* __restrict__ ws) {
+  constexpr int BYTES = NS_SLIM_X<NP> + NS_SLIM_P;
+  __shared__ __attribute__((aligned(16))) unsigned char lds[BYTES < 49152 ? 49152 : BYTES];
+  const NsClass c = find_class(cs, blockIdx.x);
+  const int local = blockIdx.x - c.start, i = local / c.per, share = local - i * c.per;
+  const NsItem it = ns_item(few, table, c.first + i);
+  if (c.mp == 32) ns_slim_rows<NP, 1, LAST, T>(c, p, it, residue, ws, lds, i, share);
+  else ns_slim_rows<NP, 2, LAST, T>(c, p, it, residue, ws, lds, i, share);
 }
 
 // ---- matrices that fit one CU's LDS whole: norm, all steps and the update in ONE launch, a workgroup of 8 waves a matrix ----------------------
@@ -1262,10 +1475,10 @@ inline size_t round_up_z(size_t v, size_t to) { return (v + to - 1) / to * to; }
 // one or two workgroups are on a CU), shares written and read at 5 TB/s and 4 us for the launch that adds them
 // (small: 1.2 us for every 16 of them in the recursion's workgroup).  23 x 256 x 2304: 230 small
 // tiles in one share 24 us (model) against 34 measured for 8 shares of 69 large ones; 3 x 512 x 4608: 8 shares of 30 large tiles.
-struct NsSplit { int tile, shares, tiles, small, mt, tiny, full, cut; size_t bytes; };      // bytes: of all shares, cut tiles' too
+struct NsSplit { int tile, shares, tiles, small, mt, tiny, full, cut; size_t bytes; int slim[NS_MAX_CLASSES]; };      // bytes: of all shares, cut tiles' too
 inline bool ns_is_tiny(const NsClass& c, int planes) { return c.mp <= 64 && c.np <= (planes == 2 ? NS_TINY_N<2> : NS_TINY_N<1>); }
 NsSplit ns_split_plan(std::vector<NsClass>& cls, int planes) {
-  NsSplit r = {64, 1, 0, 1, 2, 0, 0, 1, 0};
+  NsSplit r = {64, 1, 0, 1, 2, 0, 0, 1, 0, {}};
   if (ns_is_tiny(cls[0], planes)) {               // (and with it all of the set)
     r.tiny = 1;
     return r;
@@ -1306,7 +1519,14 @@ NsSplit ns_split_plan(std::vector<NsClass>& cls, int planes) {
   }
   r.full = cut.cut > 1 ? cut.full : r.tiles;
   r.cut = cut.cut;
-  if (r.shares > 1 || r.small) r.bytes = (size_t)r.shares * r.tiles * r.tile * r.tile * sizeof(float);
+  // matrices of up to 64 rows: columns a workgroup of the kernel that joins P X and the next Gram product takes, at most 128 shares
+  int most = r.shares;
+  for (size_t k = 0; r.small && r.mt == 2 && k < cls.size(); ++k) {
+    const int share = ((cls[k].np + 127) / 128 + 255) / 256 * 256, n = (cls[k].np + share - 1) / share;
+    r.slim[k] = share;
+    most = n > most ? n : most;
+  }
+  if (r.shares > 1 || r.small) r.bytes = (size_t)most * r.tiles * r.tile * r.tile * sizeof(float);
   // cut tiles of any of the set's products: at most 256 a job
   if (!r.small) {
     const int n = (int)cls.size();
@@ -1539,6 +1759,36 @@ int ns_rec(NsRun& r, const std::vector<NsStep>& steps, size_t s, size_t e, float
   return PXL_OK;
 }
 
+// X <- P X with the shares of its Gram product, or the result
+template <int NP, bool LAST, typename T>
+int ns_slim(NsRun& r, const NsGemm& g) {
+  NsSlim q;
+  memset(&q, 0, sizeof(q));
+  q.xplanes = g.xplanes;
+  q.p = g.job[0].a;
+  q.x = g.job[0].b;
+  q.out = g.job[0].out;
+  q.unscale = g.unscale[0];
+  q.scale = g.scale[0];
+  q.use_res = g.res_pow;
+  q.lr = g.lr;
+  q.decay = g.decay;
+  q.muon = g.muon;
+  q.part = r.shares;
+  int at = 0;
+  for (int k = 0; k < r.cs.n; ++k) {
+    NsClass& c = r.cs.c[k];
+    c.ks = r.split.slim[k];             // (and what the recursion adds up next)
+    c.per = (c.np + c.ks - 1) / c.ks;
+    c.start = at;
+    at += c.per * c.count;
+    q.matrices += c.count;
+  }
+  hipLaunchKernelGGL((ns_slim_kernel<NP, LAST, T>), dim3(at), dim3(256), 0, r.st, r.cs, q, r.few, r.table, r.residue, r.ws);
+  PXL_LAUNCH_CHECK();
+  return PXL_OK;
+}
+
 template <typename T, int NP>
 int ns_run_tiny(NsRun& r, const std::vector<NsStep>& steps, float eps, const MuonArgs& ma, int muon) {
   NsTiny q;
@@ -1604,7 +1854,8 @@ int ns_run_set(NsRun& r, const std::vector<NsStep>& steps, float eps, const Muon
     g.unscale[0] = 1.f / (sx * sx);
     g.scale[0] = sA;
     g.res_pow = NP == 1 && first ? 2 : 0;
-    NS_TRY((ns_gemm<EPI_GRAM, NP, NP, float>(r, g)));
+    const bool slim = r.split.small && r.split.mt == 2;
+    if (!slim || first) NS_TRY((ns_gemm<EPI_GRAM, NP, NP, float>(r, g)));       // (slim: later ones come with P X)
     int P = -1;
     if (r.split.small) {
       size_t e = s;
@@ -1664,12 +1915,18 @@ int ns_run_set(NsRun& r, const std::vector<NsStep>& steps, float eps, const Muon
       g.muon = muon;
       g.lr = ma.lr;
       g.decay = ma.keep;
-      NS_TRY((ns_gemm<EPI_OUT, 2, NP, T>(r, g)));
+      if (slim) NS_TRY((ns_slim<NP, true, T>(r, g)));
+      else NS_TRY((ns_gemm<EPI_OUT, 2, NP, T>(r, g)));
     } else {
       const float sx2 = plane_scale(steps[s].sigma);
       g.job[0] = {P, x, x2};
       g.scale[0] = sx2;
-      NS_TRY((ns_gemm<EPI_X, 2, NP, float>(r, g)));
+      if (slim) {
+        g.job[0].out = x2;
+        NS_TRY((ns_slim<NP, false, T>(r, g)));
+      } else {
+        NS_TRY((ns_gemm<EPI_X, 2, NP, float>(r, g)));
+      }
       sx = sx2;
       const int o = x;
       x = x2;

@@ -52,7 +52,8 @@ def gradient(shape, seed, dtype=torch.float32, rank=4):
 
 
 SHAPES = [(1, 1), (1, 64), (70, 1), (3, 5), (31, 33), (2, 32, 32), (64, 147), (147, 64), (5, 40, 70), (129, 257), (256, 256), (3, 200, 640), (300, 128),
-          (21, 4608), (2304, 96), (513, 640), (2, 3, 16, 24), (65, 65), (64, 384), (384, 63), (64, 385), (33, 256), (257, 64), (2, 32, 417), (300, 1, 5)]
+          (21, 4608), (2304, 96), (513, 640), (2, 3, 16, 24), (65, 65), (64, 384), (384, 63), (64, 385), (33, 256), (257, 64), (2, 32, 417), (300, 1, 5),
+          (48, 40007), (40007, 21), (2, 64, 1025)]
 
 
 @pytest.mark.gpu
@@ -224,11 +225,12 @@ def test_muon_update_of_mixed_shapes(nesterov, wd):
 
 
 @pytest.mark.gpu
-@pytest.mark.parametrize("rows,step", [(20, 3), (40, 30), (100, 11)])
-def test_muon_update_of_many_shapes(rows, step):
-    """15 shapes that run alike: more than the arguments of one launch hold"""
+@pytest.mark.parametrize("rows,first,step", [(20, 24, 3), (40, 24, 30), (100, 24, 11), (0, 390, 41)])
+def test_muon_update_of_many_shapes(rows, first, step):
+    """15 shapes that run alike, more than the arguments of one launch hold, tall and wide; the last of 9 to 64 rows (columns)"""
     from pixelssl_amd import functional as PF
-    trip = [make((rows, 24 + step * k) if k % 2 else (24 + step * k, rows), k) for k in range(15)]
+    small = [rows or 9 + 55 * k // 14 for k in range(15)]
+    trip = [make((small[k], first + step * k) if k % 2 else (first + step * k, small[k]), k) for k in range(15)]
     want = [muon_exact(p, g, m, 0.01) for p, g, m in trip]
     PF.muon_update(*zip(*trip), lr=0.01)
     for (p, g, m), w in zip(trip, want):
