@@ -18,7 +18,7 @@
 //
 // Measured (5 steps, us): 64 x 147 fp32 37, 23 x 256 x 2304 fp32 341, 23 x 1024 x 256 bf16 191, 2 x 2048 x 4608 fp32 2090 (0.77 PF of fp16
 // products against 1.09 of a large library product: power brings the clock from 2.4 to 1.7 - 1.8 GHz), Muon steps of 3 x 512 x 4608 350 and of
-// 4 x 21 x 18432 126.  Below some hundred rows the chain of dependent products bounds it: 4.5 us a launch until its first product, 2 us its stores.
+// 4 x 21 x 18432 78.  Below some hundred rows the chain of dependent products bounds it: 4.5 us a launch until its first product, 2 us its stores.
 //
 // No atomics, no state between calls, every sum in one order.
 #include <algorithm>
