@@ -308,7 +308,15 @@ def _node():
     return _pxlnode
 
 
-def _layer_norm(name, x, weight, bias, eps, channels):
+def _layer_norm(x, weight, bias, eps, channels):
+    y = (_pxlnode or _node()).layer_norm(x, weight, bias, eps, channels)
+    if y is None:
+        _layer_norm_refuse("layer_norm_channels" if channels else "layer_norm", x, weight, bias, eps, channels)
+    return y
+
+
+def _layer_norm_refuse(name, x, weight, bias, eps, channels):
+    """says what the node does not take about the arguments"""
     dtype = x.dtype
     if dtype is not torch.float32 and dtype is not torch.bfloat16:
         raise ValueError("%s: float32 or bfloat16, got %s" % (name, dtype))
@@ -329,22 +337,19 @@ def _layer_norm(name, x, weight, bias, eps, channels):
     if not eps >= 0:
         raise ValueError("%s: eps %r" % (name, eps))
     _gpu(x)
-    return (_pxlnode or _node()).layer_norm(x, weight, bias, eps, channels)
+    raise ValueError("%s: a dense tensor, got %s" % (name, x.layout))
 
 
 def layer_norm(x, weight=None, bias=None, eps=1e-5):
     """(x - mean) / sqrt(var + eps) * weight + bias over the LAST axis of x (fp32 or bf16; any leading axes, rows may lie apart in
     memory), statistics in fp32; weight / bias [C]: fp32 or the type of x.  Differentiable once in x, weight and bias; gradients
     are the same bits from call to call."""
-    return _layer_norm("layer_norm", x, weight, bias, eps, False)
+    return _layer_norm(x, weight, bias, eps, False)
 
 
 def layer_norm_channels(x, weight=None, bias=None, eps=1e-5):
     """`layer_norm` over axis 1 of an [N, C, ...] map at each position (a map stored channels last is read as it lies)."""
-    if x.dim() == 4 and x.dtype in (torch.float32, torch.bfloat16) and not x.is_contiguous() and \
-            x.is_contiguous(memory_format=torch.channels_last):
-        return _layer_norm("layer_norm_channels", x.permute(0, 2, 3, 1), weight, bias, eps, False).permute(0, 3, 1, 2)
-    return _layer_norm("layer_norm_channels", x, weight, bias, eps, True)
+    return _layer_norm(x, weight, bias, eps, True)
 
 
 # ---- orthogonalised updates (csrc/muon.hip) -----------------------------------------------------------------------------------

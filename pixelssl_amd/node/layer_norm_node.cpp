@@ -158,9 +158,22 @@ struct LayerNormNode : public torch::autograd::Function<LayerNormNode> {
   }
 };
 
-// arguments as functional._layer_norm has checked them
-Tensor layer_norm(const Tensor& x0, const MaybeTensor& w0, const MaybeTensor& b0, double eps, bool channels) {
+// y, or nothing where an argument is not as the kernels take it: functional._layer_norm then says what (the checks in Python take 2 - 3 us)
+MaybeTensor layer_norm(const Tensor& x0, const MaybeTensor& w0, const MaybeTensor& b0, double eps, bool channels) {
   const bool has_w = w0.has_value() && w0->defined(), has_b = b0.has_value() && b0->defined();
+  const at::ScalarType t = x0.scalar_type();
+  if (!x0.is_cuda() || x0.layout() != at::kStrided || (t != at::kFloat && t != at::kBFloat16) || x0.dim() < (channels ? 2 : 1) || !(eps >= 0)) return {};
+  const int64_t C = x0.size(channels ? 1 : -1);
+  if (C < 1 || C > (1 << 24)) return {};
+  for (const MaybeTensor* q : {&w0, &b0}) {
+    if (!(q == &w0 ? has_w : has_b)) continue;
+    const Tensor& v = **q;
+    if (v.dim() != 1 || v.size(0) != C || v.device() != x0.device() || (v.scalar_type() != at::kFloat && v.scalar_type() != t) ||
+        (has_w && v.scalar_type() != w0->scalar_type()))
+      return {};
+  }
+  if (channels && x0.dim() == 4 && !x0.is_contiguous() && x0.is_contiguous(at::MemoryFormat::ChannelsLast))      // read as it lies
+    return layer_norm(x0.permute({0, 2, 3, 1}), w0, b0, eps, false)->permute({0, 3, 1, 2});
   Tensor x = x0;
   if (!x.is_contiguous() && (channels || row_stride(x) < 0)) x = x.contiguous();
   const MaybeTensor w = has_w ? MaybeTensor(w0->contiguous()) : MaybeTensor(), b = has_b ? MaybeTensor(b0->contiguous()) : MaybeTensor();
