@@ -8,7 +8,7 @@
 // one order, so two calls on the same inputs agree bit for bit.  y and dx are rounded once.
 //
 // Bound by memory: forward moves x and y once, backward x, dy and dx once (rows and channels live in registers between the sweeps), at
-// 5.1 TB/s of a large copy.  Measured, us (rate): 33800 x 2048 bf16 forward 62 (4.5 TB/s), backward 90 (4.6); 8 x 256 x 129 x 129 fp32 64 (4.3)
+// 5.1 TB/s of a large copy.  Measured, us (rate): 33800 x 2048 bf16 forward 51 (5.4 TB/s), backward 87 (4.8); 8 x 256 x 129 x 129 fp32 64 (4.3)
 // and 100 (4.1); 8 x 2048 x 65 x 65 bf16 87 (3.2) and 180 (2.3) -- rows of 8450 bytes, so pieces lie across cache lines, and one workgroup a CU
 // that loads, sums and stores in turn.  Partial dw / db: under 5 us to write and to add.  Small calls are bound by the launches (5 us a
 // kernel) and, forward + backward, by the host: 67 us, of which an engine pass with a trivial node takes 47.
@@ -170,6 +170,19 @@ template <typename T> struct Piece {
   }
 };
 
+// a piece's worth of parameters from c on, in 16-byte loads (one by one, 64 loads a lane of 2048 features: a row 8.0 us, so 3.8)
+template <typename T> __device__ __forceinline__ void param_piece(const LnParam& w, int c, float none, float* f) {
+  constexpr int N = Piece<T>::N;
+  if (w.p == nullptr) {
+#pragma unroll
+    for (int e = 0; e < N; ++e) f[e] = none;
+  } else if (sizeof(T) == 4 || w.f32) {
+    __builtin_memcpy(f, reinterpret_cast<const float*>(w.p) + c, 4 * N);
+  } else {
+    Chunk<T>::unpack(Piece<T>::load(reinterpret_cast<const T*>(w.p) + c), f);
+  }
+}
+
 // makes the compiler take a piece as new: what is unpacked from it after this is unpacked again, not kept in registers from before
 __device__ __forceinline__ void renew(uint4& v) { asm volatile("" : "+v"(v.x), "+v"(v.y), "+v"(v.z), "+v"(v.w)); }
 
@@ -182,7 +195,7 @@ template <int LPR> __device__ __forceinline__ float row_sum(float v, float* sh) 
 
 // ---- rows that fit into registers: LPR lanes hold a row in NV pieces each, one sweep over memory; weight and bias stay in registers
 // over the rows of a workgroup.  TAIL: C is no multiple of a piece --------------------------------------------------------------
-// (Three sweeps over memory by a workgroup a row: 503 us forward + backward of 33800 x 2048 bf16, this 157.)
+// (Three sweeps over memory by a workgroup a row: 503 us forward + backward of 33800 x 2048 bf16, this 142.)
 // start of piece j of a lane, moved back where it would pass C; dup: elements it shares with the piece before (N or more: all)
 template <int N, int LPR, bool TAIL> __device__ __forceinline__ int piece_at(int j, int lane, int C, int& dup) {
   const int c = (j * LPR + lane) * N;
@@ -201,14 +214,7 @@ __global__ __launch_bounds__(256) void ln_rows_fwd(long R, int C, long xs, const
   float wv[NV][V], bv[NV][V];
   int at[NV], dup[NV];
 #pragma unroll
-  for (int j = 0; j < NV; ++j) {
-    at[j] = piece_at<V, LPR, TAIL>(j, lane, C, dup[j]);
-#pragma unroll
-    for (int e = 0; e < V; ++e) {
-      wv[j][e] = w.get<T>(at[j] + e, 1.f);
-      bv[j][e] = b.get<T>(at[j] + e, 0.f);
-    }
-  }
+  for (int j = 0; j < NV; ++j) at[j] = piece_at<V, LPR, TAIL>(j, lane, C, dup[j]);
   const float inv = 1.f / C;
   const long step = (long)gridDim.x * RPB;
   uint4 raw[NV];
@@ -218,6 +224,11 @@ __global__ __launch_bounds__(256) void ln_rows_fwd(long R, int C, long xs, const
     for (int j = 0; j < NV; ++j) raw[j] = Piece<T>::load(xr + at[j]);
   };
   fetch((long)blockIdx.x * RPB + threadIdx.x / LPR);
+#pragma unroll
+  for (int j = 0; j < NV; ++j) {
+    param_piece<T>(w, at[j], 1.f, wv[j]);
+    param_piece<T>(b, at[j], 0.f, bv[j]);
+  }
   for (long r0 = (long)blockIdx.x * RPB; r0 < R; r0 += step) {
     const long r = r0 + threadIdx.x / LPR;
     float f[NV][V];
@@ -264,10 +275,8 @@ __global__ __launch_bounds__(256) void ln_rows_bwd(long R, int C, long xs, const
   for (int j = 0; j < NV; ++j) {
     at[j] = piece_at<V, LPR, TAIL>(j, lane, C, dup[j]);
 #pragma unroll
-    for (int e = 0; e < V; ++e) {
-      wv[j][e] = w.get<T>(at[j] + e, 1.f);
-      aw[j][e] = ab[j][e] = 0.f;
-    }
+    for (int e = 0; e < V; ++e) aw[j][e] = ab[j][e] = 0.f;
+    param_piece<T>(w, at[j], 1.f, wv[j]);
   }
   const float inv = 1.f / C;
   for (long r0 = (long)blockIdx.x * RPB; r0 < R; r0 += (long)gridDim.x * RPB) {
@@ -408,6 +417,17 @@ __global__ __launch_bounds__(THREADS) void ln_chan_fwd(int tiles, int per, int C
     const int b0 = j * CY < C ? j * CY : C - 1, c = b0 + cy < C ? cy : C - 1 - b0;      // past the channels: the last one again
     raw[j] = Piece<T>::load(lane_at(x + base + (long)b0 * S, (unsigned)(c * S + at) * (unsigned)sizeof(T)));
   }
+  // parameters on their way while the channels are summed (16 channels a thread: read where they are used, no registers for them)
+  constexpr bool KEEP = NV <= 8;
+  float wk[KEEP ? NV : 1], bk[KEEP ? NV : 1];
+  if (KEEP) {
+#pragma unroll
+    for (int j = 0; j < NV; ++j) {
+      const int c = j * CY + cy < C ? j * CY + cy : C - 1;
+      wk[KEEP ? j : 0] = w.get<T>(c, 1.f);
+      bk[KEEP ? j : 0] = b.get<T>(c, 0.f);
+    }
+  }
   float s[1][V];
 #pragma unroll
   for (int e = 0; e < V; ++e) s[0][e] = 0.f;
@@ -444,7 +464,7 @@ __global__ __launch_bounds__(THREADS) void ln_chan_fwd(int tiles, int per, int C
   for (int j = 0; j < NV; ++j) {
     const int c = j * CY + cy;
     if (c >= C) continue;
-    const float wc = w.get<T>(c, 1.f), bc = b.get<T>(c, 0.f);
+    const float wc = KEEP ? wk[KEEP ? j : 0] : w.get<T>(c, 1.f), bc = KEEP ? bk[KEEP ? j : 0] : b.get<T>(c, 0.f);
     float f[V];
     renew(raw[j]);
     Chunk<T>::unpack(raw[j], f);
