@@ -16,7 +16,7 @@
 // of the fp32 ones.  A bf16 matrix scaled by a power of two IS one fp16 plane (8 of 11 bits), its norm's remainder is applied to A and
 // to the result.
 //
-// Measured (5 steps, us): 64 x 147 fp32 37, 23 x 256 x 2304 fp32 341, 23 x 1024 x 256 bf16 191, 2 x 2048 x 4608 fp32 2090 (0.77 PF of fp16
+// Measured (5 steps, us): 64 x 147 fp32 34, 23 x 256 x 2304 fp32 341, 23 x 1024 x 256 bf16 191, 2 x 2048 x 4608 fp32 2090 (0.77 PF of fp16
 // products against 1.09 of a large library product: power brings the clock from 2.4 to 1.7 - 1.8 GHz), Muon steps of 3 x 512 x 4608 350 and of
 // 4 x 21 x 18432 78.  Below some hundred rows the chain of dependent products bounds it: 4.5 us a launch until its first product, 2 us its stores.
 //
@@ -1185,13 +1185,13 @@ __global__ __launch_bounds__(256, 2) void ns_slim_kernel(NsClasses cs, NsSlim p,
 }
 
 // ---- matrices that fit one CU's LDS whole: norm, all steps and the update in ONE launch, a workgroup of 8 waves a matrix ----------------------
-// At most 64 on the smaller side, 384 (bf16: 256) on the other.  X lives in LDS as planes [mp][pitch]: 16-byte chunk ch of row r at
+// At most 64 on the smaller side, 448 (bf16: 384) on the other.  X lives in LDS as planes [mp][pitch]: 16-byte chunk ch of row r at
 // ch ^ ((r >> 2) & 3), a pitch of an odd number of 64 bytes -- 16 rows of one chunk, and the four rows of a transposing read, lie on different
 // banks.  The products are the ones of the larger matrices; only what is moved differs.
-// Measured, this against the launches of the larger ones (5 steps, us): fp32 16 x 27 24 / 56, 64 x 147 37 / 69, 64 x 256 47 / 69,
-// 64 x 448 66 / 71; bf16 64 x 64 33 / 44, 64 x 256 44 / 46, 64 x 320 48 / 46: the limits.  What bounds it is one CU's chain of small products
+// Measured, this against the launches of the larger ones (5 steps, us): fp32 16 x 27 24 / 56, 64 x 147 34 / 61, 64 x 448 56 / 63 (what LDS holds);
+// bf16 64 x 256 34 / 39, 64 x 384 40 / 40, 64 x 448 43 / 40: the limits.  What bounds it is one CU's chain of small products
 // (1 us each: 24 matrix instructions of 32 cycles on the diagonal, 512 cycles of LDS reads, the split into planes, two barriers).
-template <int NP> constexpr int NS_TINY_N = NP == 2 ? 384 : 256;
+template <int NP> constexpr int NS_TINY_N = NP == 2 ? 448 : 384;
 __host__ __device__ inline int ns_tiny_pitch(int np) { return np * 2 + (np & 32 ? 0 : 64); }
 struct NsTiny {
   NsRec rec;                            // scales and coefficients of all steps
@@ -1217,16 +1217,23 @@ __global__ __launch_bounds__(512) void ns_tiny_kernel(NsClasses cs, NsTiny p, Ns
   const bool tall = c.rows > c.cols;
 
   // momentum, update and its norm; the update stays in registers
-  const int per_line = (c.cols + 3) >> 2, groups = c.rows * per_line;
+  // fours of a line, 512 further each time (no division a step)
+  const int per_line = (c.cols + 3) >> 2, lines = 512 / per_line, fours = 512 - lines * per_line;
+  const int line0 = tid / per_line, four0 = tid - line0 * per_line;
   float u[GROUPS][4];
   double s = 0.0;
+  int line = line0, four = four0;
+  auto next = [&]() {
+    line += lines;
+    four += fours;
+    if (four >= per_line) { four -= per_line; ++line; }
+  };
 #pragma unroll
-  for (int k = 0; k < GROUPS; ++k) {
+  for (int k = 0; k < GROUPS; ++k, next()) {
 #pragma unroll
     for (int e = 0; e < 4; ++e) u[k][e] = 0.f;
-    const int n = tid + k * 512;
-    if (n < groups) {
-      const int line = n / per_line, col = (n - line * per_line) * 4;
+    if (line < c.rows) {
+      const int col = four * 4;
       const long at = (long)line * c.cols + col;
       if (col + 4 <= c.cols) {
         load4(g + at, u[k]);
@@ -1277,15 +1284,19 @@ __global__ __launch_bounds__(512) void ns_tiny_kernel(NsClasses cs, NsTiny p, Ns
     left = (float)(ldexp(1.0, e) / norm);
   }
   if (!(square < HUGE_VAL)) mul = nan("");                  // a NaN or an infinity in the matrix: all of its result is NaN
+  // (in 32 bits where they hold the factor: 2^-24 of a common factor; 64-bit operations run at half their rate)
+  const float mf = (float)mul;
+  const bool narrow = mf >= 1.2e-38f && mf <= 3e38f;
+  line = line0;
+  four = four0;
 #pragma unroll
-  for (int k = 0; k < GROUPS; ++k) {
-    const int n = tid + k * 512;
-    if (n < groups) {
-      const int line = n / per_line, col = (n - line * per_line) * 4;
+  for (int k = 0; k < GROUPS; ++k, next()) {
+    if (line < c.rows) {
+      const int col = four * 4;
       f16x4 h, l;
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
-        const float v = (float)((double)u[k][e] * mul);     // (0 behind a line's end: padding)
+        const float v = narrow ? u[k][e] * mf : (float)((double)u[k][e] * mul);     // (0 behind a line's end: padding)
         h[e] = (_Float16)v;
         l[e] = (_Float16)(v - (float)h[e]);
       }

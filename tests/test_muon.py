@@ -52,7 +52,7 @@ def gradient(shape, seed, dtype=torch.float32, rank=4):
 
 
 SHAPES = [(1, 1), (1, 64), (70, 1), (3, 5), (31, 33), (2, 32, 32), (64, 147), (147, 64), (5, 40, 70), (129, 257), (256, 256), (3, 200, 640), (300, 128),
-          (21, 4608), (2304, 96), (513, 640), (2, 3, 16, 24), (65, 65), (64, 384), (384, 63), (64, 385), (33, 256), (257, 64), (2, 32, 417), (300, 1, 5),
+          (21, 4608), (2304, 96), (513, 640), (2, 3, 16, 24), (65, 65), (64, 384), (384, 63), (64, 385), (33, 256), (257, 64), (2, 64, 448), (448, 61), (449, 64), (2, 32, 417), (300, 1, 5),
           (48, 40007), (40007, 21), (2, 64, 1025)]
 
 
@@ -225,7 +225,7 @@ def test_muon_update_of_mixed_shapes(nesterov, wd):
 
 
 @pytest.mark.gpu
-@pytest.mark.parametrize("rows,first,step", [(20, 24, 3), (40, 24, 30), (100, 24, 11), (0, 390, 41)])
+@pytest.mark.parametrize("rows,first,step", [(20, 24, 3), (40, 24, 30), (100, 24, 11), (0, 460, 41)])
 def test_muon_update_of_many_shapes(rows, first, step):
     """15 shapes that run alike, more than the arguments of one launch hold, tall and wide; the last of 9 to 64 rows (columns)"""
     from pixelssl_amd import functional as PF
