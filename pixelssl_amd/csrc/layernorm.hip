@@ -11,7 +11,7 @@
 // 5.1 TB/s of a large copy.  Measured, us (rate): 33800 x 2048 bf16 forward 51 (5.4 TB/s), backward 87 (4.8); 8 x 256 x 129 x 129 fp32 64 (4.3)
 // and 100 (4.1); 8 x 2048 x 65 x 65 bf16 87 (3.2) and 180 (2.3) -- rows of 8450 bytes, so pieces lie across cache lines, and one workgroup a CU
 // that loads, sums and stores in turn.  Partial dw / db: under 5 us to write and to add.  Small calls are bound by the launches (5 us a
-// kernel) and, forward + backward, by the host: 67 us, of which an engine pass with a trivial node takes 47.
+// kernel) and, forward + backward, by the host: 65 us, of which an engine pass with a trivial node takes 44 - 47.
 #include "common.h"
 
 namespace {

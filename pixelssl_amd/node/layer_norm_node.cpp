@@ -1,7 +1,7 @@
 // The autograd node of functional.layer_norm / layer_norm_channels: layouts, workspaces and the calls of libpixelhip's
 // pxl_layer_norm_* entry points.  The kernels of a small call take 10 - 20 us; as a Python autograd.Function the host took 104 us for
 // forward + backward of 1003 x 777 (the backward runs on a thread of the engine, where Python is two to three times as slow), as this
-// node 70 us.  Host code only; the C entry points come in through bind().
+// node 65 us.  Host code only; the C entry points come in through bind().
 #include <ATen/hip/HIPContext.h>
 #include <torch/csrc/autograd/functions/basic_ops.h>
 #include <torch/extension.h>
