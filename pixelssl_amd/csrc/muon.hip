@@ -347,7 +347,6 @@ __global__ __launch_bounds__(256, D == 2 ? 2 : 1) void ns_gemm_kernel(NsClasses 
   constexpr int KS = T == 128 ? 32 : 64;        // k a step
   constexpr int PL = T * KS * 2;                // bytes of one plane's tile
   constexpr int BUF = (NA + NB) * PL;
-  constexpr int WB = T == 128 ? 1 : 2;          // blocks of 32 x 32 a wave ends up with: 4 / 1
   __shared__ __attribute__((aligned(16))) unsigned char lds[T == 64 && 2 * BUF < 65536 ? 65536 : 2 * BUF];
   constexpr bool CUTS = T == 128 && SYM && EPI != EPI_PART;
   const bool cut = CUTS && (int)blockIdx.x >= p.full;

@@ -436,8 +436,9 @@ def muon_update(params, grads, momenta, lr, momentum=0.95, nesterov=True, weight
         momentum_k <- momentum * momentum_k + (1 - momentum) * grad_k
         u = (1 - momentum) * grad_k + momentum * momentum_k  (nesterov)  or  momentum_k
         param_k <- param_k * (1 - lr * weight_decay) - lr * muon_scale(...) * orthogonalize(u)
-    adjust: the rule of muon_scale, or one factor per parameter in its place.  params / grads fp32 or bf16 (one type per parameter), momenta fp32 with the parameter's memory layout (contiguous or channels
-    last).  Parameters and momenta may overlap nothing."""
+    adjust: the rule of muon_scale, or one factor per parameter in its place.  params / grads fp32 or bf16 (one type per parameter), momenta
+    fp32 with the parameter's memory layout (contiguous or channels last).  Parameters and momenta may overlap nothing.  Refusals that need
+    no look at memory come before anything is changed."""
     params, grads, momenta = list(params), list(grads), list(momenta)
     if not len(params) == len(grads) == len(momenta):
         raise ValueError("muon_update: %d parameters, %d gradients, %d momenta" % (len(params), len(grads), len(momenta)))
