@@ -4,6 +4,7 @@ import ctypes
 import functools
 
 import torch
+from torch.autograd import forward_ad
 
 from . import _lib
 from ._lib import check, dtype_code, lib, ptr, stream_ptr
@@ -288,6 +289,17 @@ def _launch(index, fn, *args):
         check(rc)
 
 
+def _refuse_recording(name, *tensors):
+    """A recorder (torch.jit.trace, make_fx) sees the allocations of a call but not its kernels: what it made would return what the memory held
+    before.  torch.func's wrappers have no memory, and a forward-mode tangent would stop at the outputs without a word."""
+    if torch._C._get_tracing_state() is not None or torch._C._get_dispatch_mode(torch._C._TorchDispatchModeKey.PROXY) is not None:
+        raise _lib.PixelHipError("%s cannot be traced (torch.jit.trace, make_fx): its kernels would be missing from the result" % name)
+    if torch._C._functorch.peek_interpreter_stack() is not None:
+        raise _lib.PixelHipError("%s does not run under torch.func / vmap" % name)
+    if forward_ad._current_level >= 0 and any(t is not None and forward_ad.unpack_dual(t).tangent is not None for t in tensors):
+        raise _lib.PixelHipError("%s has no forward-mode derivative" % name)
+
+
 _pxlnode = None
 
 
@@ -317,6 +329,7 @@ def _layer_norm(x, weight, bias, eps, channels):
 
 def _layer_norm_refuse(name, x, weight, bias, eps, channels):
     """says what the node does not take about the arguments"""
+    _refuse_recording(name, x, weight, bias)
     dtype = x.dtype
     if dtype is not torch.float32 and dtype is not torch.bfloat16:
         raise ValueError("%s: float32 or bfloat16, got %s" % (name, dtype))
@@ -376,6 +389,7 @@ def orthogonalize(x, steps=5, coefficients=NEWTON_SCHULZ, eps=1e-7):
     """Every matrix of x [..., rows, cols] (fp32 or bf16) with its singular values driven to about 1 by `steps` of the Newton-Schulz
     iteration X <- (a + b L + c L^2) X, L = X X', from X = x / max(|x|, eps) (Frobenius norm); for rows > cols on the transposed
     matrix.  coefficients: one (a, b, c) or one per step.  A NaN or an infinity makes its own matrix NaN.  Not differentiable."""
+    _refuse_recording("orthogonalize", x)
     if x.dim() < 2:
         raise ValueError("orthogonalize: %s is no matrix" % (tuple(x.shape),))
     if x.dtype not in (torch.float32, torch.bfloat16):
@@ -440,6 +454,7 @@ def muon_update(params, grads, momenta, lr, momentum=0.95, nesterov=True, weight
     fp32 with the parameter's memory layout (contiguous or channels last).  Parameters and momenta may overlap nothing.  Refusals that need
     no look at memory come before anything is changed."""
     params, grads, momenta = list(params), list(grads), list(momenta)
+    _refuse_recording("muon_update", *params, *grads, *momenta)
     if not len(params) == len(grads) == len(momenta):
         raise ValueError("muon_update: %d parameters, %d gradients, %d momenta" % (len(params), len(grads), len(momenta)))
     lr, momentum, weight_decay = float(lr), float(momentum), float(weight_decay)
@@ -483,6 +498,7 @@ def adam_update(params, grads, exp_avgs, exp_avg_sqs, lr, betas=(0.9, 0.999), ep
     vectors beside muon_update's matrices.  params / grads fp32 or bf16, exp_avgs / exp_avg_sqs fp32, all four of an entry dense and
     alike in memory (a gradient may lie otherwise).  Parameters and moments may overlap nothing.  step counts from 1."""
     params, grads, exp_avgs, exp_avg_sqs = list(params), list(grads), list(exp_avgs), list(exp_avg_sqs)
+    _refuse_recording("adam_update", *params, *grads, *exp_avgs, *exp_avg_sqs)
     if not len(params) == len(grads) == len(exp_avgs) == len(exp_avg_sqs):
         raise ValueError("adam_update: %d parameters, %d gradients, %d and %d moments" % (len(params), len(grads), len(exp_avgs), len(exp_avg_sqs)))
     b1, b2 = float(betas[0]), float(betas[1])

@@ -3,7 +3,9 @@
 // forward + backward of 1003 x 777 (the backward runs on a thread of the engine, where Python is two to three times as slow), as this
 // node 65 us.  Host code only; the C entry points come in through bind().
 #include <ATen/hip/HIPContext.h>
+#include <c10/core/impl/TorchDispatchModeTLS.h>
 #include <torch/csrc/autograd/functions/basic_ops.h>
+#include <torch/csrc/jit/frontend/tracer.h>
 #include <torch/extension.h>
 
 #include <optional>
@@ -158,11 +160,22 @@ struct LayerNormNode : public torch::autograd::Function<LayerNormNode> {
   }
 };
 
+// Recorders see the allocations of a call but not its kernels (a traced module would return what its memory held before), a tangent would stop
+// at the outputs, and torch.func's wrappers have no memory
+bool beyond_reach(const Tensor& x, const MaybeTensor& w, const MaybeTensor& b) {
+  if (torch::jit::tracer::isTracing() || c10::impl::tls_is_dispatch_key_included(c10::DispatchKey::FuncTorchDynamicLayerFrontMode) ||
+      c10::impl::TorchDispatchModeTLS::get_mode(c10::impl::TorchDispatchModeKey::PROXY).has_value())
+    return true;
+  auto tangent = [](const Tensor& t) { return t._fw_grad(/*level=*/0).defined(); };
+  return tangent(x) || (w.has_value() && w->defined() && tangent(*w)) || (b.has_value() && b->defined() && tangent(*b));
+}
+
 // y, or nothing where an argument is not as the kernels take it: functional._layer_norm then says what (the checks in Python take 2 - 3 us)
 MaybeTensor layer_norm(const Tensor& x0, const MaybeTensor& w0, const MaybeTensor& b0, double eps, bool channels) {
   const bool has_w = w0.has_value() && w0->defined(), has_b = b0.has_value() && b0->defined();
   const at::ScalarType t = x0.scalar_type();
-  if (!x0.is_cuda() || x0.layout() != at::kStrided || (t != at::kFloat && t != at::kBFloat16) || x0.dim() < (channels ? 2 : 1) || !(eps >= 0)) return {};
+  if (!x0.is_cuda() || x0.layout() != at::kStrided || (t != at::kFloat && t != at::kBFloat16) || x0.dim() < (channels ? 2 : 1) || !(eps >= 0) || beyond_reach(x0, w0, b0))
+    return {};
   const int64_t C = x0.size(channels ? 1 : -1);
   if (C < 1 || C > (1 << 24)) return {};
   for (const MaybeTensor* q : {&w0, &b0}) {
