@@ -53,7 +53,7 @@ def _foreign(params):
 
 def _sync_foreign_grads(groups):
     """Multi-rank: mean of the per-rank gradients of every tensor that is NOT owned by an engine model (those are
-    exchanged by the executor, overlapped with the backward pass).  One all-reduce over the concatenated gradients."""
+    exchanged by the executor, overlapped with the backward pass).  One all-reduce over the concatenated gradients of each type."""
     from .. import dist as pdist
     if not pdist.is_distributed():
         return
@@ -67,19 +67,26 @@ def _sync_foreign_grads(groups):
     # its mean is > 0 iff some rank had one): those step with the mean on EVERY rank -- a rank that had none contributed zeros to
     # the mean and must apply it too, or the replicas drift apart; tensors without a gradient anywhere keep grad = None (the
     # optimizers skip them, like torch's).  The flags are read back (a device sync) only on a rank that misses a gradient.
+    # Gradients are averaged in their own type: one all-reduce per type, in the order the types first appear (the same on every rank).
     dev = ps[0].device
-    flags = torch.tensor([0.0 if p.grad is None else 1.0 for p in ps], device=dev, dtype=ps[0].dtype)
-    flat = torch.cat([(p.grad if p.grad is not None else torch.zeros_like(p)).reshape(-1).to(ps[0].dtype) for p in ps] + [flags])
-    pdist.allreduce_mean_(flat)
-    had = flat[-len(ps):].tolist() if any(p.grad is None for p in ps) else None
-    off = 0
-    for k, p in enumerate(ps):
-        n = p.numel()
-        if p.grad is not None:
-            p.grad.copy_(flat[off:off + n].view_as(p.grad))
-        elif had[k] > 0:
-            p.grad = flat[off:off + n].view_as(p).clone().to(p.dtype)
-        off += n
+    types = list(dict.fromkeys(p.dtype for p in ps))
+    flags = torch.tensor([0.0 if p.grad is None else 1.0 for p in ps], device=dev, dtype=types[0])
+    had = None
+    for dtype in types:
+        mine = [(k, p) for k, p in enumerate(ps) if p.dtype == dtype]
+        flat = torch.cat([(p.grad if p.grad is not None else torch.zeros_like(p)).reshape(-1).to(dtype) for _, p in mine] +
+                         ([flags] if dtype == types[0] else []))
+        pdist.allreduce_mean_(flat)
+        if dtype == types[0] and any(p.grad is None for p in ps):
+            had = flat[-len(ps):].tolist()
+        off = 0
+        for k, p in mine:
+            n = p.numel()
+            if p.grad is not None:
+                p.grad.copy_(flat[off:off + n].view_as(p.grad))
+            elif had[k] > 0:
+                p.grad = flat[off:off + n].view_as(p).clone()
+            off += n
 
 
 def _flat_view(store, buf, p):
