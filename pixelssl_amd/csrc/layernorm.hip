@@ -3,7 +3,7 @@
 //   mean = sum_c x / C,  var = sum_c (x - mean)^2 / C,  rstd = 1 / sqrt(var + eps),  u = (x - mean) rstd,  y = u w + b
 //   g = dy w,  dx = rstd (g - sum_c g / C - u sum_c (g u) / C),  dw = sum_rows dy u,  db = sum_rows dy
 //
-// Statistics, sums and the parameter gradients are held in 32 bits whatever the type of x; the variance is taken around the
+// Statistics, sums and the parameter gradients are held in 32 bits or more whatever the type of x; the variance is taken around the
 // mean in a second sweep (sum x^2 - C mean^2 cancels where the mean is large against the deviation).  No atomics: every sum has
 // one order, so two calls on the same inputs agree bit for bit.  y and dx are rounded once.
 //
@@ -39,19 +39,32 @@ template <int THREADS> __device__ __forceinline__ float block_sum(float v, float
   return s;
 }
 
+// Sums of any number of terms (up to 2^24 features, 2^31 rows and more a call) are taken in 64 bits: one after the other in 32 bits, 10^6 terms of
+// one sign are off by up to 1 %.  out: over the threads of one place (threadIdx.x % TP) of a workgroup of 256, on each of them
+template <int TP> __device__ __forceinline__ double long_sum(double v, double (*sh)[TP < 64 ? TP : 64]) {
+#pragma unroll
+  for (int o = TP < 64 ? TP : 64; o < 64; o <<= 1) v += __shfl_xor(v, o, 64);
+  constexpr int W = TP < 64 ? TP : 64;
+  const int at = threadIdx.x & (W - 1);
+  __syncthreads();                      // the last reader of sh is done
+  if ((threadIdx.x & 63) < W) sh[threadIdx.x >> 6][at] = v;
+  __syncthreads();
+  return (sh[0][at] + sh[1][at]) + (sh[2][at] + sh[3][at]);
+}
+
 // ---- rows of any length: one workgroup a row, three sweeps (the second and third come out of the caches) -------------------
 template <typename T>
 __global__ __launch_bounds__(256) void ln_rows_fwd_loop(long R, int C, long xs, const T* __restrict__ x, LnParam w, LnParam b,
                                                         float eps, T* __restrict__ y, float* __restrict__ mean, float* __restrict__ rstd) {
-  __shared__ float sh[4];
+  __shared__ double sh[4][1];
   for (long r = blockIdx.x; r < R; r += gridDim.x) {
     const T* xr = x + r * xs;
-    float s = 0.f;
+    double s = 0.0;
     for (int c = threadIdx.x; c < C; c += 256) s += to_f(xr[c]);
-    const float m = block_sum<256>(s, sh) / C;
-    float q = 0.f;
+    const float m = (float)(long_sum<1>(s, sh) / C);
+    double q = 0.0;
     for (int c = threadIdx.x; c < C; c += 256) { const float d = to_f(xr[c]) - m; q += d * d; }
-    const float rs = 1.f / sqrtf(block_sum<256>(q, sh) / C + eps);
+    const float rs = 1.f / sqrtf((float)(long_sum<1>(q, sh) / C) + eps);
     T* yr = y + r * C;
     for (int c = threadIdx.x; c < C; c += 256)
       yr[c] = from_f<T>((to_f(xr[c]) - m) * rs * w.get<T>(c, 1.f) + b.get<T>(c, 0.f));
@@ -62,17 +75,17 @@ __global__ __launch_bounds__(256) void ln_rows_fwd_loop(long R, int C, long xs, 
 template <typename T>
 __global__ __launch_bounds__(256) void ln_rows_dx_loop(long R, int C, long xs, const T* __restrict__ x, const T* __restrict__ dy, LnParam w,
                                                        const float* __restrict__ mean, const float* __restrict__ rstd, T* __restrict__ dx) {
-  __shared__ float sh[4];
+  __shared__ double sh[4][1];
   for (long r = blockIdx.x; r < R; r += gridDim.x) {
     const T* xr = x + r * xs;
     const T* gr = dy + r * C;
     const float m = mean[r], rs = rstd[r];
-    float s1 = 0.f, s2 = 0.f;
+    double s1 = 0.0, s2 = 0.0;
     for (int c = threadIdx.x; c < C; c += 256) {
       const float g = to_f(gr[c]) * w.get<T>(c, 1.f), u = (to_f(xr[c]) - m) * rs;
       s1 += g; s2 += g * u;
     }
-    const float a1 = block_sum<256>(s1, sh) / C, a2 = block_sum<256>(s2, sh) / C;
+    const float a1 = (float)(long_sum<1>(s1, sh) / C), a2 = (float)(long_sum<1>(s2, sh) / C);
     T* dr = dx + r * C;
     for (int c = threadIdx.x; c < C; c += 256) {
       const float g = to_f(gr[c]) * w.get<T>(c, 1.f), u = (to_f(xr[c]) - m) * rs;
@@ -87,48 +100,61 @@ __global__ __launch_bounds__(256) void ln_rows_dwb_loop(long R, int C, long xs, 
                                                         const float* __restrict__ mean, const float* __restrict__ rstd, float* __restrict__ part) {
   const int c = blockIdx.x * 256 + threadIdx.x;
   if (c >= C) return;
-  float sw = 0.f, sb = 0.f;
+  double sw = 0.0, sb = 0.0;
   for (long r = blockIdx.y; r < R; r += gridDim.y) {
     const float g = to_f(dy[r * C + c]);
     sw += g * ((to_f(x[r * xs + c]) - mean[r]) * rstd[r]);
     sb += g;
   }
   float* p = part + (long)blockIdx.y * 2 * C;
-  p[c] = sw;
-  p[C + c] = sb;
+  p[c] = (float)sw;
+  p[C + c] = (float)sb;
 }
 
-// ---- channels of a map, any number: one thread a position ------------------------------------------------------------------
-template <typename T>
-__global__ __launch_bounds__(256) void ln_chan_fwd_loop(long P, int C, long S, const T* __restrict__ x, LnParam w, LnParam b, float eps,
+// ---- channels of a map, any number: TP positions a workgroup, 256 / TP threads over the channels of each; xn: elements from one map of x to
+// the next (rows shorter than a piece come here too, as maps of one position) -----------------------------------------------------------
+template <typename T, int TP>
+__global__ __launch_bounds__(256) void ln_chan_fwd_loop(long P, int C, long S, long xn, const T* __restrict__ x, LnParam w, LnParam b, float eps,
                                                         T* __restrict__ y, float* __restrict__ mean, float* __restrict__ rstd) {
-  for (long p = blockIdx.x * 256L + threadIdx.x; p < P; p += gridDim.x * 256L) {
-    const long n = p / S, o = n * C * S + (p - n * S);
-    float s = 0.f;
-    for (int c = 0; c < C; ++c) s += to_f(x[o + c * S]);
-    const float m = s / C;
-    float q = 0.f;
-    for (int c = 0; c < C; ++c) { const float d = to_f(x[o + c * S]) - m; q += d * d; }
-    const float rs = 1.f / sqrtf(q / C + eps);
-    for (int c = 0; c < C; ++c) y[o + c * S] = from_f<T>((to_f(x[o + c * S]) - m) * rs * w.get<T>(c, 1.f) + b.get<T>(c, 0.f));
-    if (mean != nullptr) { mean[p] = m; rstd[p] = rs; }
+  __shared__ double sh[4][TP < 64 ? TP : 64];
+  constexpr int CL = 256 / TP;
+  const int cl = threadIdx.x / TP;
+  auto sum = [&](double v) { return CL == 1 ? v : long_sum<TP>(v, sh); };
+  for (long p0 = (long)blockIdx.x * TP; p0 < P; p0 += (long)gridDim.x * TP) {
+    const long at = p0 + threadIdx.x % TP, p = at < P ? at : P - 1;         // past the end: the last position again, stored by none
+    const long n = p / S, i = p - n * S, o = n * C * S + i, ox = n * xn + i;
+    double s = 0.0;
+    for (int c = cl; c < C; c += CL) s += to_f(x[ox + c * S]);
+    const float m = (float)(sum(s) / C);
+    double q = 0.0;
+    for (int c = cl; c < C; c += CL) { const float d = to_f(x[ox + c * S]) - m; q += d * d; }
+    const float rs = 1.f / sqrtf((float)(sum(q) / C) + eps);
+    if (at >= P) continue;
+    for (int c = cl; c < C; c += CL) y[o + c * S] = from_f<T>((to_f(x[ox + c * S]) - m) * rs * w.get<T>(c, 1.f) + b.get<T>(c, 0.f));
+    if (mean != nullptr && cl == 0) { mean[p] = m; rstd[p] = rs; }
   }
 }
 
-template <typename T>
-__global__ __launch_bounds__(256) void ln_chan_dx_loop(long P, int C, long S, const T* __restrict__ x, const T* __restrict__ dy, LnParam w,
+template <typename T, int TP>
+__global__ __launch_bounds__(256) void ln_chan_dx_loop(long P, int C, long S, long xn, const T* __restrict__ x, const T* __restrict__ dy, LnParam w,
                                                        const float* __restrict__ mean, const float* __restrict__ rstd, T* __restrict__ dx) {
-  for (long p = blockIdx.x * 256L + threadIdx.x; p < P; p += gridDim.x * 256L) {
-    const long n = p / S, o = n * C * S + (p - n * S);
+  __shared__ double sh[4][TP < 64 ? TP : 64];
+  constexpr int CL = 256 / TP;
+  const int cl = threadIdx.x / TP;
+  auto sum = [&](double v) { return CL == 1 ? v : long_sum<TP>(v, sh); };
+  for (long p0 = (long)blockIdx.x * TP; p0 < P; p0 += (long)gridDim.x * TP) {
+    const long at = p0 + threadIdx.x % TP, p = at < P ? at : P - 1;
+    const long n = p / S, i = p - n * S, o = n * C * S + i, ox = n * xn + i;
     const float m = mean[p], rs = rstd[p];
-    float s1 = 0.f, s2 = 0.f;
-    for (int c = 0; c < C; ++c) {
+    double s1 = 0.0, s2 = 0.0;
+    for (int c = cl; c < C; c += CL) {
       const float g = to_f(dy[o + c * S]) * w.get<T>(c, 1.f);
-      s1 += g; s2 += g * ((to_f(x[o + c * S]) - m) * rs);
+      s1 += g; s2 += g * ((to_f(x[ox + c * S]) - m) * rs);
     }
-    const float a1 = s1 / C, a2 = s2 / C;
-    for (int c = 0; c < C; ++c) {
-      const float g = to_f(dy[o + c * S]) * w.get<T>(c, 1.f), u = (to_f(x[o + c * S]) - m) * rs;
+    const float a1 = (float)(sum(s1) / C), a2 = (float)(sum(s2) / C);
+    if (at >= P) continue;
+    for (int c = cl; c < C; c += CL) {
+      const float g = to_f(dy[o + c * S]) * w.get<T>(c, 1.f), u = (to_f(x[ox + c * S]) - m) * rs;
       dx[o + c * S] = from_f<T>(rs * (g - a1 - u * a2));
     }
   }
@@ -136,22 +162,22 @@ __global__ __launch_bounds__(256) void ln_chan_dx_loop(long P, int C, long S, co
 
 // workgroup (channel, position group) -> part[group][2][C]
 template <typename T>
-__global__ __launch_bounds__(256) void ln_chan_dwb_loop(long P, int C, long S, const T* __restrict__ x, const T* __restrict__ dy,
+__global__ __launch_bounds__(256) void ln_chan_dwb_loop(long P, int C, long S, long xn, const T* __restrict__ x, const T* __restrict__ dy,
                                                         const float* __restrict__ mean, const float* __restrict__ rstd, float* __restrict__ part) {
-  __shared__ float sh[4];
+  __shared__ double sh[4][1];
   const int c = blockIdx.x;
-  float sw = 0.f, sb = 0.f;
+  double sw = 0.0, sb = 0.0;
   for (long p = blockIdx.y * 256L + threadIdx.x; p < P; p += gridDim.y * 256L) {
-    const long n = p / S, o = (n * C + c) * S + (p - n * S);
+    const long n = p / S, i = p - n * S, o = (n * C + c) * S + i, ox = n * xn + c * S + i;
     const float g = to_f(dy[o]);
-    sw += g * ((to_f(x[o]) - mean[p]) * rstd[p]);
+    sw += g * ((to_f(x[ox]) - mean[p]) * rstd[p]);
     sb += g;
   }
-  sw = block_sum<256>(sw, sh);
-  sb = block_sum<256>(sb, sh);
+  sw = long_sum<1>(sw, sh);
+  sb = long_sum<1>(sb, sh);
   if (threadIdx.x == 0) {
-    part[(long)blockIdx.y * 2 * C + c] = sw;
-    part[(long)blockIdx.y * 2 * C + C + c] = sb;
+    part[(long)blockIdx.y * 2 * C + c] = (float)sw;
+    part[(long)blockIdx.y * 2 * C + C + c] = (float)sb;
   }
 }
 
@@ -579,10 +605,10 @@ __global__ __launch_bounds__(THREADS) void ln_chan_bwd(int tiles, int per, int C
 // part[G][2][C] -> dw[C], db[C] (either may be absent): 16 columns a workgroup, 64 lanes over the groups, in ascending order each
 template <typename T>
 __global__ __launch_bounds__(1024) void ln_dwb_fold(int G, int C, const float* __restrict__ part, void* dw, void* db, int f32) {
-  __shared__ float sh[64][17];
+  __shared__ double sh[64][17];
   const int col = threadIdx.x & 15, gl = threadIdx.x >> 4;
   const int k = blockIdx.x * 16 + col;
-  float s = 0.f;
+  double s = 0.0;                             // (up to 1280 shares)
   if (k < 2 * C) {
     int g = gl;
     for (; g + 192 < G; g += 256) {           // four loads in flight
@@ -597,14 +623,14 @@ __global__ __launch_bounds__(1024) void ln_dwb_fold(int G, int C, const float* _
   sh[gl][col] = s;
   __syncthreads();
   if (gl != 0 || k >= 2 * C) return;
-  s = 0.f;
+  s = 0.0;
 #pragma unroll 16
   for (int q = 0; q < 64; ++q) s += sh[q][col];
   void* out = k < C ? dw : db;
   if (out == nullptr) return;
   const int c = k < C ? k : k - C;
-  if (f32) reinterpret_cast<float*>(out)[c] = s;
-  else reinterpret_cast<T*>(out)[c] = from_f<T>(s);
+  if (f32) reinterpret_cast<float*>(out)[c] = (float)s;
+  else reinterpret_cast<T*>(out)[c] = from_f<T>((float)s);
 }
 
 inline unsigned blocks_for(long n, long most) { return (unsigned)(n < 1 ? 1 : (n < most ? n : most)); }
@@ -700,6 +726,13 @@ inline LnShape ln_shape(int dtype, long R, int C, long S) { return S < 0 ? ln_ro
     else if (s.nv == 8) hipLaunchKernelGGL((KERNEL<T, 512 * H, 4, 8 / H>), grid, dim3(512 * H), 0, st, __VA_ARGS__);                 \
     else hipLaunchKernelGGL((KERNEL<T, 512 * H, 4, 16 / H>), grid, dim3(512 * H), 0, st, __VA_ARGS__);                               \
   } while (0)
+// Channels beyond the register kernels: up to 16 of them one thread a position, more 8 positions a workgroup (forward + backward of 2^18 maps of
+// 2 positions, us, one thread a position / so: bf16 17 channels 179 / 219, 24 329 / 232, 64 1432 / 432; fp32 368 / 259, 551 / 298, 1720 / 625)
+#define LN_CHAN_LOOP(KERNEL, ...)                                                                                                   \
+  do {                                                                                                                              \
+    if (C <= 16) hipLaunchKernelGGL((KERNEL<T, 256>), dim3(blocks_for((R + 255) / 256, 1 << 20)), dim3(256), 0, st, __VA_ARGS__);   \
+    else hipLaunchKernelGGL((KERNEL<T, 8>), dim3(blocks_for((R + 7) / 8, 1 << 20)), dim3(256), 0, st, __VA_ARGS__);                 \
+  } while (0)
 
 template <typename T>
 int ln_fwd(long R, int C, long S, long xs, const void* x, LnParam w, LnParam b, float eps, void* y, float* mean, float* rstd, hipStream_t st) {
@@ -709,6 +742,8 @@ int ln_fwd(long R, int C, long S, long xs, const void* x, LnParam w, LnParam b, 
       // as many workgroups as are resident at once (registers: 3 a CU with 4 pieces a lane, else 6 and more), the rows evenly over them
       const long passes = (R + 256 / s.lanes - 1) / (256 / s.lanes), most = s.nv >= 4 ? 768 : 1536, each = (passes + most - 1) / most;
       LN_ROWS(ln_rows_fwd, blocks_for((passes + each - 1) / each, most), R, C, xs, (const T*)x, w, b, eps, (T*)y, mean, rstd);
+    } else if (C < Piece<T>::N) {
+      LN_CHAN_LOOP(ln_chan_fwd_loop, R, C, 1, xs, (const T*)x, w, b, eps, (T*)y, mean, rstd);
     } else {
       hipLaunchKernelGGL(ln_rows_fwd_loop<T>, dim3(blocks_for(R, 1 << 20)), dim3(256), 0, st, R, C, xs, (const T*)x, w, b, eps, (T*)y, mean, rstd);
     }
@@ -716,8 +751,7 @@ int ln_fwd(long R, int C, long S, long xs, const void* x, LnParam w, LnParam b, 
     const int per = (int)(s.tiles / (R / S));
     LN_CHAN(ln_chan_fwd, 1, (unsigned)s.tiles, (int)s.tiles, per, C, (int)S, (const T*)x, w, b, eps, (T*)y, mean, rstd);
   } else {
-    hipLaunchKernelGGL(ln_chan_fwd_loop<T>, dim3(blocks_for((R + 255) / 256, 1 << 20)), dim3(256), 0, st, R, C, S, (const T*)x, w, b, eps,
-                       (T*)y, mean, rstd);
+    LN_CHAN_LOOP(ln_chan_fwd_loop, R, C, S, C * S, (const T*)x, w, b, eps, (T*)y, mean, rstd);
   }
   PXL_LAUNCH_CHECK();
   return PXL_OK;
@@ -740,18 +774,21 @@ int ln_bwd(long R, int C, long S, long xs, const void* x, const void* dy, LnPara
     PXL_LAUNCH_CHECK();
   } else if (R > 0) {
     if (dx != nullptr) {
-      if (S < 0)
+      if (S < 0 && C < Piece<T>::N)
+        LN_CHAN_LOOP(ln_chan_dx_loop, R, C, 1, xs, (const T*)x, (const T*)dy, w, mean, rstd, (T*)dx);
+      else if (S < 0)
         hipLaunchKernelGGL(ln_rows_dx_loop<T>, dim3(blocks_for(R, 1 << 20)), dim3(256), 0, st, R, C, xs, (const T*)x, (const T*)dy, w, mean, rstd, (T*)dx);
       else
-        hipLaunchKernelGGL(ln_chan_dx_loop<T>, dim3(blocks_for((R + 255) / 256, 1 << 20)), dim3(256), 0, st, R, C, S, (const T*)x, (const T*)dy, w,
-                           mean, rstd, (T*)dx);
+        LN_CHAN_LOOP(ln_chan_dx_loop, R, C, S, C * S, (const T*)x, (const T*)dy, w, mean, rstd, (T*)dx);
       PXL_LAUNCH_CHECK();
     }
     if (params) {
-      if (S < 0)
+      if (S < 0 && C < Piece<T>::N)
+        hipLaunchKernelGGL(ln_chan_dwb_loop<T>, dim3(C, G), dim3(256), 0, st, R, C, 1, xs, (const T*)x, (const T*)dy, mean, rstd, part);
+      else if (S < 0)
         hipLaunchKernelGGL(ln_rows_dwb_loop<T>, dim3((C + 255) / 256, G), dim3(256), 0, st, R, C, xs, (const T*)x, (const T*)dy, mean, rstd, part);
       else
-        hipLaunchKernelGGL(ln_chan_dwb_loop<T>, dim3(C, G), dim3(256), 0, st, R, C, S, (const T*)x, (const T*)dy, mean, rstd, part);
+        hipLaunchKernelGGL(ln_chan_dwb_loop<T>, dim3(C, G), dim3(256), 0, st, R, C, S, C * S, (const T*)x, (const T*)dy, mean, rstd, part);
       PXL_LAUNCH_CHECK();
     }
   }
@@ -808,6 +845,7 @@ extern "C" int pxl_layer_norm_bwd(int dtype, int pdtype, long R, int C, long x_s
 extern "C" int pxl_layer_norm_nchw_fwd(int dtype, int pdtype, long N, int C, long S, const void* x, const void* w, const void* b, float eps,
                                        void* y, float* mean, float* rstd, void* stream) {
   PXL_REQUIRE(N >= 0 && S >= 0, "layer_norm_nchw_fwd: bad sizes (maps %ld, positions %ld)", N, S);
+  if (S == 1) return pxl_layer_norm_fwd(dtype, pdtype, N, C, C, x, w, b, eps, y, mean, rstd, stream);          // rows of C without gaps
   const int rc = ln_check("layer_norm_nchw_fwd", dtype, pdtype, N * S, C);
   if (rc != PXL_OK) return rc;
   if (N * S == 0) return PXL_OK;
@@ -819,6 +857,7 @@ extern "C" int pxl_layer_norm_nchw_fwd(int dtype, int pdtype, long N, int C, lon
 }
 
 extern "C" size_t pxl_layer_norm_nchw_bwd_workspace(long N, int C, long S) {
+  if (S == 1) return pxl_layer_norm_bwd_workspace(N, C);
   return N < 0 || S < 0 || C < 1 ? 0 : (size_t)ln_chan_most(N, C, S) * 2 * C * sizeof(float);
 }
 
@@ -826,6 +865,7 @@ extern "C" int pxl_layer_norm_nchw_bwd(int dtype, int pdtype, long N, int C, lon
                                        const float* mean, const float* rstd, void* dx, void* dw, void* db, void* ws, size_t ws_bytes,
                                        void* stream) {
   PXL_REQUIRE(N >= 0 && S >= 0, "layer_norm_nchw_bwd: bad sizes (maps %ld, positions %ld)", N, S);
+  if (S == 1) return pxl_layer_norm_bwd(dtype, pdtype, N, C, C, x, dy, w, mean, rstd, dx, dw, db, ws, ws_bytes, stream);
   const int rc = ln_check("layer_norm_nchw_bwd", dtype, pdtype, N * S, C);
   if (rc != PXL_OK) return rc;
   PXL_REQUIRE(N * S == 0 || (x && dy && mean && rstd), "layer_norm_nchw_bwd: bad argument");
