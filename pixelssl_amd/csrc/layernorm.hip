@@ -160,12 +160,12 @@ __global__ __launch_bounds__(256) void ln_chan_dx_loop(long P, int C, long S, lo
   }
 }
 
-// workgroup (channel, position group) -> part[group][2][C]
+// workgroup (channel from c0 on, position group) -> part[group][2][C]
 template <typename T>
-__global__ __launch_bounds__(256) void ln_chan_dwb_loop(long P, int C, long S, long xn, const T* __restrict__ x, const T* __restrict__ dy,
+__global__ __launch_bounds__(256) void ln_chan_dwb_loop(int c0, long P, int C, long S, long xn, const T* __restrict__ x, const T* __restrict__ dy,
                                                         const float* __restrict__ mean, const float* __restrict__ rstd, float* __restrict__ part) {
   __shared__ double sh[4][1];
-  const int c = blockIdx.x;
+  const int c = c0 + blockIdx.x;
   double sw = 0.0, sb = 0.0;
   for (long p = blockIdx.y * 256L + threadIdx.x; p < P; p += gridDim.y * 256L) {
     const long n = p / S, i = p - n * S, o = (n * C + c) * S + i, ox = n * xn + c * S + i;
@@ -427,13 +427,13 @@ template <typename T> __device__ __forceinline__ T* lane_at(T* base, unsigned of
 }
 
 template <typename T, int THREADS, int TSV, int NV>
-__global__ __launch_bounds__(THREADS) void ln_chan_fwd(int tiles, int per, int C, int S, const T* __restrict__ x, LnParam w, LnParam b, float eps,
+__global__ __launch_bounds__(THREADS) void ln_chan_fwd(int first, int per, int C, int S, const T* __restrict__ x, LnParam w, LnParam b, float eps,
                                                        T* __restrict__ y, float* __restrict__ mean, float* __restrict__ rstd) {
   constexpr int V = Piece<T>::N, CY = THREADS / TSV, TS = TSV * V;
   __shared__ float sh[(THREADS / 64 + 1) * TS];
   const int sv = threadIdx.x % TSV, cy = threadIdx.x / TSV;
   const float inv = 1.f / C;
-  const int t = xcd_remap(blockIdx.x, tiles);
+  const int t = first + xcd_remap(blockIdx.x, gridDim.x);
   const int n = t / per, s0 = (t - n * per) * TS + sv * V;
   const int at = s0 + V <= S ? s0 : S - V, dup = s0 - at;
   const long base = (long)n * C * S, step = (long)CY * S;
@@ -633,6 +633,7 @@ __global__ __launch_bounds__(1024) void ln_dwb_fold(int G, int C, const float* _
   else reinterpret_cast<T*>(out)[c] = from_f<T>((float)s);
 }
 
+constexpr long LN_MOST = 1l << 22;        // workgroups a launch at most: of up to 1024 threads, and a grid has fewer than 2^32
 inline unsigned blocks_for(long n, long most) { return (unsigned)(n < 1 ? 1 : (n < most ? n : most)); }
 
 // How a call is run.  Rows: 8 .. 64 lanes (a wave or a part of it) hold a row in at most 4 pieces each, else a workgroup holds it in at
@@ -749,7 +750,8 @@ int ln_fwd(long R, int C, long S, long xs, const void* x, LnParam w, LnParam b, 
     }
   } else if (s.lanes) {
     const int per = (int)(s.tiles / (R / S));
-    LN_CHAN(ln_chan_fwd, 1, (unsigned)s.tiles, (int)s.tiles, per, C, (int)S, (const T*)x, w, b, eps, (T*)y, mean, rstd);
+    for (long t = 0; t < s.tiles; t += LN_MOST)
+      LN_CHAN(ln_chan_fwd, 1, (unsigned)(s.tiles - t < LN_MOST ? s.tiles - t : LN_MOST), (int)t, per, C, (int)S, (const T*)x, w, b, eps, (T*)y, mean, rstd);
   } else {
     LN_CHAN_LOOP(ln_chan_fwd_loop, R, C, S, C * S, (const T*)x, w, b, eps, (T*)y, mean, rstd);
   }
@@ -783,12 +785,12 @@ int ln_bwd(long R, int C, long S, long xs, const void* x, const void* dy, LnPara
       PXL_LAUNCH_CHECK();
     }
     if (params) {
-      if (S < 0 && C < Piece<T>::N)
-        hipLaunchKernelGGL(ln_chan_dwb_loop<T>, dim3(C, G), dim3(256), 0, st, R, C, 1, xs, (const T*)x, (const T*)dy, mean, rstd, part);
-      else if (S < 0)
+      if (S < 0 && C >= Piece<T>::N)
         hipLaunchKernelGGL(ln_rows_dwb_loop<T>, dim3((C + 255) / 256, G), dim3(256), 0, st, R, C, xs, (const T*)x, (const T*)dy, mean, rstd, part);
       else
-        hipLaunchKernelGGL(ln_chan_dwb_loop<T>, dim3(C, G), dim3(256), 0, st, R, C, S, C * S, (const T*)x, (const T*)dy, mean, rstd, part);
+        for (long c = 0; c < C; c += LN_MOST)
+          hipLaunchKernelGGL(ln_chan_dwb_loop<T>, dim3((unsigned)(C - c < LN_MOST ? C - c : LN_MOST), G), dim3(256), 0, st, (int)c, R, C, S < 0 ? 1 : S,
+                             S < 0 ? xs : C * S, (const T*)x, (const T*)dy, mean, rstd, part);
       PXL_LAUNCH_CHECK();
     }
   }

@@ -92,3 +92,38 @@ def test_one_position_needs_the_workspace_of_rows():
     h = _lib.lib()
     for n, c in ((1, 1), (70, 33), (100000, 2048), (3, 2 ** 24)):
         assert h.pxl_layer_norm_nchw_bwd_workspace(n, c, 1) == h.pxl_layer_norm_bwd_workspace(n, c)
+
+
+@pytest.mark.gpu
+def test_more_tiles_than_a_grid_holds():
+    """2^24 small maps: as many workgroups of 256 threads as no launch takes"""
+    from pixelssl_amd import functional as PF
+    n = 2 ** 24 + 3
+    x = torch.empty(n, 2, 2, 2, device="cuda").normal_(generator=torch.Generator("cuda").manual_seed(1))
+    w, b = torch.tensor([0.7, 1.3], device="cuda"), torch.tensor([0.2, -0.1], device="cuda")
+    y = PF.layer_norm_channels(x, w, b)
+    for part, want in zip(x.split(2 ** 21 - 1), y.split(2 ** 21 - 1)):
+        assert torch.equal(PF.layer_norm_channels(part, w, b), want)
+    x.requires_grad_(True)
+    dy = torch.ones_like(y)
+    dx, = torch.autograd.grad(PF.layer_norm_channels(x, w, b), x, dy)
+    last = x[-5:].detach().requires_grad_(True)
+    assert torch.equal(torch.autograd.grad(PF.layer_norm_channels(last, w, b), last, dy[-5:])[0], dx[-5:])
+
+
+@pytest.mark.gpu
+def test_as_many_channels_as_are_taken():
+    """2^24 channels at two positions, the parameters' gradients among what is checked"""
+    from pixelssl_amd import functional as PF
+    C = 2 ** 24
+    g = torch.Generator("cuda").manual_seed(2)
+    x, dy = (torch.empty(1, C, 2, device="cuda").normal_(generator=g) for _ in range(2))
+    w, b = torch.ones(C, device="cuda"), torch.zeros(C, device="cuda")
+    leaves = [t.requires_grad_(True) for t in (x, w, b)]
+    y = PF.layer_norm_channels(*leaves)
+    dx, dw, db = torch.autograd.grad(y, leaves, dy)
+    rows = lambda t: t.detach()[0].t().contiguous()
+    want = reference(rows(x), w.detach(), b.detach(), 1e-5, rows(dy))
+    for name, t in (("y", rows(y)), ("dx", rows(dx)), ("dw", dw), ("db", db)):
+        val, bound = want[name]
+        assert ((t.double() - val).abs() <= bound(0.0) + 1e-37).all(), name
