@@ -14,7 +14,7 @@
 // power of two that puts the largest possible entry (|x_ij| <= the spectral norm, which the coefficients bound from step to step)
 // under 2^15: 22 bits and more; a product is hi hi + hi lo + lo hi summed in fp32 -- 3 of the 16-bit instructions, five times the rate
 // of the fp32 ones.  A bf16 matrix scaled by a power of two IS one fp16 plane (8 of 11 bits), its norm's remainder is applied to A and
-// to the result.
+// to the result.  (A Muon step's update is a 32-bit matrix, of bf16 parameters too: two planes.)
 //
 // Measured (5 steps, us): 64 x 147 fp32 34, 23 x 256 x 2304 fp32 341, 23 x 1024 x 256 bf16 191, 2 x 2048 x 4608 fp32 2090 (0.77 PF of fp16
 // products against 1.09 of a large library product: power brings the clock from 2.4 to 1.7 - 1.8 GHz), Muon steps of 3 x 512 x 4608 350 and of
@@ -1547,10 +1547,10 @@ NsSplit ns_split_plan(std::vector<NsClass>& cls, int planes) {
 }
 
 // slots of a region: X and its successor, NP planes each, then A, T and three for Q / P
-int ns_plan(const char* what, int dtype, const pxl_ns_item* items, int n, NsPlan& plan) {
+int ns_plan(const char* what, int dtype, const pxl_ns_item* items, int n, int planes, NsPlan& plan) {
   PXL_REQUIRE(dtype == PXL_F32 || dtype == PXL_BF16, "%s: dtype %d is neither PXL_F32 nor PXL_BF16", what, dtype);
   PXL_REQUIRE(n >= 0 && n <= (1 << 22) && (n == 0 || items != nullptr), "%s: bad item list (%d matrices, at most 2^22)", what, n);
-  plan.np = dtype == PXL_F32 ? 2 : 1;
+  plan.np = planes;
   plan.xplanes = 2 * plan.np;
   std::vector<NsPlan::Set>& sets = plan.sets;
   for (int i = 0; i < n; ++i) {
@@ -1971,8 +1971,11 @@ int ns_overlap(const char* what, int dtype, const pxl_ns_item* items, int n, int
 
 int ns_run(const char* what, int dtype, const pxl_ns_item* items, int n, int steps, const float* coef, float eps, const MuonArgs& ma, int muon,
            void* ws, size_t ws_bytes, void* stream) {
+  // A bf16 matrix is one plane; the update of a Muon step is formed in 32 bits from a 32-bit momentum whatever the gradient's type, so two
+  // (rounded to one, 11 bits: the orthogonalised update of 256 x 1024 with six directions 50 times the noise is off by 2e-2)
+  const int planes = dtype == PXL_F32 || muon ? 2 : 1;
   NsPlan plan;
-  NS_TRY(ns_plan(what, dtype, items, n, plan));
+  NS_TRY(ns_plan(what, dtype, items, n, planes, plan));
   std::vector<NsStep> st;
   NS_TRY(ns_schedule(what, steps, coef, plan.np, st));
   PXL_REQUIRE(eps > 0.f, "%s: eps %g", what, eps);
@@ -2012,6 +2015,7 @@ int ns_run(const char* what, int dtype, const pxl_ns_item* items, int n, int ste
       }
     }
     if (dtype == PXL_F32) NS_TRY((ns_run_set<float, 2>(r, st, eps, ma, muon)));
+    else if (plan.np == 2) NS_TRY((ns_run_set<bf16_t, 2>(r, st, eps, ma, muon)));
     else NS_TRY((ns_run_set<bf16_t, 1>(r, st, eps, ma, muon)));
   }
   return PXL_OK;
@@ -2021,8 +2025,13 @@ int ns_run(const char* what, int dtype, const pxl_ns_item* items, int n, int ste
 
 extern "C" size_t pxl_ns_workspace(int dtype, const pxl_ns_item* items, int n) {
   try {
-    NsPlan plan;
-    return ns_plan("ns_workspace", dtype, items, n, plan) == PXL_OK ? plan.bytes : 0;
+    size_t bytes = 0;                   // (of either form: bf16 matrices run with one plane or two)
+    for (int planes = dtype == PXL_F32 ? 2 : 1; planes <= 2; ++planes) {
+      NsPlan plan;
+      if (ns_plan("ns_workspace", dtype, items, n, planes, plan) != PXL_OK) return 0;
+      bytes = std::max(bytes, plan.bytes);
+    }
+    return bytes;
   } catch (...) {
     return 0;
   }
