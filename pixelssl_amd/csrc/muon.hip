@@ -991,6 +991,7 @@ constexpr int NS_SLIM_P = 2 * 64 * 128;                              // P
 template <int NP, int MT, bool LAST, typename T>
 __device__ __forceinline__ void ns_slim_rows(const NsClass& c, const NsSlim& p, const NsItem& it, const float* __restrict__ residue, unsigned char* __restrict__ ws,
                                              unsigned char* lds, int i, int share) {
+  static_assert(LAST || NP == 2, "a single plane has one segment");
   constexpr int PL = 64 * 128;          // a plane of a wave's columns
   constexpr int mp = 32 * MT;
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), hi = lane >> 5;
@@ -1077,7 +1078,7 @@ __device__ __forceinline__ void ns_slim_rows(const NsClass& c, const NsSlim& p, 
             }
             const int q = cb * 32 + 8 * e4 + 4 * hi, o = chunk_at<64>(v * 32 + (lane & 31), q >> 3) + (q & 7) * 2;
             *reinterpret_cast<f16x4*>(x + o) = h;
-            if (NP == 2) *reinterpret_cast<f16x4*>(x + PL + o) = l;
+            *reinterpret_cast<f16x4*>(x + PL + o) = l;
           }
         }
       } else {
@@ -1138,10 +1139,8 @@ __device__ __forceinline__ void ns_slim_rows(const NsClass& c, const NsSlim& p, 
 #pragma unroll
         for (int b = 0; b < (MT == 2 ? 3 : 1); ++b) {
           const int bi = b > 0, bj = b == 2;
-          if (NP == 2) {
-            gram[b] = __builtin_amdgcn_mfma_f32_32x32x16_f16(r[bi][0], r[bj][NP - 1], gram[b], 0, 0, 0);
-            gram[b] = __builtin_amdgcn_mfma_f32_32x32x16_f16(r[bi][NP - 1], r[bj][0], gram[b], 0, 0, 0);
-          }
+          gram[b] = __builtin_amdgcn_mfma_f32_32x32x16_f16(r[bi][0], r[bj][NP - 1], gram[b], 0, 0, 0);
+          gram[b] = __builtin_amdgcn_mfma_f32_32x32x16_f16(r[bi][NP - 1], r[bj][0], gram[b], 0, 0, 0);
           gram[b] = __builtin_amdgcn_mfma_f32_32x32x16_f16(r[bi][0], r[bj][0], gram[b], 0, 0, 0);
         }
       }
@@ -1406,7 +1405,7 @@ __global__ __launch_bounds__(512) void ns_tiny_kernel(NsClasses cs, NsTiny p, Ns
 #pragma unroll
         for (int e4 = 0; e4 < 4; ++e4) {
           const int q = nblk * 32 + 8 * e4 + 4 * hi;
-          if (!done) {
+          if (NP == 2 && !done) {        // (a single plane has one segment)
             f16x4 h, l;
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
@@ -1415,7 +1414,7 @@ __global__ __launch_bounds__(512) void ns_tiny_kernel(NsClasses cs, NsTiny p, Ns
               l[e] = (_Float16)(w - (float)h[e]);
             }
             *reinterpret_cast<f16x4*>(x + xat(r, q)) = h;
-            if (NP == 2) *reinterpret_cast<f16x4*>(x + plane + xat(r, q)) = l;
+            *reinterpret_cast<f16x4*>(x + plane + xat(r, q)) = l;
           } else if (r < c.m) {
             T* o = reinterpret_cast<T*>(it.p);
             const float f = p.muon ? -p.lr * it.scale : 1.f;
@@ -1546,12 +1545,13 @@ NsSplit ns_split_plan(std::vector<NsClass>& cls, int planes) {
   return r;
 }
 
-// slots of a region: X and its successor, NP planes each, then A, T and three for Q / P
+// slots of a region: X and its successor, two planes each (of a single plane, with one segment: X alone), then A, T and three for Q / P
+constexpr int ns_xplanes(int planes) { return planes == 2 ? 4 : 1; }
 int ns_plan(const char* what, int dtype, const pxl_ns_item* items, int n, int planes, NsPlan& plan) {
   PXL_REQUIRE(dtype == PXL_F32 || dtype == PXL_BF16, "%s: dtype %d is neither PXL_F32 nor PXL_BF16", what, dtype);
   PXL_REQUIRE(n >= 0 && n <= (1 << 22) && (n == 0 || items != nullptr), "%s: bad item list (%d matrices, at most 2^22)", what, n);
   plan.np = planes;
-  plan.xplanes = 2 * plan.np;
+  plan.xplanes = ns_xplanes(planes);
   std::vector<NsPlan::Set>& sets = plan.sets;
   for (int i = 0; i < n; ++i) {
     PXL_REQUIRE(items[i].rows >= 1 && items[i].cols >= 1 && items[i].rows <= (1 << 23) && items[i].cols <= (1 << 23) &&
@@ -1829,7 +1829,8 @@ int ns_run_tiny(NsRun& r, const std::vector<NsStep>& steps, float eps, const Muo
 template <typename T, int NP>
 int ns_run_set(NsRun& r, const std::vector<NsStep>& steps, float eps, const MuonArgs& ma, int muon) {
   if (r.split.tiny) return ns_run_tiny<T, NP>(r, steps, eps, ma, muon);
-  const int xplanes = 2 * NP, MA = xplanes, MT = xplanes + 1;
+  constexpr int xplanes = ns_xplanes(NP);
+  const int MA = xplanes, MT = xplanes + 1;
   int blocks = 0;
   for (int k = 0; k < r.cs.n; ++k) {
     NsClass& c = r.cs.c[k];
@@ -1927,7 +1928,7 @@ int ns_run_set(NsRun& r, const std::vector<NsStep>& steps, float eps, const Muon
       g.decay = ma.keep;
       if (slim) NS_TRY((ns_slim<NP, true, T>(r, g)));
       else NS_TRY((ns_gemm<EPI_OUT, 2, NP, T>(r, g)));
-    } else {
+    } else if constexpr (NP == 2) {
       const float sx2 = plane_scale(steps[s].sigma);
       g.job[0] = {P, x, x2};
       g.scale[0] = sx2;
@@ -1972,12 +1973,18 @@ int ns_overlap(const char* what, int dtype, const pxl_ns_item* items, int n, int
 int ns_run(const char* what, int dtype, const pxl_ns_item* items, int n, int steps, const float* coef, float eps, const MuonArgs& ma, int muon,
            void* ws, size_t ws_bytes, void* stream) {
   // A bf16 matrix is one plane; the update of a Muon step is formed in 32 bits from a 32-bit momentum whatever the gradient's type, so two
-  // (rounded to one, 11 bits: the orthogonalised update of 256 x 1024 with six directions 50 times the noise is off by 2e-2)
-  const int planes = dtype == PXL_F32 || muon ? 2 : 1;
+  // (rounded to one, 11 bits: the orthogonalised update of 256 x 1024 with six directions 50 times the noise is off by 2e-2).  Nor is X a bf16
+  // matrix any more behind a first segment: steps that do not fit into one run as those of 32-bit matrices
+  int planes = dtype == PXL_F32 || muon ? 2 : 1;
+  std::vector<NsStep> st;
+  NS_TRY(ns_schedule(what, steps, coef, planes, st));
+  if (planes == 1 && std::any_of(st.begin(), st.end() - 1, [](const NsStep& d) { return d.last; })) {
+    planes = 2;
+    st.clear();
+    NS_TRY(ns_schedule(what, steps, coef, planes, st));
+  }
   NsPlan plan;
   NS_TRY(ns_plan(what, dtype, items, n, planes, plan));
-  std::vector<NsStep> st;
-  NS_TRY(ns_schedule(what, steps, coef, plan.np, st));
   PXL_REQUIRE(eps > 0.f, "%s: eps %g", what, eps);
   for (int i = 0; i < n; ++i)
     PXL_REQUIRE(items[i].p != nullptr && items[i].g != nullptr && (!muon || items[i].mom != nullptr), "%s: item %d has a null pointer", what, i);

@@ -45,3 +45,13 @@ def test_the_workspace_serves_both_forms():
     for rows, cols in SHAPES + [(2048, 4608)]:
         items = (_lib.NsItem * 3)(*[(1, 1, 1, rows, cols, 1.0, 0)] * 3)
         assert h.pxl_ns_workspace(1, items, 3) >= h.pxl_ns_workspace(0, items, 3)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("steps", [6, 7, 10])
+@pytest.mark.parametrize("shape", SHAPES, ids=lambda s: "x".join(map(str, s)))
+def test_steps_past_one_segment_are_the_32_bit_steps_rounded_once(shape, steps):
+    """between two segments the iterate is no bf16 matrix any more"""
+    from pixelssl_amd import functional as PF
+    x = strong(shape, steps, 0.5).bfloat16().cuda()
+    assert torch.equal(PF.orthogonalize(x, steps=steps), PF.orthogonalize(x.float(), steps=steps).bfloat16())
