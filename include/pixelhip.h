@@ -906,7 +906,9 @@ typedef struct pxl_ns_item {
 /* items: HOST array; n <= 2^22 matrices of any mix of shapes, none of which overlap (p of one against anything of another); p == g is allowed
  * in pxl_orthogonalize.  coef: HOST array [steps][3], 1 .. 16 steps;
  *   X = G / max(|G|_F, eps);  per step  X <- a X + (b L + c L^2) X,  L = X X'  (of the transposed matrix when rows > cols)
- * fp32 results: every product to 22 bits and more, sums in fp32;  bf16: the result rounded once.  Coefficients that let singular values in
+ * Products to 22 bits of every entry down to 2^-17 of the matrix' largest possible one (X's: its norm, or eps), to 2^-39 of that below; sums in
+ * fp32.  bf16 results are rounded once; in steps that run as one segment (5 of the usual coefficients) they are off by up to 8e-4 of their norm
+ * before that.  A Muon step is computed as in fp32 whatever its parameters' type.  Coefficients that let singular values in
  * [0, 1] grow past 16 are refused.
  * pxl_muon_step:  mom <- momentum * mom + (1 - momentum) * g;  u = nesterov ? (1 - momentum) * g + momentum * mom : mom;
  *                 p <- p * (1 - lr * weight_decay) - lr * scale * orthogonalised(u)
