@@ -380,9 +380,13 @@ def _ns_coefficients(steps, coefficients):
     return (ctypes.c_float * len(flat))(*flat)
 
 
+def _coefficient_key(coefficients):
+    """one (a, b, c) or one per step, as nested tuples whatever sequences they came in"""
+    return tuple(tuple(float(v) for v in t) if isinstance(t, (tuple, list)) else float(t) for t in coefficients)
+
+
 def _coefficients(steps, coefficients):
-    c = tuple(tuple(t) if isinstance(t, (tuple, list)) else float(t) for t in coefficients)
-    return _ns_coefficients(int(steps), c)
+    return _ns_coefficients(int(steps), _coefficient_key(coefficients))
 
 
 def orthogonalize(x, steps=5, coefficients=NEWTON_SCHULZ, eps=1e-7):

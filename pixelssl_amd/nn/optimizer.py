@@ -623,7 +623,8 @@ class FusedMuon(_FlatStateMixin, Optimizer):
                     entry = tuple(self._slot(getattr(ref[0], k), p) for k in ('params', 'grads') + tuple(a for _, a in self._keys_of(p)))
                 if matrix:
                     scale = PF.muon_scale(p.shape, group['adjust_lr'])
-                    key = tuple(group[k] for k in ('lr', 'momentum', 'nesterov', 'weight_decay', 'ns_steps', 'ns_coefficients', 'ns_eps'))
+                    key = (float(group['lr']), float(group['momentum']), bool(group['nesterov']), float(group['weight_decay']), int(group['ns_steps']),
+                           PF._coefficient_key(group['ns_coefficients']), float(group['ns_eps']))
                     calls.setdefault(key, []).append(entry + (scale,))
                 else:
                     vectors.append(entry)
