@@ -919,6 +919,9 @@ int pxl_orthogonalize(int dtype, const pxl_ns_item* items, int n, int steps, con
                       void* stream);
 int pxl_muon_step(int dtype, const pxl_ns_item* items, int n, int steps, const float* coef, float eps, double lr, double momentum, int nesterov,
                   double weight_decay, void* ws, size_t ws_bytes, void* stream);
+/* what pxl_muon_step / pxl_adam_list would refuse about these arguments, the workspace apart; nothing is launched.  For a step of several calls that
+ * is to happen as a whole or not at all. */
+int pxl_muon_check(int dtype, const pxl_ns_item* items, int n, int steps, const float* coef, float eps, double lr, double momentum, double weight_decay);
 
 /* pxl_adam_step without weight decay on n tensors, 40 to a launch: the vectors that the Muon optimizer leaves to Adam.  items: HOST array,
  * copied at the call; p / g of type dtype, moments fp32; p and moments of one may overlap nothing of the call. */
@@ -929,6 +932,7 @@ typedef struct pxl_adam_item {
   float* exp_avg_sq;
   int64_t n;
 } pxl_adam_item;
+int pxl_adam_check(int dtype, const pxl_adam_item* items, int n, double beta1, double beta2, double eps, int step);
 int pxl_adam_list(int dtype, const pxl_adam_item* items, int n, double lr, double beta1, double beta2, double eps, int step, void* stream);
 
 #ifdef __cplusplus

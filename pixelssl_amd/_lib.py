@@ -292,6 +292,8 @@ SIGNATURES = {
     "pxl_ns_workspace": (_Z, [_I, _P, _I]),
     "pxl_orthogonalize": (_I, [_I, _P, _I, _I, _P, _F, _P, _Z, _P]),
     "pxl_muon_step": (_I, [_I, _P, _I, _I, _P, _F, C.c_double, C.c_double, _I, C.c_double, _P, _Z, _P]),
+    "pxl_muon_check": (_I, [_I, _P, _I, _I, _P, _F, C.c_double, C.c_double, C.c_double]),
+    "pxl_adam_check": (_I, [_I, _P, _I, C.c_double, C.c_double, C.c_double, _I]),
     "pxl_adam_list": (_I, [_I, _P, _I, C.c_double, C.c_double, C.c_double, C.c_double, _I, _P]),
     "pxl_net_backward": (_I, [_P, _P, _P, _P, _P, _P, _P, _P, _Z, _P, _Z, _I, _P]),
 }

@@ -1973,26 +1973,33 @@ int ns_overlap(const char* what, int dtype, const pxl_ns_item* items, int n, int
   return PXL_OK;
 }
 
-int ns_run(const char* what, int dtype, const pxl_ns_item* items, int n, int steps, const float* coef, float eps, const MuonArgs& ma, int muon,
-           void* ws, size_t ws_bytes, void* stream) {
+// everything about a call but its workspace; nothing is launched
+int ns_check(const char* what, int dtype, const pxl_ns_item* items, int n, int steps, const float* coef, float eps, int muon, NsPlan& plan,
+             std::vector<NsStep>& st) {
   // A bf16 matrix is one plane; the update of a Muon step is formed in 32 bits from a 32-bit momentum whatever the gradient's type, so two
   // (rounded to one, 11 bits: the orthogonalised update of 256 x 1024 with six directions 50 times the noise is off by 2e-2).  Nor is X a bf16
   // matrix any more behind a first segment: steps that do not fit into one run as those of 32-bit matrices
   int planes = dtype == PXL_F32 || muon ? 2 : 1;
-  std::vector<NsStep> st;
   NS_TRY(ns_schedule(what, steps, coef, planes, st));
   if (planes == 1 && std::any_of(st.begin(), st.end() - 1, [](const NsStep& d) { return d.last; })) {
     planes = 2;
     st.clear();
     NS_TRY(ns_schedule(what, steps, coef, planes, st));
   }
-  NsPlan plan;
   NS_TRY(ns_plan(what, dtype, items, n, planes, plan));
   PXL_REQUIRE(eps > 0.f, "%s: eps %g", what, eps);
   for (int i = 0; i < n; ++i)
     PXL_REQUIRE(items[i].p != nullptr && items[i].g != nullptr && (!muon || items[i].mom != nullptr), "%s: item %d has a null pointer", what, i);
+  if (n > 0) NS_TRY(ns_overlap(what, dtype, items, n, muon));
+  return PXL_OK;
+}
+
+int ns_run(const char* what, int dtype, const pxl_ns_item* items, int n, int steps, const float* coef, float eps, const MuonArgs& ma, int muon,
+           void* ws, size_t ws_bytes, void* stream) {
+  NsPlan plan;
+  std::vector<NsStep> st;
+  NS_TRY(ns_check(what, dtype, items, n, steps, coef, eps, muon, plan, st));
   if (n == 0) return PXL_OK;
-  NS_TRY(ns_overlap(what, dtype, items, n, muon));
   if (ws == nullptr || ws_bytes < plan.bytes)
     return pxl_set_error(PXL_ERR_WORKSPACE, "%s: workspace of %zu bytes, %zu needed", what, ws_bytes, plan.bytes);
   NsRun r;
@@ -2056,10 +2063,27 @@ extern "C" int pxl_orthogonalize(int dtype, const pxl_ns_item* items, int n, int
   }
 }
 
-extern "C" int pxl_muon_step(int dtype, const pxl_ns_item* items, int n, int steps, const float* coef, float eps, double lr, double momentum,
-                             int nesterov, double weight_decay, void* ws, size_t ws_bytes, void* stream) {
+static int muon_scalars(double lr, double momentum, double weight_decay) {
   if (!(momentum >= 0.0 && momentum < 1.0) || !std::isfinite(lr) || !std::isfinite(weight_decay))
     return pxl_set_error(PXL_ERR_ARG, "muon_step: lr %g, momentum %g (0 <= momentum < 1), weight decay %g", lr, momentum, weight_decay);
+  return PXL_OK;
+}
+
+extern "C" int pxl_muon_check(int dtype, const pxl_ns_item* items, int n, int steps, const float* coef, float eps, double lr, double momentum,
+                              double weight_decay) {
+  NS_TRY(muon_scalars(lr, momentum, weight_decay));
+  try {
+    NsPlan plan;
+    std::vector<NsStep> st;
+    return ns_check("muon_step", dtype, items, n, steps, coef, eps, 1, plan, st);
+  } catch (...) {
+    return pxl_set_error(PXL_ERR_ARG, "muon_step: out of host memory");
+  }
+}
+
+extern "C" int pxl_muon_step(int dtype, const pxl_ns_item* items, int n, int steps, const float* coef, float eps, double lr, double momentum,
+                             int nesterov, double weight_decay, void* ws, size_t ws_bytes, void* stream) {
+  NS_TRY(muon_scalars(lr, momentum, weight_decay));
   try {
     return ns_run("muon_step", dtype, items, n, steps, coef, eps, MuonArgs{(float)lr, (float)momentum, (float)(1.0 - momentum), (float)(1.0 - lr * weight_decay), nesterov}, 1, ws, ws_bytes, stream);
   } catch (...) {

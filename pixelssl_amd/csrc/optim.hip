@@ -311,18 +311,22 @@ static int adam_overlap(int dtype, const pxl_adam_item* items, int n) {
   return PXL_OK;
 }
 
-extern "C" int pxl_adam_list(int dtype, const pxl_adam_item* items, int n, double lr, double beta1, double beta2, double eps, int step, void* stream) {
+extern "C" int pxl_adam_check(int dtype, const pxl_adam_item* items, int n, double beta1, double beta2, double eps, int step) {
   PXL_REQUIRE(dtype == PXL_F32 || dtype == PXL_BF16, "adam_list: dtype %d is neither PXL_F32 nor PXL_BF16", dtype);
   PXL_REQUIRE(n >= 0 && (n == 0 || items != nullptr) && step >= 1 && beta1 >= 0 && beta1 < 1 && beta2 >= 0 && beta2 < 1 && eps > 0,
               "adam_list: bad argument (step counts from 1)");
   for (int k = 0; k < n; ++k)
     PXL_REQUIRE(items[k].p && items[k].g && items[k].exp_avg && items[k].exp_avg_sq && items[k].n >= 1, "adam_list: item %d: null pointer or no elements", k);
   try {
-    const int rc = adam_overlap(dtype, items, n);
-    if (rc != PXL_OK) return rc;
+    return adam_overlap(dtype, items, n);
   } catch (...) {
     return pxl_set_error(PXL_ERR_ARG, "adam_list: out of host memory");
   }
+}
+
+extern "C" int pxl_adam_list(int dtype, const pxl_adam_item* items, int n, double lr, double beta1, double beta2, double eps, int step, void* stream) {
+  const int rc = pxl_adam_check(dtype, items, n, beta1, beta2, eps, step);
+  if (rc != PXL_OK) return rc;
   const double bc1 = 1.0 - pow(beta1, step), bc2 = 1.0 - pow(beta2, step);
   for (int at = 0; at < n; at += 40) {
     AdamList list;

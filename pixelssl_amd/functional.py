@@ -2,6 +2,7 @@
 orthogonalised updates of weight matrices."""
 import ctypes
 import functools
+import threading
 
 import torch
 from torch.autograd import forward_ad
@@ -289,6 +290,32 @@ def _launch(index, fn, *args):
         check(rc)
 
 
+_held = threading.local()
+
+
+class _AllOrNothing:
+    """`with _AllOrNothing():` -- the updates called inside check their arguments there and are launched together at the end; an exception, and
+    none of them is."""
+
+    def __enter__(self):
+        self.outer, _held.calls = getattr(_held, "calls", None), []
+
+    def __exit__(self, kind, *_):
+        calls, _held.calls = _held.calls, self.outer
+        if kind is None:
+            _submit(calls)
+
+
+def _submit(calls):
+    """calls: (device index, C function, arguments, what has to live until the launch), all checked; launched one after the other"""
+    held = getattr(_held, "calls", None)
+    if held is not None:
+        held += calls
+        return
+    for index, fn, args, _ in calls:
+        _launch(index, fn, *args)
+
+
 def _refuse_recording(name, *tensors):
     """A recorder (torch.jit.trace, make_fx) sees the allocations of a call but not its kernels: what it made would return what the memory held
     before.  torch.func's wrappers have no memory, and a forward-mode tangent would stop at the outputs without a word."""
@@ -412,16 +439,18 @@ def orthogonalize(x, steps=5, coefficients=NEWTON_SCHULZ, eps=1e-7):
         src, dst = x.data_ptr(), out.data_ptr()
         n = x.numel() // (rows * cols)
         items = (_lib.NsItem * n)(*[(dst + k * size, src + k * size, None, rows, cols, 1.0, 0) for k in range(n)])
-        _run_ns(lib().pxl_orthogonalize, x.device, dtype_code(x.dtype), items, n, steps, coef, eps)
+        index, fn, args, ws = _ns_call(lib().pxl_orthogonalize, x.device, dtype_code(x.dtype), items, n, steps, coef, eps)
+        _launch(index, fn, *args)
     return out
 
 
-def _run_ns(fn, dev, code, items, n, steps, coef, eps, *scalars):
+def _ns_call(fn, dev, code, items, n, steps, coef, eps, *scalars):
+    """one call with its workspace, as _submit takes it"""
     nbytes = lib().pxl_ns_workspace(code, items, n)
     if nbytes == 0:
         raise _lib.PixelHipError("libpixelhip: %s" % lib().pxl_last_error().decode())
     ws = torch.empty(nbytes, device=dev, dtype=torch.uint8)
-    _launch(dev.index, fn, code, items, n, int(steps), coef, float(eps), *scalars, ptr(ws), nbytes)
+    return dev.index, fn, (code, items, n, int(steps), coef, float(eps)) + scalars + (ptr(ws), nbytes), ws
 
 
 def _dense_strides(t):
@@ -455,8 +484,8 @@ def muon_update(params, grads, momenta, lr, momentum=0.95, nesterov=True, weight
         u = (1 - momentum) * grad_k + momentum * momentum_k  (nesterov)  or  momentum_k
         param_k <- param_k * (1 - lr * weight_decay) - lr * muon_scale(...) * orthogonalize(u)
     adjust: the rule of muon_scale, or one factor per parameter in its place.  params / grads fp32 or bf16 (one type per parameter), momenta
-    fp32 with the parameter's memory layout (contiguous or channels last).  Parameters and momenta may overlap nothing.  Refusals that need
-    no look at memory come before anything is changed."""
+    fp32 with the parameter's memory layout (contiguous or channels last).  Parameters and momenta may overlap nothing.  What is refused is
+    refused before anything is changed."""
     params, grads, momenta = list(params), list(grads), list(momenta)
     _refuse_recording("muon_update", *params, *grads, *momenta)
     if not len(params) == len(grads) == len(momenta):
@@ -491,16 +520,21 @@ def muon_update(params, grads, momenta, lr, momentum=0.95, nesterov=True, weight
             scales[shape] = (shape[0], p.numel() // shape[0], muon_scale(shape, adjust) if named else 0.0, 0)
         geo = scales[shape] if named else scales[shape][:2] + (float(adjust[k]), 0)
         work.setdefault((p.device, p.dtype), []).append((p.data_ptr(), g.data_ptr(), m.data_ptr()) + geo)
+    calls = []
     for (dev, dtype), entries in work.items():
-        _run_ns(lib().pxl_muon_step, dev, dtype_code(dtype), (_lib.NsItem * len(entries))(*entries), len(entries), steps, coef, eps, lr, momentum,
-                int(bool(nesterov)), weight_decay)
+        items, n = (_lib.NsItem * len(entries))(*entries), len(entries)
+        check(lib().pxl_muon_check(dtype_code(dtype), items, n, int(steps), coef, float(eps), lr, momentum, weight_decay))
+        index, fn, args, ws = _ns_call(lib().pxl_muon_step, dev, dtype_code(dtype), items, n, steps, coef, eps, lr, momentum, int(bool(nesterov)), weight_decay)
+        calls.append((index, fn, args, (ws, keep)))
+    _submit(calls)
     torch.autograd.graph.increment_version([t for t in params + momenta if t.numel()])
 
 
 def adam_update(params, grads, exp_avgs, exp_avg_sqs, lr, betas=(0.9, 0.999), eps=1e-8, step=1):
     """torch.optim.Adam's update without weight decay (FusedAdam's arithmetic) on lists of tensors, in place, many in one launch: the
     vectors beside muon_update's matrices.  params / grads fp32 or bf16, exp_avgs / exp_avg_sqs fp32, all four of an entry dense and
-    alike in memory (a gradient may lie otherwise).  Parameters and moments may overlap nothing.  step counts from 1."""
+    alike in memory (a gradient may lie otherwise).  Parameters and moments may overlap nothing.  step counts from 1.  What is refused is refused
+    before anything is changed."""
     params, grads, exp_avgs, exp_avg_sqs = list(params), list(grads), list(exp_avgs), list(exp_avg_sqs)
     _refuse_recording("adam_update", *params, *grads, *exp_avgs, *exp_avg_sqs)
     if not len(params) == len(grads) == len(exp_avgs) == len(exp_avg_sqs):
@@ -527,7 +561,10 @@ def adam_update(params, grads, exp_avgs, exp_avg_sqs, lr, betas=(0.9, 0.999), ep
             keep.append(g)
         work.setdefault((p.device, p.dtype), []).append((p.data_ptr(), g.data_ptr(), m.data_ptr(), v.data_ptr(), p.numel()))
         touched += [p, m, v]
+    calls = []
     for (dev, dtype), entries in work.items():
-        _launch(dev.index, lib().pxl_adam_list, dtype_code(dtype), (_lib.AdamItem * len(entries))(*entries), len(entries), float(lr), b1, b2, float(eps),
-                int(step))
+        items, n = (_lib.AdamItem * len(entries))(*entries), len(entries)
+        check(lib().pxl_adam_check(dtype_code(dtype), items, n, b1, b2, float(eps), int(step)))
+        calls.append((dev.index, lib().pxl_adam_list, (dtype_code(dtype), items, n, float(lr), b1, b2, float(eps), int(step)), keep))
+    _submit(calls)
     torch.autograd.graph.increment_version(touched)

@@ -601,8 +601,20 @@ class FusedMuon(_FlatStateMixin, Optimizer):
             with torch.enable_grad():
                 loss = closure()
         _sync_foreign_grads(self._foreign)
+        with PF._AllOrNothing():        # (a step that is refused has moved nothing)
+            self._update(PF, self._step + 1)
         self._step += 1
         self._steps_taken = self._step
+        for foreign in self._foreign:
+            for p in foreign:
+                if p.grad is not None:
+                    self.state[p]['step'] = torch.tensor(float(self._step))
+        for store in self._stores.values():
+            store.touch()
+        return loss
+
+    def _update(self, PF, step):
+        """the vectors' and the matrices' updates of all groups as step number `step`"""
         calls = {}                      # settings -> the matrices that share them
         for group in self.param_groups:
             b1, b2 = group['betas']
@@ -617,7 +629,6 @@ class FusedMuon(_FlatStateMixin, Optimizer):
                     for k, _ in self._keys_of(p):
                         if st.get(k) is None:
                             st[k] = torch.zeros_like(p, dtype=torch.float32)
-                    st['step'] = torch.tensor(float(self._step))
                     entry = (p, p.grad) + tuple(st[k] for k, _ in self._keys_of(p))
                 else:
                     entry = tuple(self._slot(getattr(ref[0], k), p) for k in ('params', 'grads') + tuple(a for _, a in self._keys_of(p)))
@@ -629,14 +640,11 @@ class FusedMuon(_FlatStateMixin, Optimizer):
                 else:
                     vectors.append(entry)
             if vectors:
-                PF.adam_update(*zip(*vectors), lr=float(group['lr']) * float(group['vector_scale']), betas=(b1, b2), eps=group['eps'], step=self._step)
+                PF.adam_update(*zip(*vectors), lr=float(group['lr']) * float(group['vector_scale']), betas=(b1, b2), eps=group['eps'], step=step)
         for (lr, momentum, nesterov, wd, steps, coefs, eps), entries in calls.items():
             p, g, m, scales = zip(*entries)
             PF.muon_update(p, g, m, lr=lr, momentum=momentum, nesterov=nesterov, weight_decay=wd, steps=steps, coefficients=coefs, eps=eps,
                            adjust=scales)
-        for store in self._stores.values():
-            store.touch()
-        return loss
 
     def zero_grad(self, set_to_none=False):
         for store in self._stores.values():
