@@ -3,6 +3,7 @@ against torch's headers), in-tree.
 
     python -m pixelssl_amd.build            # incremental
     python -m pixelssl_amd.build --force
+    python -m pixelssl_amd.build --library  # libpixelhip.so alone: what a user of the C ABI needs (no g++, no torch headers)
 
 hipcc cross-compiles without a GPU; the resulting .so is git-ignored but travels with the
 snapshot to the GPU box (it is NOT listed in .gpurunignore).
@@ -53,10 +54,11 @@ NODE_SRC = os.path.join(HERE, "node", "layer_norm_node.cpp")
 NODE_LIB = os.path.join(HERE, "_pxlnode.so")
 
 
+NODE_STAMP = os.path.join(OBJDIR, "_pxlnode.cmd")       # what _pxlnode.so was compiled with: torch's version among it
+
+
 def _build_node(force):
     """host code only: the kernels are reached through addresses that functional.py hands over, so libpixelhip.so is loaded once"""
-    if not force and not _stale(NODE_LIB, [NODE_SRC] + HEADERS):
-        return False
     import sysconfig
     import torch
     from torch.utils import cpp_extension
@@ -66,32 +68,46 @@ def _build_node(force):
     for d in cpp_extension.include_paths() + [sysconfig.get_paths()["include"], "/opt/rocm/include"]:
         cmd += ["-isystem", d]
     cmd += ["-L" + libdir] + ["-l" + n for n in ("c10", "torch_cpu", "torch_python", "c10_hip", "torch_hip")]
+    stamp = "torch %s\n%s\n" % (torch.__version__, "\n".join(cmd))
+    if not force and not _stale(NODE_LIB, [NODE_SRC] + HEADERS) and _read(NODE_STAMP) == stamp:
+        return False
     r = subprocess.run(cmd, capture_output=True, text=True)
     if r.returncode != 0:
         raise RuntimeError("compiling %s failed:\n%s\n%s" % (NODE_SRC, r.stdout, r.stderr))
+    with open(NODE_STAMP, "w") as f:
+        f.write(stamp)
     return True
 
 
-def build(force=False, verbose=True):
+def _read(path):
+    try:
+        with open(path) as f:
+            return f.read()
+    except OSError:
+        return None
+
+
+def build(force=False, verbose=True, node=True):
+    """the library, and with `node` the autograd nodes: compiled beside it, but nothing that goes wrong with them keeps the library from being linked"""
     os.makedirs(OBJDIR, exist_ok=True)
     srcs = sources()
     with ThreadPoolExecutor(max_workers=min(8, len(srcs) + 1)) as ex:
-        node = ex.submit(_build_node, force)
+        nodes = ex.submit(_build_node, force) if node else None
         results = list(ex.map(lambda s: _compile(s, force), srcs))
-        if node.result() and verbose:
+        objs = [o for o, _ in results]
+        if force or any(c for _, c in results) or _stale(LIB, objs):
+            cmd = [HIPCC, "--offload-arch=" + ARCH, "-shared", "-fPIC", "-o", LIB] + objs
+            r = subprocess.run(cmd, capture_output=True, text=True)
+            if r.returncode != 0:
+                raise RuntimeError("link failed:\n%s\n%s" % (r.stdout, r.stderr))
+            if verbose:
+                print("built", LIB)
+        elif verbose:
+            print("up to date:", LIB)
+        if nodes is not None and nodes.result() and verbose:
             print("built", NODE_LIB)
-    objs = [o for o, _ in results]
-    if force or any(c for _, c in results) or _stale(LIB, objs):
-        cmd = [HIPCC, "--offload-arch=" + ARCH, "-shared", "-fPIC", "-o", LIB] + objs
-        r = subprocess.run(cmd, capture_output=True, text=True)
-        if r.returncode != 0:
-            raise RuntimeError("link failed:\n%s\n%s" % (r.stdout, r.stderr))
-        if verbose:
-            print("built", LIB)
-    elif verbose:
-        print("up to date:", LIB)
     return LIB
 
 
 if __name__ == "__main__":
-    build(force="--force" in sys.argv)
+    build(force="--force" in sys.argv, node="--library" not in sys.argv)
