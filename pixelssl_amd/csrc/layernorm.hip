@@ -504,7 +504,10 @@ __global__ __launch_bounds__(THREADS) void ln_chan_fwd(int first, int per, int C
   }
 }
 
-template <typename T, int THREADS, int TSV, int NV>
+// FULL: every thread has NV channels.  Else what channels past the end would add to the sums is replaced by 0 (times a weight of 0, an infinite
+// dy of the last channel made every channel's sums NaN): forward + backward of 8 x 2000 x 65 x 65 bf16 272 us, 268 without; replaced where dy is
+// loaded or unpacked, in all threads, it cost registers (8 x 2048 x 65 x 65 289 - 300 us, so 270).
+template <typename T, int THREADS, int TSV, int NV, bool FULL>
 __global__ __launch_bounds__(THREADS) void ln_chan_bwd(int tiles, int per, int C, int S, const T* __restrict__ x, const T* __restrict__ dy, LnParam w,
                                                        const float* __restrict__ mean, const float* __restrict__ rstd, T* __restrict__ dx,
                                                        float* __restrict__ part) {
@@ -557,8 +560,9 @@ __global__ __launch_bounds__(THREADS) void ln_chan_bwd(int tiles, int per, int C
         const float own = e >= dup ? d[e] : 0.f;          // a position that the piece before holds too counts there
         aw[j] += e >= dup ? d[e] * u[e] : 0.f;
         ab[j] += own;
-        s[0][e] += d[e] * wj;
-        s[1][e] += d[e] * wj * u[e];
+        const float gj = FULL || j * CY + cy < C ? d[e] * wj : 0.f;
+        s[0][e] += gj;
+        s[1][e] += gj * u[e];
       }
       // every sum is taken here: left to the compiler, some sink to the loop's end and keep all pieces unpacked until then (196 registers, 144 so)
       asm volatile("" : "+v"(aw[j]), "+v"(ab[j]));
@@ -715,18 +719,25 @@ inline LnShape ln_shape(int dtype, long R, int C, long S) { return S < 0 ? ln_ro
   } while (0)
 // Backward (H = 2), which holds x and dy: 8 channels a thread and more go to twice the threads with half of them each (8 x 256 x 129 x 129 fp32
 // 100 us, with 8 a thread 109; 8 x 2048 x 65 x 65 bf16 180 us, with 16 a thread 194; forward the other way round, 87 with 16 and 104 with 8)
-#define LN_CHAN(KERNEL, H, BLOCKS, ...)                                                                                              \
+#define LN_CHAN_FWD(TH, TSV, NV, ...) hipLaunchKernelGGL((ln_chan_fwd<T, TH, TSV, NV>), grid, dim3(TH), 0, st, __VA_ARGS__)
+#define LN_CHAN_BWD(TH, TSV, NV, ...)                                                                                                \
+  do {                                                                                                                               \
+    if (C == TH / TSV * NV) hipLaunchKernelGGL((ln_chan_bwd<T, TH, TSV, NV, true>), grid, dim3(TH), 0, st, __VA_ARGS__);             \
+    else hipLaunchKernelGGL((ln_chan_bwd<T, TH, TSV, NV, false>), grid, dim3(TH), 0, st, __VA_ARGS__);                               \
+  } while (0)
+#define LN_CHAN(LAUNCH, H, BLOCKS, ...)                                                                                              \
   do {                                                                                                                               \
     const dim3 grid(BLOCKS);                                                                                                         \
     if (s.tsv == 8) {                                                                                                                \
-      if (s.nv == 1) hipLaunchKernelGGL((KERNEL<T, 256, 8, 1>), grid, dim3(256), 0, st, __VA_ARGS__);                                \
-      else if (s.nv == 2) hipLaunchKernelGGL((KERNEL<T, 256, 8, 2>), grid, dim3(256), 0, st, __VA_ARGS__);                           \
-      else if (s.nv == 4) hipLaunchKernelGGL((KERNEL<T, 256, 8, 4>), grid, dim3(256), 0, st, __VA_ARGS__);                           \
-      else hipLaunchKernelGGL((KERNEL<T, 256 * H, 8, 8 / H>), grid, dim3(256 * H), 0, st, __VA_ARGS__);                              \
-    } else if (s.threads == 256) hipLaunchKernelGGL((KERNEL<T, 256 * H, 4, 8 / H>), grid, dim3(256 * H), 0, st, __VA_ARGS__);        \
-    else if (s.nv == 8) hipLaunchKernelGGL((KERNEL<T, 512 * H, 4, 8 / H>), grid, dim3(512 * H), 0, st, __VA_ARGS__);                 \
-    else hipLaunchKernelGGL((KERNEL<T, 512 * H, 4, 16 / H>), grid, dim3(512 * H), 0, st, __VA_ARGS__);                               \
+      if (s.nv == 1) LAUNCH(256, 8, 1, __VA_ARGS__);                                                                                 \
+      else if (s.nv == 2) LAUNCH(256, 8, 2, __VA_ARGS__);                                                                            \
+      else if (s.nv == 4) LAUNCH(256, 8, 4, __VA_ARGS__);                                                                            \
+      else LAUNCH((256 * H), 8, (8 / H), __VA_ARGS__);                                                                               \
+    } else if (s.threads == 256) LAUNCH((256 * H), 4, (8 / H), __VA_ARGS__);                                                         \
+    else if (s.nv == 8) LAUNCH((512 * H), 4, (8 / H), __VA_ARGS__);                                                                  \
+    else LAUNCH((512 * H), 4, (16 / H), __VA_ARGS__);                                                                                \
   } while (0)
+
 // Channels beyond the register kernels: up to 16 of them one thread a position, more 8 positions a workgroup (forward + backward of 2^18 maps of
 // 2 positions, us, one thread a position / so: bf16 17 channels 179 / 219, 24 329 / 232, 64 1432 / 432; fp32 368 / 259, 551 / 298, 1720 / 625)
 #define LN_CHAN_LOOP(KERNEL, ...)                                                                                                   \
@@ -751,7 +762,7 @@ int ln_fwd(long R, int C, long S, long xs, const void* x, LnParam w, LnParam b, 
   } else if (s.lanes) {
     const int per = (int)(s.tiles / (R / S));
     for (long t = 0; t < s.tiles; t += LN_MOST)
-      LN_CHAN(ln_chan_fwd, 1, (unsigned)(s.tiles - t < LN_MOST ? s.tiles - t : LN_MOST), (int)t, per, C, (int)S, (const T*)x, w, b, eps, (T*)y, mean, rstd);
+      LN_CHAN(LN_CHAN_FWD, 1, (unsigned)(s.tiles - t < LN_MOST ? s.tiles - t : LN_MOST), (int)t, per, C, (int)S, (const T*)x, w, b, eps, (T*)y, mean, rstd);
   } else {
     LN_CHAN_LOOP(ln_chan_fwd_loop, R, C, S, C * S, (const T*)x, w, b, eps, (T*)y, mean, rstd);
   }
@@ -771,7 +782,7 @@ int ln_bwd(long R, int C, long S, long xs, const void* x, const void* dy, LnPara
       LN_ROWS(ln_rows_bwd, (unsigned)G, R, C, xs, (const T*)x, (const T*)dy, w, mean, rstd, (T*)dx, p);
     } else {
       const int per = (int)(s.tiles / (R / S));
-      LN_CHAN(ln_chan_bwd, 2, (unsigned)G, (int)s.tiles, per, C, (int)S, (const T*)x, (const T*)dy, w, mean, rstd, (T*)dx, p);
+      LN_CHAN(LN_CHAN_BWD, 2, (unsigned)G, (int)s.tiles, per, C, (int)S, (const T*)x, (const T*)dy, w, mean, rstd, (T*)dx, p);
     }
     PXL_LAUNCH_CHECK();
   } else if (R > 0) {
