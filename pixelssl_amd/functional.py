@@ -468,7 +468,7 @@ def muon_scale(shape, adjust="original"):
     for n in shape[1:]:
         cols *= n
     if adjust == "original":
-        return max(1.0, rows / cols) ** 0.5
+        return max(1.0, rows / cols) ** 0.5 if cols else 1.0
     if adjust == "match_rms_adamw":
         return 0.2 * max(rows, cols) ** 0.5
     if adjust == "none":

@@ -539,30 +539,41 @@ class FusedMuon(_FlatStateMixin, Optimizer):
         super().__init__(params, dict(lr=lr, momentum=momentum, nesterov=nesterov, weight_decay=weight_decay, ns_steps=ns_steps,
                                       ns_coefficients=coefs, ns_eps=ns_eps, adjust_lr=adjust_lr, betas=tuple(betas), eps=eps,
                                       vector_scale=vector_scale, muon=muon))
-        self._foreign = []
-        self._stores = {}
-        for group in self.param_groups:
-            if not 0 <= group['momentum'] < 1:
-                raise ValueError('FusedMuon: momentum %r' % (group['momentum'],))
-            b1, b2 = group['betas']
-            if not (0 <= b1 < 1 and 0 <= b2 < 1) or not group['eps'] > 0 or not group['ns_eps'] > 0:
-                raise ValueError('FusedMuon: betas %r, eps %r, ns_eps %r' % (group['betas'], group['eps'], group['ns_eps']))
-            PF.muon_scale((1, 1), group['adjust_lr'])
-            PF._coefficients(group['ns_steps'], group['ns_coefficients'])
-            self._foreign.append(_foreign(group['params']))
-            for p in self._foreign[-1]:
-                if p.dtype not in (torch.float32, torch.bfloat16) or PF._dense_strides(p) is None:
-                    raise ValueError('FusedMuon: parameters are dense float32 or bfloat16 tensors, got %s of strides %s' % (p.dtype, p.stride()))
-            for p in group['params']:
-                if getattr(p, '_pxl_flat', None) is not None:
-                    self._stores[id(p._pxl_flat[0])] = p._pxl_flat[0]
-        for store in self._stores.values():
-            for _, attr in self._ALL_KEYS:
-                if not hasattr(store, attr):
-                    setattr(store, attr, torch.zeros_like(store.params))
-        self._matrix = {id(p): bool(group['muon']) and p.dim() >= 2 for group in self.param_groups for p in group['params']}
         self._step = 0
         self._steps_taken = 0
+
+    def add_param_group(self, param_group):
+        """as torch's; also what the constructor passes each of its groups through"""
+        if not hasattr(self, '_matrix'):
+            self._foreign, self._stores, self._matrix = [], {}, {}
+        super().add_param_group(param_group)
+        try:
+            self._admit(self.param_groups[-1])
+        except ValueError:
+            self.param_groups.pop()
+            raise
+
+    def _admit(self, group):
+        from .. import functional as PF
+        if not 0 <= group['momentum'] < 1:
+            raise ValueError('FusedMuon: momentum %r' % (group['momentum'],))
+        b1, b2 = group['betas']
+        if not (0 <= b1 < 1 and 0 <= b2 < 1) or not group['eps'] > 0 or not group['ns_eps'] > 0:
+            raise ValueError('FusedMuon: betas %r, eps %r, ns_eps %r' % (group['betas'], group['eps'], group['ns_eps']))
+        PF.muon_scale((1, 1), group['adjust_lr'])
+        PF._coefficients(group['ns_steps'], group['ns_coefficients'])
+        foreign = _foreign(group['params'])
+        for p in foreign:
+            if p.dtype not in (torch.float32, torch.bfloat16) or PF._dense_strides(p) is None:
+                raise ValueError('FusedMuon: parameters are dense float32 or bfloat16 tensors, got %s of strides %s' % (p.dtype, p.stride()))
+        self._foreign.append(foreign)
+        for p in group['params']:
+            self._matrix[id(p)] = bool(group['muon']) and p.dim() >= 2
+            if getattr(p, '_pxl_flat', None) is not None:
+                store = self._stores[id(p._pxl_flat[0])] = p._pxl_flat[0]
+                for _, attr in self._ALL_KEYS:
+                    if not hasattr(store, attr):
+                        setattr(store, attr, torch.zeros_like(store.params))
 
     def _keys_of(self, p):
         return self._ALL_KEYS[:1] if self._matrix[id(p)] else self._ALL_KEYS[1:]

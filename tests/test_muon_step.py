@@ -127,3 +127,31 @@ def test_a_refused_step_moves_no_parameter():
     b.grad = None
     opt.step()
     assert opt._step == 1 and not any(torch.equal(t, o) for t, o in zip((flat, v.detach(), c.detach()), before))
+
+
+def test_parameters_without_elements(launches):
+    """an axis of length 0 is left alone, beside parameters that step"""
+    from pixelssl_amd import functional as PF
+    from pixelssl_amd.nn.optimizer import FusedMuon
+    ps = [nn.Parameter(torch.randn(s)) for s in ((5, 0), (0, 5), (4, 6), (0,), (3,))]
+    for p in ps:
+        p.grad = torch.randn(p.shape)
+    opt = FusedMuon(ps)
+    opt.step()
+    assert launches == ["pxl_adam_list", "pxl_muon_step"] and opt._step == 1
+    assert PF.muon_scale((5, 0)) == PF.muon_scale((0, 5)) == 1.0
+
+
+def test_a_group_added_later(launches):
+    from pixelssl_amd.nn.optimizer import FusedMuon
+    mats, vecs = parameters()
+    opt = FusedMuon(mats[:1])
+    opt.step()
+    with pytest.raises(ValueError, match="dense"):
+        opt.add_param_group({"params": [nn.Parameter(torch.randn(4, 6).t())]})
+    assert len(opt.param_groups) == 1
+    opt.add_param_group({"params": mats[1:] + vecs, "lr": 0.1})
+    launches.clear()
+    opt.step()
+    assert launches == ["pxl_adam_list", "pxl_muon_step", "pxl_muon_step"] and opt._foreign[1] == mats[1:] + vecs
+    assert set(opt.state_dict()["state"][2]) == {"exp_avg", "exp_avg_sq", "step"}
