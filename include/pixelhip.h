@@ -903,7 +903,7 @@ typedef struct pxl_ns_item {
   float scale;
   int32_t reserved;
 } pxl_ns_item;
-/* items: HOST array; n <= 2^22 matrices of any mix of shapes, none of which overlap (p of one against anything of another); p == g is allowed
+/* items: HOST array; n <= 2^22 matrices (and fewer than 2^24 tiles of 64 x 64, 2^35 elements) of any mix of shapes, none of which overlap (p of one against anything of another); p == g is allowed
  * in pxl_orthogonalize.  coef: HOST array [steps][3], 1 .. 16 steps;
  *   X = G / max(|G|_F, eps);  per step  X <- a X + (b L + c L^2) X,  L = X X'  (of the transposed matrix when rows > cols)
  * Products to 22 bits of every entry down to 2^-17 of the matrix' largest possible one (X's: its norm, or eps), to 2^-39 of that below; sums in

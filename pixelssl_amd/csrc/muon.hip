@@ -1599,6 +1599,14 @@ int ns_plan(const char* what, int dtype, const pxl_ns_item* items, int n, int pl
     int first = 0;
     for (auto& c : s.cls) { c.first = first; first += c.count; }
     s.items = first;
+    // no launch of a set has more workgroups than the larger of these two passes; one of 256 threads each, and a grid has fewer than 2^32
+    long norm = 0, split = 0;
+    for (auto& c : s.cls) {
+      norm += (long)c.parts * c.count;
+      split += (long)((c.np + 63) / 64) * ((c.mp + 63) / 64) * c.count;
+    }
+    PXL_REQUIRE(ns_is_tiny(s.cls[0], plan.np) || (norm < (1l << 24) && split < (1l << 24)),
+                "%s: %d matrices like %d x %d are too many for one call (2^24 tiles of 64 x 64, 2^35 elements)", what, first, s.cls[0].rows, s.cls[0].cols);
     const size_t table = round_up_z(first * sizeof(NsItem), 256);
     const size_t head = ns_is_tiny(s.cls[0], plan.np) ? table : table + round_up_z(first * sizeof(double) * NS_PARTS, 256) + round_up_z(first * sizeof(float), 256);
     if (head > plan.head) plan.head = head;

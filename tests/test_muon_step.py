@@ -155,3 +155,23 @@ def test_a_group_added_later(launches):
     opt.step()
     assert launches == ["pxl_adam_list", "pxl_muon_step", "pxl_muon_step"] and opt._foreign[1] == mats[1:] + vecs
     assert set(opt.state_dict()["state"][2]) == {"exp_avg", "exp_avg_sq", "step"}
+
+
+def test_as_many_workgroups_as_no_grid_holds_are_refused():
+    """2^22 matrices of 1 x 449 are 2^25 tiles: with 256 threads each past the 2^32 of a grid"""
+    import ctypes
+    import numpy as np
+    from pixelssl_amd import _lib
+    h = _lib.lib()
+    n = 1 << 22
+    items = np.zeros(n, dtype=np.dtype([("p", "u8"), ("g", "u8"), ("mom", "u8"), ("rows", "i4"), ("cols", "i4"), ("scale", "f4"), ("reserved", "i4")]))
+    assert items.itemsize == ctypes.sizeof(_lib.NsItem)
+    items["p"], items["g"], items["mom"], items["rows"], items["cols"] = 1, 1, 1, 1, 449
+    at = items.ctypes.data_as(ctypes.c_void_p)
+    for dtype in (0, 1):
+        assert h.pxl_ns_workspace(dtype, at, n) == 0 and b"too many" in h.pxl_last_error()
+        assert h.pxl_ns_workspace(dtype, at, n // 4) > 0
+    items["cols"] = 300                                  # on one CU each: a workgroup a matrix
+    assert h.pxl_ns_workspace(1, at, n) > 0
+    items["rows"], items["cols"] = 4096, 4096             # 2^15 tiles are fine, 2^24 are not
+    assert h.pxl_ns_workspace(0, at, 8) > 0 and h.pxl_ns_workspace(0, at, 1 << 12) == 0 and b"too many" in h.pxl_last_error()
