@@ -862,7 +862,8 @@ template <int MT> struct NsOnCu {
   // steps first .. last from A in slot 0 (a barrier has been passed since it was written) -> this wave's block of P, times its planes'
   // scale.  Every thread of the workgroup calls it.  Slot 1 is read until its end.
   __device__ __forceinline__ f32x16 run(const NsRec& p, int first, int last) {
-    return mp == 32 * MT ? run_k<2 * MT>(p, first, last) : run_k<2 * MT - 2>(p, first, last);
+    if constexpr (MT == 2) return run_k<4>(p, first, last);          // (mp = 32: ns_rec_one)
+    else return mp == 32 * MT ? run_k<2 * MT>(p, first, last) : run_k<2 * MT - 2>(p, first, last);
   }
   template <int KT> __device__ __forceinline__ f32x16 run_k(const NsRec& p, int first, int last) {
     const int u = I < J ? J : I;
@@ -913,6 +914,56 @@ template <int MT> struct NsOnCu {
   }
 };
 
+// ---- the same for at most 32 rows: one wave, everything in its registers and in fp32 ---------------------------------------------------------
+// Planes of 22 bits, whose rounding acts on whole rows of Q and P, left results of so few rows further off than a plain fp32 iteration is (16 x 300
+// 2.3e-6 of the norm, so 1.3e-6, for 1.0e-6).  The fp32 matrix instructions take 1024 cycles a product, and no operand has to be moved: of a symmetric
+// matrix, element e of a lane (row 8 (e / 4) + 4 (lane / 32) + e % 4, column lane % 32) is both what the lane has to bring as left operand (that
+// column's row, that row's column) and as right operand, with k running over the rows in the order of e.
+__device__ __forceinline__ f32x16 ns_product_one(const f32x16& x, const f32x16& y) {
+  f32x16 r;
+#pragma unroll
+  for (int e = 0; e < 16; ++e) r[e] = 0.f;
+#pragma unroll
+  for (int e = 0; e < 16; ++e) r = __builtin_amdgcn_mfma_f32_32x32x2f32(x[e], y[e], r, 0, 0, 0);
+  return r;
+}
+// f times the mean of v and its transpose, exactly symmetric; through 32 x 33 floats of LDS that no other wave uses
+__device__ __forceinline__ f32x16 ns_symmetric_one(const f32x16& v, float f, float* t) {
+  const int lane = threadIdx.x & 63, q = lane & 31, h = 4 * (lane >> 5);
+#pragma unroll
+  for (int e = 0; e < 16; ++e) t[(8 * (e >> 2) + h + (e & 3)) * 33 + q] = v[e];
+  __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+  __builtin_amdgcn_wave_barrier();
+  __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+  f32x16 r;
+  f *= 0.5f;
+#pragma unroll
+  for (int e = 0; e < 16; ++e) r[e] = (v[e] + t[q * 33 + 8 * (e >> 2) + h + (e & 3)]) * f;
+  __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+  __builtin_amdgcn_wave_barrier();
+  return r;
+}
+// steps first .. last from the sums A (times `un`) of a segment's first product -> P, times its planes' scale
+__device__ __forceinline__ f32x16 ns_rec_one(const NsRec& p, int first, int last, const f32x16& sums, float un, float* t) {
+  const int lane = threadIdx.x & 63;
+  f32x16 A = ns_symmetric_one(sums, un * p.sA[first], t), P;
+  for (int s = first; s <= last; ++s) {
+    const NsRecStep d = p.step[s];
+    f32x16 Q = ns_product_one(A, A);                     // (x y summed in the order of y x: symmetric as it is)
+#pragma unroll
+    for (int e = 0; e < 16; ++e) {
+      Q[e] = __fmaf_rn(d.g, Q[e], d.ia * A[e]);
+      Q[e] += 8 * (e >> 2) + 4 * (lane >> 5) + (e & 3) == (lane & 31) ? d.a : 0.f;
+    }
+    P = s == first ? Q : ns_symmetric_one(ns_product_one(Q, P), d.fP, t);
+    if (s < last) {
+      const f32x16 T = ns_symmetric_one(ns_product_one(Q, A), d.fT, t);
+      A = ns_symmetric_one(ns_product_one(Q, T), d.fA, t);
+    }
+  }
+  return P;
+}
+
 template <int MT>
 __global__ __launch_bounds__(MT == 2 ? 512 : 1024) void ns_rec_kernel(NsClasses cs, NsRec p, int tiles, const float* __restrict__ residue, unsigned char* __restrict__ ws) {
   __shared__ __attribute__((aligned(16))) unsigned char lds[2 * NsOnCu<MT>::SLOT];
@@ -950,14 +1001,20 @@ __global__ __launch_bounds__(MT == 2 ? 512 : 1024) void ns_rec_kernel(NsClasses 
     const int t = (I >> 1) * ((I >> 1) + 1) / 2 + (J >> 1);
     V = ns_share_sum<2>(p.part, ns_shares(c), (size_t)tiles * 4, ((size_t)c.tn + (size_t)i * c.per + t) * 4 + (I & 1) * 2 + (J & 1));
   }
-  if (lower) {
+  f32x16 P;
+  if (MT == 2 && c.mp == 32) {
+    if (!m.inside) return;              // (one wave has a block)
+    P = ns_rec_one(p, 0, p.steps - 1, V, un, reinterpret_cast<float*>(lds));
+  } else {
+    if (lower) {
 #pragma unroll
-    for (int e = 0; e < 16; ++e) V[e] *= un;
-    m.put_gram(V, p.sA[0], I, J);
+      for (int e = 0; e < 16; ++e) V[e] *= un;
+      m.put_gram(V, p.sA[0], I, J);
+    }
+    __syncthreads();
+    P = m.run(p, 0, p.steps - 1);
+    if (!m.inside) return;
   }
-  __syncthreads();
-  const f32x16 P = m.run(p, 0, p.steps - 1);
-  if (!m.inside) return;
   _Float16* out = reinterpret_cast<_Float16*>(ws + c.base + (size_t)i * c.stride + slot_off(c, p.xplanes, p.out));
   const size_t pm = (size_t)c.mp * c.mp;
 #pragma unroll
@@ -1189,7 +1246,7 @@ __global__ __launch_bounds__(256, 2) void ns_slim_kernel(NsClasses cs, NsSlim p,
 // At most 64 on the smaller side, 448 (bf16: 384) on the other.  X lives in LDS as planes [mp][pitch]: 16-byte chunk ch of row r at
 // ch ^ ((r >> 2) & 3), a pitch of an odd number of 64 bytes -- 16 rows of one chunk, and the four rows of a transposing read, lie on different
 // banks.  The products are the ones of the larger matrices; only what is moved differs.
-// Measured, this against the launches of the larger ones (5 steps, us): fp32 16 x 27 24 / 56, 64 x 147 34 / 61, 64 x 448 56 / 63 (what LDS holds);
+// Measured, this against the launches of the larger ones (5 steps, us): fp32 64 x 147 34 / 61, 64 x 448 56 / 63 (what LDS holds);
 // bf16 64 x 256 34 / 39, 64 x 384 40 / 40, 64 x 448 43 / 40: the limits.  What bounds it is one CU's chain of small products
 // (1 us each: 24 matrix instructions of 32 cycles on the diagonal, 512 cycles of LDS reads, the split into planes, two barriers).
 template <int NP> constexpr int NS_TINY_N = NP == 2 ? 448 : 384;
@@ -1201,7 +1258,8 @@ struct NsTiny {
   float eps, lr, decay;
   int muon;
 };
-template <typename T, int NP>
+// ONE: at most 32 rows (a kernel of its own: in the other's registers its recursion cost that one 2 %)
+template <typename T, int NP, bool ONE>
 __global__ __launch_bounds__(512) void ns_tiny_kernel(NsClasses cs, NsTiny p, NsInline few, const NsItem* __restrict__ table, MuonArgs ma) {
   constexpr int XB = 64 * (NS_TINY_N<NP> * 2 + 64);             // bytes of one plane of X at most
   constexpr int GROUPS = 64 * NS_TINY_N<NP> / 4 / 512;          // fours of elements a thread holds at most
@@ -1323,7 +1381,8 @@ __global__ __launch_bounds__(512) void ns_tiny_kernel(NsClasses cs, NsTiny p, Ns
     while (!(p.ends >> s1 & 1)) ++s1;
     const float sx = p.sx[s0], res = s0 == 0 ? left : 1.f;
     // A = X X': wave w has block w % nb of the nb on and below the diagonal, and every (8 / nb)-th 16 of K from w / nb on
-    const int nb = c.mp > 32 ? 3 : 1, parts = 8 / nb, blk = wave % nb, part = wave / nb;
+    constexpr int nb = ONE ? 1 : 3, parts = 8 / nb;
+    const int blk = wave % nb, part = wave / nb;
     const int bi = blk > 0, bj = blk == 2;
     f32x16 a;
 #pragma unroll
@@ -1357,16 +1416,20 @@ __global__ __launch_bounds__(512) void ns_tiny_kernel(NsClasses cs, NsTiny p, Ns
       }
     }
     __syncthreads();
-    if (part == 0) {
-      const float un = res * res / (sx * sx);
+    const float una = res * res / (sx * sx);
+    if constexpr (ONE) {
+      if (wave == 0) m.put(0, ns_rec_one(p.rec, s0, s1, a, una, reinterpret_cast<float*>(lds + NsOnCu<2>::SLOT)));
+    } else {
+      if (part == 0) {
 #pragma unroll
-      for (int e = 0; e < 16; ++e) a[e] *= un;
-      m.put_gram(a, p.rec.sA[s0], bi, bj);
+        for (int e = 0; e < 16; ++e) a[e] *= una;
+        m.put_gram(a, p.rec.sA[s0], bi, bj);
+      }
+      __syncthreads();
+      const f32x16 P = m.run(p.rec, s0, s1);
+      __syncthreads();
+      if (m.inside) m.put(0, P);
     }
-    __syncthreads();
-    const f32x16 P = m.run(p.rec, s0, s1);
-    __syncthreads();
-    if (m.inside) m.put(0, P);
     __syncthreads();
     // X <- P X in place: a wave takes blocks of 32 columns, all rows of them (nobody else reads those columns)
     const bool done = s1 == steps - 1;
@@ -1438,6 +1501,230 @@ __global__ __launch_bounds__(512) void ns_tiny_kernel(NsClasses cs, NsTiny p, Ns
   }
 }
 
+// ---- matrices of up to 64 x 64 and 32 x 128 on one CU: in fp32, step by step as written --------------------------------------------------------
+// Near-square matrices of so few rows have weak directions, which the iteration amplifies 485 times, beside strong ones, which the P of several steps
+// has to keep in spite of its size (11.9 after two); with planes and with fp32 alike that showed against a plain fp32 iteration: 32 x 32 1.4e-6 of the norm,
+// 64 x 64 1.4e-6 (all in fp32 1.8e-6), 94 x 22 1.7e-6 for 0.9e-6, 1.0e-6, 1.0e-6.  Here X X', its square and (b A + c A^2) X are the only
+// products of a step, three of nearly the same size, so that commuting factors would save none: X <- a X + (b A + c A^2) X.
+// The fp32 instructions take 64 cycles for 32 x 32 x 2: 2048 a product of 64 x 64 on each wave.  Rows of X and of the symmetric matrices lie in LDS an
+// odd number of 16 bytes apart; wave w < 3 has block (w > 0, w == 2) of those on and below the diagonal and writes its mirror image too.
+// Measured (5 steps, us, with planes before): 16 x 27 15 / 24, 32 x 128 18 / 26, 64 x 64 29 / 30; bf16, where planes are exact enough, 15 / 20, 18 / 21,
+// 29 / 27.  32 x 300 so would take 40, with planes and the recursion in fp32 26 at 1.3e-6 of the norm for the plain iteration's 1.0e-6.
+struct NsF32 {
+  static constexpr int PM = 64 + 4;
+  int q, h, I, J;
+  // sum over k of a[32 I + row][k] b[32 J + column][k]
+  static __device__ __forceinline__ f32x16 rows(const float* a, const float* b, int from, int to, int step, f32x16 r) {
+#pragma unroll 4
+    for (int k = from; k < to; k += step) {
+      const float4 x = *reinterpret_cast<const float4*>(a + k), y = *reinterpret_cast<const float4*>(b + k);
+      r = __builtin_amdgcn_mfma_f32_32x32x2f32(x.x, y.x, r, 0, 0, 0);
+      r = __builtin_amdgcn_mfma_f32_32x32x2f32(x.y, y.y, r, 0, 0, 0);
+      r = __builtin_amdgcn_mfma_f32_32x32x2f32(x.z, y.z, r, 0, 0, 0);
+      r = __builtin_amdgcn_mfma_f32_32x32x2f32(x.w, y.w, r, 0, 0, 0);
+    }
+    return r;
+  }
+  static __device__ __forceinline__ f32x16 zero() {
+    f32x16 r;
+#pragma unroll
+    for (int e = 0; e < 16; ++e) r[e] = 0.f;
+    return r;
+  }
+  // this wave's block of the product of two symmetric 64 x 64 matrices
+  __device__ __forceinline__ f32x16 product(const float* a, const float* b) const {
+    return rows(a + (32 * I + q) * PM + h, b + (32 * J + q) * PM + h, 0, 64, 8, zero());
+  }
+  // exactly symmetric: of a block on the diagonal the elements on and below it
+  __device__ __forceinline__ void put(float* m, const f32x16& v) const {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const int r0 = 32 * I + 8 * i + h, c = 32 * J + q;
+#pragma unroll
+      for (int e = 0; e < 4; ++e)
+        if (I > J || r0 + e >= c) {
+          m[(r0 + e) * PM + c] = v[i * 4 + e];
+          m[c * PM + r0 + e] = v[i * 4 + e];
+        }
+    }
+  }
+  __device__ __forceinline__ f32x16 get(const float* m) const {
+    f32x16 v;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const float4 t = *reinterpret_cast<const float4*>(m + (32 * J + q) * PM + 32 * I + 8 * i + h);
+      v[i * 4] = t.x; v[i * 4 + 1] = t.y; v[i * 4 + 2] = t.z; v[i * 4 + 3] = t.w;
+    }
+    return v;
+  }
+};
+struct NsF32Args {
+  int steps;
+  float a[NS_MAX_STEPS], b[NS_MAX_STEPS], c[NS_MAX_STEPS];
+  float eps, lr, decay;
+  int muon;
+};
+template <typename T>
+__global__ __launch_bounds__(256) void ns_f32_kernel(NsClasses cs, NsF32Args p, NsInline few, const NsItem* __restrict__ table, MuonArgs ma) {
+  constexpr int PM = NsF32::PM, GROUPS = 64 * 64 / 4 / 256;
+  __shared__ __attribute__((aligned(16))) float x[64 * PM];          // (32 * 132 is less)
+  __shared__ __attribute__((aligned(16))) float mat[2][64 * PM];
+  __shared__ double sh[4];
+  const NsClass c = find_class(cs, blockIdx.x);
+  const int i = blockIdx.x - c.start;
+  const NsItem it = ns_item(few, table, c.first + i);
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const T* g = reinterpret_cast<const T*>(it.g);
+  const bool tall = c.rows > c.cols;
+
+  // momentum, update and its norm; the update stays in registers (fours of a line, 256 further each time)
+  const int per_line = (c.cols + 3) >> 2, lines = 256 / per_line, fours = 256 - lines * per_line;
+  const int line0 = tid / per_line, four0 = tid - line0 * per_line;
+  float u[GROUPS][4];
+  double s = 0.0;
+  int line = line0, four = four0;
+  auto next = [&]() {
+    line += lines;
+    four += fours;
+    if (four >= per_line) { four -= per_line; ++line; }
+  };
+#pragma unroll
+  for (int k = 0; k < GROUPS; ++k, next()) {
+#pragma unroll
+    for (int e = 0; e < 4; ++e) u[k][e] = 0.f;
+    if (line < c.rows) {
+      const int col = four * 4;
+      const long at = (long)line * c.cols + col;
+      if (col + 4 <= c.cols) {
+        load4(g + at, u[k]);
+        if (it.mom != nullptr) {
+          float m[4];
+          load4(it.mom + at, m);
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            m[e] = muon_momentum(m[e], u[k][e], ma);
+            u[k][e] = muon_update(m[e], u[k][e], ma);
+          }
+          store4(it.mom + at, m);
+        }
+      } else {
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+          if (col + e < c.cols) {
+            float v = to_f(g[at + e]);
+            if (it.mom != nullptr) {
+              const float m = muon_momentum(it.mom[at + e], v, ma);
+              it.mom[at + e] = m;
+              v = muon_update(m, v, ma);
+            }
+            u[k][e] = v;
+          }
+      }
+#pragma unroll
+      for (int e = 0; e < 4; ++e) s += (double)u[k][e] * u[k][e];
+    }
+  }
+#pragma unroll
+  for (int o = 32; o > 0; o >>= 1) s += __shfl_xor(s, o, 64);
+  if (lane == 0) sh[wave] = s;
+  const int px = c.np + 4;
+  for (int e = tid * 4; e < c.mp * px; e += 1024) *reinterpret_cast<float4*>(x + e) = make_float4(0.f, 0.f, 0.f, 0.f);     // the padding
+  __syncthreads();
+  const double square = (sh[0] + sh[1]) + (sh[2] + sh[3]);
+  // (a NaN or an infinity in the matrix: all of its result is NaN)
+  const double mul = square < HUGE_VAL ? 1.0 / fmax(sqrt(square), (double)p.eps) : nan("");
+  line = line0;
+  four = four0;
+#pragma unroll
+  for (int k = 0; k < GROUPS; ++k, next()) {
+    if (line >= c.rows) continue;
+#pragma unroll
+    for (int e = 0; e < 4; ++e)
+      if (four * 4 + e < c.cols) x[tall ? (four * 4 + e) * px + line : line * px + four * 4 + e] = (float)((double)u[k][e] * mul);
+  }
+  __syncthreads();
+
+  const NsF32 m{lane & 31, 4 * (lane >> 5), wave > 0, wave == 2};
+  const int q = m.q, h = m.h;
+  const bool two = c.mp > 32;
+  // block of X <- a X + S X that a wave has: four at most
+  const int v = two ? wave & 1 : 0, col = (two ? wave >> 1 : wave) * 32;
+  const bool mine = col < c.np;
+  float *A = mat[0], *S = mat[1];
+  for (int st = 0;; ++st) {
+    const float ca = p.a[st], cb = p.b[st], cc = p.c[st];
+    if (two) {                             // (wave 3 only waits)
+      if (wave < 3) m.put(A, NsF32::rows(x + (32 * m.I + q) * px + h, x + (32 * m.J + q) * px + h, 0, c.np, 8, NsF32::zero()));
+      __syncthreads();
+      if (wave < 3) {
+        f32x16 t = m.product(A, A);
+        const f32x16 a = m.get(A);
+#pragma unroll
+        for (int e = 0; e < 16; ++e) t[e] = __fmaf_rn(cc, t[e], cb * a[e]);
+        m.put(S, t);
+      }
+    } else {
+      // four waves share the sum over K
+      f32x16 t = NsF32::rows(x + q * px + h, x + q * px + h, wave * 8, c.np, 32, NsF32::zero());
+      float4* o = reinterpret_cast<float4*>(A);
+      if (wave > 0) {
+#pragma unroll
+        for (int e4 = 0; e4 < 4; ++e4) o[((wave - 1) * 4 + e4) * 64 + lane] = make_float4(t[e4 * 4], t[e4 * 4 + 1], t[e4 * 4 + 2], t[e4 * 4 + 3]);
+      }
+      __syncthreads();
+      if (wave == 0) {
+        for (int w = 0; w < 3; ++w)
+#pragma unroll
+          for (int e4 = 0; e4 < 4; ++e4) {
+            const float4 a = o[(w * 4 + e4) * 64 + lane];
+            t[e4 * 4] += a.x; t[e4 * 4 + 1] += a.y; t[e4 * 4 + 2] += a.z; t[e4 * 4 + 3] += a.w;
+          }
+        const f32x16 w = ns_product_one(t, t);         // (sums of x y in the order of y x: t is symmetric as it is)
+#pragma unroll
+        for (int e = 0; e < 16; ++e) t[e] = __fmaf_rn(cc, w[e], cb * t[e]);
+#pragma unroll
+        for (int e4 = 0; e4 < 4; ++e4) *reinterpret_cast<float4*>(S + q * PM + 8 * e4 + h) = make_float4(t[e4 * 4], t[e4 * 4 + 1], t[e4 * 4 + 2], t[e4 * 4 + 3]);
+      }
+    }
+    __syncthreads();
+    // X <- a X + S X.  A lane: rows 32 v + 8 e4 + h + 0 .. 3, column col + q
+    f32x16 y = NsF32::zero();
+    if (mine) {
+#pragma unroll 4
+      for (int k = 0; k < c.mp; k += 8) {
+        const float4 a = *reinterpret_cast<const float4*>(S + (32 * v + q) * PM + k + h);
+        const float* b = x + (k + h) * px + col + q;
+        y = __builtin_amdgcn_mfma_f32_32x32x2f32(a.x, b[0], y, 0, 0, 0);
+        y = __builtin_amdgcn_mfma_f32_32x32x2f32(a.y, b[px], y, 0, 0, 0);
+        y = __builtin_amdgcn_mfma_f32_32x32x2f32(a.z, b[2 * px], y, 0, 0, 0);
+        y = __builtin_amdgcn_mfma_f32_32x32x2f32(a.w, b[3 * px], y, 0, 0, 0);
+      }
+#pragma unroll
+      for (int e = 0; e < 16; ++e) y[e] = __fmaf_rn(ca, x[(32 * v + 8 * (e >> 2) + h + (e & 3)) * px + col + q], y[e]);
+    }
+    if (st == p.steps - 1) {
+      if (!mine || col + q >= c.n) return;
+      T* o = reinterpret_cast<T*>(it.p);
+      const float f = p.muon ? -p.lr * it.scale : 1.f;
+#pragma unroll
+      for (int e = 0; e < 16; ++e) {
+        const int r = 32 * v + 8 * (e >> 2) + h + (e & 3), n = col + q;
+        if (r >= c.m) continue;
+        const size_t at = tall ? (size_t)n * c.cols + r : (size_t)r * c.cols + n;
+        const float w = y[e] * f;
+        o[at] = from_f<T>(p.muon ? to_f(o[at]) * p.decay + w : w);
+      }
+      return;
+    }
+    __syncthreads();
+    if (mine) {
+#pragma unroll
+      for (int e = 0; e < 16; ++e) x[(32 * v + 8 * (e >> 2) + h + (e & 3)) * px + col + q] = y[e];
+    }
+    __syncthreads();
+  }
+}
+
 // ---- host ---------------------------------------------------------------------------------------------------------------------
 struct NsPlan {
   struct Set { std::vector<NsClass> cls; size_t bytes; int items; };
@@ -1488,11 +1775,12 @@ inline size_t round_up_z(size_t v, size_t to) { return (v + to - 1) / to * to; }
 // (small: 1.2 us for every 16 of them in the recursion's workgroup).  23 x 256 x 2304: 230 small
 // tiles in one share 24 us (model) against 34 measured for 8 shares of 69 large ones; 3 x 512 x 4608: 8 shares of 30 large tiles.
 struct NsSplit { int tile, shares, tiles, small, mt, tiny, full, cut; size_t bytes; int slim[NS_MAX_CLASSES]; };      // bytes: of all shares, cut tiles' too
+inline bool ns_is_f32(const NsClass& c, int planes) { return c.mp == 32 ? c.np <= 128 : c.np <= 64 && planes == 2; }          // (and tiny with it)
 inline bool ns_is_tiny(const NsClass& c, int planes) { return c.mp <= 64 && c.np <= (planes == 2 ? NS_TINY_N<2> : NS_TINY_N<1>); }
 NsSplit ns_split_plan(std::vector<NsClass>& cls, int planes) {
   NsSplit r = {64, 1, 0, 1, 2, 0, 0, 1, 0, {}};
   if (ns_is_tiny(cls[0], planes)) {               // (and with it all of the set)
-    r.tiny = 1;
+    r.tiny = ns_is_f32(cls[0], planes) ? 2 : 1;
     return r;
   }
   int longest = 0;
@@ -1581,7 +1869,7 @@ int ns_plan(const char* what, int dtype, const pxl_ns_item* items, int n, int pl
       c.parts = (int)((size + chunk - 1) / chunk);
       c.stride = round_up_z((size_t)plan.xplanes * c.mp * c.np * 2 + (size_t)5 * 2 * c.mp * c.mp * 2, 256);
       // matrices that run on one CU whole, those whose recursion does, by its two sizes, and the others: in sets of their own
-      auto kind = [&](const NsClass& x) { return ns_is_tiny(x, plan.np) ? 0 : (x.mp <= 64 ? 1 : (x.mp <= 128 ? 2 : 3)); };
+      auto kind = [&](const NsClass& x) { return ns_is_f32(x, plan.np) ? -1 : ns_is_tiny(x, plan.np) ? (x.mp == 32 ? -2 : 0) : (x.mp <= 64 ? 1 : (x.mp <= 128 ? 2 : 3)); };
       if (ns_is_tiny(c, plan.np)) c.stride = 0;
       for (size_t q = 0; q < sets.size(); ++q)
         if (kind(sets[q].cls[0]) == kind(c) && sets[q].cls.size() < (size_t)NS_MAX_CLASSES) sk = (int)q;
@@ -1832,13 +2120,35 @@ int ns_run_tiny(NsRun& r, const std::vector<NsStep>& steps, float eps, const Muo
     r.cs.c[k].start = at;
     at += r.cs.c[k].count;
   }
-  hipLaunchKernelGGL((ns_tiny_kernel<T, NP>), dim3(at), dim3(512), 0, r.st, r.cs, q, r.few, r.table, ma);
+  if (r.cs.c[0].mp == 32) hipLaunchKernelGGL((ns_tiny_kernel<T, NP, true>), dim3(at), dim3(512), 0, r.st, r.cs, q, r.few, r.table, ma);
+  else hipLaunchKernelGGL((ns_tiny_kernel<T, NP, false>), dim3(at), dim3(512), 0, r.st, r.cs, q, r.few, r.table, ma);
+  PXL_LAUNCH_CHECK();
+  return PXL_OK;
+}
+
+template <typename T>
+int ns_run_f32(NsRun& r, const std::vector<NsStep>& steps, float eps, const MuonArgs& ma, int muon) {
+  NsF32Args q;
+  memset(&q, 0, sizeof(q));
+  q.steps = (int)steps.size();
+  for (size_t s = 0; s < steps.size(); ++s) { q.a[s] = (float)steps[s].a; q.b[s] = (float)steps[s].b; q.c[s] = (float)steps[s].c; }
+  q.eps = eps;
+  q.lr = ma.lr;
+  q.decay = ma.keep;
+  q.muon = muon;
+  int at = 0;
+  for (int k = 0; k < r.cs.n; ++k) {
+    r.cs.c[k].start = at;
+    at += r.cs.c[k].count;
+  }
+  hipLaunchKernelGGL((ns_f32_kernel<T>), dim3(at), dim3(256), 0, r.st, r.cs, q, r.few, r.table, ma);
   PXL_LAUNCH_CHECK();
   return PXL_OK;
 }
 
 template <typename T, int NP>
 int ns_run_set(NsRun& r, const std::vector<NsStep>& steps, float eps, const MuonArgs& ma, int muon) {
+  if (r.split.tiny == 2) return ns_run_f32<T>(r, steps, eps, ma, muon);
   if (r.split.tiny) return ns_run_tiny<T, NP>(r, steps, eps, ma, muon);
   constexpr int xplanes = ns_xplanes(NP);
   const int MA = xplanes, MT = xplanes + 1;
