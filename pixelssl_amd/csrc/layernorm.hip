@@ -612,7 +612,7 @@ __global__ __launch_bounds__(1024) void ln_dwb_fold(int G, int C, const float* _
   __shared__ double sh[64][17];
   const int col = threadIdx.x & 15, gl = threadIdx.x >> 4;
   const int k = blockIdx.x * 16 + col;
-  double s = 0.0;                             // (up to 1280 shares)
+  double s = 0.0;                             // (up to 8192 shares)
   if (k < 2 * C) {
     int g = gl;
     for (; g + 192 < G; g += 256) {           // four loads in flight
@@ -643,6 +643,16 @@ inline unsigned blocks_for(long n, long most) { return (unsigned)(n < 1 ? 1 : (n
 // How a call is run.  Rows: 8 .. 64 lanes (a wave or a part of it) hold a row in at most 4 pieces each, else a workgroup holds it in at
 // most 4 (fp32: 8); channels: at most 16 pieces a thread; beyond: the three-sweep kernels, which take any length.
 struct LnShape { int lanes, nv, threads, tsv; int groups; long tiles; };
+// Workgroups of a backward pass over `n` turns: as many as run at once, the turns evenly over them; several times as many where a thread would add
+// up the parameters' gradients over more than `longest` turns, one after the other in 32 bits (2^20 x 2048 fp32 of a constant gradient: 2048 turns, db
+// 1.6e-5 off, with 256 2e-6; the plain sum 2e-6) -- up to 8192, whose shares take 128 KB a 2 features.
+inline int ln_groups(long n, long resident, long longest) {
+  long most = resident * ((n + resident * longest - 1) / (resident * longest));
+  if (most < resident) most = resident;
+  if (most > 8192) most = 8192 / resident * resident;
+  const long each = (n + most - 1) / most;
+  return (int)(n < 1 ? 1 : (n + each - 1) / each);
+}
 LnShape ln_rows_shape(int dtype, long R, int C) {
   LnShape s = {0, 0, 256, 0, 1, 0};
   const int v = dtype == PXL_F32 ? 4 : 8, pieces = (C + v - 1) / v;
@@ -658,8 +668,7 @@ LnShape ln_rows_shape(int dtype, long R, int C) {
   }
   if (s.lanes) {
     const long passes = (R + 256 / s.lanes - 1) / (256 / s.lanes);
-    const long each = (passes + 511) / 512;
-    s.groups = (int)(passes < 1 ? 1 : (passes + each - 1) / each);
+    s.groups = ln_groups(passes, 512, 256);
   } else {
     const long g = (R + 63) / 64;
     s.groups = (int)(g < 1 ? 1 : (g > 256 ? 256 : g));
@@ -687,8 +696,7 @@ LnShape ln_chan_shape(int dtype, long N, int C, long S) {
     // sums too (8 x 64 x 257 x 257 fp32 108 us + 5 to add 1175 of them, a workgroup for every 4 tiles 106 + 20)
     const int threads = s.nv >= 8 ? 2 * s.threads : s.threads;
     const long most = threads == 1024 ? 256 : (threads == 512 ? 512 : 1280);
-    const long each = (s.tiles + most - 1) / most;
-    s.groups = (int)(s.tiles < 1 ? 1 : (s.tiles + each - 1) / each);
+    s.groups = ln_groups(s.tiles, most, 128 / v);
   }
   if (!s.nv) {
     const long g = (N * S + 63) / 64;

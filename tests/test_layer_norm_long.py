@@ -127,3 +127,19 @@ def test_as_many_channels_as_are_taken():
     for name, t in (("y", rows(y)), ("dx", rows(dx)), ("dw", dw), ("db", db)):
         val, bound = want[name]
         assert ((t.double() - val).abs() <= bound(0.0) + 1e-37).all(), name
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("shape,channels", [((2 ** 20, 2048), False), ((2 ** 24, 16), False), ((16, 32, 1025, 1025), True)], ids=lambda v: "x".join(map(str, v)) if isinstance(v, tuple) else "")
+def test_parameter_gradients_of_a_constant_gradient(shape, channels):
+    """one addend over and over is what a running sum in 32 bits drifts with: n of them, each addition off by up to 2^-24 of what there is, by up to
+    2^-25 n of the sum.  At most 256 rows, or 512 positions of these maps, are added up so; what adds up those sums is in 64 bits"""
+    from pixelssl_amd import functional as PF
+    C = shape[1]
+    x = torch.empty(shape, device="cuda").normal_(generator=torch.Generator("cuda").manual_seed(1)).bfloat16()
+    w, b = torch.ones(C, device="cuda", requires_grad=True), torch.zeros(C, device="cuda", requires_grad=True)
+    dy = torch.full(shape, 0.1, device="cuda")
+    y = (PF.layer_norm_channels if channels else PF.layer_norm)(x.float(), w, b)
+    db, = torch.autograd.grad(y, b, dy)
+    want = x.numel() // C * float(dy.flatten()[0])
+    assert (db.double() / want - 1).abs().max().item() <= 2.0 ** -25 * 512 * (1 if channels else 0.5)
