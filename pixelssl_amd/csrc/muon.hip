@@ -19,9 +19,9 @@
 // instructions, five times the rate of the fp32 ones.  A bf16 matrix scaled by a power of two IS one fp16 plane (8 of 11 bits), its norm's remainder is applied to A and
 // to the result.  (A Muon step's update is a 32-bit matrix, of bf16 parameters too: two planes.)
 //
-// Measured (5 steps, us): 64 x 147 fp32 34, 23 x 256 x 2304 fp32 341, 23 x 1024 x 256 bf16 191, 2 x 2048 x 4608 fp32 2090 (0.77 PF of fp16
-// products against 1.09 of a large library product: power brings the clock from 2.4 to 1.7 - 1.8 GHz), Muon steps of 3 x 512 x 4608 350 and of
-// 4 x 21 x 18432 78.  Below some hundred rows the chain of dependent products bounds it: 4.5 us a launch until its first product, 2 us its stores.
+// Measured (5 steps, us): 64 x 147 fp32 34, 23 x 256 x 2304 fp32 341 - 349, 23 x 1024 x 256 bf16 191 - 196, 2 x 2048 x 4608 fp32 2090 - 2150 (0.77 PF
+// of fp16 products against 1.09 of a large library product: power brings the clock from 2.4 to 1.7 - 1.8 GHz), Muon steps of 3 x 512 x 4608 350 - 354
+// (bf16 parameters too) and of 4 x 21 x 18432 74.  Below some hundred rows the chain of dependent products bounds it: 4.5 us a launch until its first product, 2 us its stores.
 //
 // No atomics, no state between calls, every sum in one order.
 #include <algorithm>
@@ -1036,7 +1036,7 @@ __global__ __launch_bounds__(MT == 2 ? 512 : 1024) void ns_rec_kernel(NsClasses 
 // A wave takes all rows of 64 columns at a time, in LDS of its own (no barrier): [row][64] per plane, chunks permuted as in the products (chunk_at).
 // P's fragments stay in registers, X's come through the transposing LDS load, the result goes back in place, from there to memory in rows of 128
 // bytes and, K being columns now, into the Gram product's sums: a launch less a segment, and no tiles of 64 rows for matrices of 32.  5 steps of
-// 4 x 21 x 18432 fp32 121 -> 78 us, of 32 x 2304 x 64 110 -> 102, of 1 x 64 x 576 64 either way.
+// 4 x 21 x 18432 fp32 121 -> 78 us (74 with the recursion in fp32), of 32 x 2304 x 64 110 -> 102, of 1 x 64 x 576 64 either way.
 struct NsSlim {
   int xplanes, p, x, out;               // slots
   float unscale, scale;                 // sums -> value;  value -> planes

@@ -696,8 +696,8 @@ def adam(args):
 
 def muon(args):
     """`muon(args)`: an optimizer of this framework (not one of VALID_OPTIMIZER, which are the reference's), chosen like them
-    -- `nn.optimizer.muon(args)(param_groups)`.  The shared flags: --lr (default 0.02), --momentum (0.95), --nesterov, --weight-decay (0),
-    and --beta1 / --beta2 / --eps (0.9, 0.999, 1e-8) of the vectors' Adam step."""
+    -- `nn.optimizer.muon(args)(param_groups)`.  The shared flags: --lr (default 0.02), --momentum (0.95), --nesterov (off unless given, as for
+    sgd; FusedMuon's own default, Nesterov's form, takes --nesterov true), --weight-decay (0), and --beta1 / --beta2 / --eps (0.9, 0.999, 1e-8) of the vectors' Adam step."""
     args.lr = 0.02 if args.lr == -1 else args.lr
     args.momentum = 0.95 if args.momentum == -1 else args.momentum
     args.weight_decay = 0.0 if args.weight_decay == -1 else args.weight_decay
