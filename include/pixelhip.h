@@ -915,6 +915,8 @@ typedef struct pxl_ns_item {
  * ws: pxl_ns_workspace(dtype, items, n) bytes (0: a bad argument), 256-byte aligned, not shared with another call in flight.
  * The item list is copied at the call (kernel arguments): nothing of it is read later.  Equal inputs give equal bits; capturable. */
 size_t pxl_ns_workspace(int dtype, const pxl_ns_item* items, int n);
+/* what pxl_orthogonalize needs of it for these steps: a quarter for bf16 matrices whose steps run as one segment */
+size_t pxl_orthogonalize_workspace(int dtype, const pxl_ns_item* items, int n, int steps, const float* coef);
 int pxl_orthogonalize(int dtype, const pxl_ns_item* items, int n, int steps, const float* coef, float eps, void* ws, size_t ws_bytes,
                       void* stream);
 int pxl_muon_step(int dtype, const pxl_ns_item* items, int n, int steps, const float* coef, float eps, double lr, double momentum, int nesterov,

@@ -290,6 +290,7 @@ SIGNATURES = {
     "pxl_layer_norm_nchw_bwd_workspace": (_Z, [_L, _I, _L]),
     "pxl_layer_norm_nchw_bwd": (_I, [_I, _I, _L, _I, _L, _P, _P, _P, _P, _P, _P, _P, _P, _P, _Z, _P]),
     "pxl_ns_workspace": (_Z, [_I, _P, _I]),
+    "pxl_orthogonalize_workspace": (_Z, [_I, _P, _I, _I, _P]),
     "pxl_orthogonalize": (_I, [_I, _P, _I, _I, _P, _F, _P, _Z, _P]),
     "pxl_muon_step": (_I, [_I, _P, _I, _I, _P, _F, C.c_double, C.c_double, _I, C.c_double, _P, _Z, _P]),
     "pxl_muon_check": (_I, [_I, _P, _I, _I, _P, _F, C.c_double, C.c_double, C.c_double]),

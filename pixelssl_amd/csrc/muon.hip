@@ -2291,19 +2291,25 @@ int ns_overlap(const char* what, int dtype, const pxl_ns_item* items, int n, int
   return PXL_OK;
 }
 
-// everything about a call but its workspace; nothing is launched
-int ns_check(const char* what, int dtype, const pxl_ns_item* items, int n, int steps, const float* coef, float eps, int muon, NsPlan& plan,
-             std::vector<NsStep>& st) {
-  // A bf16 matrix is one plane; the update of a Muon step is formed in 32 bits from a 32-bit momentum whatever the gradient's type, so two
-  // (rounded to one, 11 bits: the orthogonalised update of 256 x 1024 with six directions 50 times the noise is off by 2e-2).  Nor is X a bf16
-  // matrix any more behind a first segment: steps that do not fit into one run as those of 32-bit matrices
-  int planes = dtype == PXL_F32 || muon ? 2 : 1;
+// The steps of a call and its matrices' planes.  A bf16 matrix is one plane; the update of a Muon step is formed in 32 bits from a 32-bit momentum
+// whatever the gradient's type, so two (rounded to one, 11 bits: the orthogonalised update of 256 x 1024 with six directions 50 times the noise is off
+// by 2e-2).  Nor is X a bf16 matrix any more behind a first segment: steps that do not fit into one run as those of 32-bit matrices
+int ns_form(const char* what, int dtype, int steps, const float* coef, int muon, int& planes, std::vector<NsStep>& st) {
+  planes = dtype == PXL_F32 || muon ? 2 : 1;
   NS_TRY(ns_schedule(what, steps, coef, planes, st));
   if (planes == 1 && std::any_of(st.begin(), st.end() - 1, [](const NsStep& d) { return d.last; })) {
     planes = 2;
     st.clear();
     NS_TRY(ns_schedule(what, steps, coef, planes, st));
   }
+  return PXL_OK;
+}
+
+// everything about a call but its workspace; nothing is launched
+int ns_check(const char* what, int dtype, const pxl_ns_item* items, int n, int steps, const float* coef, float eps, int muon, NsPlan& plan,
+             std::vector<NsStep>& st) {
+  int planes;
+  NS_TRY(ns_form(what, dtype, steps, coef, muon, planes, st));
   NS_TRY(ns_plan(what, dtype, items, n, planes, plan));
   PXL_REQUIRE(eps > 0.f, "%s: eps %g", what, eps);
   for (int i = 0; i < n; ++i)
@@ -2367,6 +2373,18 @@ extern "C" size_t pxl_ns_workspace(int dtype, const pxl_ns_item* items, int n) {
       bytes = std::max(bytes, plan.bytes);
     }
     return bytes;
+  } catch (...) {
+    return 0;
+  }
+}
+
+extern "C" size_t pxl_orthogonalize_workspace(int dtype, const pxl_ns_item* items, int n, int steps, const float* coef) {
+  try {
+    int planes;
+    std::vector<NsStep> st;
+    NsPlan plan;
+    return ns_form("orthogonalize_workspace", dtype, steps, coef, 0, planes, st) == PXL_OK && ns_plan("orthogonalize_workspace", dtype, items, n, planes, plan) == PXL_OK
+               ? plan.bytes : 0;
   } catch (...) {
     return 0;
   }

@@ -439,14 +439,14 @@ def orthogonalize(x, steps=5, coefficients=NEWTON_SCHULZ, eps=1e-7):
         src, dst = x.data_ptr(), out.data_ptr()
         n = x.numel() // (rows * cols)
         items = (_lib.NsItem * n)(*[(dst + k * size, src + k * size, None, rows, cols, 1.0, 0) for k in range(n)])
-        index, fn, args, ws = _ns_call(lib().pxl_orthogonalize, x.device, dtype_code(x.dtype), items, n, steps, coef, eps)
+        nbytes = lib().pxl_orthogonalize_workspace(dtype_code(x.dtype), items, n, int(steps), coef)
+        index, fn, args, ws = _ns_call(lib().pxl_orthogonalize, nbytes, x.device, dtype_code(x.dtype), items, n, steps, coef, eps)
         _launch(index, fn, *args)
     return out
 
 
-def _ns_call(fn, dev, code, items, n, steps, coef, eps, *scalars):
-    """one call with its workspace, as _submit takes it"""
-    nbytes = lib().pxl_ns_workspace(code, items, n)
+def _ns_call(fn, nbytes, dev, code, items, n, steps, coef, eps, *scalars):
+    """one call with its workspace of nbytes (0: refused), as _submit takes it"""
     if nbytes == 0:
         raise _lib.PixelHipError("libpixelhip: %s" % lib().pxl_last_error().decode())
     ws = torch.empty(nbytes, device=dev, dtype=torch.uint8)
@@ -524,7 +524,8 @@ def muon_update(params, grads, momenta, lr, momentum=0.95, nesterov=True, weight
     for (dev, dtype), entries in work.items():
         items, n = (_lib.NsItem * len(entries))(*entries), len(entries)
         check(lib().pxl_muon_check(dtype_code(dtype), items, n, int(steps), coef, float(eps), lr, momentum, weight_decay))
-        index, fn, args, ws = _ns_call(lib().pxl_muon_step, dev, dtype_code(dtype), items, n, steps, coef, eps, lr, momentum, int(bool(nesterov)), weight_decay)
+        nbytes = lib().pxl_ns_workspace(dtype_code(dtype), items, n)
+        index, fn, args, ws = _ns_call(lib().pxl_muon_step, nbytes, dev, dtype_code(dtype), items, n, steps, coef, eps, lr, momentum, int(bool(nesterov)), weight_decay)
         calls.append((index, fn, args, (ws, keep)))
     _submit(calls)
     torch.autograd.graph.increment_version([t for t in params + momenta if t.numel()])

@@ -55,3 +55,18 @@ def test_steps_past_one_segment_are_the_32_bit_steps_rounded_once(shape, steps):
     from pixelssl_amd import functional as PF
     x = strong(shape, steps, 0.5).bfloat16().cuda()
     assert torch.equal(PF.orthogonalize(x, steps=steps), PF.orthogonalize(x.float(), steps=steps).bfloat16())
+
+
+def test_workspace_of_the_form_that_runs():
+    """bf16 matrices in five steps are one plane: their workspace is that of one, and enough for the call; refusals are 0"""
+    import ctypes
+    from pixelssl_amd import _lib
+    h = _lib.lib()
+    coef = (ctypes.c_float * 21)(*((3.4445, -4.7750, 2.0315) * 7))
+    items = (_lib.NsItem * 2)((1 << 20, 1 << 26, 0, 512, 4608, 1.0, 0), (1 << 30, 1 << 31, 0, 512, 4608, 1.0, 0))
+    five, seven, both = h.pxl_orthogonalize_workspace(1, items, 2, 5, coef), h.pxl_orthogonalize_workspace(1, items, 2, 7, coef), h.pxl_ns_workspace(1, items, 2)
+    assert 0 < five < 0.6 * seven and seven <= both
+    assert h.pxl_orthogonalize_workspace(0, items, 2, 5, coef) == h.pxl_ns_workspace(0, items, 2)
+    assert h.pxl_orthogonalize(1, items, 2, 5, coef, 1e-7, 1, five - 1, None) == -4
+    assert h.pxl_orthogonalize_workspace(1, items, 2, 17, coef) == 0 and h.pxl_orthogonalize_workspace(2, items, 2, 5, coef) == 0
+    assert h.pxl_orthogonalize_workspace(1, None, 2, 5, coef) == 0 and h.pxl_orthogonalize_workspace(1, items, 2, 5, None) == 0
